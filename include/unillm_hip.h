@@ -310,4 +310,8 @@ int unillm_hip_graph_destroy(unillm_graph* g);
 #ifdef __cplusplus
 }
 #endif
+
+/* Many sequences on one pool of KV pages: page tables and attention over them. */
+#include "unillm_hip_paged.h"
+
 #endif /* UNILLM_HIP_H */

@@ -16,6 +16,7 @@ __all__ = [
     "Q4_0", "Q4_K", "Q5_0", "Q5_K", "Q6_K", "Q8_0",
     "HipError",
     "QuantLinear", "quantize_blocks", "lm_head_forward", "KvCache",
+    "PageTable", "PagedKvCache",
 ]
 
 
@@ -27,4 +28,7 @@ def __getattr__(name):
     if name == "KvCache":
         from . import attention
         return attention.KvCache
+    if name in ("PageTable", "PagedKvCache"):
+        from . import paged
+        return getattr(paged, name)
     raise AttributeError(name)

@@ -11,6 +11,7 @@ import re
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libunillm_hip.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "unillm_hip.h")
+PAGED_HEADER = os.path.join(os.path.dirname(HERE), "include", "unillm_hip_paged.h")
 
 Q4_0 = 2
 Q8_0 = 8
@@ -98,11 +99,30 @@ SIGNATURES = {
     "unillm_hip_graph_launch": ([P, P], ctypes.c_int),
     "unillm_hip_graph_destroy": ([P], ctypes.c_int),
 }
+# include/unillm_hip_paged.h
+PAGED_SIGNATURES = {
+    "unillm_hip_page_table_bytes": (
+        [I64, I64, I64, I64, I64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "unillm_hip_page_table_create": ([I64, I64, I64, I64, I64, P, ctypes.POINTER(P)], ctypes.c_int),
+    "unillm_hip_page_table_destroy": ([P], ctypes.c_int),
+    "unillm_hip_page_table_buffers": ([P] + [ctypes.POINTER(P)] * 7, ctypes.c_int),
+    "unillm_hip_page_table_clear": ([P, P], ctypes.c_int),
+    "unillm_hip_page_table_extend": ([P, P, P, I64, P], ctypes.c_int),
+    "unillm_hip_page_table_truncate": ([P, P, P, I64, P], ctypes.c_int),
+    "unillm_hip_page_table_check": ([P, P], ctypes.c_int),
+    "unillm_hip_paged_kv_create": (
+        [ctypes.c_int, I64, I64, I64, I64, ctypes.c_float, P, P, ctypes.POINTER(P)], ctypes.c_int),
+    "unillm_hip_paged_kv_destroy": ([P], ctypes.c_int),
+    "unillm_hip_paged_kv_buffers": (
+        [P, ctypes.POINTER(P), ctypes.POINTER(P), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "unillm_hip_paged_attention": ([P, P, P, I64, I64, I64, I64, I64, P, I64, P], ctypes.c_int),
+    "unillm_hip_paged_attention_reserve": ([P, P, I64, I64, P], ctypes.c_int),
+}
 
 
-def header_symbols() -> list[str]:
-    """Every function the public header declares."""
-    with open(HEADER) as f:
+def header_symbols(header: str = HEADER) -> list[str]:
+    """Every function a public header declares."""
+    with open(header) as f:
         text = f.read()
     return sorted(set(re.findall(r"\b(unillm_hip_\w+)\s*\(", text)))
 
@@ -115,7 +135,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -m unillm_amd.build` "
                 "(the HIP library is required; there is no CPU fallback)")
         l = ctypes.CDLL(LIB_PATH)
-        for name, (args, res) in SIGNATURES.items():
+        for name, (args, res) in {**SIGNATURES, **PAGED_SIGNATURES}.items():
             fn = getattr(l, name)
             fn.argtypes = args
             fn.restype = res

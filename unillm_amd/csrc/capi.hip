@@ -403,7 +403,7 @@ int fail_launch(hipError_t e, const std::string& what) {
                         std::to_string(g_ws_capture_need) +
                         " bytes, which cannot happen while the stream is being captured; "
                         "reserve it before capture (unillm_hip_qmatmul_reserve / "
-                        "unillm_hip_attention_reserve) or make the same call once eagerly");
+                        "unillm_hip_attention_reserve / unillm_hip_paged_attention_reserve) or make the same call once eagerly");
     return fail_hip(e, what.c_str());
 }
 
@@ -845,6 +845,345 @@ int unillm_hip_attention_decode(unillm_kv_cache* c, const float* qkv_dev, int64_
     if (e != hipSuccess) return fail_launch(e, "attention launch");
     c->len += m;  // the kernels advance the device copy in stream order
     return UNILLM_OK;
+}
+
+// ---- page tables and paged attention ---------------------------------------------------------
+namespace {
+
+// Byte offsets of a table's parts in its storage, each on a 256-byte boundary.
+struct PageLayout {
+    size_t table, lens, free_pages, cu, ids, step_lens, slots, positions, counts, bytes;
+};
+
+int page_layout(int64_t max_seqs, int64_t max_pages, int64_t n_pages, int64_t page_size,
+                int64_t max_tokens, PageLayout* out) {
+    const int64_t far = (int64_t)INT32_MAX;
+    const bool size_ok = page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128 ||
+                         page_size == 256;
+    if (!size_ok || max_seqs < 1 || max_seqs > kPagesMaxSeqs || max_pages < 1 ||
+        max_pages > kPagesMaxEach || n_pages < 1 || n_pages > far / page_size ||
+        max_pages > far / page_size || max_tokens < 1 || max_tokens > kPagesMaxEach)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    "page table: need page_size 16 / 32 / 64 / 128 / 256, max_seqs in [1, " +
+                        std::to_string(kPagesMaxSeqs) + "], max_pages and max_tokens in [1, " +
+                        std::to_string(kPagesMaxEach) +
+                        "], n_pages >= 1, and n_pages and max_pages times page_size below 2^31");
+    size_t at = 0;
+    auto take = [&](int64_t ints) {
+        const size_t here = at;
+        at += ((size_t)ints * sizeof(int) + 255) & ~(size_t)255;
+        return here;
+    };
+    out->table = take(max_seqs * max_pages);
+    out->lens = take(max_seqs);
+    out->free_pages = take(n_pages);
+    out->cu = take(max_seqs + 1);
+    out->ids = take(max_seqs);
+    out->step_lens = take(max_seqs);
+    out->slots = take(max_tokens);
+    out->positions = take(max_tokens);
+    out->counts = take(kPagesCounts);
+    out->bytes = at;
+    return UNILLM_OK;
+}
+
+int check_entries(const unillm_page_table* t, const void* ids, const void* lens, bool need_lens,
+                  int64_t n, const char* what) {
+    if (!t) return fail(UNILLM_ERR_INVALID_ARG, std::string(what) + ": table is NULL");
+    if (n < 0 || n > t->st.max_seqs)
+        return fail(UNILLM_ERR_INVALID_ARG, std::string(what) + ": n_seqs " + std::to_string(n) +
+                                                " outside [0, " + std::to_string(t->st.max_seqs) + "]");
+    if (n > 0 && (!ids || (need_lens && !lens)))
+        return fail(UNILLM_ERR_INVALID_ARG, std::string(what) + ": ids or lengths is NULL");
+    if (((uintptr_t)ids & 3u) != 0 || ((uintptr_t)lens & 3u) != 0)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    std::string(what) + ": ids and lengths must be 4-byte aligned (int32)");
+    return UNILLM_OK;
+}
+
+// What a paged attention call and its reserve check alike.
+int check_paged(const unillm_paged_kv* c, const unillm_page_table* t, int64_t n, int64_t n_heads,
+                const std::string& what) {
+    if (!c || !t) return fail(UNILLM_ERR_INVALID_ARG, what + ": cache or table is NULL");
+    if (c->n_pages != t->st.n_pages || c->page_size != t->st.page_size)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + ": the cache has " + std::to_string(c->n_pages) + " pages of " +
+                        std::to_string(c->page_size) + ", the table " +
+                        std::to_string(t->st.n_pages) + " of " + std::to_string(t->st.page_size));
+    if (n_heads < c->n_kv_heads || n_heads % c->n_kv_heads != 0 || n_heads > 65535)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": need n_heads a multiple of n_kv_heads");
+    if (n < 0 || n > t->st.max_tokens)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": n_tokens " + std::to_string(n) +
+                                                " outside [0, " + std::to_string(t->st.max_tokens) +
+                                                "]");
+    return UNILLM_OK;
+}
+
+}  // namespace
+
+int unillm_hip_page_table_bytes(int64_t max_seqs, int64_t max_pages, int64_t n_pages,
+                                int64_t page_size, int64_t max_tokens, size_t* bytes) {
+    if (!bytes) return fail(UNILLM_ERR_INVALID_ARG, "bytes is NULL");
+    *bytes = 0;
+    PageLayout l;
+    if (int rc = page_layout(max_seqs, max_pages, n_pages, page_size, max_tokens, &l)) return rc;
+    *bytes = l.bytes;
+    return UNILLM_OK;
+}
+
+int unillm_hip_page_table_create(int64_t max_seqs, int64_t max_pages, int64_t n_pages,
+                                 int64_t page_size, int64_t max_tokens, void* storage_dev,
+                                 unillm_page_table** out) {
+    if (!out) return fail(UNILLM_ERR_INVALID_ARG, "out is NULL");
+    *out = nullptr;
+    PageLayout l;
+    if (int rc = page_layout(max_seqs, max_pages, n_pages, page_size, max_tokens, &l)) return rc;
+    if (((uintptr_t)storage_dev & 255u) != 0)
+        return fail(UNILLM_ERR_INVALID_ARG, "page table: storage must be 256-byte aligned");
+    if (int rc = ensure_init()) return rc;
+    unillm_page_table* t = new (std::nothrow) unillm_page_table{};
+    if (!t) return fail(UNILLM_ERR_OUT_OF_MEMORY, "host allocation failed");
+    hipError_t e = hipSuccess;
+    t->owned = storage_dev == nullptr;
+    t->storage = storage_dev;
+    if (t->owned && (e = hipMalloc(&t->storage, l.bytes)) != hipSuccess) {
+        delete t;
+        return e == hipErrorOutOfMemory ? fail(UNILLM_ERR_OUT_OF_MEMORY, "page table allocation")
+                                        : fail_hip(e, "page table allocation");
+    }
+    auto at = [&](size_t off) { return reinterpret_cast<int*>(static_cast<uint8_t*>(t->storage) + off); };
+    int shift = 0;
+    while (((int64_t)1 << shift) < page_size) ++shift;
+    t->st = {(int)max_seqs, (int)max_pages, (int)n_pages, (int)page_size, shift, (int)max_tokens,
+             at(l.table), at(l.lens), at(l.free_pages), at(l.cu), at(l.ids), at(l.step_lens),
+             at(l.slots), at(l.positions), at(l.counts)};
+    t->device = g_device;
+    t->entries = 0;
+    if ((e = launch_pages_clear(t->st, nullptr)) != hipSuccess ||
+        (e = hipStreamSynchronize(nullptr)) != hipSuccess) {
+        if (t->owned) (void)hipFree(t->storage);
+        delete t;
+        return fail_hip(e, "clearing the page table");
+    }
+    *out = t;
+    return UNILLM_OK;
+}
+
+int unillm_hip_page_table_destroy(unillm_page_table* t) {
+    if (!t) return UNILLM_OK;
+    const hipError_t e = t->owned ? hipFree(t->storage) : hipSuccess;
+    delete t;
+    return e == hipSuccess ? UNILLM_OK : fail_hip(e, "hipFree (page table)");
+}
+
+int unillm_hip_page_table_buffers(const unillm_page_table* t, int32_t** block_table,
+                                  int32_t** seq_lens, int32_t** free_pages, int32_t** n_free,
+                                  int32_t** cu_tokens, int32_t** slots, int32_t** positions) {
+    if (!t) return fail(UNILLM_ERR_INVALID_ARG, "page table is NULL");
+    if (block_table) *block_table = t->st.table;
+    if (seq_lens) *seq_lens = t->st.lens;
+    if (free_pages) *free_pages = t->st.free_pages;
+    if (n_free) *n_free = t->st.counts + kPagesFree;
+    if (cu_tokens) *cu_tokens = t->st.cu;
+    if (slots) *slots = t->st.slots;
+    if (positions) *positions = t->st.positions;
+    return UNILLM_OK;
+}
+
+int unillm_hip_page_table_clear(unillm_page_table* t, void* stream) {
+    if (!t) return fail(UNILLM_ERR_INVALID_ARG, "page table is NULL");
+    if (int rc = ensure_init()) return rc;
+    hipError_t e = launch_pages_clear(t->st, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? UNILLM_OK : fail_hip(e, "page table clear");
+}
+
+int unillm_hip_page_table_extend(unillm_page_table* t, const int32_t* seq_ids_dev,
+                                 const int32_t* new_lens_dev, int64_t n_seqs, void* stream) {
+    if (int rc = check_entries(t, seq_ids_dev, new_lens_dev, true, n_seqs, "page table extend"))
+        return rc;
+    if (int rc = ensure_init()) return rc;
+    hipError_t e = launch_pages_extend(t->st, seq_ids_dev, new_lens_dev, n_seqs,
+                                       static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail_hip(e, "page table extend");
+    t->entries = n_seqs;
+    return UNILLM_OK;
+}
+
+int unillm_hip_page_table_truncate(unillm_page_table* t, const int32_t* seq_ids_dev,
+                                   const int32_t* lens_dev, int64_t n_seqs, void* stream) {
+    if (int rc = check_entries(t, seq_ids_dev, lens_dev, false, n_seqs, "page table truncate"))
+        return rc;
+    if (int rc = ensure_init()) return rc;
+    hipError_t e = launch_pages_truncate(t->st, seq_ids_dev, lens_dev, n_seqs,
+                                         static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? UNILLM_OK : fail_hip(e, "page table truncate");
+}
+
+int unillm_hip_page_table_check(unillm_page_table* t, void* stream) {
+    if (!t) return fail(UNILLM_ERR_INVALID_ARG, "page table is NULL");
+    if (int rc = ensure_init()) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    int code = 0;
+    const int none = 0;
+    hipError_t e = hipMemcpyAsync(&code, t->st.counts + kPagesError, sizeof(code),
+                                  hipMemcpyDeviceToHost, s);
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    if (e == hipSuccess && code != 0) {
+        e = hipMemcpyAsync(t->st.counts + kPagesError, &none, sizeof(none), hipMemcpyHostToDevice, s);
+        if (e == hipSuccess) e = hipStreamSynchronize(s);
+    }
+    if (e != hipSuccess) return fail_hip(e, "page table check");
+    const std::string what = "page table: ";
+    switch (code) {
+        case 0: return UNILLM_OK;
+        case kPagesBadId:
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + "a sequence id past max_seqs, or twice in one batch");
+        case kPagesBadLength:
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + "a negative number of new tokens, or a truncate outside [0, length]");
+        case kPagesSeqFull:
+            return fail(UNILLM_ERR_INVALID_ARG, what + "a sequence longer than max_pages pages");
+        case kPagesStepFull:
+            return fail(UNILLM_ERR_INVALID_ARG, what + "a step of more than max_tokens tokens");
+        case kPagesNoPages:
+            return fail(UNILLM_ERR_OUT_OF_MEMORY, what + "the pool has too few free pages");
+        case kPagesNoPlan:
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + "attention without a plan (extend comes first, after any truncate)");
+        case kPagesRows:
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + "attention on fewer rows than the step's plan has");
+        default:
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + "its state is not one that its calls leave (a length, n_free or a "
+                               "page id out of range)");
+    }
+}
+
+int unillm_hip_paged_kv_create(int kv_type, int64_t n_kv_heads, int64_t head_dim, int64_t n_pages,
+                               int64_t page_size, float rope_theta, void* k_dev, void* v_dev,
+                               unillm_paged_kv** out) {
+    if (!out) return fail(UNILLM_ERR_INVALID_ARG, "out is NULL");
+    *out = nullptr;
+    if (!is_dense(kv_type))
+        return fail(UNILLM_ERR_UNSUPPORTED, "paged KV cache: unsupported type " + std::to_string(kv_type) +
+                                                " (want 0 = F32, 1 = F16, 30 = BF16)");
+    PageLayout l;
+    if (n_kv_heads < 1 || n_kv_heads > 65535 || !(head_dim == 64 || head_dim == 128 || head_dim == 256) ||
+        !(rope_theta > 0.0f) || !isfinite(rope_theta))
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    "paged KV cache: need n_kv_heads >= 1, head_dim 64 / 128 / 256, rope_theta > 0");
+    if (int rc = page_layout(1, 1, n_pages, page_size, 1, &l)) return rc;
+    if ((k_dev == nullptr) != (v_dev == nullptr) || !aligned16(k_dev) || !aligned16(v_dev))
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    "paged KV cache: give both of k and v, 16-byte aligned, or neither");
+    if (int rc = ensure_init()) return rc;
+    unillm_paged_kv* c = new (std::nothrow) unillm_paged_kv{};
+    if (!c) return fail(UNILLM_ERR_OUT_OF_MEMORY, "host allocation failed");
+    c->device = g_device;
+    c->type = kv_type;
+    c->n_kv_heads = n_kv_heads;
+    c->head_dim = head_dim;
+    c->n_pages = n_pages;
+    c->page_size = page_size;
+    while (((int64_t)1 << c->page_shift) < page_size) ++c->page_shift;
+    c->rope_theta = rope_theta;
+    c->k = k_dev;
+    c->v = v_dev;
+    c->owned = k_dev == nullptr;
+    std::vector<double> freq((size_t)head_dim / 2);
+    for (size_t i = 0; i < freq.size(); ++i)
+        freq[i] = pow((double)rope_theta, -2.0 * (double)i / (double)head_dim) / M_PI;
+    const size_t bytes = (size_t)(n_pages * page_size) * (size_t)(n_kv_heads * head_dim) *
+                         (size_t)dense_elem_bytes(kv_type);
+    void* f = nullptr;
+    hipError_t e = hipMalloc(&f, freq.size() * sizeof(double));
+    if (e == hipSuccess)
+        e = hipMemcpy(f, freq.data(), freq.size() * sizeof(double), hipMemcpyHostToDevice);
+    if (c->owned && e == hipSuccess && (e = hipMalloc(&c->k, bytes)) == hipSuccess &&
+        (e = hipMalloc(&c->v, bytes)) == hipSuccess && (e = hipMemset(c->k, 0, bytes)) == hipSuccess)
+        e = hipMemset(c->v, 0, bytes);
+    if (e != hipSuccess) {
+        (void)hipFree(f);
+        if (c->owned) {
+            (void)hipFree(c->k);
+            (void)hipFree(c->v);
+        }
+        delete c;
+        return e == hipErrorOutOfMemory ? fail(UNILLM_ERR_OUT_OF_MEMORY, "paged KV cache allocation")
+                                        : fail_hip(e, "paged KV cache allocation");
+    }
+    c->freq = static_cast<double*>(f);
+    *out = c;
+    return UNILLM_OK;
+}
+
+int unillm_hip_paged_kv_destroy(unillm_paged_kv* c) {
+    if (!c) return UNILLM_OK;
+    hipError_t e = hipFree(c->freq);
+    if (c->owned) {
+        const hipError_t e2 = hipFree(c->k), e3 = hipFree(c->v);
+        if (e == hipSuccess) e = e2;
+        if (e == hipSuccess) e = e3;
+    }
+    delete c;
+    return e == hipSuccess ? UNILLM_OK : fail_hip(e, "hipFree (paged KV cache)");
+}
+
+int unillm_hip_paged_kv_buffers(const unillm_paged_kv* c, void** k, void** v, size_t* bytes) {
+    if (!c) return fail(UNILLM_ERR_INVALID_ARG, "cache is NULL");
+    if (k) *k = c->k;
+    if (v) *v = c->v;
+    if (bytes)
+        *bytes = (size_t)(c->n_pages * c->page_size) * (size_t)(c->n_kv_heads * c->head_dim) *
+                 (size_t)dense_elem_bytes(c->type);
+    return UNILLM_OK;
+}
+
+int unillm_hip_paged_attention(unillm_paged_kv* c, const unillm_page_table* t,
+                               const float* qkv_dev, int64_t qkv_stride, int64_t n_tokens,
+                               int64_t n_heads, int64_t window, int64_t sinks, float* out_dev,
+                               int64_t out_stride, void* stream) {
+    const std::string what = "paged attention";
+    if (int rc = check_paged(c, t, n_tokens, n_heads, what)) return rc;
+    if (window < 0 || sinks < 0 || (window == 0 && sinks != 0))
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + ": need window >= 0 and sinks >= 0 (0 without a window)");
+    if (n_tokens == 0) return UNILLM_OK;
+    const int64_t width = (n_heads + 2 * c->n_kv_heads) * c->head_dim, owidth = n_heads * c->head_dim;
+    const int64_t far = (int64_t)1 << 40;
+    if (qkv_stride < width || out_stride < owidth || qkv_stride % 4 != 0 || out_stride % 4 != 0 ||
+        qkv_stride > far || out_stride > far)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + ": row strides must be multiples of 4 floats, of at least " +
+                        std::to_string(width) + " (qkv) and " + std::to_string(owidth) + " (out)");
+    if (!qkv_dev || !out_dev) return fail(UNILLM_ERR_INVALID_ARG, what + ": qkv or out is NULL");
+    if (!aligned16(qkv_dev) || !aligned16(out_dev))
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": qkv and out must be 16-byte aligned");
+    const uintptr_t q0 = (uintptr_t)qkv_dev, o0 = (uintptr_t)out_dev;
+    const uintptr_t q1 = q0 + (uintptr_t)((n_tokens - 1) * qkv_stride + width) * sizeof(float),
+                    o1 = o0 + (uintptr_t)((n_tokens - 1) * out_stride + owidth) * sizeof(float);
+    if (q0 < o1 && o0 < q1)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": out must not share memory with qkv");
+    if (int rc = ensure_init()) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const std::unique_lock<std::mutex> order = stream_order(s);
+    hipError_t e = launch_paged_attention(*c, *t, qkv_dev, qkv_stride, n_tokens, n_heads, window,
+                                          sinks, out_dev, out_stride, s);
+    return e == hipSuccess ? UNILLM_OK : fail_launch(e, what);
+}
+
+int unillm_hip_paged_attention_reserve(const unillm_paged_kv* c, const unillm_page_table* t,
+                                       int64_t n_tokens, int64_t n_heads, void* stream) {
+    const std::string what = "paged attention reserve";
+    if (int rc = check_paged(c, t, n_tokens, n_heads, what)) return rc;
+    if (n_tokens == 0) return UNILLM_OK;
+    if (int rc = ensure_init()) return rc;
+    void* p = nullptr;
+    hipError_t e = stream_workspace(static_cast<hipStream_t>(stream),
+                                    paged_workspace_bytes(*c, *t, n_tokens, n_heads), &p, kPagedSlot);
+    return e == hipSuccess ? UNILLM_OK : fail_launch(e, what);
 }
 
 int unillm_hip_malloc(void** ptr, size_t bytes) {

@@ -80,6 +80,44 @@ struct unillm_kv_cache {
     bool captured;
 };
 
+// The state of a page table (pages.hip), all in device memory: the kernels take it by value.
+struct unillm_page_state {
+    int max_seqs, max_pages, n_pages, page_size, page_shift, max_tokens;
+    int* table;       // [max_seqs][max_pages] page ids, -1 where none
+    int* lens;        // [max_seqs] tokens held
+    int* free_pages;  // [n_pages] stack
+    int* cu;          // the step's plan: [max_seqs + 1] first row of each entry,
+    int* step_ids;    // [max_seqs] its sequence (-1: a padding entry)
+    int* step_lens;   // [max_seqs] and its tokens with the new ones
+    int* slots;       // [max_tokens] page * page_size + offset of each row
+    int* positions;   // [max_tokens]
+    int* counts;      // [kPagesCounts], below
+};
+
+// The opaque page-table handle.  entries: the batch of the last extend (what an attention
+// call sizes its grid for; its kernels take the device's own count).
+struct unillm_page_table {
+    unillm_page_state st;
+    int device;
+    void* storage;
+    bool owned;
+    int64_t entries;
+};
+
+// The opaque handle of one layer's pool of KV pages: K [n_pages][n_kv_heads][page_size][hd],
+// V [n_pages][n_kv_heads][hd][page_size], both of `type` (F32, F16 or BF16).
+struct unillm_paged_kv {
+    int device;
+    int type;
+    int64_t n_kv_heads, head_dim, n_pages, page_size;
+    int page_shift;
+    float rope_theta;
+    void* k;
+    void* v;
+    double* freq;  // [hd / 2] theta^(-2 i / hd) / pi: a token's angle in half turns a position
+    bool owned;
+};
+
 namespace unillm {
 
 constexpr int QK = 32;  // weights per block
@@ -171,9 +209,10 @@ const DeviceInfo& device_info();
 // attention's partials (and, for hd 256 prompts, the rotated queries); slot 3 an
 // aligned copy of x; slot kSyncSlot the batched decode's arrival tickets, zeroed
 // when allocated (every launch leaves them zero again); slot kDenseSlot a dense
-// weight's x in bf16 parts and its split-k slabs.
+// weight's x in bf16 parts and its split-k slabs; slot kPagedSlot paged attention's partials.
 constexpr int kSyncSlot = 4;
 constexpr int kDenseSlot = 5;
+constexpr int kPagedSlot = 6;
 hipError_t stream_workspace(hipStream_t s, size_t bytes, void** out, int slot = 0);
 // UNILLM_DEBUG_LAUNCH=1 prints each kernel's launch shape to stderr.
 bool debug_launch();
@@ -276,6 +315,33 @@ hipError_t launch_attention(const KvCache& kv, const float* qkv, int64_t m, int6
 size_t attention_workspace_bytes(const KvCache& kv, int64_t m, int64_t H);
 int attention_max_queries();  // m * H / KVH per decode call
 int64_t attention_max_positions();  // len + m per call
+
+// Page tables (pages.hip).  counts: n_free, whether a step's plan is valid, its rows and
+// entries; on cache lines of their own the ticket of a launch's last workgroup and the first
+// error since the last check.
+using PageTable = ::unillm_page_state;
+constexpr int kPagesFree = 0, kPagesStep = 1, kPagesTokens = 2, kPagesEntries = 3, kPagesTicket = 32,
+              kPagesError = 64, kPagesCounts = 96;
+constexpr int kPagesBadId = 1, kPagesBadLength = 2, kPagesSeqFull = 3, kPagesStepFull = 4,
+              kPagesNoPages = 5, kPagesBadState = 6, kPagesNoPlan = 7, kPagesRows = 8;
+constexpr int64_t kPagesMaxSeqs = 8192;       // (a call's entries are scanned in LDS)
+constexpr int64_t kPagesMaxEach = 1 << 22;    // max_tokens, max_pages
+hipError_t launch_pages_clear(const PageTable& t, hipStream_t s);
+hipError_t launch_pages_extend(const PageTable& t, const int32_t* ids, const int32_t* news,
+                               int64_t B, hipStream_t s);
+// lens == nullptr: all 0
+hipError_t launch_pages_truncate(const PageTable& t, const int32_t* ids, const int32_t* lens,
+                                 int64_t B, hipStream_t s);
+
+// Attention over pages (paged.hip): the step's rows qkv[n][(H + 2 KVH) hd] (qstride floats
+// apart), rotated at their positions, k and v into their slots, then causal attention (window
+// > 0: the last `window` positions and the first `sinks`) into out[n][H hd] (ostride apart).
+using PagedKv = ::unillm_paged_kv;
+hipError_t launch_paged_attention(const PagedKv& c, const unillm_page_table& t, const float* qkv,
+                                  int64_t qstride, int64_t n, int64_t H, int64_t window,
+                                  int64_t sinks, float* out, int64_t ostride, hipStream_t s);
+// Workspace (slot kPagedSlot) of such a call of up to n rows.
+size_t paged_workspace_bytes(const PagedKv& c, const unillm_page_table& t, int64_t n, int64_t H);
 
 constexpr int64_t kGemvMaxM = 4;
 constexpr int64_t kDecodeMaxM = 64;

@@ -19,6 +19,8 @@ const SOURCES: &[&str] = &[
     "prefill.hip",
     "attention.hip",
     "dense.hip",
+    "pages.hip",
+    "paged.hip",
 ];
 
 // Libraries the link adds besides HIP's own.  Keep in step with LIBS in unillm_amd/build.py.

@@ -10,6 +10,8 @@
 //! * [`KvCache`] takes the slot of `LayerKVCache` (crates/runtime/src/kv_cache.rs:28-150)
 //!   together with the attention of `LlamaAttention::forward_with_cache` after the
 //!   projections (llama.rs:1044-1150).
+//! * [`PageTable`] and [`PagedKvCache`] are many sequences on one pool of KV pages, the cache
+//!   that `crates/kv` declares without a device behind it (crates/kv/src/gpu_memory.rs:110).
 //!
 //! No dependencies: errors are [`HipError`], which implements `std::error::Error`, so
 //! `?` turns it into the reference's `anyhow::Error`.  Its message is the library's
@@ -130,6 +132,55 @@ pub mod sys {
         pub fn unillm_hip_graph_end(stream: *mut c_void, out: *mut *mut unillm_graph) -> c_int;
         pub fn unillm_hip_graph_launch(g: *const unillm_graph, stream: *mut c_void) -> c_int;
         pub fn unillm_hip_graph_destroy(g: *mut unillm_graph) -> c_int;
+    }
+
+    // include/unillm_hip_paged.h
+    /// Opaque page table: which page holds which positions of which sequence.
+    #[repr(C)]
+    pub struct unillm_page_table {
+        _private: [u8; 0],
+    }
+    /// Opaque pool of one layer's KV pages.
+    #[repr(C)]
+    pub struct unillm_paged_kv {
+        _private: [u8; 0],
+    }
+
+    extern "C" {
+        pub fn unillm_hip_page_table_bytes(max_seqs: i64, max_pages: i64, n_pages: i64,
+                                           page_size: i64, max_tokens: i64, bytes: *mut usize) -> c_int;
+        pub fn unillm_hip_page_table_create(max_seqs: i64, max_pages: i64, n_pages: i64,
+                                            page_size: i64, max_tokens: i64,
+                                            storage_dev: *mut c_void,
+                                            out: *mut *mut unillm_page_table) -> c_int;
+        pub fn unillm_hip_page_table_destroy(t: *mut unillm_page_table) -> c_int;
+        pub fn unillm_hip_page_table_buffers(t: *const unillm_page_table,
+                                             block_table: *mut *mut i32, seq_lens: *mut *mut i32,
+                                             free_pages: *mut *mut i32, n_free: *mut *mut i32,
+                                             cu_tokens: *mut *mut i32, slots: *mut *mut i32,
+                                             positions: *mut *mut i32) -> c_int;
+        pub fn unillm_hip_page_table_clear(t: *mut unillm_page_table, stream: *mut c_void) -> c_int;
+        pub fn unillm_hip_page_table_extend(t: *mut unillm_page_table, seq_ids_dev: *const i32,
+                                            new_lens_dev: *const i32, n_seqs: i64,
+                                            stream: *mut c_void) -> c_int;
+        pub fn unillm_hip_page_table_truncate(t: *mut unillm_page_table, seq_ids_dev: *const i32,
+                                              lens_dev: *const i32, n_seqs: i64,
+                                              stream: *mut c_void) -> c_int;
+        pub fn unillm_hip_page_table_check(t: *mut unillm_page_table, stream: *mut c_void) -> c_int;
+        pub fn unillm_hip_paged_kv_create(kv_type: c_int, n_kv_heads: i64, head_dim: i64,
+                                          n_pages: i64, page_size: i64, rope_theta: f32,
+                                          k_dev: *mut c_void, v_dev: *mut c_void,
+                                          out: *mut *mut unillm_paged_kv) -> c_int;
+        pub fn unillm_hip_paged_kv_destroy(c: *mut unillm_paged_kv) -> c_int;
+        pub fn unillm_hip_paged_kv_buffers(c: *const unillm_paged_kv, k: *mut *mut c_void,
+                                           v: *mut *mut c_void, bytes: *mut usize) -> c_int;
+        pub fn unillm_hip_paged_attention(c: *mut unillm_paged_kv, t: *const unillm_page_table,
+                                          qkv_dev: *const f32, qkv_stride: i64, n_tokens: i64,
+                                          n_heads: i64, window: i64, sinks: i64,
+                                          out_dev: *mut f32, out_stride: i64, stream: *mut c_void) -> c_int;
+        pub fn unillm_hip_paged_attention_reserve(c: *const unillm_paged_kv,
+                                                  t: *const unillm_page_table, n_tokens: i64,
+                                                  n_heads: i64, stream: *mut c_void) -> c_int;
     }
 }
 
@@ -563,6 +614,125 @@ impl Drop for KvCache {
     fn drop(&mut self) {
         unsafe {
             sys::unillm_hip_kv_cache_destroy(self.c);
+        }
+    }
+}
+
+// ---- many sequences on one pool of KV pages ----------------------------------------------
+
+/// Which page holds which positions of which sequence, and the current step's plan, in device
+/// memory.  Calls are asynchronous on `stream`; [`PageTable::check`] reports what failed there.
+pub struct PageTable {
+    t: *mut sys::unillm_page_table,
+}
+
+unsafe impl Send for PageTable {}
+
+impl PageTable {
+    pub fn new(max_seqs: usize, max_pages: usize, n_pages: usize, page_size: usize,
+               max_tokens: usize) -> Result<Self> {
+        let mut t = ptr::null_mut();
+        check(unsafe {
+            sys::unillm_hip_page_table_create(to_i64(max_seqs, "max_seqs")?,
+                                              to_i64(max_pages, "max_pages")?,
+                                              to_i64(n_pages, "n_pages")?,
+                                              to_i64(page_size, "page_size")?,
+                                              to_i64(max_tokens, "max_tokens")?, ptr::null_mut(),
+                                              &mut t)
+        })?;
+        Ok(Self { t })
+    }
+
+    /// Room for `new_lens[b]` more tokens of sequence `seq_ids[b]`, and the step's plan.
+    ///
+    /// # Safety
+    /// `seq_ids` and `new_lens` point to n_seqs i32 in device memory; `stream` is a HIP stream
+    /// of the library's device, or null.
+    pub unsafe fn extend_raw(&mut self, seq_ids: *const i32, new_lens: *const i32, n_seqs: usize,
+                             stream: *mut c_void) -> Result<()> {
+        check(sys::unillm_hip_page_table_extend(self.t, seq_ids, new_lens,
+                                                to_i64(n_seqs, "n_seqs")?, stream))
+    }
+
+    /// Sequence `seq_ids[b]` keeps its first `lens[b]` tokens (`lens` null: none).
+    ///
+    /// # Safety
+    /// As [`PageTable::extend_raw`].
+    pub unsafe fn truncate_raw(&mut self, seq_ids: *const i32, lens: *const i32, n_seqs: usize,
+                               stream: *mut c_void) -> Result<()> {
+        check(sys::unillm_hip_page_table_truncate(self.t, seq_ids, lens,
+                                                  to_i64(n_seqs, "n_seqs")?, stream))
+    }
+
+    /// Waits for `stream`; the first call since the last check that failed on the device.
+    ///
+    /// # Safety
+    /// `stream` is a HIP stream of the library's device, or null.
+    pub unsafe fn check(&mut self, stream: *mut c_void) -> Result<()> {
+        check(sys::unillm_hip_page_table_check(self.t, stream))
+    }
+}
+
+impl Drop for PageTable {
+    fn drop(&mut self) {
+        unsafe {
+            sys::unillm_hip_page_table_destroy(self.t);
+        }
+    }
+}
+
+/// One layer's pool of KV pages, of `kv_type` `sys::UNILLM_QTYPE_F32`, `_F16` or `_BF16`.
+pub struct PagedKvCache {
+    c: *mut sys::unillm_paged_kv,
+}
+
+unsafe impl Send for PagedKvCache {}
+
+impl PagedKvCache {
+    pub fn new(kv_type: c_int, n_kv_heads: usize, head_dim: usize, n_pages: usize,
+               page_size: usize, rope_theta: f32) -> Result<Self> {
+        let mut c = ptr::null_mut();
+        check(unsafe {
+            sys::unillm_hip_paged_kv_create(kv_type, to_i64(n_kv_heads, "n_kv_heads")?,
+                                            to_i64(head_dim, "head_dim")?,
+                                            to_i64(n_pages, "n_pages")?,
+                                            to_i64(page_size, "page_size")?, rope_theta,
+                                            ptr::null_mut(), ptr::null_mut(), &mut c)
+        })?;
+        Ok(Self { c })
+    }
+
+    /// Grows `stream`'s workspace for calls of up to n_tokens rows (before a graph capture).
+    pub fn reserve(&self, table: &PageTable, n_tokens: usize, n_heads: usize,
+                   stream: *mut c_void) -> Result<()> {
+        check(unsafe {
+            sys::unillm_hip_paged_attention_reserve(self.c, table.t, to_i64(n_tokens, "n_tokens")?,
+                                                    to_i64(n_heads, "n_heads")?, stream)
+        })
+    }
+
+    /// RoPE, append and attention of the plan's rows: qkv [n_tokens, (n_heads + 2 n_kv_heads)
+    /// head_dim] -> out [n_tokens, n_heads head_dim], rows `_stride` floats apart.
+    ///
+    /// # Safety
+    /// `qkv` and `out` point to device memory of those sizes, 16-byte aligned, not overlapping;
+    /// `stream` is a HIP stream of the library's device, or null.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn attention_raw(&mut self, table: &PageTable, qkv: *const f32, qkv_stride: usize,
+                                n_tokens: usize, n_heads: usize, window: usize, sinks: usize,
+                                out: *mut f32, out_stride: usize, stream: *mut c_void) -> Result<()> {
+        check(sys::unillm_hip_paged_attention(self.c, table.t, qkv, to_i64(qkv_stride, "qkv_stride")?,
+                                              to_i64(n_tokens, "n_tokens")?,
+                                              to_i64(n_heads, "n_heads")?, to_i64(window, "window")?,
+                                              to_i64(sinks, "sinks")?, out,
+                                              to_i64(out_stride, "out_stride")?, stream))
+    }
+}
+
+impl Drop for PagedKvCache {
+    fn drop(&mut self) {
+        unsafe {
+            sys::unillm_hip_paged_kv_destroy(self.c);
         }
     }
 }
