@@ -10,6 +10,7 @@
 // the true value; sums, maxima and quotients are f32.
 #include <hip/hip_runtime.h>
 
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -62,6 +63,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // One piece of a call's work: the visits v0 .. v0 + nv - 1 of a tile of `rows` query rows
 // (row r of an entry is head r % G of its token r / G, for each kv head).  Of a tile dealt out
 // in S > 1 pieces this is piece s; its partial sums go to rows base + (g S + s) rows + r.
+// An entry of up to kNarrowRows rows has narrow tiles, a longer one wide ones, each kind with
+// a list and a kernel of its own.
 struct Item {
     int entry, row0, rows, v0, nv, base, s, S;
 };
@@ -77,18 +80,26 @@ struct Call {
     int64_t qstride, ostride;
     int n, H, KVH, G;
     int window, sinks;
-    int target;     // pieces to deal the call's work out in, over all kv heads
-    int most_rows;  // partial rows there is room for
-    int* head;      // [0] items, [1] splits
-    Item* items;
-    Split* splits;
-    float2* turn;   // [n][hd / 2] cos, sin of each row's angles
-    float2* ms;     // [most_rows] maximum (log2), sum of the weights
-    float* po;      // [most_rows][hd] unnormalized sums
+    float2* turn;  // [n][hd / 2] cos, sin of each row's angles
+    float2* ms;    // partial rows: maximum (log2), sum of the weights
+    float* po;     // [hd] unnormalized sums
+    struct Kind {
+        int target;     // pieces to deal the kind's work out in, over all kv heads
+        int least;      // visits of the smallest piece
+        int row0, most_rows;  // its partial rows
+        int* head;      // [0] items, [1] splits
+        Item* items;
+        Split* splits;
+    } kind[2];
 };
 
-constexpr int kTileRows = 16;  // query rows of a tile
-constexpr int kUnit = 32;      // keys of a visit
+constexpr int kNarrow = 0, kWide = 1;
+constexpr int kNarrowRows = 64;  // most query rows of an entry (a kv head) for narrow tiles
+constexpr int kTileRows[2] = {16, 128};  // query rows of a tile
+constexpr int kUnit = 32;        // keys of a narrow tile's visit
+// keys of a wide tile's visit: what leaves room for two workgroups a CU (one of f32 at hd 256)
+template <class T, int D>
+constexpr int kWideUnit = sizeof(T) == 2 && D < 256 ? 64 : 32;
 
 // Whether the step can run: a plan, of at most the call's rows.
 __device__ __forceinline__ bool step_fits(const PageTable& t, int n) {
@@ -135,22 +146,34 @@ __device__ __forceinline__ int2 block_scan2(int2 v, int2* tmp) {
     return make_int2(v.x + base.x, v.y + base.y);
 }
 
-// Deals the step's work out (one workgroup): every entry's rows in tiles of kTileRows, every
-// tile's visits in equal pieces of at most C, where C makes a.target pieces over all kv heads.
-// tp: LDS [entries + 1].
-__device__ void plan(const PageTable& t, const Call& a, int* tp, int2* tmp) {
-    const int tid = threadIdx.x, B = t.counts[kPagesEntries];
-    int carry = 0;
+// Deals one kind's work out (one workgroup): every entry's rows in tiles, every tile's visits of
+// U keys in equal pieces of at most C, where C makes the kind's target of pieces over all kv
+// heads.  An entry's last tile, whose rows see the most keys, is dealt out first.
+// sm: LDS, tp[B + 1] (tiles before each entry) | m[B] | ctx[B].
+template <int U>
+__device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
+    __shared__ int2 tmp[4];
+    __shared__ float part[4];
+    __shared__ int off[257], info[256][6], last[2];
+    const Call::Kind& kd = a.kind[kind];
+    const int tid = threadIdx.x, B = t.counts[kPagesEntries], TR = kTileRows[kind];
+    int *tp = sm, *ms = tp + B + 1, *ctxs = ms + B;
+    int tiles = 0;
     if (tid == 0) tp[0] = 0;
     for (int b0 = 0; b0 < B; b0 += 256) {
         const int b = b0 + tid;
-        const int m = b < B ? t.cu[b + 1] - t.cu[b] : 0;
-        const int2 s = block_scan2(make_int2((m * a.G + kTileRows - 1) / kTileRows, 0), tmp);
-        if (b < B) tp[b + 1] = carry + s.x;
+        int n = 0;
+        if (b < B) {
+            const int m = t.cu[b + 1] - t.cu[b], rows = m * a.G;
+            ms[b] = m;
+            ctxs[b] = t.step_lens[b] - m;
+            if ((rows <= kNarrowRows) == (kind == kNarrow)) n = (rows + TR - 1) / TR;
+        }
+        const int2 s = block_scan2(make_int2(n, 0), tmp);
+        if (b < B) tp[b + 1] = tiles + s.x;
         __syncthreads();
-        carry = tp[min(b0 + 256, B)];
+        tiles = tp[min(b0 + 256, B)];
     }
-    const int tiles = carry;
     struct Tile {
         int b, row0, rows, nv;
     };
@@ -161,22 +184,18 @@ __device__ void plan(const PageTable& t, const Call& a, int* tp, int2* tmp) {
             if (tp[mid] <= i) lo = mid;
             else hi = mid;
         }
-        const int m = t.cu[lo + 1] - t.cu[lo], ctx = t.step_lens[lo] - m;
-        Tile x{lo, (i - tp[lo]) * kTileRows, 0, 0};
-        x.rows = min(kTileRows, m * a.G - x.row0);
-        x.nv = Visits<kUnit>(ctx + x.row0 / a.G, ctx + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks).count;
+        Tile x{lo, (tp[lo + 1] - 1 - i) * TR, 0, 0};
+        x.rows = min(TR, ms[lo] * a.G - x.row0);
+        x.nv = Visits<U>(ctxs[lo] + x.row0 / a.G, ctxs[lo] + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks).count;
         return x;
     };
-    // (visits of a call: below 2^31 / 32 keys a tile; their sum in f32 is exact enough to divide)
-    float sum = 0.0f;
+    float sum = 0.0f;  // (as a float: it is only divided by)
     for (int i = tid; i < tiles; i += 256) sum += (float)tile(i).nv;
     sum = wave_add(sum);
-    __shared__ float part[4];
-    __syncthreads();
     if ((tid & 63) == 0) part[tid >> 6] = sum;
     __syncthreads();
     const float all = (part[0] + part[1]) + (part[2] + part[3]);
-    const int C = max(4, (int)ceilf(all * (float)a.KVH / (float)a.target));
+    const int C = max(kd.least, (int)ceilf(all * (float)a.KVH / (float)kd.target));
     int items = 0, splits = 0, rows = 0;
     for (int i0 = 0; i0 < tiles; i0 += 256) {
         const int i = i0 + tid;
@@ -189,54 +208,62 @@ __device__ void plan(const PageTable& t, const Call& a, int* tp, int2* tmp) {
         const int want = S > 1 ? S * a.KVH * x.rows : 0;
         const int2 r = block_scan2(make_int2(want, S > 1 ? 1 : 0), tmp);
         const int base = rows + r.x - want;
-        if (S > 1 && base + want > a.most_rows) S = 1;  // (no room: whole)
+        if (S > 1 && base + want > kd.most_rows) S = 1;  // (no room: whole)
         const int2 n = block_scan2(make_int2(S, 0), tmp);
-        for (int s = 0; s < S; ++s) {
-            const int v0 = (int)((int64_t)s * x.nv / S), v1 = (int)((int64_t)(s + 1) * x.nv / S);
-            a.items[items + n.x - S + s] = {x.b, x.row0, x.rows, v0, v1 - v0, base, s, S};
-        }
-        if (want) a.splits[splits + r.y - 1] = {x.b, x.row0, x.rows, base, S, {}};
-        __shared__ int last[3];
+        off[tid + 1] = n.x;
+        if (tid == 0) off[0] = 0;
         if (tid == 255) {
-            last[0] = n.x;
-            last[1] = r.y;
-            last[2] = r.x;
+            last[0] = r.y;
+            last[1] = r.x;
         }
+        const int v[6] = {x.b, x.row0, x.rows, x.nv, kd.row0 + base, S};
+#pragma unroll
+        for (int e = 0; e < 6; ++e) info[tid][e] = v[e];
+        if (want) kd.splits[splits + r.y - 1] = {x.b, x.row0, x.rows, kd.row0 + base, S, {}};
         __syncthreads();
-        items += last[0];
-        splits += last[1];
-        rows += last[2];
+        for (int k = tid; k < off[256]; k += 256) {
+            int lo = 0, hi = 256;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (off[mid] <= k) lo = mid;
+                else hi = mid;
+            }
+            const int* w = info[lo];
+            const int s = k - off[lo], nv = w[3], Sw = w[5];
+            const int v0 = (int)((int64_t)s * nv / Sw), v1 = (int)((int64_t)(s + 1) * nv / Sw);
+            kd.items[items + k] = {w[0], w[1], w[2], v0, v1 - v0, w[4], s, Sw};
+        }
+        items += off[256];
+        splits += last[0];
+        rows += last[1];
         __syncthreads();
     }
     if (tid == 0) {
-        a.head[0] = items;
-        a.head[1] = splits;
+        kd.head[0] = items;
+        kd.head[1] = splits;
     }
 }
 
-// The first kernel of a call.  Workgroup 0 deals the work out; each other one takes R rows of
-// the step: the rotation of their angles (kept for the queries), the keys rotated and stored,
+// The first kernel of a call.  Workgroups 0 and 1 deal the work out; each other one takes R
+// rows of the step: the rotation of their angles (kept for the queries), the keys rotated and stored,
 // the values stored.
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable t, Call a, int R) {
     constexpr int HALF = D / 2;
     __shared__ double2 turn[HALF];
-    __shared__ int2 tmp[4];
-    extern __shared__ int tp[];
+    extern __shared__ int plan_lds[];
     if (!step_fits(t, a.n)) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) a.head[0] = a.head[1] = 0;
+        if (blockIdx.x < 2 && threadIdx.x < 2) a.kind[blockIdx.x].head[threadIdx.x] = 0;
         fail_call(t, a, D, blockIdx.x, gridDim.x);
         return;
     }
-    if (blockIdx.x == 0) {
-        plan(t, a, tp, tmp);
-        return;
-    }
+    if (blockIdx.x == 0) return plan<kUnit>(t, a, kNarrow, plan_lds);
+    if (blockIdx.x == 1) return plan<kWideUnit<T, D>>(t, a, kWide, plan_lds);
     const int total = t.counts[kPagesTokens];
     const int KVH = a.KVH;
     const int64_t ps = c.page_size;
     for (int r = 0; r < R; ++r) {
-        const int row = ((int)blockIdx.x - 1) * R + r;
+        const int row = ((int)blockIdx.x - 2) * R + r;
         if (row >= total) return;
         const int slot = t.slots[row];
         __syncthreads();
@@ -495,9 +522,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
     const int col = lane & 15, qd = lane >> 4;
     const int64_t ps = c.page_size;
     const int KVH = a.KVH, G = a.G;
-    const int total = a.head[0] * KVH;
+    const int total = a.kind[kNarrow].head[0] * KVH;
     for (int idx = blockIdx.x; idx < total; idx += gridDim.x) {
-        const Item it = a.items[idx / KVH];
+        const Item it = a.kind[kNarrow].items[idx / KVH];
         const int g = idx % KVH;
         const int first = t.cu[it.entry], m = t.cu[it.entry + 1] - first;
         const int len = t.step_lens[it.entry], ctx = len - m;
@@ -624,10 +651,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
                 const bool whole = j0 + kUnit - 1 <= pmin &&
                                    (a.window == 0 || j0 > pmax - a.window || j0 + kUnit <= a.sinks);
                 if (!whole) {
+                    const int at = ppos - j0 - 8 * qd, far = a.window > 0 ? at - a.window : INT_MIN;
+                    const int sk = a.sinks - j0 - 8 * qd;
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
-                        const int j = j0 + 8 * qd + r;
-                        if (j > ppos || (a.window > 0 && j <= ppos - a.window && j >= a.sinks)) s[r] = -INFINITY;
+                        const bool hidden = (r > at) | ((r <= far) & (r >= sk));
+                        s[r] = hidden ? -INFINITY : s[r];
                     }
                 }
                 float top = s[0];
@@ -757,67 +786,502 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
     }
 }
 
+// ---- many query rows: tiles of keys shared through LDS -----------------------------------------
+//
+// A workgroup takes an item of a tile of 128 query rows of a kv head, 32 to each of its four
+// waves (32x32x16 MFMAs), and visits U keys at a time through LDS: K [U][2 D bytes] and V^T [D][2 U
+// bytes] (of f32 three planes of parts each), 16-byte chunks XOR-swizzled so that the lanes a
+// read serves together touch all banks.  As above both products are transposed, a lane's 16
+// accumulators of a 32-key group are one row's scores of keys 16 k + 8 (l / 32) + 0 .. 7 (the row
+// of K that operand row i reads is i with bits 2 and 3 exchanged), and those are the keys its
+// operand of the second product contracts; q's parts stay in registers.
+// K and V pass through registers on their way to LDS, V's of this visit stored after the first
+// product, K's of the next one after the second, so one buffer each is enough and every request
+// has a product to arrive in; two workgroups a CU fill each other's waits.
+// Bound by the matrix cores: Parts::N times the products of a 16-bit attention.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <class T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 x, u32x4 y, f32x16 z) {
+    if constexpr (std::is_same_v<T, f16_t>)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x),
+                                                      __builtin_bit_cast(f16x8, y), z, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
+                                                       __builtin_bit_cast(bf16x8, y), z, 0, 0, 0);
+}
+
+template <class T, int D>
+struct WideLds {
+    static constexpr int U = kWideUnit<T, D>, KPARTS = Parts<T>::K;
+    static constexpr int KROW = 2 * D, VROW = 2 * U;
+    static constexpr int PLANE = U * KROW;                  // of K, and of V^T
+    static constexpr int K = 0, V = K + KPARTS * PLANE;
+    static constexpr int QL = V + KPARTS * PLANE;           // q's last part, where registers lack
+    static constexpr bool kQl = sizeof(T) == 2 && D == 128;
+    static constexpr int QREGS = Parts<T>::Q - (kQl ? 1 : 0);
+    static constexpr int IDS = QL + (kQl ? 4 * D / 16 * 1024 : 0);  // a page id per 16 keys of SEG visits
+    static constexpr int PER = U / 16, SEG = 512 / PER;
+    static constexpr int STAT = IDS + 2048;                 // rows to redo, a bad page
+    static constexpr int BYTES = STAT + 64;
+    static constexpr int TASKS = U * D / 8 / 256;           // 8-element chunks a thread
+    static_assert(4 * (D + 64) * 4 <= V, "");               // (redone rows' queries)
+    __device__ static uint32_t kslot(uint32_t r, uint32_t c) {
+        return D >= 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
+    }
+    __device__ static uint32_t vslot(uint32_t d, uint32_t c) {
+        return U == 64 ? c ^ ((d >> 1) & 7) : c ^ ((d >> 2) & 3);
+    }
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(PagedKv c, PageTable t, Call a) {
+    using L = WideLds<T, D>;
+    using P = Parts<T>;
+    constexpr int U = L::U, NB = D / 16, OT = D / 32, NG = U / 32;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    int* ids = reinterpret_cast<int*>(lds + L::IDS);
+    int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0 .. 3] rows to redo, [4] a bad page
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, hf = lane >> 5;
+    const int ps = c.page_size, shift = c.page_shift;
+    const int KVH = a.KVH, G = a.G;
+    constexpr int LOG_D = D == 64 ? 6 : D == 128 ? 7 : 8;
+    const int kread = ((col & 16) | (col & 4) << 1 | (col & 8) >> 1 | (col & 3));  // operand row's key
+    // where the lane's operand rows begin, chunk hf
+    const uint32_t kat = kread * L::KROW + L::kslot(kread, hf) * 16;
+    const uint32_t vat = col * L::VROW + L::vslot(col, hf) * 16;
+    const int total = a.kind[kWide].head[0] * KVH;
+    for (int idx = blockIdx.x; idx < total; idx += gridDim.x) {
+        const Item it = a.kind[kWide].items[idx / KVH];
+        const int g = idx % KVH;
+        const int first = t.cu[it.entry], m = t.cu[it.entry + 1] - first;
+        const int len = t.step_lens[it.entry], ctx = len - m;
+        const int* pages = t.table + (int64_t)t.step_ids[it.entry] * t.max_pages;
+        const Visits<U> vis(ctx + it.row0 / G, ctx + (it.row0 + it.rows - 1) / G, a.window, a.sinks);
+        // the wave's rows and their positions
+        const int w0 = 32 * wv;
+        const bool any = w0 < it.rows;
+        const int wmin = ctx + (it.row0 + w0) / G;
+        const int wmax = ctx + (it.row0 + min(w0 + 31, it.rows - 1)) / G;
+        const int myrow = it.row0 + min(w0 + col, it.rows - 1);  // (rows past the tile repeat its last)
+        const int ppos = ctx + myrow / G;
+        u32x4 q[L::QREGS][NB];
+        u32x4* ql = reinterpret_cast<u32x4*>(lds + L::QL) + wv * NB * 64 + lane;
+        __syncthreads();  // (the item before is done with the LDS)
+        float inv = 1.0f;
+        if (any) {
+            float up = 1.0f;
+            if (std::is_same_v<T, f16_t>) {
+                float amax = 0.0f;
+#pragma unroll 2
+                for (int b = 0; b < NB; ++b) {
+                    const f32x8 v = rotated8<D>(a, first, g, myrow, 16 * b + 8 * hf);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
+                }
+                amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+                const float2 sc = row_scale(amax);
+                up = sc.x;
+                inv = sc.y;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                f32x8 v = rotated8<D>(a, first, g, myrow, 16 * b + 8 * hf);
+                if (std::is_same_v<T, f16_t>) v *= up;
+                u32x4 p[P::Q];
+                split_q<T>(v, p);
+#pragma unroll
+                for (int i = 0; i < L::QREGS; ++i) q[i][b] = p[i];
+                if (L::kQl) ql[b * 64] = p[P::Q - 1];
+                if (b % 2) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        float ref = -INFINITY, l = 0.0f;
+        f32x16 o[OT];
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+
+        if (tid < 5) flags[tid] = 0;
+        for (int seg = 0; seg < it.nv; seg += L::SEG) {
+            const int nseg = min(L::SEG, it.nv - seg);
+            __syncthreads();
+            for (int i = tid; i < nseg * L::PER; i += 256) {
+                const int j0 = vis.key(it.v0 + seg + i / L::PER);
+                int j = j0 + i % L::PER * 16;
+                if (j >= len) j = j0;  // (past the sequence: the visit's first keys again)
+                int pg = pages[j >> shift];
+                if ((unsigned)pg >= (unsigned)c.n_pages) {
+                    pg = 0;
+                    flags[4] = 1;
+                }
+                ids[i] = pg;
+            }
+            __syncthreads();
+            Raw<T> st[L::TASKS];
+            // A thread's chunk i of K is 8 dimensions of row kr0 + i KSTEP, whose page is one for the
+            // whole wave; of V, 8 keys of dimension vd0 + i VSTEP.  (Its number is made opaque, so
+            // that addresses are formed again each visit and not kept in registers.)
+            constexpr int KSTEP = 2048 / D, VSTEP = 2048 / U;
+            auto request_k = [&](int v) {
+                const int j0 = vis.key(it.v0 + seg + v);
+                int ti = tid;
+                asm volatile("" : "+v"(ti));
+                const int kr0 = ti / (D / 8);
+                const uint32_t lane_at = (uint32_t)(kr0 % 16 * D + ti % (D / 8) * 8);
+#pragma unroll
+                for (int i = 0; i < L::TASKS; ++i) {
+                    const int grp = __builtin_amdgcn_readfirstlane((kr0 + i * KSTEP) / 16);
+                    const uint32_t pg = __builtin_amdgcn_readfirstlane(ids[v * L::PER + grp]);
+                    const int j = j0 + (j0 + 16 * grp < len ? 16 * grp : 0);
+                    const int64_t at = ((int64_t)(pg * (uint32_t)KVH + (uint32_t)g) << shift) + (j & (ps - 1));
+                    // (rows 8 and on of a group are chunk i odd's where a chunk step is 8 rows)
+                    st[i] = load8<T>(static_cast<const T*>(c.k) + (at << LOG_D) +
+                                     (lane_at + (KSTEP == 8 ? i % 2 * 8 * D : 0)));
+                }
+            };
+            auto request_v = [&](int v) {
+                const int j0 = vis.key(it.v0 + seg + v);
+                int ti = tid;
+                asm volatile("" : "+v"(ti));
+                const int ch = ti % (U / 8), vd0 = ti / (U / 8), grp = ch / 2;
+                const uint32_t pg = ids[v * L::PER + grp];
+                const int j = j0 + (j0 + 16 * grp < len ? 16 * grp : 0);
+                const int64_t at = (((int64_t)(pg * (uint32_t)KVH + (uint32_t)g) << LOG_D) + vd0) << shift;
+                const T* from = static_cast<const T*>(c.v) + at + (j & (ps - 1)) + 8 * (ch % 2);
+#pragma unroll
+                for (int i = 0; i < L::TASKS; ++i) st[i] = load8<T>(from + ((int64_t)(i * VSTEP) << shift));
+            };
+            auto store_k = [&] {
+                int ti = tid;
+                asm volatile("" : "+v"(ti));
+                const uint32_t kr0 = ti / (D / 8), at = kr0 * L::KROW + L::kslot(kr0, ti % (D / 8)) * 16;
+#pragma unroll
+                for (int i = 0; i < L::TASKS; ++i) {
+                    u32x4 p[P::K];
+                    split_k<T>(st[i], p);
+                    // (a chunk step of 8 rows turns bit 3 of the slot)
+                    const uint32_t to = (KSTEP == 8 && i % 2 ? at ^ 128 : at) + i * KSTEP * L::KROW;
+#pragma unroll
+                    for (int n = 0; n < P::K; ++n) *reinterpret_cast<u32x4*>(lds + L::K + n * L::PLANE + to) = p[n];
+                }
+            };
+            auto store_v = [&](int v) {
+                const int j0 = vis.key(it.v0 + seg + v);
+                int ti = tid;
+                asm volatile("" : "+v"(ti));
+                const uint32_t ch = ti % (U / 8), vd0 = ti / (U / 8);
+                const uint32_t at = vd0 * L::VROW + L::vslot(vd0, ch) * 16;
+                if (j0 + U > len) {  // past the sequence's end a page holds anything
+                    constexpr int E = 4 / sizeof(T);
+#pragma unroll
+                    for (int i = 0; i < L::TASKS; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (j0 + 8 * (int)ch + e >= len) {
+                                uint32_t& w = reinterpret_cast<uint32_t*>(&st[i])[e / E];
+                                if constexpr (E == 1) w = 0;
+                                else w &= e % 2 ? 0xFFFFu : 0xFFFF0000u;
+                            }
+                }
+#pragma unroll
+                for (int i = 0; i < L::TASKS; ++i) {
+                    u32x4 p[P::K];
+                    split_k<T>(st[i], p);
+#pragma unroll
+                    for (int n = 0; n < P::K; ++n)
+                        *reinterpret_cast<u32x4*>(lds + L::V + n * L::PLANE + at + i * VSTEP * L::VROW) = p[n];
+                }
+            };
+            request_k(0);
+            store_k();
+            request_v(0);
+            for (int v = 0; v < nseg; ++v) {
+                __syncthreads();  // K of this visit is staged, V of the one before read
+                const int j0 = vis.key(it.v0 + seg + v);
+                // (a group of 32 keys that no row of the wave sees is left out)
+                bool live[NG];
+                f32x16 s[NG];
+                bool some = false;
+                uint32_t ka = kat, va = vat;  // (opaque: no address is kept across visits)
+                asm volatile("" : "+v"(ka), "+v"(va));
+#pragma unroll
+                for (int u = 0; u < NG; ++u) {
+                    const int ju = j0 + 32 * u;
+                    live[u] = any && ju <= wmax && (a.window == 0 || ju + 31 > wmin - a.window || ju < a.sinks);
+                    some |= live[u];
+                    if (!live[u]) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[u][e] = -INFINITY;
+                    } else {
+                        f32x16 lo;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[u][e] = lo[e] = 0.0f;
+                        // a block's parts are read ahead of the MFMAs of the one before (chunk 2 b + hf
+                        // of the row: the swizzle is an XOR, so b's bits can be turned last)
+                        u32x4 kp[2][P::K], qx[2];
+                        auto read = [&](int b) {
+#pragma unroll
+                            for (int n = 0; n < P::K; ++n)
+                                kp[b % 2][n] = *reinterpret_cast<const u32x4*>(
+                                    lds + L::K + n * L::PLANE + 32 * u * L::KROW + (ka ^ 32 * b));
+                            if (L::kQl) qx[b % 2] = ql[b * 64];
+                        };
+                        read(0);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            if (b + 1 < NB) read(b + 1);
+                            __builtin_amdgcn_sched_barrier(0);
+                            // (the small products in a sum of their own)
+#pragma unroll
+                            for (int n = 0; n < P::N - 1; ++n)
+                                lo = mfma32<T>(kp[b % 2][P::ki[n]],
+                                               P::qi[n] < L::QREGS ? q[P::qi[n] < L::QREGS ? P::qi[n] : 0][b] : qx[b % 2], lo);
+                            s[u] = mfma32<T>(kp[b % 2][0], q[0][b], s[u]);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        s[u] += lo;
+                    }
+                }
+                store_v(v);
+                if (v + 1 < nseg) request_k(v + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                u32x4 p[NG][2][P::Q];
+                if (some) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < NG; ++u) {
+                        const int ju = j0 + 32 * u;
+                        if (std::is_same_v<T, f16_t>) s[u] *= inv;
+                        const bool whole = ju + 31 <= wmin &&
+                                           (a.window == 0 || ju > wmax - a.window || ju + 32 <= a.sinks);
+                        if (!whole) {
+                            const int at = ppos - ju - 8 * hf, far = a.window > 0 ? at - a.window : INT_MIN;
+                            const int sk = a.sinks - ju - 8 * hf;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const int j = 16 * (e / 8) + e % 8;
+                                const bool hidden = (j > at) | ((j <= far) & (j >= sk));
+                                s[u][e] = hidden ? -INFINITY : s[u][e];
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
+                    }
+                    if (__any(top > ref + 8.0f)) {
+                        top = fmaxf(top, __shfl_xor(top, 32, 64));
+                        const float to = fmaxf(ref, top);
+                        const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+                        l *= f;
+#pragma unroll
+                        for (int i = 0; i < OT; ++i) o[i] *= f;
+                        ref = to;
+                    }
+                    const float from = ref == -INFINITY ? 0.0f : ref - P::shift;
+#pragma unroll
+                    for (int u = 0; u < NG; ++u)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            f32x8 w;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                w[e] = __builtin_amdgcn_exp2f(s[u][8 * k + e] - from);
+                                l += w[e];
+                            }
+                            split_q<T>(w, p[u][k]);
+                        }
+                }
+                __syncthreads();  // V of this visit is staged, K read
+                if (some) {
+                    // step i: dimensions 32 (i % OT) .., keys of MFMA i / OT; read ahead as above
+                    u32x4 vp[2][P::K];
+                    auto read = [&](int i) {
+#pragma unroll
+                        for (int n = 0; n < P::K; ++n)
+                            vp[i % 2][n] = *reinterpret_cast<const u32x4*>(
+                                lds + L::V + n * L::PLANE + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
+                    };
+                    read(0);
+#pragma unroll
+                    for (int i = 0; i < 2 * NG * OT; ++i) {
+                        if (i + 1 < 2 * NG * OT) read(i + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int n = 0; n < P::N; ++n)
+                            o[i % OT] = mfma32<T>(vp[i % 2][P::ki[n]], p[i / OT / 2][i / OT % 2][P::qi[n]], o[i % OT]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                if (v + 1 < nseg) {
+                    store_k();
+                    request_v(v + 1);
+                }
+            }
+        }
+
+        const bool whole = it.S == 1;
+        const bool mine = any && w0 + col < it.rows;
+        l += __shfl_xor(l, 32, 64);
+        const float inv_l = 1.0f / l;
+        float chk = l * 0.0f;
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                // the quotient: the rounded product, corrected by its remainder
+                const float y = o[i][e] * inv_l;
+                if (whole) o[i][e] = fmaf(fmaf(-y, l, o[i][e]), inv_l, y);
+                chk = fmaf(o[i][e], 0.0f, chk);
+            }
+        bool bad = mine && chk != 0.0f;
+        bad |= (bool)__shfl_xor((int)bad, 32, 64);
+        const bool bad_page = flags[4] != 0;
+        if (bad_page) {
+            bad = false;
+            l = __builtin_nanf("");
+            if (tid == 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
+        }
+        const uint32_t again = (uint32_t)__ballot(bad);  // (both halves of a row agree)
+        const int64_t piece = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows;
+        auto place = [&](int r) {  // row r of the tile
+            const int rr = it.row0 + r;
+            return whole ? a.out + (int64_t)(first + rr / G) * a.ostride + (int64_t)(g * G + rr % G) * D
+                         : a.po + (piece + r) * D;
+        };
+        if (mine && !bad) {
+            float* dst = place(w0 + col);
+#pragma unroll
+            for (int i = 0; i < OT; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const f32x4 x = {o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]};
+                    *reinterpret_cast<f32x4*>(dst + 32 * i + 8 * u + 4 * hf) =
+                        bad_page ? f32x4(__builtin_nanf("")) : x;
+                }
+            if (!whole && hf == 0) a.ms[piece + w0 + col] = make_float2(ref - P::shift, l);
+        }
+        if (lane == 0 && again) flags[wv] = (int)again;
+        __syncthreads();
+        float* qf = reinterpret_cast<float*>(lds) + wv * (D + 64);
+        int turn = 0;
+        for (int w = 0; w < 4; ++w) {
+            uint32_t left = (uint32_t)flags[w];
+            while (left) {
+                const int r = 32 * w + __builtin_ctz(left);
+                left &= left - 1;
+                if (turn++ % 4 != wv) continue;
+                float mx, sw, acc[D / 64];
+                attend_row<T, D, U>(c, a, pages, vis, it, first, ctx, g, it.row0 + r, qf, qf + D, mx, sw, acc);
+                float* y = place(r);
+#pragma unroll
+                for (int e = 0; e < D / 64; ++e) y[lane + 64 * e] = whole ? acc[e] / sw : acc[e];
+                if (!whole && lane == 0) a.ms[piece + r] = make_float2(mx, sw);
+            }
+        }
+    }
+}
+
 // The pieces of a tile dealt out, joined: out = sum_s 2^(M_s - M) o_s / sum_s 2^(M_s - M) l_s over the
 // pieces' (M_s, l_s, o_s); a piece in which a row sees no key has M_s = -inf, weight 0.  A
-// group of D / 4 threads per (tile, kv head, row).
+// workgroup per (16 rows of a tile, kv head), D / 4 threads to a row; where there are fewer rows
+// than such groups, several share a row's pieces and meet in LDS.
 template <int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PageTable t, Call a) {
     constexpr int W = D / 4, N = 256 / W;
-    const int d4 = threadIdx.x % W, sub = threadIdx.x / W;
-    const int64_t per = (int64_t)a.KVH * kTileRows, total = (int64_t)a.head[1] * per;
-    for (int64_t i = (int64_t)blockIdx.x * N + sub; i < total; i += (int64_t)gridDim.x * N) {
-        const Split sp = a.splits[i / per];
-        const int g = (int)(i % per) / kTileRows, r = (int)(i % kTileRows);
-        if (r >= sp.rows || sp.S < 2) continue;
-        const int64_t p0 = (int64_t)sp.base + (int64_t)g * sp.S * sp.rows + r;
-        float M = -INFINITY;
-        for (int s = 0; s < sp.S; ++s) M = fmaxf(M, a.ms[p0 + (int64_t)s * sp.rows].x);
-        float l = 0.0f;
-        f32x4 o = 0.0f;
-        for (int s = 0; s < sp.S; ++s) {
-            const int64_t p = p0 + (int64_t)s * sp.rows;
-            const float2 x = a.ms[p];
-            const float f = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - M);
-            const f32x4 v = *reinterpret_cast<const f32x4*>(a.po + p * D + 4 * d4);
-            l = fmaf(x.y, f, l);
+    __shared__ f32x4 so[N][W];
+    __shared__ float sl[N];
+    const int ln = threadIdx.x % W, sub = threadIdx.x / W;
+    const int nn = a.kind[kNarrow].head[1] * a.KVH;
+    const int nw = a.kind[kWide].head[1] * a.KVH * (kTileRows[kWide] / 16);
+    for (int i = blockIdx.x; i < nn + nw; i += gridDim.x) {
+        const bool wide = i >= nn;
+        const int k = wide ? (i - nn) / (kTileRows[kWide] / 16) : i;
+        const int r0 = wide ? (i - nn) % (kTileRows[kWide] / 16) * 16 : 0;
+        const Split sp = a.kind[wide ? kWide : kNarrow].splits[k / a.KVH];
+        const int g = k % a.KVH, rows = min(16, sp.rows - r0);
+        if (rows <= 0 || sp.S < 2) continue;  // (uniform)
+        int share = 1;
+        while (share * 2 * rows <= N) share *= 2;
+        const int per = N / share;  // rows at a time
+        const int part = sub % share;
+        const int64_t first = t.cu[sp.entry];
+        for (int rb = 0; rb < rows; rb += per) {
+            const int r = rb + sub / share;
+            const bool live = r < rows;
+            const int64_t p0 = (int64_t)sp.base + (int64_t)g * sp.S * sp.rows + r0 + min(r, rows - 1);
+            float M = -INFINITY;
+            for (int s = ln; s < sp.S; s += W) M = fmaxf(M, a.ms[p0 + (int64_t)s * sp.rows].x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], f, o[e]);
+            for (int x = W / 2; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, W));
+            float l = 0.0f;
+            f32x4 o = 0.0f;
+#pragma unroll 8
+            for (int s = part; s < sp.S; s += share) {
+                const int64_t p = p0 + (int64_t)s * sp.rows;
+                const float2 x = a.ms[p];
+                const f32x4 v = *reinterpret_cast<const f32x4*>(a.po + p * D + 4 * ln);
+                const float f = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - M);
+                l = fmaf(x.y, f, l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], f, o[e]);
+            }
+            if (share > 1) {
+                so[sub][ln] = o;
+                if (ln == 0) sl[sub] = l;
+                __syncthreads();
+                if (part == 0)
+                    for (int x = 1; x < share; ++x) {
+                        o += so[sub + x][ln];
+                        l += sl[sub + x];
+                    }
+                __syncthreads();
+            }
+            if (live && part == 0) {
+                const int rr = sp.row0 + r0 + r;
+                *reinterpret_cast<f32x4*>(a.out + (first + rr / a.G) * a.ostride +
+                                          (int64_t)(g * a.G + rr % a.G) * D + 4 * ln) = o / l;
+            }
         }
-        const int rr = sp.row0 + r;
-        const int64_t row = t.cu[sp.entry] + rr / a.G;
-        *reinterpret_cast<f32x4*>(a.out + row * a.ostride + (int64_t)(g * a.G + rr % a.G) * D + 4 * d4) = o / l;
     }
 }
 
 // How a call's workspace is laid out, and its grids.
 struct Layout {
-    int64_t items, most_rows;
-    size_t items_at, splits_at, turn_at, ms_at, po_at, bytes;
+    int64_t items[2], rows[2];
+    size_t head_at[2], items_at[2], splits_at[2], turn_at, ms_at, po_at, bytes;
 };
 
-// Pieces a call is dealt out in: four workgroups of four waves for every CU.
-int target_pieces() { return 4 * device_info().cu_count; }
+// Pieces a kind's work is dealt out in: narrow, four workgroups of four waves for every CU; wide,
+// one for every place that its kernel has (two a CU), which leaves a causal prompt's tiles, at
+// most twice the mean, whole.
+int target_pieces(int kind) { return (kind == kNarrow ? 4 : 1) * device_info().cu_count; }
 
 Layout layout(const PagedKv& c, const unillm_page_table& t, int64_t n, int64_t H) {
     const int64_t KVH = c.n_kv_heads, G = H / KVH, D = c.head_dim;
     Layout l;
-    // tiles: an entry's last may be ragged.  A tile of nv visits makes at most nv / C + 1 pieces,
-    // and the nv / C add up to target / KVH.
-    const int64_t tiles = n * G / kTileRows + std::min<int64_t>(n, t.st.max_seqs);
-    l.items = tiles + target_pieces() / KVH + 1;
-    // a tile in more than one piece has at most 2 nv / C of them
-    l.most_rows = 2 * (int64_t)target_pieces() * std::min<int64_t>(kTileRows, n * G);
-    size_t at = 256;
+    size_t at = 0;
     auto take = [&](int64_t bytes) {
         const size_t here = at;
         at += ((size_t)bytes + 255) & ~(size_t)255;
         return here;
     };
-    l.items_at = take(l.items * (int64_t)sizeof(Item));
-    l.splits_at = take(tiles * (int64_t)sizeof(Split));
+    for (int k = 0; k < 2; ++k) {
+        // tiles: an entry's last may be ragged.  A tile of nv visits makes at most nv / C + 1
+        // pieces, and the nv / C add up to target / KVH; more than one piece, at most 2 nv / C.
+        const int64_t tiles = n * G / kTileRows[k] + std::min<int64_t>(n, t.st.max_seqs);
+        const bool some = k == kNarrow || n * G > kNarrowRows;
+        l.items[k] = some ? tiles + target_pieces(k) / KVH + 1 : 0;
+        l.rows[k] = some ? 2 * (int64_t)target_pieces(k) * std::min<int64_t>(kTileRows[k], n * G) : 0;
+        l.head_at[k] = take(2 * sizeof(int));
+        l.items_at[k] = take(l.items[k] * (int64_t)sizeof(Item));
+        l.splits_at[k] = take(tiles * (int64_t)sizeof(Split));
+    }
     l.turn_at = take(n * D / 2 * (int64_t)sizeof(float2));
-    l.ms_at = take(l.most_rows * (int64_t)sizeof(float2));
-    l.po_at = take(l.most_rows * D * (int64_t)sizeof(float));
+    l.ms_at = take((l.rows[0] + l.rows[1]) * (int64_t)sizeof(float2));
+    l.po_at = take((l.rows[0] + l.rows[1]) * D * (int64_t)sizeof(float));
     l.bytes = at;
     return l;
 }
@@ -826,22 +1290,30 @@ template <class T, int D>
 hipError_t launch_typed(const PagedKv& c, const unillm_page_table& t, const Call& a, const Layout& l,
                         hipStream_t s) {
     using L = NarrowLds<T, D>;
+    using LW = WideLds<T, D>;
     static const bool attr =
         hipFuncSetAttribute((const void*)paged_narrow_kernel<T, D>,
-                            hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES) == hipSuccess;
+                            hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES) == hipSuccess &&
+        hipFuncSetAttribute((const void*)paged_wide_kernel<T, D>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, LW::BYTES) == hipSuccess &&
+        hipFuncSetAttribute((const void*)paged_append_kernel<T, D>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024) == hipSuccess;
     if (!attr) return hipErrorInvalidValue;
     const int R = (int)std::max<int64_t>(1, std::min<int64_t>(16, a.n / 1024));
-    // (the plan keeps a prefix sum of the entries in LDS)
-    const size_t plan_lds = (size_t)(t.st.max_seqs + 1) * sizeof(int);
-    paged_append_kernel<T, D><<<(unsigned)(1 + (a.n + R - 1) / R), 256, plan_lds, s>>>(c, t.st, a, R);
+    // (the plan keeps three ints an entry in LDS)
+    const size_t plan_lds = (size_t)(3 * t.st.max_seqs + 1) * sizeof(int);
+    paged_append_kernel<T, D><<<(unsigned)(2 + (a.n + R - 1) / R), 256, plan_lds, s>>>(c, t.st, a, R);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const unsigned grid = (unsigned)std::min<int64_t>(l.items * a.KVH, 1 << 16);
+    if (l.items[kWide] > 0) {
+        const unsigned grid = (unsigned)std::min<int64_t>(l.items[kWide] * a.KVH, 1 << 16);
+        paged_wide_kernel<T, D><<<grid, 256, LW::BYTES, s>>>(c, t.st, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    const unsigned grid = (unsigned)std::min<int64_t>(l.items[kNarrow] * a.KVH, 1 << 16);
     paged_narrow_kernel<T, D><<<grid, 256, L::BYTES, s>>>(c, t.st, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    const int64_t merged = (l.most_rows / 2 * (D / 4) + 255) / 256;
-    paged_merge_kernel<D><<<(unsigned)std::min<int64_t>(merged, 4 * device_info().cu_count), 256, 0, s>>>(
-        t.st, a);
+    paged_merge_kernel<D><<<(unsigned)(4 * device_info().cu_count), 256, 0, s>>>(t.st, a);
     return hipGetLastError();
 }
 
@@ -865,11 +1337,15 @@ hipError_t launch_paged_attention(const PagedKv& c, const unillm_page_table& t, 
     uint8_t* w = static_cast<uint8_t*>(ws);
     // a window or sinks past any position are all of them
     const int64_t far = (int64_t)1 << 30;
-    const Call a{qkv, out, qstride, ostride, (int)n, (int)H, (int)c.n_kv_heads, (int)(H / c.n_kv_heads),
-                 (int)std::min(window, far), (int)std::min(sinks, far), target_pieces(),
-                 (int)l.most_rows, reinterpret_cast<int*>(w), reinterpret_cast<Item*>(w + l.items_at),
-                 reinterpret_cast<Split*>(w + l.splits_at), reinterpret_cast<float2*>(w + l.turn_at),
-                 reinterpret_cast<float2*>(w + l.ms_at), reinterpret_cast<float*>(w + l.po_at)};
+    Call a{qkv, out, qstride, ostride, (int)n, (int)H, (int)c.n_kv_heads, (int)(H / c.n_kv_heads),
+           (int)std::min(window, far), (int)std::min(sinks, far),
+           reinterpret_cast<float2*>(w + l.turn_at), reinterpret_cast<float2*>(w + l.ms_at),
+           reinterpret_cast<float*>(w + l.po_at), {}};
+    for (int k = 0; k < 2; ++k)
+        a.kind[k] = {target_pieces(k), k == kNarrow ? 4 : 2, k == kNarrow ? 0 : (int)l.rows[0],
+                     (int)l.rows[k], reinterpret_cast<int*>(w + l.head_at[k]),
+                     reinterpret_cast<Item*>(w + l.items_at[k]),
+                     reinterpret_cast<Split*>(w + l.splits_at[k])};
     if (c.type == UNILLM_QTYPE_F32) return launch_type<float>(c, t, a, l, s);
     if (c.type == UNILLM_QTYPE_F16) return launch_type<f16_t>(c, t, a, l, s);
     return launch_type<bf16_t>(c, t, a, l, s);
