@@ -54,9 +54,11 @@ __device__ __forceinline__ float wave_add(float v) {
     return v;
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -244,50 +246,109 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     }
 }
 
-// The first kernel of a call.  Workgroups 0 and 1 deal the work out; each other one takes R
-// rows of the step: the rotation of their angles (kept for the queries), the keys rotated and stored,
-// the values stored.
+// The first kernel of a call.  Workgroups 0 and 1 deal the work out; each other one takes 16 rows
+// of the step and `heads` kv heads: the rows' rotations (kept in f32 for the queries), their
+// keys rotated and stored, their values stored.  A V page runs along the keys, so where 8 rows
+// are 8 neighbouring slots of a page, aligned (a prompt's rows, but for its ends), a thread
+// stores a dimension's 8 values at once; other rows value by value.  (2048 rows of 32 heads of
+// 128: 65 us with every value on its own, a row after the other.)
+constexpr int kAppendRows = 16;
+
 template <class T, int D>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable t, Call a, int R) {
-    constexpr int HALF = D / 2;
-    __shared__ double2 turn[HALF];
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable t, Call a, int heads) {
+    constexpr int HALF = D / 2, Q4 = HALF / 4, NR = kAppendRows;
+    __shared__ double2 turn[NR][HALF];
+    __shared__ int slots[NR + 14];  // of the rows from 7 before the workgroup's to 7 after
     extern __shared__ int plan_lds[];
+    const int tid = threadIdx.x;
+    const int bx = (int)blockIdx.x - 2, groups = (a.KVH + heads - 1) / heads;
+    const int row0 = bx / groups * NR, g0 = bx % groups * heads;
+    // (rows' slots and positions are requested with the plan's header: both arrays hold max_tokens)
+    int slot = -1, pos = 0;
+    if (bx >= 0 && tid < NR + 14) {
+        const int row = row0 + tid - 7;
+        if (row >= 0 && row < t.max_tokens) slot = t.slots[row];
+    }
+    if (bx >= 0 && tid < NR && row0 + tid < t.max_tokens) pos = t.positions[row0 + tid];
     if (!step_fits(t, a.n)) {
-        if (blockIdx.x < 2 && threadIdx.x < 2) a.kind[blockIdx.x].head[threadIdx.x] = 0;
+        if (blockIdx.x < 2 && tid < 2) a.kind[blockIdx.x].head[tid] = 0;
         fail_call(t, a, D, blockIdx.x, gridDim.x);
         return;
     }
     if (blockIdx.x == 0) return plan<kUnit>(t, a, kNarrow, plan_lds);
     if (blockIdx.x == 1) return plan<kWideUnit<T, D>>(t, a, kWide, plan_lds);
     const int total = t.counts[kPagesTokens];
-    const int KVH = a.KVH;
+    if (row0 >= total) return;
+    const int rows = min(NR, total - row0);
+    __shared__ int at[NR];
+    if (tid < NR + 14) slots[tid] = row0 + tid - 7 < total ? slot : -1;
+    if (tid < NR) at[tid] = pos;
+    __syncthreads();
+    for (int i = tid; i < rows * HALF; i += 256) {
+        const int r = i / HALF, p = i % HALF;
+        double sn, cs;
+        sincospi((double)at[r] * c.freq[p], &sn, &cs);
+        turn[r][p] = make_double2(cs, sn);
+        if (g0 == 0) a.turn[(int64_t)(row0 + r) * HALF + p] = make_float2((float)cs, (float)sn);
+    }
+    __syncthreads();
+    const int KVH = a.KVH, shift = c.page_shift;
     const int64_t ps = c.page_size;
-    for (int r = 0; r < R; ++r) {
-        const int row = ((int)blockIdx.x - 2) * R + r;
-        if (row >= total) return;
-        const int slot = t.slots[row];
-        __syncthreads();
-        if (threadIdx.x < HALF) {
-            double sn, cs;
-            sincospi((double)t.positions[row] * c.freq[threadIdx.x], &sn, &cs);
-            turn[threadIdx.x] = make_double2(cs, sn);
-            a.turn[(int64_t)row * HALF + threadIdx.x] = make_float2((float)cs, (float)sn);
+    const int g1 = min(g0 + heads, KVH);
+    const float* xk = a.qkv + (int64_t)row0 * a.qstride + (int64_t)a.H * D;
+    const float* xv = xk + (int64_t)KVH * D;
+    // keys: 4 dimensions and their partners a thread
+    for (int i = tid; i < (g1 - g0) * rows * Q4; i += 256) {
+        const int g = g0 + i / (rows * Q4), r = i / Q4 % rows, p = i % Q4 * 4;
+        const int sl = slots[r + 7];
+        const float* x = xk + r * a.qstride + (int64_t)g * D + p;
+        const f32x4 u = *reinterpret_cast<const f32x4*>(x), w = *reinterpret_cast<const f32x4*>(x + HALF);
+        struct alignas(4 * sizeof(T)) Four {
+            T v[4];
+        } lo, hi;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double2 z = turn[r][p + e];
+            const double uu = u[e], ww = w[e];
+            lo.v[e] = narrow<T>((float)(uu * z.x - ww * z.y));
+            hi.v[e] = narrow<T>((float)(uu * z.y + ww * z.x));
         }
-        __syncthreads();
-        if (slot < 0) continue;
-        const int64_t page = slot >> c.page_shift, off = slot & (c.page_size - 1);
-        const float* xk = a.qkv + row * a.qstride + (int64_t)a.H * D;
-        const float* xv = xk + (int64_t)KVH * D;
-        for (int i = threadIdx.x; i < KVH * HALF; i += 256) {
-            const int g = i / HALF, p = i % HALF;
-            const double2 cs = turn[p];
-            const double u = xk[g * D + p], v = xk[g * D + p + HALF];
-            T* dst = static_cast<T*>(c.k) + ((page * KVH + g) * ps + off) * D;
-            dst[p] = narrow<T>((float)(u * cs.x - v * cs.y));
-            dst[p + HALF] = narrow<T>((float)(u * cs.y + v * cs.x));
+        if (sl < 0) continue;
+        T* dst = static_cast<T*>(c.k) +
+                 (((((int64_t)(sl >> shift) * KVH + g) << shift) + (sl & (ps - 1))) * D + p);
+        *reinterpret_cast<Four*>(dst) = lo;
+        *reinterpret_cast<Four*>(dst + HALF) = hi;
+    }
+    // values: a wave a task of 64 dimensions; row r is in a run of 8 if the row r - slot % 8 and
+    // the one 7 after it are 7 slots apart
+    const int lane = tid & 63;
+    constexpr int DG = D / 64;
+    auto runs = [&](int r) {  // r from -7 on
+        const int sl = slots[r + 7], s0 = r - (sl & 7);
+        return sl >= 0 && s0 >= -7 && s0 + 7 < NR + 7 && slots[s0 + 7] == (sl & ~7) &&
+               slots[s0 + 14] == (sl | 7);
+    };
+    for (int i = __builtin_amdgcn_readfirstlane(tid >> 6); i < (g1 - g0) * rows * DG; i += 4) {
+        const int g = g0 + i / (rows * DG), r = i / DG % rows, d = i % DG * 64 + lane;
+        const int sl = slots[r + 7];
+        if (sl < 0) continue;
+        const bool run = runs(r);
+        if (run && (sl & 7) != 0) continue;  // (stored with the run's first row)
+        T* dst = static_cast<T*>(c.v) + (((((int64_t)(sl >> shift) * KVH + g) * D + d) << shift) + (sl & (ps - 1)));
+        const float* x = xv + r * a.qstride + (int64_t)g * D + d;
+        if (run) {
+            struct alignas(16) Eight {
+                T v[8];
+            } y;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = x[e * a.qstride];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y.v[e] = narrow<T>(f[e]);
+            *reinterpret_cast<Eight*>(dst) = y;
+        } else {
+            *dst = narrow<T>(*x);
         }
-        for (int i = threadIdx.x; i < KVH * D; i += 256)
-            static_cast<T*>(c.v)[(page * KVH * D + i) * ps + off] = narrow<T>(xv[i]);
     }
 }
 
@@ -337,6 +398,25 @@ __device__ __forceinline__ void split_q(const f32x8& v, u32x4 (&p)[Parts<T>::Q])
             p[1][j] = y;
             p[2][j] = z;
         }
+    }
+}
+
+// 8 weights -> their parts.  f16: the first part cut off (a mask, exact in f16 but below 2^-14),
+// what is left of up to 2^-10 rounded: 2^-22 of the weight, in either direction, for three
+// instructions a weight where two roundings take four.
+template <class T>
+__device__ __forceinline__ void split_w(const f32x8& v, u32x4 (&p)[Parts<T>::Q]) {
+    if constexpr (std::is_same_v<T, f16_t>) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = __uint_as_float(__float_as_uint(v[2 * j]) & 0xFFFFE000u);
+            const float b = __uint_as_float(__float_as_uint(v[2 * j + 1]) & 0xFFFFE000u);
+            p[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+            p[1][j] = __builtin_bit_cast(
+                uint32_t, __builtin_convertvector(f32x2{v[2 * j] - a, v[2 * j + 1] - b}, f16x2));
+        }
+    } else {
+        split_q<T>(v, p);
     }
 }
 
@@ -1002,48 +1082,44 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(Paged
             for (int v = 0; v < nseg; ++v) {
                 __syncthreads();  // K of this visit is staged, V of the one before read
                 const int j0 = vis.key(it.v0 + seg + v);
-                // (a group of 32 keys that no row of the wave sees is left out)
-                bool live[NG];
+                // (the groups of 32 keys, from u0 on, that some row of the wave sees)
                 f32x16 s[NG];
-                bool some = false;
-                uint32_t ka = kat, va = vat;  // (opaque: no address is kept across visits)
-                asm volatile("" : "+v"(ka), "+v"(va));
+                bool live[NG], some = false;
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
                     const int ju = j0 + 32 * u;
                     live[u] = any && ju <= wmax && (a.window == 0 || ju + 31 > wmin - a.window || ju < a.sinks);
                     some |= live[u];
-                    if (!live[u]) {
+                }
+                uint32_t ka = kat, va = vat;  // (opaque: no address is kept across visits)
+                asm volatile("" : "+v"(ka), "+v"(va));
+                if (some) {
+                    // a block's parts are read ahead of the MFMAs of the one before (chunk 2 b + hf
+                    // of the row: the swizzle is an XOR, so b's bits can be turned last)
+                    u32x4 kp[2][NG][P::K], qx[2];
+                    auto read = [&](int b) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) s[u][e] = -INFINITY;
-                    } else {
-                        f32x16 lo;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) s[u][e] = lo[e] = 0.0f;
-                        // a block's parts are read ahead of the MFMAs of the one before (chunk 2 b + hf
-                        // of the row: the swizzle is an XOR, so b's bits can be turned last)
-                        u32x4 kp[2][P::K], qx[2];
-                        auto read = [&](int b) {
+                        for (int u = 0; u < NG; ++u)
 #pragma unroll
                             for (int n = 0; n < P::K; ++n)
-                                kp[b % 2][n] = *reinterpret_cast<const u32x4*>(
+                                kp[b % 2][u][n] = *reinterpret_cast<const u32x4*>(
                                     lds + L::K + n * L::PLANE + 32 * u * L::KROW + (ka ^ 32 * b));
-                            if (L::kQl) qx[b % 2] = ql[b * 64];
-                        };
-                        read(0);
+                        if (L::kQl) qx[b % 2] = ql[b * 64];
+                    };
+                    read(0);
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            if (b + 1 < NB) read(b + 1);
-                            __builtin_amdgcn_sched_barrier(0);
-                            // (the small products in a sum of their own)
+                    for (int b = 0; b < NB; ++b) {
+                        if (b + 1 < NB) read(b + 1);
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                            for (int n = 0; n < P::N - 1; ++n)
-                                lo = mfma32<T>(kp[b % 2][P::ki[n]],
-                                               P::qi[n] < L::QREGS ? q[P::qi[n] < L::QREGS ? P::qi[n] : 0][b] : qx[b % 2], lo);
-                            s[u] = mfma32<T>(kp[b % 2][0], q[0][b], s[u]);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                        s[u] += lo;
+                        for (int n = 0; n < P::N; ++n)
+#pragma unroll
+                            for (int u = 0; u < NG; ++u) {
+                                const f32x16 zero = {};
+                                const u32x4 x = P::qi[n] < L::QREGS ? q[P::qi[n] < L::QREGS ? P::qi[n] : 0][b] : qx[b % 2];
+                                s[u] = mfma32<T>(kp[b % 2][u][P::ki[n]], x, b + n == 0 ? zero : s[u]);
+                            }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
                 store_v(v);
@@ -1055,7 +1131,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(Paged
 #pragma unroll
                     for (int u = 0; u < NG; ++u) {
                         const int ju = j0 + 32 * u;
-                        if (std::is_same_v<T, f16_t>) s[u] *= inv;
                         const bool whole = ju + 31 <= wmin &&
                                            (a.window == 0 || ju > wmax - a.window || ju + 32 <= a.sinks);
                         if (!whole) {
@@ -1071,6 +1146,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(Paged
 #pragma unroll
                         for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
                     }
+                    if (std::is_same_v<T, f16_t>) top *= inv;  // (a power of two)
                     if (__any(top > ref + 8.0f)) {
                         top = fmaxf(top, __shfl_xor(top, 32, 64));
                         const float to = fmaxf(ref, top);
@@ -1088,10 +1164,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(Paged
                             f32x8 w;
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
-                                w[e] = __builtin_amdgcn_exp2f(s[u][8 * k + e] - from);
+                                w[e] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * k + e], inv, -from));
                                 l += w[e];
                             }
-                            split_q<T>(w, p[u][k]);
+                            split_w<T>(w, p[u][k]);
                         }
                 }
                 __syncthreads();  // V of this visit is staged, K read
@@ -1297,23 +1373,27 @@ hipError_t launch_typed(const PagedKv& c, const unillm_page_table& t, const Call
         hipFuncSetAttribute((const void*)paged_wide_kernel<T, D>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, LW::BYTES) == hipSuccess &&
         hipFuncSetAttribute((const void*)paged_append_kernel<T, D>,
-                            hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024) == hipSuccess;
+                            hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)((3 * kPagesMaxSeqs + 1) * sizeof(int))) == hipSuccess;
     if (!attr) return hipErrorInvalidValue;
-    const int R = (int)std::max<int64_t>(1, std::min<int64_t>(16, a.n / 1024));
     // (the plan keeps three ints an entry in LDS)
     const size_t plan_lds = (size_t)(3 * t.st.max_seqs + 1) * sizeof(int);
-    paged_append_kernel<T, D><<<(unsigned)(2 + (a.n + R - 1) / R), 256, plan_lds, s>>>(c, t.st, a, R);
+    // kv heads a workgroup: one, or what makes four workgroups a CU
+    const int64_t blocks = (a.n + kAppendRows - 1) / kAppendRows, most = 4 * device_info().cu_count;
+    const int heads = (int)std::min<int64_t>(a.KVH, std::max<int64_t>(1, blocks * a.KVH / most));
+    const int64_t append = blocks * ((a.KVH + heads - 1) / heads);
+    paged_append_kernel<T, D><<<(unsigned)(2 + append), 256, plan_lds, s>>>(c, t.st, a, heads);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (l.items[kWide] > 0) {
-        const unsigned grid = (unsigned)std::min<int64_t>(l.items[kWide] * a.KVH, 1 << 16);
+        const unsigned grid = (unsigned)std::min<int64_t>(l.items[kWide] * a.KVH, most);
         paged_wide_kernel<T, D><<<grid, 256, LW::BYTES, s>>>(c, t.st, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    const unsigned grid = (unsigned)std::min<int64_t>(l.items[kNarrow] * a.KVH, 1 << 16);
+    const unsigned grid = (unsigned)std::min<int64_t>(l.items[kNarrow] * a.KVH, most);
     paged_narrow_kernel<T, D><<<grid, 256, L::BYTES, s>>>(c, t.st, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    paged_merge_kernel<D><<<(unsigned)(4 * device_info().cu_count), 256, 0, s>>>(t.st, a);
+    paged_merge_kernel<D><<<(unsigned)std::min<int64_t>((l.rows[0] + l.rows[1]) / 2, most), 256, 0, s>>>(t.st, a);
     return hipGetLastError();
 }
 
