@@ -916,8 +916,8 @@ int check_paged(const unillm_paged_kv* c, const unillm_page_table* t, int64_t n,
         return fail(UNILLM_ERR_INVALID_ARG, what + ": n_tokens " + std::to_string(n) +
                                                 " outside [0, " + std::to_string(t->st.max_tokens) +
                                                 "]");
-    if (n * (n_heads / c->n_kv_heads) > (int64_t)INT32_MAX / 2)
-        return fail(UNILLM_ERR_INVALID_ARG, what + ": too many query rows a kv head");
+    if (n * n_heads > (int64_t)INT32_MAX / 2)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": n_tokens * n_heads must be below 2^30");
     return UNILLM_OK;
 }
 

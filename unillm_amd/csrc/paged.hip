@@ -85,7 +85,10 @@ struct Call {
     float2* turn;  // [n][hd / 2] cos, sin of each row's angles
     float2* ms;    // partial rows: maximum (log2), sum of the weights
     float* po;     // [hd] unnormalized sums
+    int* redo_count;  // rows and heads (row H + head) whose products of parts came out non-finite
+    int* redo;
     struct Kind {
+        int tile_rows;  // most query rows of a tile
         int target;     // pieces to deal the kind's work out in, over all kv heads
         int least;      // visits of the smallest piece
         int row0, most_rows;  // its partial rows
@@ -97,11 +100,14 @@ struct Call {
 
 constexpr int kNarrow = 0, kWide = 1;
 constexpr int kNarrowRows = 64;  // most query rows of an entry (a kv head) for narrow tiles
-constexpr int kTileRows[2] = {16, 128};  // query rows of a tile
+constexpr int kTileRows = 16;    // query rows of a narrow tile
 constexpr int kUnit = 32;        // keys of a narrow tile's visit
-// keys of a wide tile's visit: what leaves room for two workgroups a CU (one of f32 at hd 256)
+// Wide tiles: groups of four waves of 32 rows each (what the registers hold: two groups, one at
+// hd 256), and keys of a visit.
 template <class T, int D>
-constexpr int kWideUnit = sizeof(T) == 2 && D < 256 ? 64 : 32;
+constexpr int kGroups = D < 256 ? 2 : 1;
+template <class T, int D>
+constexpr int kWideUnit = D == 64 || (sizeof(T) == 2 && D == 128) ? 64 : 32;
 
 // Whether the step can run: a plan, of at most the call's rows.
 __device__ __forceinline__ bool step_fits(const PageTable& t, int n) {
@@ -148,7 +154,7 @@ __device__ __forceinline__ int2 block_scan2(int2 v, int2* tmp) {
     return make_int2(v.x + base.x, v.y + base.y);
 }
 
-// Deals one kind's work out (one workgroup): every entry's rows in tiles, every tile's visits of
+// Deals one kind's work out (one workgroup): every entry's rows in equal tiles, every tile's visits of
 // U keys in equal pieces of at most C, where C makes the kind's target of pieces over all kv
 // heads.  An entry's last tile, whose rows see the most keys, is dealt out first.
 // sm: LDS, tp[B + 1] (tiles before each entry) | m[B] | ctx[B].
@@ -158,7 +164,7 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     __shared__ float part[4];
     __shared__ int off[257], info[256][6], last[2];
     const Call::Kind& kd = a.kind[kind];
-    const int tid = threadIdx.x, B = t.counts[kPagesEntries], TR = kTileRows[kind];
+    const int tid = threadIdx.x, B = t.counts[kPagesEntries], TR = kd.tile_rows;
     int *tp = sm, *ms = tp + B + 1, *ctxs = ms + B;
     int tiles = 0;
     if (tid == 0) tp[0] = 0;
@@ -186,8 +192,11 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
             if (tp[mid] <= i) lo = mid;
             else hi = mid;
         }
-        Tile x{lo, (tp[lo + 1] - 1 - i) * TR, 0, 0};
-        x.rows = min(TR, ms[lo] * a.G - x.row0);
+        // (wide: in whole waves of 32 rows; no tile comes out empty, as rows > (tiles - 1) TR)
+        const int rows = ms[lo] * a.G, n = tp[lo + 1] - tp[lo];
+        const int each = kind == kNarrow ? TR : ((rows + n - 1) / n + 31) / 32 * 32;
+        Tile x{lo, (tp[lo + 1] - 1 - i) * each, 0, 0};
+        x.rows = min(each, rows - x.row0);
         x.nv = Visits<U>(ctxs[lo] + x.row0 / a.G, ctxs[lo] + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks).count;
         return x;
     };
@@ -272,9 +281,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable 
     if (bx >= 0 && tid < NR && row0 + tid < t.max_tokens) pos = t.positions[row0 + tid];
     if (!step_fits(t, a.n)) {
         if (blockIdx.x < 2 && tid < 2) a.kind[blockIdx.x].head[tid] = 0;
+        if (blockIdx.x == 0 && tid == 0) *a.redo_count = 0;
         fail_call(t, a, D, blockIdx.x, gridDim.x);
         return;
     }
+    if (blockIdx.x == 0 && tid == 0) *a.redo_count = 0;
     if (blockIdx.x == 0) return plan<kUnit>(t, a, kNarrow, plan_lds);
     if (blockIdx.x == 1) return plan<kWideUnit<T, D>>(t, a, kWide, plan_lds);
     const int total = t.counts[kPagesTokens];
@@ -466,6 +477,10 @@ __device__ __forceinline__ float2 row_scale(float amax) {
     return make_float2(ldexpf(1.0f, e), ldexpf(1.0f, -e));
 }
 
+__device__ __forceinline__ void redo_row(const Call& a, int64_t row, int h) {
+    a.redo[atomicAdd(a.redo_count, 1)] = (int)row * a.H + h;
+}
+
 // Query row r of an entry (its first step row `first`): 1 / sqrt(D) and log2 e times the
 // rotated dimensions d .. d + 7 (d a multiple of 8).
 template <int D>
@@ -484,77 +499,6 @@ __device__ __forceinline__ f32x8 rotated8(const Call& a, int first, int g, int r
         v[j] = (d < HALF ? u * z.x - w * z.y : u * z.y + w * z.x) * scale;
     }
     return v;
-}
-
-// One query row over an item's visits by a wave, in plain f32: for rows whose products of parts
-// came out non-finite (an infinity times a part that is 0, or what a masked place holds).
-// qf: LDS [D] for the query; sc: LDS [64].  Lane el gets dimensions el + 64 i of the
-// unnormalized sum, with the maximum (log2) and the sum of the weights.
-template <class T, int D, int U>
-__device__ void attend_row(const PagedKv& c, const Call& a, const int* pages, const Visits<U>& vis,
-                           const Item& it, int first, int ctx, int g, int r, float* qf, float* sc,
-                           float& mx, float& l, float (&acc)[D / 64]) {
-    const int el = threadIdx.x & 63;
-    const int64_t ps = c.page_size;
-    const int p = ctx + r / a.G;
-    auto settle = [] {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    };
-    auto page_of = [&](int j) {  // (ids out of range make the tile NaN elsewhere; never read)
-        const int pg = pages[j >> c.page_shift];
-        return (int64_t)((unsigned)pg < (unsigned)c.n_pages ? pg : 0);
-    };
-    settle();
-    if (el < D / 8) {
-        const f32x8 v = rotated8<D>(a, first, g, r, 8 * el);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) qf[8 * el + j] = v[j];
-    }
-    settle();
-    mx = -INFINITY;
-    l = 0.0f;
-    for (int i = 0; i < D / 64; ++i) acc[i] = 0.0f;
-    for (int v = it.v0; v < it.v0 + it.nv; ++v) {
-        const int j0 = vis.key(v);
-        if (j0 > p) break;
-        for (int i = 0; i < U / 8; ++i) {  // 8 lanes a key
-            const int j = min(j0 + 8 * i + el / 8, p);
-            const T* kr = static_cast<const T*>(c.k) +
-                          ((page_of(j) * a.KVH + g) * ps + (j & (ps - 1))) * D + el % 8 * (D / 8);
-            float dot = 0.0f;
-            for (int d = 0; d < D / 8; ++d) dot = fmaf(widen(kr[d]), qf[el % 8 * (D / 8) + d], dot);
-            dot += __shfl_xor(dot, 1, 64);
-            dot += __shfl_xor(dot, 2, 64);
-            dot += __shfl_xor(dot, 4, 64);
-            if (el % 8 == 0) sc[8 * i + el / 8] = dot;
-        }
-        settle();
-        const int j = j0 + el;
-        const bool seen = el < U && j <= p && (a.window == 0 || j > p - a.window || j < a.sinks);
-        const float s = seen ? sc[el] : -INFINITY;
-        const float mnew = fmaxf(mx, wave_max(s));
-        const float alpha = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mnew);
-        const float w = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - mnew);
-        l = l * alpha + wave_add(w);
-        mx = mnew;
-        settle();
-        sc[el] = w;
-        settle();
-        const uint64_t mask = __ballot(seen);
-        for (int i = 0; i < D / 64; ++i) acc[i] *= alpha;
-        for (int u = 0; u < U / 8; ++u) {
-            if ((mask >> (8 * u) & 0xFF) == 0) continue;
-            const int j8 = j0 + 8 * u;
-            const T* vr = static_cast<const T*>(c.v) + (page_of(j8) * a.KVH + g) * D * ps + (j8 & (ps - 1));
-            for (int e = 0; e < 8; ++e)
-                if (mask >> (8 * u + e) & 1)
-                    for (int i = 0; i < D / 64; ++i)
-                        acc[i] = fmaf(sc[8 * u + e], widen(vr[(el + 64 * i) * ps + e]), acc[i]);
-        }
-        settle();
-    }
 }
 
 // ---- few query rows: keys stream through registers --------------------------------------------
@@ -828,39 +772,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
         if (live && chk != 0.0f) atomicOr(&flags[1], 1 << col);
         __syncthreads();
         const bool bad_page = flags[0] != 0;
-        const int redo = bad_page ? 0 : flags[1];
-        if (bad_page) {
-            sum = __builtin_nanf("");
-            if (tid == 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
-        }
-        const int r0 = it.row0 + col;
-        const int64_t prow = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows + col;
-        float* dst = whole ? a.out + (int64_t)(first + r0 / G) * a.ostride + (int64_t)(g * G + r0 % G) * D
-                           : a.po + prow * D;
-        if (live && !(redo >> col & 1)) {
+        if (bad_page && tid == 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
+        if (live) {
+            const bool again = !bad_page && (flags[1] >> col & 1);
+            const int rr = it.row0 + col;
+            const int64_t row = first + rr / G;
+            const int h = g * G + rr % G;
+            const int64_t piece = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows + col;
+            // (a row with a bad page is NaN, whatever its other pieces hold)
+            float* dst = whole || bad_page ? a.out + row * a.ostride + (int64_t)h * D : a.po + piece * D;
+            if (!again)
 #pragma unroll
-            for (int i = 0; i < OT / 4; ++i)
-                *reinterpret_cast<f32x4*>(dst + (4 * i + wv) * 16 + 4 * qd) =
-                    bad_page ? f32x4(__builtin_nanf("")) : res[i];
-            if (!whole && wv == 0 && qd == 0) a.ms[prow] = make_float2(top - P::shift, sum);
-        }
-        if (redo) {
-            __syncthreads();
-            float* qf = reinterpret_cast<float*>(lds + L::O) + wv * (D + 64);
-            int left = redo, turn = 0;
-            while (left) {
-                const int r = __builtin_ctz(left);
-                left &= left - 1;
-                if (turn++ % 4 != wv) continue;
-                float mx, sw, acc[D / 64];
-                attend_row<T, D, kUnit>(c, a, pages, vis, it, first, ctx, g, it.row0 + r, qf, qf + D, mx, sw, acc);
-                const int64_t pr = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows + r;
-                const int rr = it.row0 + r;
-                float* y = whole ? a.out + (int64_t)(first + rr / G) * a.ostride + (int64_t)(g * G + rr % G) * D
-                                 : a.po + pr * D;
-#pragma unroll
-                for (int e = 0; e < D / 64; ++e) y[lane + 64 * e] = whole ? acc[e] / sw : acc[e];
-                if (!whole && lane == 0) a.ms[pr] = make_float2(mx, sw);
+                for (int i = 0; i < OT / 4; ++i)
+                    *reinterpret_cast<f32x4*>(dst + (4 * i + wv) * 16 + 4 * qd) =
+                        bad_page ? f32x4(__builtin_nanf("")) : res[i];
+            if (wv == 0 && qd == 0) {
+                if (again) redo_row(a, row, h);
+                if (!whole) a.ms[piece] = make_float2(top - P::shift, again || bad_page ? __builtin_nanf("") : sum);
             }
         }
     }
@@ -868,16 +796,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
 
 // ---- many query rows: tiles of keys shared through LDS -----------------------------------------
 //
-// A workgroup takes an item of a tile of 128 query rows of a kv head, 32 to each of its four
-// waves (32x32x16 MFMAs), and visits U keys at a time through LDS: K [U][2 D bytes] and V^T [D][2 U
-// bytes] (of f32 three planes of parts each), 16-byte chunks XOR-swizzled so that the lanes a
-// read serves together touch all banks.  As above both products are transposed, a lane's 16
+// A workgroup takes an item of a tile of up to 256 query rows of a kv head (128 at hd 256), 32 to
+// each of its waves (32x32x16 MFMAs), and visits U keys at a time through LDS: K [U][2 D bytes] and V^T
+// [D][2 U bytes] (of f32 three planes of parts each), 16-byte chunks XOR-swizzled so that the lanes
+// a read serves together touch all banks.  As above both products are transposed, a lane's 16
 // accumulators of a 32-key group are one row's scores of keys 16 k + 8 (l / 32) + 0 .. 7 (the row
 // of K that operand row i reads is i with bits 2 and 3 exchanged), and those are the keys its
-// operand of the second product contracts; q's parts stay in registers.
-// K and V pass through registers on their way to LDS, V's of this visit stored after the first
-// product, K's of the next one after the second, so one buffer each is enough and every request
-// has a product to arrive in; two workgroups a CU fill each other's waits.
+// operand of the second product contracts.
+// Visit n is a matrix phase, p v of visit n - 1 and q k of visit n, and a vector phase, the
+// weights of visit n; a barrier ends each.  The two groups of four waves, a wave of each on every
+// SIMD, are a phase apart, so the matrix cores and the vector units are both at work: without
+// that the two workgroups of a CU ran their phases together (a 2048-token prompt of 32 heads of
+// 128, f16: matrix cores busy 20 % of the time, 142 us).  V of n - 1 and K of n share one of two
+// LDS buffers; each group stores its half of the next pair in its vector phase, requested one
+// visit before.
 // Bound by the matrix cores: Parts::N times the products of a 16-bit attention.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -893,19 +825,17 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 x, u32x4 y, f32x16 z) {
 
 template <class T, int D>
 struct WideLds {
+    static constexpr int GR = kGroups<T, D>, NT = 256 * GR;
     static constexpr int U = kWideUnit<T, D>, KPARTS = Parts<T>::K;
     static constexpr int KROW = 2 * D, VROW = 2 * U;
     static constexpr int PLANE = U * KROW;                  // of K, and of V^T
-    static constexpr int K = 0, V = K + KPARTS * PLANE;
-    static constexpr int QL = V + KPARTS * PLANE;           // q's last part, where registers lack
+    static constexpr int K = 0, V = KPARTS * PLANE, PAIR = 2 * V;
+    static constexpr int QL = GR * PAIR;                    // q's last part, where registers lack
     static constexpr bool kQl = sizeof(T) == 2 && D == 128;
     static constexpr int QREGS = Parts<T>::Q - (kQl ? 1 : 0);
-    static constexpr int IDS = QL + (kQl ? 4 * D / 16 * 1024 : 0);  // a page id per 16 keys of SEG visits
-    static constexpr int PER = U / 16, SEG = 512 / PER;
-    static constexpr int STAT = IDS + 2048;                 // rows to redo, a bad page
+    static constexpr int STAT = QL + (kQl ? NT / 64 * (D / 16) * 1024 : 0);  // whether a page is bad
     static constexpr int BYTES = STAT + 64;
-    static constexpr int TASKS = U * D / 8 / 256;           // 8-element chunks a thread
-    static_assert(4 * (D + 64) * 4 <= V, "");               // (redone rows' queries)
+    static constexpr int TASKS = U * D / 8 / NT;            // 8-element chunks of K (or V) a thread
     __device__ static uint32_t kslot(uint32_t r, uint32_t c) {
         return D >= 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
     }
@@ -915,19 +845,20 @@ struct WideLds {
 };
 
 template <class T, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(PagedKv c, PageTable t, Call a) {
+__global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void paged_wide_kernel(PagedKv c, PageTable t, Call a) {
     using L = WideLds<T, D>;
     using P = Parts<T>;
-    constexpr int U = L::U, NB = D / 16, OT = D / 32, NG = U / 32;
+    constexpr int U = L::U, NB = D / 16, OT = D / 32, NG = U / 32, GR = L::GR, NT = L::NT;
+    constexpr int LOG_D = D == 64 ? 6 : D == 128 ? 7 : 8;
+    constexpr int KSTEP = NT * 8 / D, VSTEP = NT * 8 / U;  // rows (dimensions) between a thread's chunks
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    int* ids = reinterpret_cast<int*>(lds + L::IDS);
-    int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0 .. 3] rows to redo, [4] a bad page
+    int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
     const int tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wv / 4;
     const int col = lane & 31, hf = lane >> 5;
     const int ps = c.page_size, shift = c.page_shift;
     const int KVH = a.KVH, G = a.G;
-    constexpr int LOG_D = D == 64 ? 6 : D == 128 ? 7 : 8;
     const int kread = ((col & 16) | (col & 4) << 1 | (col & 8) >> 1 | (col & 3));  // operand row's key
     // where the lane's operand rows begin, chunk hf
     const uint32_t kat = kread * L::KROW + L::kslot(kread, hf) * 16;
@@ -947,9 +878,97 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(Paged
         const int wmax = ctx + (it.row0 + min(w0 + 31, it.rows - 1)) / G;
         const int myrow = it.row0 + min(w0 + col, it.rows - 1);  // (rows past the tile repeat its last)
         const int ppos = ctx + myrow / G;
+
+        // Staging.  A thread's chunk i of K is 8 dimensions of key kr0 + i KSTEP of the visit, of V 8 keys
+        // of dimension vd0 + i VSTEP.  The page of each is read a visit ahead of its request, that
+        // a visit ahead of its use.  Past the item's ends the nearest visit is staged again, unused:
+        // with no branch around a load the waits count only what they need.  (Thread numbers
+        // are made opaque: addresses are formed again each time and not kept in registers.)
+        Raw<T> sk[L::TASKS], sv[L::TASKS];
+        uint32_t pk[L::TASKS], pv;
+        bool bad_id = false;
+        auto key_of = [&](int n) { return vis.key(it.v0 + max(0, min(n, it.nv - 1))); };
+        auto page_at = [&](int j0, uint32_t grp16) {
+            const int j = j0 + 16 * (int)grp16;
+            return (uint32_t)pages[(j < len ? j : j0) >> shift];  // (past the sequence: the visit's first)
+        };
+        auto sound = [&](uint32_t pg) {  // (looked at when it is used: its load has a visit to arrive in)
+            const bool bad = pg >= (uint32_t)c.n_pages;
+            bad_id |= bad;
+            return bad ? 0u : pg;
+        };
+        auto read_pages = [&](int n) {  // of pair n: V of visit n - 1, K of visit n
+            uint32_t ti = tid;
+            asm volatile("" : "+v"(ti));
+            const int j0 = key_of(n);
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) pk[i] = page_at(j0, (ti / (D / 8) + i * KSTEP) / 16);
+            pv = page_at(key_of(n - 1), ti % (U / 8) / 2);
+        };
+        auto request = [&](int n) {
+            uint32_t ti = tid;
+            asm volatile("" : "+v"(ti));
+            const int j0 = key_of(n);
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) {
+                const uint32_t r = ti / (D / 8) + i * KSTEP;
+                const uint32_t at = (uint32_t)j0 + (j0 + (int)(r & ~15u) < len ? r : r & 15u);
+                const int64_t row = ((int64_t)(sound(pk[i]) * (uint32_t)KVH + (uint32_t)g) << shift) + (at & (uint32_t)(ps - 1));
+                sk[i] = load8<T>(static_cast<const T*>(c.k) + (row << LOG_D) + ti % (D / 8) * 8);
+            }
+            const int i0 = key_of(n - 1);
+            const uint32_t ch = ti % (U / 8);
+            const uint32_t at = (uint32_t)i0 + (i0 + (int)(ch / 2 * 16) < len ? 8 * ch : 8 * (ch & 1));
+            const int64_t row = ((int64_t)(sound(pv) * (uint32_t)KVH + (uint32_t)g) << LOG_D) + ti / (U / 8);
+            const T* from = static_cast<const T*>(c.v) + (row << shift) + (at & (uint32_t)(ps - 1));
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) sv[i] = load8<T>(from + ((int64_t)(i * VSTEP) << shift));
+        };
+        auto store = [&](int n) {
+            uint32_t ti = tid;
+            asm volatile("" : "+v"(ti));
+            uint8_t* buf = lds + n % GR * L::PAIR;
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) {
+                const uint32_t r = ti / (D / 8) + i * KSTEP;
+                u32x4 p[P::K];
+                split_k<T>(sk[i], p);
+#pragma unroll
+                for (int x = 0; x < P::K; ++x)
+                    *reinterpret_cast<u32x4*>(buf + L::K + x * L::PLANE + r * L::KROW +
+                                              L::kslot(r, ti % (D / 8)) * 16) = p[x];
+            }
+            const int left = len - key_of(n - 1) - (int)(ti % (U / 8) * 8);  // keys of the chunk and on
+            if (__any(left < 8)) {  // past the sequence's end a page holds anything
+                constexpr int E = 4 / sizeof(T);
+#pragma unroll
+                for (int i = 0; i < L::TASKS; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        uint32_t& w = reinterpret_cast<uint32_t*>(&sv[i])[e / E];
+                        const uint32_t keep = E == 1 ? 0u : e % 2 ? 0xFFFFu : 0xFFFF0000u;
+                        w = e >= left ? w & keep : w;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) {
+                const uint32_t d = ti / (U / 8) + i * VSTEP;
+                u32x4 p[P::K];
+                split_k<T>(sv[i], p);
+#pragma unroll
+                for (int x = 0; x < P::K; ++x)
+                    *reinterpret_cast<u32x4*>(buf + L::V + x * L::PLANE + d * L::VROW +
+                                              L::vslot(d, ti % (U / 8)) * 16) = p[x];
+            }
+        };
+        read_pages(0);
+        request(0);
+        read_pages(1);
+
         u32x4 q[L::QREGS][NB];
         u32x4* ql = reinterpret_cast<u32x4*>(lds + L::QL) + wv * NB * 64 + lane;
         __syncthreads();  // (the item before is done with the LDS)
+        if (tid == 0) flags[0] = 0;
         float inv = 1.0f;
         if (any) {
             float up = 1.0f;
@@ -985,218 +1004,131 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(Paged
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
 
-        if (tid < 5) flags[tid] = 0;
-        for (int seg = 0; seg < it.nv; seg += L::SEG) {
-            const int nseg = min(L::SEG, it.nv - seg);
+        store(0);
+        request(1);
+        read_pages(2);
+        __syncthreads();
+        if (grp == 1) {  // (its half of pair 1, while the first group's first products run)
+            store(1);
+            request(2);
+            read_pages(3);
             __syncthreads();
-            for (int i = tid; i < nseg * L::PER; i += 256) {
-                const int j0 = vis.key(it.v0 + seg + i / L::PER);
-                int j = j0 + i % L::PER * 16;
-                if (j >= len) j = j0;  // (past the sequence: the visit's first keys again)
-                int pg = pages[j >> shift];
-                if ((unsigned)pg >= (unsigned)c.n_pages) {
-                    pg = 0;
-                    flags[4] = 1;
+        }
+        bool some = false;  // the visit has keys that some row of the wave sees
+        u32x4 p[NG][2][P::Q];
+        for (int n = 0; n <= it.nv; ++n) {
+            const uint8_t* buf = lds + n % GR * L::PAIR;
+            uint32_t ka = kat, va = vat;  // (opaque: no address is kept across visits)
+            asm volatile("" : "+v"(ka), "+v"(va));
+            if (some) {
+                // step i: dimensions 32 (i % OT) .., keys of MFMA i / OT; operands read ahead of the MFMAs
+                // of the step before (chunk 2 (i / OT) + hf: the swizzle is an XOR, turned last)
+                u32x4 vp[2][P::K];
+                auto read = [&](int i) {
+#pragma unroll
+                    for (int x = 0; x < P::K; ++x)
+                        vp[i % 2][x] = *reinterpret_cast<const u32x4*>(
+                            buf + L::V + x * L::PLANE + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
+                };
+                read(0);
+#pragma unroll
+                for (int i = 0; i < 2 * NG * OT; ++i) {
+                    if (i + 1 < 2 * NG * OT) read(i + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int x = 0; x < P::N; ++x)
+                        o[i % OT] = mfma32<T>(vp[i % 2][P::ki[x]], p[i / OT / 2][i / OT % 2][P::qi[x]], o[i % OT]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                ids[i] = pg;
             }
-            __syncthreads();
-            Raw<T> st[L::TASKS];
-            // A thread's chunk i of K is 8 dimensions of row kr0 + i KSTEP, whose page is one for the
-            // whole wave; of V, 8 keys of dimension vd0 + i VSTEP.  (Its number is made opaque, so
-            // that addresses are formed again each visit and not kept in registers.)
-            constexpr int KSTEP = 2048 / D, VSTEP = 2048 / U;
-            auto request_k = [&](int v) {
-                const int j0 = vis.key(it.v0 + seg + v);
-                int ti = tid;
-                asm volatile("" : "+v"(ti));
-                const int kr0 = ti / (D / 8);
-                const uint32_t lane_at = (uint32_t)(kr0 % 16 * D + ti % (D / 8) * 8);
-#pragma unroll
-                for (int i = 0; i < L::TASKS; ++i) {
-                    const int grp = __builtin_amdgcn_readfirstlane((kr0 + i * KSTEP) / 16);
-                    const uint32_t pg = __builtin_amdgcn_readfirstlane(ids[v * L::PER + grp]);
-                    const int j = j0 + (j0 + 16 * grp < len ? 16 * grp : 0);
-                    const int64_t at = ((int64_t)(pg * (uint32_t)KVH + (uint32_t)g) << shift) + (j & (ps - 1));
-                    // (rows 8 and on of a group are chunk i odd's where a chunk step is 8 rows)
-                    st[i] = load8<T>(static_cast<const T*>(c.k) + (at << LOG_D) +
-                                     (lane_at + (KSTEP == 8 ? i % 2 * 8 * D : 0)));
-                }
-            };
-            auto request_v = [&](int v) {
-                const int j0 = vis.key(it.v0 + seg + v);
-                int ti = tid;
-                asm volatile("" : "+v"(ti));
-                const int ch = ti % (U / 8), vd0 = ti / (U / 8), grp = ch / 2;
-                const uint32_t pg = ids[v * L::PER + grp];
-                const int j = j0 + (j0 + 16 * grp < len ? 16 * grp : 0);
-                const int64_t at = (((int64_t)(pg * (uint32_t)KVH + (uint32_t)g) << LOG_D) + vd0) << shift;
-                const T* from = static_cast<const T*>(c.v) + at + (j & (ps - 1)) + 8 * (ch % 2);
-#pragma unroll
-                for (int i = 0; i < L::TASKS; ++i) st[i] = load8<T>(from + ((int64_t)(i * VSTEP) << shift));
-            };
-            auto store_k = [&] {
-                int ti = tid;
-                asm volatile("" : "+v"(ti));
-                const uint32_t kr0 = ti / (D / 8), at = kr0 * L::KROW + L::kslot(kr0, ti % (D / 8)) * 16;
-#pragma unroll
-                for (int i = 0; i < L::TASKS; ++i) {
-                    u32x4 p[P::K];
-                    split_k<T>(st[i], p);
-                    // (a chunk step of 8 rows turns bit 3 of the slot)
-                    const uint32_t to = (KSTEP == 8 && i % 2 ? at ^ 128 : at) + i * KSTEP * L::KROW;
-#pragma unroll
-                    for (int n = 0; n < P::K; ++n) *reinterpret_cast<u32x4*>(lds + L::K + n * L::PLANE + to) = p[n];
-                }
-            };
-            auto store_v = [&](int v) {
-                const int j0 = vis.key(it.v0 + seg + v);
-                int ti = tid;
-                asm volatile("" : "+v"(ti));
-                const uint32_t ch = ti % (U / 8), vd0 = ti / (U / 8);
-                const uint32_t at = vd0 * L::VROW + L::vslot(vd0, ch) * 16;
-                if (j0 + U > len) {  // past the sequence's end a page holds anything
-                    constexpr int E = 4 / sizeof(T);
-#pragma unroll
-                    for (int i = 0; i < L::TASKS; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (j0 + 8 * (int)ch + e >= len) {
-                                uint32_t& w = reinterpret_cast<uint32_t*>(&st[i])[e / E];
-                                if constexpr (E == 1) w = 0;
-                                else w &= e % 2 ? 0xFFFFu : 0xFFFF0000u;
-                            }
-                }
-#pragma unroll
-                for (int i = 0; i < L::TASKS; ++i) {
-                    u32x4 p[P::K];
-                    split_k<T>(st[i], p);
-#pragma unroll
-                    for (int n = 0; n < P::K; ++n)
-                        *reinterpret_cast<u32x4*>(lds + L::V + n * L::PLANE + at + i * VSTEP * L::VROW) = p[n];
-                }
-            };
-            request_k(0);
-            store_k();
-            request_v(0);
-            for (int v = 0; v < nseg; ++v) {
-                __syncthreads();  // K of this visit is staged, V of the one before read
-                const int j0 = vis.key(it.v0 + seg + v);
-                // (the groups of 32 keys, from u0 on, that some row of the wave sees)
-                f32x16 s[NG];
-                bool live[NG], some = false;
-#pragma unroll
-                for (int u = 0; u < NG; ++u) {
-                    const int ju = j0 + 32 * u;
-                    live[u] = any && ju <= wmax && (a.window == 0 || ju + 31 > wmin - a.window || ju < a.sinks);
-                    some |= live[u];
-                }
-                uint32_t ka = kat, va = vat;  // (opaque: no address is kept across visits)
-                asm volatile("" : "+v"(ka), "+v"(va));
-                if (some) {
-                    // a block's parts are read ahead of the MFMAs of the one before (chunk 2 b + hf
-                    // of the row: the swizzle is an XOR, so b's bits can be turned last)
-                    u32x4 kp[2][NG][P::K], qx[2];
-                    auto read = [&](int b) {
-#pragma unroll
-                        for (int u = 0; u < NG; ++u)
-#pragma unroll
-                            for (int n = 0; n < P::K; ++n)
-                                kp[b % 2][u][n] = *reinterpret_cast<const u32x4*>(
-                                    lds + L::K + n * L::PLANE + 32 * u * L::KROW + (ka ^ 32 * b));
-                        if (L::kQl) qx[b % 2] = ql[b * 64];
-                    };
-                    read(0);
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        if (b + 1 < NB) read(b + 1);
-                        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                        for (int n = 0; n < P::N; ++n)
-#pragma unroll
-                            for (int u = 0; u < NG; ++u) {
-                                const f32x16 zero = {};
-                                const u32x4 x = P::qi[n] < L::QREGS ? q[P::qi[n] < L::QREGS ? P::qi[n] : 0][b] : qx[b % 2];
-                                s[u] = mfma32<T>(kp[b % 2][u][P::ki[n]], x, b + n == 0 ? zero : s[u]);
-                            }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-                store_v(v);
-                if (v + 1 < nseg) request_k(v + 1);
-                __builtin_amdgcn_sched_barrier(0);
-                u32x4 p[NG][2][P::Q];
-                if (some) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int u = 0; u < NG; ++u) {
-                        const int ju = j0 + 32 * u;
-                        const bool whole = ju + 31 <= wmin &&
-                                           (a.window == 0 || ju > wmax - a.window || ju + 32 <= a.sinks);
-                        if (!whole) {
-                            const int at = ppos - ju - 8 * hf, far = a.window > 0 ? at - a.window : INT_MIN;
-                            const int sk = a.sinks - ju - 8 * hf;
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const int j = 16 * (e / 8) + e % 8;
-                                const bool hidden = (j > at) | ((j <= far) & (j >= sk));
-                                s[u][e] = hidden ? -INFINITY : s[u][e];
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
-                    }
-                    if (std::is_same_v<T, f16_t>) top *= inv;  // (a power of two)
-                    if (__any(top > ref + 8.0f)) {
-                        top = fmaxf(top, __shfl_xor(top, 32, 64));
-                        const float to = fmaxf(ref, top);
-                        const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
-                        l *= f;
-#pragma unroll
-                        for (int i = 0; i < OT; ++i) o[i] *= f;
-                        ref = to;
-                    }
-                    const float from = ref == -INFINITY ? 0.0f : ref - P::shift;
+            if (n == it.nv) break;
+            const int j0 = vis.key(it.v0 + n);
+            some = any && j0 <= wmax && (a.window == 0 || j0 + U - 1 > wmin - a.window || j0 < a.sinks);
+            f32x16 s[NG];
+            if (some) {
+                u32x4 kp[2][NG][P::K], qx[2];
+                auto read = [&](int b) {
 #pragma unroll
                     for (int u = 0; u < NG; ++u)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            f32x8 w;
+                        for (int x = 0; x < P::K; ++x)
+                            kp[b % 2][u][x] = *reinterpret_cast<const u32x4*>(
+                                buf + L::K + x * L::PLANE + 32 * u * L::KROW + (ka ^ 32 * b));
+                    if (L::kQl) qx[b % 2] = ql[b * 64];
+                };
+                read(0);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                w[e] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * k + e], inv, -from));
-                                l += w[e];
-                            }
-                            split_w<T>(w, p[u][k]);
+                for (int b = 0; b < NB; ++b) {
+                    if (b + 1 < NB) read(b + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int x = 0; x < P::N; ++x)
+#pragma unroll
+                        for (int u = 0; u < NG; ++u) {
+                            const f32x16 zero = {};
+                            const u32x4 y = P::qi[x] < L::QREGS ? q[P::qi[x] < L::QREGS ? P::qi[x] : 0][b] : qx[b % 2];
+                            s[u] = mfma32<T>(kp[b % 2][u][P::ki[x]], y, b + x == 0 ? zero : s[u]);
                         }
-                }
-                __syncthreads();  // V of this visit is staged, K read
-                if (some) {
-                    // step i: dimensions 32 (i % OT) .., keys of MFMA i / OT; read ahead as above
-                    u32x4 vp[2][P::K];
-                    auto read = [&](int i) {
-#pragma unroll
-                        for (int n = 0; n < P::K; ++n)
-                            vp[i % 2][n] = *reinterpret_cast<const u32x4*>(
-                                lds + L::V + n * L::PLANE + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
-                    };
-                    read(0);
-#pragma unroll
-                    for (int i = 0; i < 2 * NG * OT; ++i) {
-                        if (i + 1 < 2 * NG * OT) read(i + 1);
-                        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                        for (int n = 0; n < P::N; ++n)
-                            o[i % OT] = mfma32<T>(vp[i % 2][P::ki[n]], p[i / OT / 2][i / OT % 2][P::qi[n]], o[i % OT]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-                if (v + 1 < nseg) {
-                    store_k();
-                    request_v(v + 1);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            __syncthreads();  // the matrix phase ends
+            if (some) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < NG; ++u) {
+                    const int ju = j0 + 32 * u;
+                    const bool whole = ju + 31 <= wmin &&
+                                       (a.window == 0 || ju > wmax - a.window || ju + 32 <= a.sinks);
+                    if (!whole) {
+                        const int at = ppos - ju - 8 * hf, far = a.window > 0 ? at - a.window : INT_MIN;
+                        const int sk0 = a.sinks - ju - 8 * hf;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int j = 16 * (e / 8) + e % 8;
+                            const bool hidden = (j > at) | ((j <= far) & (j >= sk0));
+                            s[u][e] = hidden ? -INFINITY : s[u][e];
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
+                }
+                if (std::is_same_v<T, f16_t>) top *= inv;  // (a power of two)
+                if (__any(top > ref + 8.0f)) {
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float to = fmaxf(ref, top);
+                    const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+                    l *= f;
+#pragma unroll
+                    for (int i = 0; i < OT; ++i) o[i] *= f;
+                    ref = to;
+                }
+                const float from = ref == -INFINITY ? 0.0f : ref - P::shift;
+#pragma unroll
+                for (int u = 0; u < NG; ++u)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        f32x8 w;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            w[e] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * k + e], inv, -from));
+                            l += w[e];
+                        }
+                        split_w<T>(w, p[u][k]);
+                    }
+            }
+            const int next = n + 1 + (GR == 2 ? grp : 0);
+            store(next);
+            request(next + 1);
+            read_pages(next + 2);
+            __syncthreads();  // the vector phase ends
         }
+        if (GR == 2) {  // (both groups pass 2 nv + 2 barriers from the first pair on)
+            __syncthreads();
+            if (grp == 0) __syncthreads();
+        }
+        if (bad_id) flags[0] = 1;
+        __syncthreads();
 
         const bool whole = it.S == 1;
         const bool mine = any && w0 + col < it.rows;
@@ -1213,69 +1145,126 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_wide_kernel(Paged
                 chk = fmaf(o[i][e], 0.0f, chk);
             }
         bool bad = mine && chk != 0.0f;
-        bad |= (bool)__shfl_xor((int)bad, 32, 64);
-        const bool bad_page = flags[4] != 0;
-        if (bad_page) {
-            bad = false;
-            l = __builtin_nanf("");
-            if (tid == 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
-        }
-        const uint32_t again = (uint32_t)__ballot(bad);  // (both halves of a row agree)
-        const int64_t piece = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows;
-        auto place = [&](int r) {  // row r of the tile
-            const int rr = it.row0 + r;
-            return whole ? a.out + (int64_t)(first + rr / G) * a.ostride + (int64_t)(g * G + rr % G) * D
-                         : a.po + (piece + r) * D;
-        };
-        if (mine && !bad) {
-            float* dst = place(w0 + col);
+        bad |= (bool)__shfl_xor((int)bad, 32, 64);  // (both halves of a row)
+        const bool bad_page = flags[0] != 0;
+        if (bad_page && tid == 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
+        if (mine) {
+            const bool again = !bad_page && bad;
+            const int rr = it.row0 + w0 + col;
+            const int64_t row = first + rr / G;
+            const int h = g * G + rr % G;
+            const int64_t piece = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows + w0 + col;
+            // (a row with a bad page is NaN, whatever its other pieces hold)
+            float* dst = whole || bad_page ? a.out + row * a.ostride + (int64_t)h * D : a.po + piece * D;
+            if (!again)
 #pragma unroll
-            for (int i = 0; i < OT; ++i)
+                for (int i = 0; i < OT; ++i)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const f32x4 x = {o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]};
-                    *reinterpret_cast<f32x4*>(dst + 32 * i + 8 * u + 4 * hf) =
-                        bad_page ? f32x4(__builtin_nanf("")) : x;
-                }
-            if (!whole && hf == 0) a.ms[piece + w0 + col] = make_float2(ref - P::shift, l);
-        }
-        if (lane == 0 && again) flags[wv] = (int)again;
-        __syncthreads();
-        float* qf = reinterpret_cast<float*>(lds) + wv * (D + 64);
-        int turn = 0;
-        for (int w = 0; w < 4; ++w) {
-            uint32_t left = (uint32_t)flags[w];
-            while (left) {
-                const int r = 32 * w + __builtin_ctz(left);
-                left &= left - 1;
-                if (turn++ % 4 != wv) continue;
-                float mx, sw, acc[D / 64];
-                attend_row<T, D, U>(c, a, pages, vis, it, first, ctx, g, it.row0 + r, qf, qf + D, mx, sw, acc);
-                float* y = place(r);
-#pragma unroll
-                for (int e = 0; e < D / 64; ++e) y[lane + 64 * e] = whole ? acc[e] / sw : acc[e];
-                if (!whole && lane == 0) a.ms[piece + r] = make_float2(mx, sw);
+                    for (int u = 0; u < 4; ++u) {
+                        const f32x4 x = {o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]};
+                        *reinterpret_cast<f32x4*>(dst + 32 * i + 8 * u + 4 * hf) =
+                            bad_page ? f32x4(__builtin_nanf("")) : x;
+                    }
+            if (hf == 0) {
+                if (again) redo_row(a, row, h);
+                if (!whole) a.ms[piece] = make_float2(ref - P::shift, again || bad_page ? __builtin_nanf("") : l);
             }
         }
     }
 }
 
-// The pieces of a tile dealt out, joined: out = sum_s 2^(M_s - M) o_s / sum_s 2^(M_s - M) l_s over the
+// One row and head by a wave, in plain f32: for rows whose products of parts came out non-finite
+// (an infinity times a part that is 0, also where a mask hides it).  qf: LDS [D], the query;
+// sc: LDS [64].  Lane el gets dimensions el + 64 i of out.
+template <class T, int D>
+__device__ void attend_row(const PagedKv& c, const Call& a, const int* pages, int row, int h, int p,
+                           float* qf, float* sc, float (&acc)[D / 64]) {
+    constexpr int U = 64;
+    const int el = threadIdx.x & 63, g = h / a.G;
+    const int64_t ps = c.page_size;
+    auto settle = [] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    bool bad = false;
+    auto page_of = [&](int j) {
+        const int pg = pages[j >> c.page_shift];
+        if ((unsigned)pg < (unsigned)c.n_pages) return (int64_t)pg;
+        bad = true;
+        return (int64_t)0;
+    };
+    settle();
+    if (el < D / 8) {
+        const f32x8 v = rotated8<D>(a, row, g, h % a.G, 8 * el);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) qf[8 * el + j] = v[j];
+    }
+    settle();
+    float mx = -INFINITY, l = 0.0f;
+    for (int i = 0; i < D / 64; ++i) acc[i] = 0.0f;
+    const Visits<U> vis(p, p, a.window, a.sinks);
+    for (int v = 0; v < vis.count && !(l != l); ++v) {  // (a NaN sum stays one)
+        const int j0 = vis.key(v);
+        for (int i = 0; i < U / 8; ++i) {  // 8 lanes a key
+            const int j = min(j0 + 8 * i + el / 8, p);
+            const T* kr = static_cast<const T*>(c.k) +
+                          ((page_of(j) * a.KVH + g) * ps + (j & (ps - 1))) * D + el % 8 * (D / 8);
+            float dot = 0.0f;
+            for (int d = 0; d < D / 8; ++d) dot = fmaf(widen(kr[d]), qf[el % 8 * (D / 8) + d], dot);
+            dot += __shfl_xor(dot, 1, 64);
+            dot += __shfl_xor(dot, 2, 64);
+            dot += __shfl_xor(dot, 4, 64);
+            if (el % 8 == 0) sc[8 * i + el / 8] = dot;
+        }
+        settle();
+        const int j = j0 + el;
+        const bool seen = j <= p && (a.window == 0 || j > p - a.window || j < a.sinks);
+        const float s = seen ? sc[el] : -INFINITY;
+        const float mnew = fmaxf(mx, wave_max(s));
+        const float alpha = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mnew);
+        const float w = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - mnew);
+        l = l * alpha + wave_add(w);
+        mx = mnew;
+        settle();
+        sc[el] = w;
+        settle();
+        const uint64_t mask = __ballot(seen);
+        for (int i = 0; i < D / 64; ++i) acc[i] *= alpha;
+        for (int u = 0; u < U / 8; ++u) {
+            if ((mask >> (8 * u) & 0xFF) == 0) continue;
+            const int j8 = j0 + 8 * u;
+            const T* vr = static_cast<const T*>(c.v) + (page_of(j8) * a.KVH + g) * D * ps + (j8 & (ps - 1));
+            for (int e = 0; e < 8; ++e)
+                if (mask >> (8 * u + e) & 1)
+                    for (int i = 0; i < D / 64; ++i)
+                        acc[i] = fmaf(sc[8 * u + e], widen(vr[(el + 64 * i) * ps + e]), acc[i]);
+        }
+        settle();
+    }
+    if (__any(bad)) l = __builtin_nanf("");
+    for (int i = 0; i < D / 64; ++i) acc[i] = l != l ? l : acc[i] / l;
+}
+
+// The last kernel of a call.  The pieces of a tile dealt out, joined: out = sum_s 2^(M_s - M) o_s / sum_s 2^(M_s - M) l_s over the
 // pieces' (M_s, l_s, o_s); a piece in which a row sees no key has M_s = -inf, weight 0.  A
 // workgroup per (16 rows of a tile, kv head), D / 4 threads to a row; where there are fewer rows
-// than such groups, several share a row's pieces and meet in LDS.
-template <int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PageTable t, Call a) {
+// than such groups, several share a row's pieces and meet in LDS.  A row with a piece of NaN sum
+// is left: its output is written (a bad page), or it is one of the rows listed to be done again,
+// which follow.
+template <class T, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv c, PageTable t, Call a) {
     constexpr int W = D / 4, N = 256 / W;
     __shared__ f32x4 so[N][W];
     __shared__ float sl[N];
     const int ln = threadIdx.x % W, sub = threadIdx.x / W;
     const int nn = a.kind[kNarrow].head[1] * a.KVH;
-    const int nw = a.kind[kWide].head[1] * a.KVH * (kTileRows[kWide] / 16);
+    const int bl = a.kind[kWide].tile_rows / 16;
+    const int nw = a.kind[kWide].head[1] * a.KVH * bl;
     for (int i = blockIdx.x; i < nn + nw; i += gridDim.x) {
         const bool wide = i >= nn;
-        const int k = wide ? (i - nn) / (kTileRows[kWide] / 16) : i;
-        const int r0 = wide ? (i - nn) % (kTileRows[kWide] / 16) * 16 : 0;
+        const int k = wide ? (i - nn) / bl : i;
+        const int r0 = wide ? (i - nn) % bl * 16 : 0;
         const Split sp = a.kind[wide ? kWide : kNarrow].splits[k / a.KVH];
         const int g = k % a.KVH, rows = min(16, sp.rows - r0);
         if (rows <= 0 || sp.S < 2) continue;  // (uniform)
@@ -1315,25 +1304,46 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PageTable t, Call a) {
                     }
                 __syncthreads();
             }
-            if (live && part == 0) {
+            if (live && part == 0 && l == l) {
                 const int rr = sp.row0 + r0 + r;
                 *reinterpret_cast<f32x4*>(a.out + (first + rr / a.G) * a.ostride +
                                           (int64_t)(g * a.G + rr % a.G) * D + 4 * ln) = o / l;
             }
         }
     }
+    const int again = *a.redo_count;
+    if (again == 0) return;
+    __shared__ float rows[4][D + 64];
+    const int wv = threadIdx.x / 64, B = t.counts[kPagesEntries];
+    for (int i = (int)blockIdx.x * 4 + wv; i < again; i += (int)gridDim.x * 4) {
+        const int row = a.redo[i] / a.H, h = a.redo[i] % a.H;
+        int lo = 0, hi = B;  // its entry
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (t.cu[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        const int p = t.step_lens[lo] - t.cu[lo + 1] + row;
+        float acc[D / 64];
+        attend_row<T, D>(c, a, t.table + (int64_t)t.step_ids[lo] * t.max_pages, row, h, p, rows[wv],
+                         rows[wv] + D, acc);
+        float* o = a.out + row * a.ostride + (int64_t)h * D + (threadIdx.x & 63);
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) o[64 * e] = acc[e];
+    }
 }
 
 // How a call's workspace is laid out, and its grids.
 struct Layout {
     int64_t items[2], rows[2];
-    size_t head_at[2], items_at[2], splits_at[2], turn_at, ms_at, po_at, bytes;
+    size_t head_at[2], items_at[2], splits_at[2], turn_at, ms_at, po_at, count_at, redo_at, bytes;
 };
 
 // Pieces a kind's work is dealt out in: narrow, four workgroups of four waves for every CU; wide,
-// one for every place that its kernel has (two a CU), which leaves a causal prompt's tiles, at
-// most twice the mean, whole.
+// the one of eight waves (of four at hd 256) that a CU holds.
 int target_pieces(int kind) { return (kind == kNarrow ? 4 : 1) * device_info().cu_count; }
+
+int tile_rows(int kind, int64_t D) { return kind == kNarrow ? kTileRows : D < 256 ? 256 : 128; }
 
 Layout layout(const PagedKv& c, const unillm_page_table& t, int64_t n, int64_t H) {
     const int64_t KVH = c.n_kv_heads, G = H / KVH, D = c.head_dim;
@@ -1347,10 +1357,10 @@ Layout layout(const PagedKv& c, const unillm_page_table& t, int64_t n, int64_t H
     for (int k = 0; k < 2; ++k) {
         // tiles: an entry's last may be ragged.  A tile of nv visits makes at most nv / C + 1
         // pieces, and the nv / C add up to target / KVH; more than one piece, at most 2 nv / C.
-        const int64_t tiles = n * G / kTileRows[k] + std::min<int64_t>(n, t.st.max_seqs);
+        const int64_t tiles = n * G / tile_rows(k, D) + std::min<int64_t>(n, t.st.max_seqs);
         const bool some = k == kNarrow || n * G > kNarrowRows;
         l.items[k] = some ? tiles + target_pieces(k) / KVH + 1 : 0;
-        l.rows[k] = some ? 2 * (int64_t)target_pieces(k) * std::min<int64_t>(kTileRows[k], n * G) : 0;
+        l.rows[k] = some ? 2 * (int64_t)target_pieces(k) * std::min<int64_t>(tile_rows(k, D), n * G) : 0;
         l.head_at[k] = take(2 * sizeof(int));
         l.items_at[k] = take(l.items[k] * (int64_t)sizeof(Item));
         l.splits_at[k] = take(tiles * (int64_t)sizeof(Split));
@@ -1358,6 +1368,9 @@ Layout layout(const PagedKv& c, const unillm_page_table& t, int64_t n, int64_t H
     l.turn_at = take(n * D / 2 * (int64_t)sizeof(float2));
     l.ms_at = take((l.rows[0] + l.rows[1]) * (int64_t)sizeof(float2));
     l.po_at = take((l.rows[0] + l.rows[1]) * D * (int64_t)sizeof(float));
+    // rows to do again: every (row, head), and again for each piece
+    l.count_at = take(sizeof(int));
+    l.redo_at = take((n * H + l.rows[0] + l.rows[1]) * (int64_t)sizeof(int));
     l.bytes = at;
     return l;
 }
@@ -1386,14 +1399,15 @@ hipError_t launch_typed(const PagedKv& c, const unillm_page_table& t, const Call
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (l.items[kWide] > 0) {
-        const unsigned grid = (unsigned)std::min<int64_t>(l.items[kWide] * a.KVH, most);
-        paged_wide_kernel<T, D><<<grid, 256, LW::BYTES, s>>>(c, t.st, a);
+        const unsigned grid = (unsigned)std::min<int64_t>(l.items[kWide] * a.KVH, 4 * most);
+        paged_wide_kernel<T, D><<<grid, LW::NT, LW::BYTES, s>>>(c, t.st, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     const unsigned grid = (unsigned)std::min<int64_t>(l.items[kNarrow] * a.KVH, most);
     paged_narrow_kernel<T, D><<<grid, 256, L::BYTES, s>>>(c, t.st, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    paged_merge_kernel<D><<<(unsigned)std::min<int64_t>((l.rows[0] + l.rows[1]) / 2, most), 256, 0, s>>>(t.st, a);
+    paged_merge_kernel<T, D><<<(unsigned)std::min<int64_t>((l.rows[0] + l.rows[1]) / 2, most), 256, 0, s>>>(
+        c, t.st, a);
     return hipGetLastError();
 }
 
@@ -1420,9 +1434,10 @@ hipError_t launch_paged_attention(const PagedKv& c, const unillm_page_table& t, 
     Call a{qkv, out, qstride, ostride, (int)n, (int)H, (int)c.n_kv_heads, (int)(H / c.n_kv_heads),
            (int)std::min(window, far), (int)std::min(sinks, far),
            reinterpret_cast<float2*>(w + l.turn_at), reinterpret_cast<float2*>(w + l.ms_at),
-           reinterpret_cast<float*>(w + l.po_at), {}};
+           reinterpret_cast<float*>(w + l.po_at), reinterpret_cast<int*>(w + l.count_at),
+           reinterpret_cast<int*>(w + l.redo_at), {}};
     for (int k = 0; k < 2; ++k)
-        a.kind[k] = {target_pieces(k), k == kNarrow ? 4 : 2, k == kNarrow ? 0 : (int)l.rows[0],
+        a.kind[k] = {tile_rows(k, c.head_dim), target_pieces(k), k == kNarrow ? 4 : 2, k == kNarrow ? 0 : (int)l.rows[0],
                      (int)l.rows[k], reinterpret_cast<int*>(w + l.head_at[k]),
                      reinterpret_cast<Item*>(w + l.items_at[k]),
                      reinterpret_cast<Split*>(w + l.splits_at[k])};
