@@ -68,11 +68,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // An entry of up to kNarrowRows rows has narrow tiles, a longer one wide ones, each kind with
 // a list and a kernel of its own.
 struct Item {
-    int entry, row0, rows, v0, nv, base, s, S;
+    int first, ctx, len, id;  // of the entry: its first step row, tokens before the step and with it, sequence
+    int row0, rows, v0, nv, base, s, S, pad;
 };
 // A tile dealt out, for the merge.
 struct Split {
-    int entry, row0, rows, base, S, pad[3];
+    int first, row0, rows, base, S, pad[3];
 };
 
 // What the kernels of a call share.
@@ -230,7 +231,7 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         const int v[6] = {x.b, x.row0, x.rows, x.nv, kd.row0 + base, S};
 #pragma unroll
         for (int e = 0; e < 6; ++e) info[tid][e] = v[e];
-        if (want) kd.splits[splits + r.y - 1] = {x.b, x.row0, x.rows, kd.row0 + base, S, {}};
+        if (want) kd.splits[splits + r.y - 1] = {t.cu[x.b], x.row0, x.rows, kd.row0 + base, S, {}};
         __syncthreads();
         for (int k = tid; k < off[256]; k += 256) {
             int lo = 0, hi = 256;
@@ -242,7 +243,8 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
             const int* w = info[lo];
             const int s = k - off[lo], nv = w[3], Sw = w[5];
             const int v0 = (int)((int64_t)s * nv / Sw), v1 = (int)((int64_t)(s + 1) * nv / Sw);
-            kd.items[items + k] = {w[0], w[1], w[2], v0, v1 - v0, w[4], s, Sw};
+            const int b = w[0], ctx = ctxs[b];
+            kd.items[items + k] = {t.cu[b], ctx, ctx + ms[b], t.step_ids[b], w[1], w[2], v0, v1 - v0, w[4], s, Sw, 0};
         }
         items += off[256];
         splits += last[0];
@@ -550,9 +552,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
     for (int idx = blockIdx.x; idx < total; idx += gridDim.x) {
         const Item it = a.kind[kNarrow].items[idx / KVH];
         const int g = idx % KVH;
-        const int first = t.cu[it.entry], m = t.cu[it.entry + 1] - first;
-        const int len = t.step_lens[it.entry], ctx = len - m;
-        const int* pages = t.table + (int64_t)t.step_ids[it.entry] * t.max_pages;
+        const int first = it.first, len = it.len, ctx = it.ctx;
+        const int* pages = t.table + (int64_t)it.id * t.max_pages;
         const int pmin = ctx + it.row0 / G, pmax = ctx + (it.row0 + it.rows - 1) / G;
         const Visits<kUnit> vis(pmin, pmax, a.window, a.sinks);
         // q's parts: task (block, lane) as the B operand takes it
@@ -850,7 +851,8 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
     using P = Parts<T>;
     constexpr int U = L::U, NB = D / 16, OT = D / 32, NG = U / 32, GR = L::GR, NT = L::NT;
     constexpr int LOG_D = D == 64 ? 6 : D == 128 ? 7 : 8;
-    constexpr int KSTEP = NT * 8 / D, VSTEP = NT * 8 / U;  // rows (dimensions) between a thread's chunks
+    constexpr int KSTEP = NT * 8 / D, KROWS = 512 / D;  // keys between a thread's chunks, keys of a wave's
+    constexpr int VGROUPS = U / 16;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
     const int tid = threadIdx.x, lane = tid & 63;
@@ -863,103 +865,101 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
     // where the lane's operand rows begin, chunk hf
     const uint32_t kat = kread * L::KROW + L::kslot(kread, hf) * 16;
     const uint32_t vat = col * L::VROW + L::vslot(col, hf) * 16;
+    // its staging: offsets of its chunks of K and V from their group's first, and in a buffer
+    const int kr0 = tid / (D / 8), vgroup = wv % VGROUPS;
+    const uint32_t vd0 = wv / VGROUPS * (32 * L::TASKS) + lane / 2;
+    const uint32_t klane = (uint32_t)(kr0 % 16 * D + tid % (D / 8) * 8);
+    const uint32_t vlane = (vd0 << shift) + 8 * (lane & 1);
+    const uint32_t kto = kr0 * L::KROW + L::kslot(kr0, tid % (D / 8)) * 16;
+    const uint32_t vto = vd0 * L::VROW + L::vslot(vd0, 2 * vgroup + (lane & 1)) * 16;
     const int total = a.kind[kWide].head[0] * KVH;
     for (int idx = blockIdx.x; idx < total; idx += gridDim.x) {
         const Item it = a.kind[kWide].items[idx / KVH];
         const int g = idx % KVH;
-        const int first = t.cu[it.entry], m = t.cu[it.entry + 1] - first;
-        const int len = t.step_lens[it.entry], ctx = len - m;
-        const int* pages = t.table + (int64_t)t.step_ids[it.entry] * t.max_pages;
+        const int first = it.first, len = it.len, ctx = it.ctx;
+        const int* pages = t.table + (int64_t)it.id * t.max_pages;
         const Visits<U> vis(ctx + it.row0 / G, ctx + (it.row0 + it.rows - 1) / G, a.window, a.sinks);
         // the wave's rows and their positions
         const int w0 = 32 * wv;
-        const bool any = w0 < it.rows;
-        const int wmin = ctx + (it.row0 + w0) / G;
+        const int wmin = ctx + (it.row0 + min(w0, it.rows - 1)) / G;
         const int wmax = ctx + (it.row0 + min(w0 + 31, it.rows - 1)) / G;
         const int myrow = it.row0 + min(w0 + col, it.rows - 1);  // (rows past the tile repeat its last)
         const int ppos = ctx + myrow / G;
 
-        // Staging.  A thread's chunk i of K is 8 dimensions of key kr0 + i KSTEP of the visit, of V 8 keys
-        // of dimension vd0 + i VSTEP.  The page of each is read a visit ahead of its request, that
-        // a visit ahead of its use.  Past the item's ends the nearest visit is staged again, unused:
-        // with no branch around a load the waits count only what they need.  (Thread numbers
-        // are made opaque: addresses are formed again each time and not kept in registers.)
+        // Staging.  A wave's chunks of K are 8 dimensions of keys kr0 + i KSTEP of the visit each, of V 8
+        // keys of dimensions vd0 + 32 i, all chunk i of one group of 16 keys and so of one page:
+        // addresses are a uniform base and the lane's fixed offset.  A page id is read a visit ahead
+        // of its request, that a visit ahead of its use.  Past the item's ends the nearest visit is
+        // staged again, unused: with no branch around a load the waits count only what they need.
         Raw<T> sk[L::TASKS], sv[L::TASKS];
-        uint32_t pk[L::TASKS], pv;
+        int pk[L::TASKS], pv;
         bool bad_id = false;
         auto key_of = [&](int n) { return vis.key(it.v0 + max(0, min(n, it.nv - 1))); };
-        auto page_at = [&](int j0, uint32_t grp16) {
-            const int j = j0 + 16 * (int)grp16;
-            return (uint32_t)pages[(j < len ? j : j0) >> shift];  // (past the sequence: the visit's first)
-        };
-        auto sound = [&](uint32_t pg) {  // (looked at when it is used: its load has a visit to arrive in)
+        // (past the sequence: the visit's first group again)
+        auto group_key = [&](int j0, int grp16) { return j0 + 16 * grp16 < len ? j0 + 16 * grp16 : j0; };
+        auto sound = [&](int page) {  // (looked at when it is used: its load has a visit to arrive in)
+            const uint32_t pg = (uint32_t)__builtin_amdgcn_readfirstlane(page);
             const bool bad = pg >= (uint32_t)c.n_pages;
             bad_id |= bad;
             return bad ? 0u : pg;
         };
+        auto kgroup = [&](int i) { return (wv * KROWS + i * KSTEP) / 16; };
         auto read_pages = [&](int n) {  // of pair n: V of visit n - 1, K of visit n
-            uint32_t ti = tid;
-            asm volatile("" : "+v"(ti));
-            const int j0 = key_of(n);
 #pragma unroll
-            for (int i = 0; i < L::TASKS; ++i) pk[i] = page_at(j0, (ti / (D / 8) + i * KSTEP) / 16);
-            pv = page_at(key_of(n - 1), ti % (U / 8) / 2);
+            for (int i = 0; i < L::TASKS; ++i) pk[i] = pages[group_key(key_of(n), kgroup(i)) >> shift];
+            pv = pages[group_key(key_of(n - 1), vgroup) >> shift];
         };
         auto request = [&](int n) {
-            uint32_t ti = tid;
-            asm volatile("" : "+v"(ti));
-            const int j0 = key_of(n);
 #pragma unroll
             for (int i = 0; i < L::TASKS; ++i) {
-                const uint32_t r = ti / (D / 8) + i * KSTEP;
-                const uint32_t at = (uint32_t)j0 + (j0 + (int)(r & ~15u) < len ? r : r & 15u);
-                const int64_t row = ((int64_t)(sound(pk[i]) * (uint32_t)KVH + (uint32_t)g) << shift) + (at & (uint32_t)(ps - 1));
-                sk[i] = load8<T>(static_cast<const T*>(c.k) + (row << LOG_D) + ti % (D / 8) * 8);
+                const int at = group_key(key_of(n), kgroup(i)) & (ps - 1);
+                const int64_t row = ((int64_t)(sound(pk[i]) * (uint32_t)KVH + (uint32_t)g) << shift) + at;
+                sk[i] = load8<T>(static_cast<const T*>(c.k) + (row << LOG_D) +
+                                 (klane + (KSTEP == 8 ? i % 2 * 8 * D : 0)));
             }
-            const int i0 = key_of(n - 1);
-            const uint32_t ch = ti % (U / 8);
-            const uint32_t at = (uint32_t)i0 + (i0 + (int)(ch / 2 * 16) < len ? 8 * ch : 8 * (ch & 1));
-            const int64_t row = ((int64_t)(sound(pv) * (uint32_t)KVH + (uint32_t)g) << LOG_D) + ti / (U / 8);
-            const T* from = static_cast<const T*>(c.v) + (row << shift) + (at & (uint32_t)(ps - 1));
+            const int at = group_key(key_of(n - 1), vgroup) & (ps - 1);
+            const int64_t row = (int64_t)(sound(pv) * (uint32_t)KVH + (uint32_t)g) << LOG_D;
+            const T* from = static_cast<const T*>(c.v) + (row << shift) + at;
 #pragma unroll
-            for (int i = 0; i < L::TASKS; ++i) sv[i] = load8<T>(from + ((int64_t)(i * VSTEP) << shift));
+            for (int i = 0; i < L::TASKS; ++i) sv[i] = load8<T>(from + ((int64_t)(32 * i) << shift) + vlane);
         };
         auto store = [&](int n) {
-            uint32_t ti = tid;
-            asm volatile("" : "+v"(ti));
             uint8_t* buf = lds + n % GR * L::PAIR;
 #pragma unroll
             for (int i = 0; i < L::TASKS; ++i) {
-                const uint32_t r = ti / (D / 8) + i * KSTEP;
                 u32x4 p[P::K];
                 split_k<T>(sk[i], p);
+                // (a chunk step of 8 rows turns bit 3 of the slot)
+                const uint32_t at = (KSTEP == 8 && i % 2 ? kto ^ 128 : kto) + i * KSTEP * L::KROW;
 #pragma unroll
-                for (int x = 0; x < P::K; ++x)
-                    *reinterpret_cast<u32x4*>(buf + L::K + x * L::PLANE + r * L::KROW +
-                                              L::kslot(r, ti % (D / 8)) * 16) = p[x];
+                for (int x = 0; x < P::K; ++x) *reinterpret_cast<u32x4*>(buf + L::K + x * L::PLANE + at) = p[x];
             }
-            const int left = len - key_of(n - 1) - (int)(ti % (U / 8) * 8);  // keys of the chunk and on
-            if (__any(left < 8)) {  // past the sequence's end a page holds anything
+            const int left = len - key_of(n - 1);  // keys of the visit and on
+            if (left < U) {                        // past the sequence's end a page holds anything
                 constexpr int E = 4 / sizeof(T);
+                const int mine = left - 16 * vgroup - 8 * (lane & 1);
 #pragma unroll
                 for (int i = 0; i < L::TASKS; ++i)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         uint32_t& w = reinterpret_cast<uint32_t*>(&sv[i])[e / E];
                         const uint32_t keep = E == 1 ? 0u : e % 2 ? 0xFFFFu : 0xFFFF0000u;
-                        w = e >= left ? w & keep : w;
+                        w = e >= mine ? w & keep : w;
                     }
             }
 #pragma unroll
             for (int i = 0; i < L::TASKS; ++i) {
-                const uint32_t d = ti / (U / 8) + i * VSTEP;
                 u32x4 p[P::K];
                 split_k<T>(sv[i], p);
 #pragma unroll
                 for (int x = 0; x < P::K; ++x)
-                    *reinterpret_cast<u32x4*>(buf + L::V + x * L::PLANE + d * L::VROW +
-                                              L::vslot(d, ti % (U / 8)) * 16) = p[x];
+                    *reinterpret_cast<u32x4*>(buf + L::V + x * L::PLANE + vto + 32 * i * L::VROW) = p[x];
             }
+        };
+        auto stage = [&](int n) {
+            store(n);
+            request(n + 1);
+            read_pages(n + 2);
         };
         read_pages(0);
         request(0);
@@ -970,16 +970,47 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
         __syncthreads();  // (the item before is done with the LDS)
         if (tid == 0) flags[0] = 0;
         float inv = 1.0f;
-        if (any) {
+        {
+            // dimensions 16 b + 8 hf .. and their partners D / 2 on, every load before its use
+            const int64_t row = first + myrow / G;
+            const float* x = a.qkv + row * a.qstride + (int64_t)(g * G + myrow % G) * D + 8 * hf;
+            const float2* turn = a.turn + row * (D / 2) + 8 * hf;
+            const float scale = kLog2e / sqrtf((float)D);
+            f32x8 r[NB];
+            constexpr int PART = 2;
+#pragma unroll
+            for (int b0 = 0; b0 < NB / 2; b0 += PART) {
+                f32x4 u[PART][2], w[PART][2], z[PART][4];
+#pragma unroll
+                for (int b = 0; b < PART; ++b) {
+                    const float* xb = x + 16 * (b0 + b);
+                    const f32x4* zb = reinterpret_cast<const f32x4*>(turn + 16 * (b0 + b));
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        u[b][k] = reinterpret_cast<const f32x4*>(xb)[k];
+                        w[b][k] = reinterpret_cast<const f32x4*>(xb + D / 2)[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) z[b][k] = zb[k];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int b = 0; b < PART; ++b)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float uu = u[b][j / 4][j % 4], ww = w[b][j / 4][j % 4];
+                        const float cs = z[b][j / 2][j % 2 * 2], sn = z[b][j / 2][j % 2 * 2 + 1];
+                        r[b0 + b][j] = (uu * cs - ww * sn) * scale;
+                        r[b0 + b + NB / 2][j] = (uu * sn + ww * cs) * scale;
+                    }
+            }
             float up = 1.0f;
             if (std::is_same_v<T, f16_t>) {
                 float amax = 0.0f;
-#pragma unroll 2
-                for (int b = 0; b < NB; ++b) {
-                    const f32x8 v = rotated8<D>(a, first, g, myrow, 16 * b + 8 * hf);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
-                }
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(r[b][j]));
                 amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
                 const float2 sc = row_scale(amax);
                 up = sc.x;
@@ -987,14 +1018,12 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                f32x8 v = rotated8<D>(a, first, g, myrow, 16 * b + 8 * hf);
-                if (std::is_same_v<T, f16_t>) v *= up;
+                if (std::is_same_v<T, f16_t>) r[b] *= up;
                 u32x4 p[P::Q];
-                split_q<T>(v, p);
+                split_q<T>(r[b], p);
 #pragma unroll
                 for (int i = 0; i < L::QREGS; ++i) q[i][b] = p[i];
                 if (L::kQl) ql[b * 64] = p[P::Q - 1];
-                if (b % 2) __builtin_amdgcn_sched_barrier(0);
             }
         }
         float ref = -INFINITY, l = 0.0f;
@@ -1004,83 +1033,61 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
 
-        store(0);
-        request(1);
-        read_pages(2);
+        stage(0);
         __syncthreads();
-        if (grp == 1) {  // (its half of pair 1, while the first group's first products run)
-            store(1);
-            request(2);
-            read_pages(3);
-            __syncthreads();
-        }
-        bool some = false;  // the visit has keys that some row of the wave sees
-        u32x4 p[NG][2][P::Q];
-        for (int n = 0; n <= it.nv; ++n) {
+        if (grp == 1) __syncthreads();
+        // s = q k of visit n: operands read ahead of the MFMAs of the block before (chunk 2 b + hf of a
+        // row: the swizzle is an XOR, so b's bits can be turned last).  Every wave forms all its
+        // products, seen or not: the phase lasts as long as the longest wave's.
+        f32x16 s[NG];
+        auto scores = [&](int n) {
             const uint8_t* buf = lds + n % GR * L::PAIR;
-            uint32_t ka = kat, va = vat;  // (opaque: no address is kept across visits)
-            asm volatile("" : "+v"(ka), "+v"(va));
-            if (some) {
-                // step i: dimensions 32 (i % OT) .., keys of MFMA i / OT; operands read ahead of the MFMAs
-                // of the step before (chunk 2 (i / OT) + hf: the swizzle is an XOR, turned last)
-                u32x4 vp[2][P::K];
-                auto read = [&](int i) {
+            uint32_t ka = kat;  // (opaque: no address is kept across visits, nor 32 zeros)
+            float zero = 0.0f;
+            asm volatile("" : "+v"(ka), "+v"(zero));
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[u][e] = zero;
+            u32x4 kp[2][NG][P::K], qx[2];
+            auto read = [&](int b) {
+#pragma unroll
+                for (int u = 0; u < NG; ++u)
 #pragma unroll
                     for (int x = 0; x < P::K; ++x)
-                        vp[i % 2][x] = *reinterpret_cast<const u32x4*>(
-                            buf + L::V + x * L::PLANE + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
-                };
-                read(0);
+                        kp[b % 2][u][x] = *reinterpret_cast<const u32x4*>(
+                            buf + L::K + x * L::PLANE + 32 * u * L::KROW + (ka ^ 32 * b));
+                if (L::kQl) qx[b % 2] = ql[b * 64];
+            };
+            read(0);
 #pragma unroll
-                for (int i = 0; i < 2 * NG * OT; ++i) {
-                    if (i + 1 < 2 * NG * OT) read(i + 1);
-                    __builtin_amdgcn_sched_barrier(0);
+            for (int b = 0; b < NB; ++b) {
+                if (b + 1 < NB) read(b + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int x = 0; x < P::N; ++x)
-                        o[i % OT] = mfma32<T>(vp[i % 2][P::ki[x]], p[i / OT / 2][i / OT % 2][P::qi[x]], o[i % OT]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                for (int x = 0; x < P::N; ++x)
+#pragma unroll
+                    for (int u = 0; u < NG; ++u) {
+                        const u32x4 y = P::qi[x] < L::QREGS ? q[P::qi[x] < L::QREGS ? P::qi[x] : 0][b] : qx[b % 2];
+                        s[u] = mfma32<T>(kp[b % 2][u][P::ki[x]], y, s[u]);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (n == it.nv) break;
+        };
+        if (GR == 2) stage(1);
+        scores(0);
+        __syncthreads();  // the first matrix phase ends
+        for (int n = 0;; ++n) {
             const int j0 = vis.key(it.v0 + n);
-            some = any && j0 <= wmax && (a.window == 0 || j0 + U - 1 > wmin - a.window || j0 < a.sinks);
-            f32x16 s[NG];
-            if (some) {
-                u32x4 kp[2][NG][P::K], qx[2];
-                auto read = [&](int b) {
-#pragma unroll
-                    for (int u = 0; u < NG; ++u)
-#pragma unroll
-                        for (int x = 0; x < P::K; ++x)
-                            kp[b % 2][u][x] = *reinterpret_cast<const u32x4*>(
-                                buf + L::K + x * L::PLANE + 32 * u * L::KROW + (ka ^ 32 * b));
-                    if (L::kQl) qx[b % 2] = ql[b * 64];
-                };
-                read(0);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if (b + 1 < NB) read(b + 1);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int x = 0; x < P::N; ++x)
-#pragma unroll
-                        for (int u = 0; u < NG; ++u) {
-                            const f32x16 zero = {};
-                            const u32x4 y = P::qi[x] < L::QREGS ? q[P::qi[x] < L::QREGS ? P::qi[x] : 0][b] : qx[b % 2];
-                            s[u] = mfma32<T>(kp[b % 2][u][P::ki[x]], y, b + x == 0 ? zero : s[u]);
-                        }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-            __syncthreads();  // the matrix phase ends
-            if (some) {
+            u32x4 p[NG][2][P::Q];
+            {
                 float top = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
                     const int ju = j0 + 32 * u;
-                    const bool whole = ju + 31 <= wmin &&
-                                       (a.window == 0 || ju > wmax - a.window || ju + 32 <= a.sinks);
-                    if (!whole) {
+                    const bool all = ju + 31 <= wmin &&
+                                     (a.window == 0 || ju > wmax - a.window || ju + 32 <= a.sinks);
+                    if (!all) {
                         const int at = ppos - ju - 8 * hf, far = a.window > 0 ? at - a.window : INT_MIN;
                         const int sk0 = a.sinks - ju - 8 * hf;
 #pragma unroll
@@ -1117,11 +1124,35 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                         split_w<T>(w, p[u][k]);
                     }
             }
-            const int next = n + 1 + (GR == 2 ? grp : 0);
-            store(next);
-            request(next + 1);
-            read_pages(next + 2);
+            if (GR == 1) stage(n + 1);
             __syncthreads();  // the vector phase ends
+            {
+                // o += p v of visit n.  Step i: dimensions 32 (i % OT) .., keys of MFMA i / OT
+                const uint8_t* buf = lds + (n + 1) % GR * L::PAIR;
+                uint32_t va = vat;
+                asm volatile("" : "+v"(va));
+                u32x4 vp[2][P::K];
+                auto read = [&](int i) {
+#pragma unroll
+                    for (int x = 0; x < P::K; ++x)
+                        vp[i % 2][x] = *reinterpret_cast<const u32x4*>(
+                            buf + L::V + x * L::PLANE + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
+                };
+                read(0);
+#pragma unroll
+                for (int i = 0; i < 2 * NG * OT; ++i) {
+                    if (i + 1 < 2 * NG * OT) read(i + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int x = 0; x < P::N; ++x)
+                        o[i % OT] = mfma32<T>(vp[i % 2][P::ki[x]], p[i / OT / 2][i / OT % 2][P::qi[x]], o[i % OT]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (n + 1 == it.nv) break;
+            if (GR == 2) stage(n + 2);  // (the buffer's pair before is read by both groups)
+            scores(n + 1);
+            __syncthreads();  // the matrix phase ends
         }
         if (GR == 2) {  // (both groups pass 2 nv + 2 barriers from the first pair on)
             __syncthreads();
@@ -1131,7 +1162,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
         __syncthreads();
 
         const bool whole = it.S == 1;
-        const bool mine = any && w0 + col < it.rows;
+        const bool mine = w0 + col < it.rows;
         l += __shfl_xor(l, 32, 64);
         const float inv_l = 1.0f / l;
         float chk = l * 0.0f;
@@ -1272,7 +1303,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv c, PageTable t
         while (share * 2 * rows <= N) share *= 2;
         const int per = N / share;  // rows at a time
         const int part = sub % share;
-        const int64_t first = t.cu[sp.entry];
+        const int64_t first = sp.first;
         for (int rb = 0; rb < rows; rb += per) {
             const int r = rb + sub / share;
             const bool live = r < rows;
