@@ -853,6 +853,12 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
     constexpr int LOG_D = D == 64 ? 6 : D == 128 ? 7 : 8;
     constexpr int KSTEP = NT * 8 / D, KROWS = 512 / D;  // keys between a thread's chunks, keys of a wave's
     constexpr int VGROUPS = U / 16;
+    // Staging goes with the shorter phase.  A buffer's pair m - 2 was last read in the second group's
+    // matrix phase m - 2, so either group may store its share of pair m in the two phases after:
+    // its matrix phase m - 1, or the vector phase m - 1 (m - 2 in the second group).  Measured
+    // (f16): at hd 128 a matrix phase takes 2330 cycles, a vector phase 1290 and staging 780; at hd
+    // 64 1350, 1600 and 600.
+    constexpr bool kStageEarly = GR == 2 && D == 64 && sizeof(T) == 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
     const int tid = threadIdx.x, lane = tid & 63;
@@ -1035,7 +1041,10 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 
         stage(0);
         __syncthreads();
-        if (grp == 1) __syncthreads();
+        if (grp == 1) {  // (a phase behind)
+            if (!kStageEarly) stage(1);
+            __syncthreads();
+        }
         // s = q k of visit n: operands read ahead of the MFMAs of the block before (chunk 2 b + hf of a
         // row: the swizzle is an XOR, so b's bits can be turned last).  Every wave forms all its
         // products, seen or not: the phase lasts as long as the longest wave's.
@@ -1074,7 +1083,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        if (GR == 2) stage(1);
+        if (kStageEarly) stage(1);
         scores(0);
         __syncthreads();  // the first matrix phase ends
         for (int n = 0;; ++n) {
@@ -1124,7 +1133,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                         split_w<T>(w, p[u][k]);
                     }
             }
-            if (GR == 1) stage(n + 1);
+            if (!kStageEarly) stage(GR == 2 ? n + 1 + grp : n + 1);
             __syncthreads();  // the vector phase ends
             {
                 // o += p v of visit n.  Step i: dimensions 32 (i % OT) .., keys of MFMA i / OT
@@ -1150,7 +1159,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                 }
             }
             if (n + 1 == it.nv) break;
-            if (GR == 2) stage(n + 2);  // (the buffer's pair before is read by both groups)
+            if (kStageEarly) stage(n + 2);
             scores(n + 1);
             __syncthreads();  // the matrix phase ends
         }
