@@ -1077,6 +1077,10 @@ int unillm_hip_paged_kv_create(int kv_type, int64_t n_kv_heads, int64_t head_dim
         return fail(UNILLM_ERR_INVALID_ARG,
                     "paged KV cache: need n_kv_heads >= 1, head_dim 64 / 128 / 256, rope_theta > 0");
     if (int rc = page_layout(1, 1, n_pages, page_size, 1, &l)) return rc;
+    if (n_kv_heads * page_size * head_dim > (int64_t)INT32_MAX || n_pages * n_kv_heads > (int64_t)INT32_MAX)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    "paged KV cache: need n_kv_heads * page_size * head_dim and n_pages * n_kv_heads "
+                    "below 2^31");
     if ((k_dev == nullptr) != (v_dev == nullptr) || !aligned16(k_dev) || !aligned16(v_dev))
         return fail(UNILLM_ERR_INVALID_ARG,
                     "paged KV cache: give both of k and v, 16-byte aligned, or neither");

@@ -92,7 +92,7 @@ struct Call {
         int tile_rows;  // most query rows of a tile
         int target;     // pieces to deal the kind's work out in, over all kv heads
         int least;      // visits of the smallest piece
-        int row0, most_rows;  // its partial rows
+        int row0;       // its first partial row
         int* head;      // [0] items, [1] splits
         Item* items;
         Split* splits;
@@ -157,13 +157,13 @@ __device__ __forceinline__ int2 block_scan2(int2 v, int2* tmp) {
 
 // Deals one kind's work out (one workgroup): every entry's rows in equal tiles, every tile's visits of
 // U keys in equal pieces of at most C, where C makes the kind's target of pieces over all kv
-// heads.  An entry's last tile, whose rows see the most keys, is dealt out first.
+// heads.
 // sm: LDS, tp[B + 1] (tiles before each entry) | m[B] | ctx[B].
 template <int U>
 __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     __shared__ int2 tmp[4];
-    __shared__ float part[4];
-    __shared__ int off[257], info[256][6], last[2];
+    __shared__ long long part[4];
+    __shared__ int off[257], info[256][7], last[6];
     const Call::Kind& kd = a.kind[kind];
     const int tid = threadIdx.x, B = t.counts[kPagesEntries], TR = kd.tile_rows;
     int *tp = sm, *ms = tp + B + 1, *ctxs = ms + B;
@@ -196,41 +196,66 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         // (wide: in whole waves of 32 rows; no tile comes out empty, as rows > (tiles - 1) TR)
         const int rows = ms[lo] * a.G, n = tp[lo + 1] - tp[lo];
         const int each = kind == kNarrow ? TR : ((rows + n - 1) / n + 31) / 32 * 32;
-        Tile x{lo, (tp[lo + 1] - 1 - i) * each, 0, 0};
+        Tile x{lo, (tp[lo + 1] - 1 - i) * each, 0, 0};  // (an entry's last, which sees the most keys, first)
         x.rows = min(each, rows - x.row0);
         x.nv = Visits<U>(ctxs[lo] + x.row0 / a.G, ctxs[lo] + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks).count;
         return x;
     };
-    float sum = 0.0f;  // (as a float: it is only divided by)
-    for (int i = tid; i < tiles; i += 256) sum += (float)tile(i).nv;
-    sum = wave_add(sum);
+    long long sum = 0;
+    for (int i = tid; i < tiles; i += 256) sum += tile(i).nv;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if ((tid & 63) == 0) part[tid >> 6] = sum;
     __syncthreads();
-    const float all = (part[0] + part[1]) + (part[2] + part[3]);
-    const int C = max(kd.least, (int)ceilf(all * (float)a.KVH / (float)kd.target));
-    int items = 0, splits = 0, rows = 0;
+    sum = part[0] + part[1] + part[2] + part[3];
+    // (exact: the lists' and the partial rows' room is what this C can need)
+    const int C = max(kd.least, (int)((sum * a.KVH + kd.target - 1) / kd.target));
+    // Pieces in order of their size, in quarters of C, the largest first (and a tile's neighbours
+    // beside it, whose keys are the same): what is dealt out last fills the gaps.
+    __shared__ int count[4];
+    if (tid < 4) count[tid] = 0;
+    __syncthreads();
+    auto pieces = [&](int nv) { return (nv + C - 1) / C; };
+    auto rank = [&](int nv, int S) { return 3 - min(3, 4 * (nv / S) / C); };
+    for (int i = tid; i < tiles; i += 256) {
+        const int nv = tile(i).nv, S = pieces(nv);
+        atomicAdd(&count[rank(nv, S)], S);
+    }
+    __syncthreads();
+    int fill[4] = {0, count[0], count[0] + count[1], count[0] + count[1] + count[2]};
+    if (tid == 0) kd.head[0] = fill[3] + count[3];
+    int splits = 0, rows = 0;
     for (int i0 = 0; i0 < tiles; i0 += 256) {
         const int i = i0 + tid;
         Tile x{0, 0, 0, 0};
         int S = 0;
         if (i < tiles) {
             x = tile(i);
-            S = (x.nv + C - 1) / C;
+            S = pieces(x.nv);
         }
         const int want = S > 1 ? S * a.KVH * x.rows : 0;
         const int2 r = block_scan2(make_int2(want, S > 1 ? 1 : 0), tmp);
-        const int base = rows + r.x - want;
-        if (S > 1 && base + want > kd.most_rows) S = 1;  // (no room: whole)
         const int2 n = block_scan2(make_int2(S, 0), tmp);
+        const int rk = S > 0 ? rank(x.nv, S) : 0;
+        const int2 n01 = block_scan2(make_int2(rk == 0 ? S : 0, rk == 1 ? S : 0), tmp);
+        const int2 n23 = block_scan2(make_int2(rk == 2 ? S : 0, rk == 3 ? S : 0), tmp);
+        const int upto[4] = {n01.x, n01.y, n23.x, n23.y};
+        int at = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (rk == e) at = fill[e] + upto[e] - S;
+        const int base = rows + r.x - want;
         off[tid + 1] = n.x;
         if (tid == 0) off[0] = 0;
         if (tid == 255) {
             last[0] = r.y;
             last[1] = r.x;
-        }
-        const int v[6] = {x.b, x.row0, x.rows, x.nv, kd.row0 + base, S};
 #pragma unroll
-        for (int e = 0; e < 6; ++e) info[tid][e] = v[e];
+            for (int e = 0; e < 4; ++e) last[2 + e] = upto[e];
+        }
+        const int v[7] = {x.b, x.row0, x.rows, x.nv, kd.row0 + base, S, at};
+#pragma unroll
+        for (int e = 0; e < 7; ++e) info[tid][e] = v[e];
         if (want) kd.splits[splits + r.y - 1] = {t.cu[x.b], x.row0, x.rows, kd.row0 + base, S, {}};
         __syncthreads();
         for (int k = tid; k < off[256]; k += 256) {
@@ -244,17 +269,15 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
             const int s = k - off[lo], nv = w[3], Sw = w[5];
             const int v0 = (int)((int64_t)s * nv / Sw), v1 = (int)((int64_t)(s + 1) * nv / Sw);
             const int b = w[0], ctx = ctxs[b];
-            kd.items[items + k] = {t.cu[b], ctx, ctx + ms[b], t.step_ids[b], w[1], w[2], v0, v1 - v0, w[4], s, Sw, 0};
+            kd.items[w[6] + s] = {t.cu[b], ctx, ctx + ms[b], t.step_ids[b], w[1], w[2], v0, v1 - v0, w[4], s, Sw, 0};
         }
-        items += off[256];
         splits += last[0];
         rows += last[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) fill[e] += last[2 + e];
         __syncthreads();
     }
-    if (tid == 0) {
-        kd.head[0] = items;
-        kd.head[1] = splits;
-    }
+    if (tid == 0) kd.head[1] = splits;
 }
 
 // The first kernel of a call.  Workgroups 0 and 1 deal the work out; each other one takes 16 rows
@@ -824,6 +847,13 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 x, u32x4 y, f32x16 z) {
                                                        __builtin_bit_cast(bf16x8, y), z, 0, 0, 0);
 }
 
+// the wave's LDS stores before its reads after them
+__device__ __forceinline__ void settle_wave() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <class T, int D>
 struct WideLds {
     static constexpr int GR = kGroups<T, D>, NT = 256 * GR;
@@ -834,7 +864,9 @@ struct WideLds {
     static constexpr int QL = GR * PAIR;                    // q's last part, where registers lack
     static constexpr bool kQl = sizeof(T) == 2 && D == 128;
     static constexpr int QREGS = Parts<T>::Q - (kQl ? 1 : 0);
-    static constexpr int STAT = QL + (kQl ? NT / 64 * (D / 16) * 1024 : 0);  // whether a page is bad
+    static constexpr int QROWS = 32 * D * 4;                // a wave's rows in f32, before and after
+    static constexpr int USED = QL + (kQl ? NT / 64 * (D / 16) * 1024 : 0), ROWS = NT / 64 * QROWS;
+    static constexpr int STAT = USED > ROWS ? USED : ROWS;  // whether a page is bad
     static constexpr int BYTES = STAT + 64;
     static constexpr int TASKS = U * D / 8 / NT;            // 8-element chunks of K (or V) a thread
     __device__ static uint32_t kslot(uint32_t r, uint32_t c) {
@@ -853,12 +885,11 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
     constexpr int LOG_D = D == 64 ? 6 : D == 128 ? 7 : 8;
     constexpr int KSTEP = NT * 8 / D, KROWS = 512 / D;  // keys between a thread's chunks, keys of a wave's
     constexpr int VGROUPS = U / 16;
-    // Staging goes with the shorter phase.  A buffer's pair m - 2 was last read in the second group's
-    // matrix phase m - 2, so either group may store its share of pair m in the two phases after:
-    // its matrix phase m - 1, or the vector phase m - 1 (m - 2 in the second group).  Measured
-    // (f16): at hd 128 a matrix phase takes 2330 cycles, a vector phase 1290 and staging 780; at hd
-    // 64 1350, 1600 and 600.
-    constexpr bool kStageEarly = GR == 2 && D == 64 && sizeof(T) == 2;
+    // A buffer's pair m - 2 was last read in the second group's matrix phase m - 2, so either group may
+    // store its share of pair m in the two phases after: its matrix phase m - 1, or the vector
+    // phase m - 1 (m - 2 in the second group).  The stores go with the shorter phase (f16: at hd 128
+    // a matrix phase takes 2330 cycles, the weights 1290; at hd 64 1350 and 1600).
+    constexpr bool kStoreEarly = GR == 2 && D == 64 && sizeof(T) == 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
     const int tid = threadIdx.x, lane = tid & 63;
@@ -894,43 +925,65 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 
         // Staging.  A wave's chunks of K are 8 dimensions of keys kr0 + i KSTEP of the visit each, of V 8
         // keys of dimensions vd0 + 32 i, all chunk i of one group of 16 keys and so of one page:
-        // addresses are a uniform base and the lane's fixed offset.  A page id is read a visit ahead
-        // of its request, that a visit ahead of its use.  Past the item's ends the nearest visit is
+        // addresses are a uniform base and the lane's fixed offset.  A page id is read a pair ahead
+        // of its request, that a pair ahead of its store.  Past the item's ends the nearest visit is
         // staged again, unused: with no branch around a load the waits count only what they need.
         Raw<T> sk[L::TASKS], sv[L::TASKS];
         int pk[L::TASKS], pv;
         bool bad_id = false;
         auto key_of = [&](int n) { return vis.key(it.v0 + max(0, min(n, it.nv - 1))); };
+        // the keys of visits m - 1, m and m + 1 where pair m (V of m - 1, K of m) is fetched next, and
+        // of V's visit in the pair fetched last
+        int k0 = key_of(-1), k1 = key_of(0), k2 = key_of(1), kstored = k0;
         // (past the sequence: the visit's first group again)
         auto group_key = [&](int j0, int grp16) { return j0 + 16 * grp16 < len ? j0 + 16 * grp16 : j0; };
-        auto sound = [&](int page) {  // (looked at when it is used: its load has a visit to arrive in)
+        auto sound = [&](int page) {  // (looked at when it is used: its load has a pair to arrive in)
             const uint32_t pg = (uint32_t)__builtin_amdgcn_readfirstlane(page);
-            const bool bad = pg >= (uint32_t)c.n_pages;
-            bad_id |= bad;
-            return bad ? 0u : pg;
+            bad_id |= pg >= (uint32_t)c.n_pages;
+            return min(pg, (uint32_t)c.n_pages - 1);
         };
         auto kgroup = [&](int i) { return (wv * KROWS + i * KSTEP) / 16; };
-        auto read_pages = [&](int n) {  // of pair n: V of visit n - 1, K of visit n
+        const T* kbase = static_cast<const T*>(c.k) + ((int64_t)g << (shift + LOG_D));
+        const T* vbase = static_cast<const T*>(c.v) + ((int64_t)g << (shift + LOG_D));
+        const uint32_t page_elems = (uint32_t)KVH << (shift + LOG_D);
+        auto read_pages = [&](int jk, int jv) {
 #pragma unroll
-            for (int i = 0; i < L::TASKS; ++i) pk[i] = pages[group_key(key_of(n), kgroup(i)) >> shift];
-            pv = pages[group_key(key_of(n - 1), vgroup) >> shift];
+            for (int i = 0; i < L::TASKS; ++i) pk[i] = pages[group_key(jk, kgroup(i)) >> shift];
+            pv = pages[group_key(jv, vgroup) >> shift];
         };
-        auto request = [&](int n) {
-#pragma unroll
-            for (int i = 0; i < L::TASKS; ++i) {
-                const int at = group_key(key_of(n), kgroup(i)) & (ps - 1);
-                const int64_t row = ((int64_t)(sound(pk[i]) * (uint32_t)KVH + (uint32_t)g) << shift) + at;
-                sk[i] = load8<T>(static_cast<const T*>(c.k) + (row << LOG_D) +
-                                 (klane + (KSTEP == 8 ? i % 2 * 8 * D : 0)));
-            }
-            const int at = group_key(key_of(n - 1), vgroup) & (ps - 1);
-            const int64_t row = (int64_t)(sound(pv) * (uint32_t)KVH + (uint32_t)g) << LOG_D;
-            const T* from = static_cast<const T*>(c.v) + (row << shift) + at;
-#pragma unroll
-            for (int i = 0; i < L::TASKS; ++i) sv[i] = load8<T>(from + ((int64_t)(32 * i) << shift) + vlane);
+        auto fetch_k = [&](int i) {
+            const uint32_t at = (uint32_t)group_key(k1, kgroup(i)) & (uint32_t)(ps - 1);
+            sk[i] = load8<T>(kbase + ((uint64_t)sound(pk[i]) * page_elems + (at << LOG_D)) +
+                             (klane + (KSTEP == 8 ? i % 2 * 8 * D : 0)));
         };
-        auto store = [&](int n) {
-            uint8_t* buf = lds + n % GR * L::PAIR;
+        auto fetch_v = [&] {
+            const uint32_t at = (uint32_t)group_key(k0, vgroup) & (uint32_t)(ps - 1);
+            const T* from = vbase + ((uint64_t)sound(pv) * page_elems + at);
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) sv[i] = load8<T>(from + (32 * i << shift) + vlane);
+        };
+        auto fetch_pages = [&](int m) {  // of pair m + 1, after pair m's requests
+            read_pages(k2, k1);
+            kstored = k0;
+            k0 = k1;
+            k1 = k2;
+            k2 = key_of(m + 2);
+        };
+        // pair m in four pieces, to go between MFMAs
+        auto fetch_piece = [&](int m, int piece) {
+            constexpr int HALF_T = (L::TASKS + 1) / 2;
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i)
+                if (piece == (i < HALF_T ? 0 : 1)) fetch_k(i);
+            if (piece == 2) fetch_v();
+            if (piece == 3) fetch_pages(m);
+        };
+        auto fetch = [&](int m) {
+#pragma unroll
+            for (int piece = 0; piece < 4; ++piece) fetch_piece(m, piece);
+        };
+        auto store = [&](int m) {
+            uint8_t* buf = lds + m % GR * L::PAIR;
 #pragma unroll
             for (int i = 0; i < L::TASKS; ++i) {
                 u32x4 p[P::K];
@@ -940,8 +993,8 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 #pragma unroll
                 for (int x = 0; x < P::K; ++x) *reinterpret_cast<u32x4*>(buf + L::K + x * L::PLANE + at) = p[x];
             }
-            const int left = len - key_of(n - 1);  // keys of the visit and on
-            if (left < U) {                        // past the sequence's end a page holds anything
+            const int left = len - kstored;  // keys of V's visit and on
+            if (left < U) {                  // past the sequence's end a page holds anything
                 constexpr int E = 4 / sizeof(T);
                 const int mine = left - 16 * vgroup - 8 * (lane & 1);
 #pragma unroll
@@ -962,54 +1015,62 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                     *reinterpret_cast<u32x4*>(buf + L::V + x * L::PLANE + vto + 32 * i * L::VROW) = p[x];
             }
         };
-        auto stage = [&](int n) {
-            store(n);
-            request(n + 1);
-            read_pages(n + 2);
-        };
-        read_pages(0);
-        request(0);
-        read_pages(1);
+        read_pages(k1, k0);
+        fetch(0);
 
         u32x4 q[L::QREGS][NB];
         u32x4* ql = reinterpret_cast<u32x4*>(lds + L::QL) + wv * NB * 64 + lane;
         __syncthreads();  // (the item before is done with the LDS)
         if (tid == 0) flags[0] = 0;
         float inv = 1.0f;
+        // The wave's rows of q and of their rotations come whole rows at a time and through its own
+        // part of the LDS: a lane's operand is 32 bytes of a row, and loaded so every request would
+        // touch 32 lines (22000 cycles an item at hd 128 before, of 115000).
+        u32x4 qlast[L::kQl ? NB : 1];
         {
-            // dimensions 16 b + 8 hf .. and their partners D / 2 on, every load before its use
-            const int64_t row = first + myrow / G;
-            const float* x = a.qkv + row * a.qstride + (int64_t)(g * G + myrow % G) * D + 8 * hf;
-            const float2* turn = a.turn + row * (D / 2) + 8 * hf;
-            const float scale = kLog2e / sqrtf((float)D);
-            f32x8 r[NB];
-            constexpr int PART = 2;
+            // (opaque lane numbers here and at the end: no address of these is kept through the visits)
+            int el = lane;
+            asm volatile("" : "+v"(el));
+            constexpr int CH = D / 4, N = 32 * CH / 64;  // 16-byte chunks of a row, requests of 32 rows
+            f32x4* own = reinterpret_cast<f32x4*>(lds + wv * L::QROWS);
+            auto slot = [&](int r, int ch) { return r * CH + (ch ^ (r & (CH - 1 < 31 ? CH - 1 : 31))); };
+            f32x4 x[N];
+            // (a lane's own row is `myrow`: its place is handed to the lanes that load it)
+            auto rows = [&](const float* from, int64_t place) {
 #pragma unroll
-            for (int b0 = 0; b0 < NB / 2; b0 += PART) {
-                f32x4 u[PART][2], w[PART][2], z[PART][4];
-#pragma unroll
-                for (int b = 0; b < PART; ++b) {
-                    const float* xb = x + 16 * (b0 + b);
-                    const f32x4* zb = reinterpret_cast<const f32x4*>(turn + 16 * (b0 + b));
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        u[b][k] = reinterpret_cast<const f32x4*>(xb)[k];
-                        w[b][k] = reinterpret_cast<const f32x4*>(xb + D / 2)[k];
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) z[b][k] = zb[k];
-                }
+                for (int i = 0; i < N; ++i)
+                    x[i] = reinterpret_cast<const f32x4*>(from + __shfl(place, (i * 64 + el) / CH, 64))[el % CH];
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int b = 0; b < PART; ++b)
+                for (int i = 0; i < N; ++i) own[slot((i * 64 + el) / CH, el % CH)] = x[i];
+                settle_wave();
+            };
+            f32x8 r[NB];
+            const int64_t myq = first + myrow / G;
+            rows(a.qkv, myq * a.qstride + (int64_t)(g * G + myrow % G) * D);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float uu = u[b][j / 4][j % 4], ww = w[b][j / 4][j % 4];
-                        const float cs = z[b][j / 2][j % 2 * 2], sn = z[b][j / 2][j % 2 * 2 + 1];
-                        r[b0 + b][j] = (uu * cs - ww * sn) * scale;
-                        r[b0 + b + NB / 2][j] = (uu * sn + ww * cs) * scale;
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const f32x4 v = own[slot(el % 32, 4 * b + 2 * (el / 32) + k)];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) r[b][4 * k + j] = v[j];
+                }
+            settle_wave();
+            rows(reinterpret_cast<const float*>(a.turn), myq * D);
+            const float scale = kLog2e / sqrtf((float)D);
+#pragma unroll
+            for (int b = 0; b < NB / 2; ++b)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f32x4 v = own[slot(el % 32, 8 * b + 4 * (el / 32) + k)];  // two (cos, sin)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float uu = r[b][2 * k + j], ww = r[b + NB / 2][2 * k + j];
+                        r[b][2 * k + j] = (uu * v[2 * j] - ww * v[2 * j + 1]) * scale;
+                        r[b + NB / 2][2 * k + j] = (uu * v[2 * j + 1] + ww * v[2 * j]) * scale;
                     }
-            }
+                }
             float up = 1.0f;
             if (std::is_same_v<T, f16_t>) {
                 float amax = 0.0f;
@@ -1029,9 +1090,13 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                 split_q<T>(r[b], p);
 #pragma unroll
                 for (int i = 0; i < L::QREGS; ++i) q[i][b] = p[i];
-                if (L::kQl) ql[b * 64] = p[P::Q - 1];
+                if (L::kQl) qlast[L::kQl ? b : 0] = p[P::Q - 1];
             }
         }
+        __syncthreads();  // (every wave is done with its rows: the buffers and q's last parts go there)
+        if (L::kQl)
+#pragma unroll
+            for (int b = 0; b < (L::kQl ? NB : 0); ++b) ql[b * 64] = qlast[b];
         float ref = -INFINITY, l = 0.0f;
         f32x16 o[OT];
 #pragma unroll
@@ -1039,10 +1104,14 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
 
-        stage(0);
+        store(0);
+        fetch(1);
         __syncthreads();
         if (grp == 1) {  // (a phase behind)
-            if (!kStageEarly) stage(1);
+            if (!kStoreEarly) {
+                store(1);
+                fetch(2);
+            }
             __syncthreads();
         }
         // s = q k of visit n: operands read ahead of the MFMAs of the block before (chunk 2 b + hf of a
@@ -1072,6 +1141,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (b + 1 < NB) read(b + 1);
+                if (kStoreEarly && b % (NB / 4) == 0) fetch_piece(n + 2, b / (NB / 4));
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int x = 0; x < P::N; ++x)
@@ -1083,7 +1153,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        if (kStageEarly) stage(1);
+        if (kStoreEarly) store(1);
         scores(0);
         __syncthreads();  // the first matrix phase ends
         for (int n = 0;; ++n) {
@@ -1133,8 +1203,11 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                         split_w<T>(w, p[u][k]);
                     }
             }
-            if (!kStageEarly) stage(GR == 2 ? n + 1 + grp : n + 1);
+            if (!kStoreEarly) store(n + 1 + grp);
             __syncthreads();  // the vector phase ends
+            // (where the matrix phase is the longer one, its wave goes first on the SIMD: three chunks
+            // among 24 sequences, bf16, 175 us against 181; at hd 64, 225 against 205)
+            if (!kStoreEarly) __builtin_amdgcn_s_setprio(1);
             {
                 // o += p v of visit n.  Step i: dimensions 32 (i % OT) .., keys of MFMA i / OT
                 const uint8_t* buf = lds + (n + 1) % GR * L::PAIR;
@@ -1151,6 +1224,8 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 #pragma unroll
                 for (int i = 0; i < 2 * NG * OT; ++i) {
                     if (i + 1 < 2 * NG * OT) read(i + 1);
+                    // (what is stored next is requested between the first MFMAs after the stores before)
+                    if (!kStoreEarly && i % (NG * OT / 2) == 0) fetch_piece(n + 2 + grp, i / (NG * OT / 2));
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int x = 0; x < P::N; ++x)
@@ -1158,9 +1233,13 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (n + 1 == it.nv) break;
-            if (kStageEarly) stage(n + 2);
+            if (n + 1 == it.nv) {
+                __builtin_amdgcn_s_setprio(0);
+                break;
+            }
+            if (kStoreEarly) store(n + 2);
             scores(n + 1);
+            if (!kStoreEarly) __builtin_amdgcn_s_setprio(0);
             __syncthreads();  // the matrix phase ends
         }
         if (GR == 2) {  // (both groups pass 2 nv + 2 barriers from the first pair on)
@@ -1188,27 +1267,39 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
         bad |= (bool)__shfl_xor((int)bad, 32, 64);  // (both halves of a row)
         const bool bad_page = flags[0] != 0;
         if (bad_page && tid == 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
-        if (mine) {
-            const bool again = !bad_page && bad;
+        const bool again = mine && !bad_page && bad;
+        const int64_t piece = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows;
+        if (mine && hf == 0) {
             const int rr = it.row0 + w0 + col;
-            const int64_t row = first + rr / G;
-            const int h = g * G + rr % G;
-            const int64_t piece = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows + w0 + col;
-            // (a row with a bad page is NaN, whatever its other pieces hold)
-            float* dst = whole || bad_page ? a.out + row * a.ostride + (int64_t)h * D : a.po + piece * D;
-            if (!again)
+            if (again) redo_row(a, first + rr / G, g * G + rr % G);
+            if (!whole) a.ms[piece + w0 + col] = make_float2(ref - P::shift, again || bad_page ? __builtin_nanf("") : l);
+        }
+        // whole rows out, through the wave's part of the LDS (a row with a bad page is NaN, whatever its
+        // other pieces hold)
+        const uint32_t skip = (uint32_t)__ballot(again);
+        constexpr int CH = D / 4, N = 32 * CH / 64;
+        int el = lane;
+        asm volatile("" : "+v"(el));
+        f32x4* own = reinterpret_cast<f32x4*>(lds + wv * L::QROWS);
+        auto slot = [&](int r, int ch) { return r * CH + (ch ^ (r & (CH - 1 < 31 ? CH - 1 : 31))); };
 #pragma unroll
-                for (int i = 0; i < OT; ++i)
+        for (int i = 0; i < OT; ++i)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const f32x4 x = {o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]};
-                        *reinterpret_cast<f32x4*>(dst + 32 * i + 8 * u + 4 * hf) =
-                            bad_page ? f32x4(__builtin_nanf("")) : x;
-                    }
-            if (hf == 0) {
-                if (again) redo_row(a, row, h);
-                if (!whole) a.ms[piece] = make_float2(ref - P::shift, again || bad_page ? __builtin_nanf("") : l);
-            }
+            for (int u = 0; u < 4; ++u)
+                own[slot(el % 32, 8 * i + 2 * u + el / 32)] =
+                    f32x4{o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]};
+        settle_wave();
+        const bool direct = whole || bad_page;
+        float* to = direct ? a.out : a.po;
+        const int64_t place = direct ? (int64_t)(first + myrow / G) * a.ostride + (int64_t)(g * G + myrow % G) * D
+                                     : (piece + w0 + col) * D;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = (i * 64 + el) / CH;
+            float* dst = to + __shfl(place, r, 64) + el % CH * 4;
+            const f32x4 v = own[slot(r, el % CH)];
+            if (w0 + r < it.rows && !(skip >> r & 1))
+                *reinterpret_cast<f32x4*>(dst) = bad_page ? f32x4(__builtin_nanf("")) : v;
         }
     }
 }
@@ -1477,8 +1568,7 @@ hipError_t launch_paged_attention(const PagedKv& c, const unillm_page_table& t, 
            reinterpret_cast<float*>(w + l.po_at), reinterpret_cast<int*>(w + l.count_at),
            reinterpret_cast<int*>(w + l.redo_at), {}};
     for (int k = 0; k < 2; ++k)
-        a.kind[k] = {tile_rows(k, c.head_dim), target_pieces(k), k == kNarrow ? 4 : 2, k == kNarrow ? 0 : (int)l.rows[0],
-                     (int)l.rows[k], reinterpret_cast<int*>(w + l.head_at[k]),
+        a.kind[k] = {tile_rows(k, c.head_dim), target_pieces(k), k == kNarrow ? 4 : 2, k == kNarrow ? 0 : (int)l.rows[0], reinterpret_cast<int*>(w + l.head_at[k]),
                      reinterpret_cast<Item*>(w + l.items_at[k]),
                      reinterpret_cast<Split*>(w + l.splits_at[k])};
     if (c.type == UNILLM_QTYPE_F32) return launch_type<float>(c, t, a, l, s);
