@@ -92,6 +92,7 @@ struct Call {
         int tile_rows;  // most query rows of a tile
         int target;     // pieces to deal the kind's work out in, over all kv heads
         int least;      // visits of the smallest piece
+        int overhead;   // of a piece, in visits
         int row0;       // its first partial row
         int* head;      // [0] items, [1] splits
         Item* items;
@@ -208,15 +209,64 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     if ((tid & 63) == 0) part[tid >> 6] = sum;
     __syncthreads();
     sum = part[0] + part[1] + part[2] + part[3];
-    // (exact: the lists' and the partial rows' room is what this C can need)
-    const int C = max(kd.least, (int)((sum * a.KVH + kd.target - 1) / kd.target));
-    // Pieces in order of their size, in quarters of C, the largest first (and a tile's neighbours
+    // The lists' and the partial rows' room is what this C can need, and a larger one needs less.
+    const int C0 = max(kd.least, (int)((sum * a.KVH + kd.target - 1) / kd.target));
+    // Wide: of C0, 5 / 4, 3 / 2 and 2 C0 and whole tiles the one of the shortest time, in visits: an
+    // item's own time is `overhead` visits, and as much again where its sums go through memory;
+    // items that all have a place take the largest one's time, others the mean place's load
+    // and 3 / 4 of an item more (three chunks among 24 sequences: 155 us with pieces for 3 / 4 of the
+    // places, 188 with a few more pieces than places).
+    int C = C0, longest = INT_MAX;
+    if (kind == kWide && tiles > 0) {
+        constexpr int TRY = 5;
+        __shared__ int made[TRY + 1][4], split_made[TRY][4];
+        auto candidate = [&](int k) { return k == 0 ? C0 : k == 1 ? C0 + C0 / 4 : k == 2 ? C0 + C0 / 2 : k == 3 ? 2 * C0 : INT_MAX / 2; };
+        int m[TRY + 1] = {}, sp[TRY] = {};
+        for (int i = tid; i < tiles; i += 256) {
+            const int nv = tile(i).nv;
+            m[TRY] = max(m[TRY], nv);
+#pragma unroll
+            for (int k = 0; k < TRY; ++k) {
+                const int S = (nv - 1) / candidate(k) + 1;
+                m[k] += S;
+                sp[k] += S > 1 ? S : 0;
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            m[TRY] = max(m[TRY], __shfl_xor(m[TRY], o, 64));
+#pragma unroll
+            for (int k = 0; k < TRY; ++k) m[k] += __shfl_xor(m[k], o, 64), sp[k] += __shfl_xor(sp[k], o, 64);
+        }
+        if ((tid & 63) == 0) {
+            made[TRY][tid >> 6] = m[TRY];
+#pragma unroll
+            for (int k = 0; k < TRY; ++k) made[k][tid >> 6] = m[k], split_made[k][tid >> 6] = sp[k];
+        }
+        __syncthreads();
+        longest = max(max(made[TRY][0], made[TRY][1]), max(made[TRY][2], made[TRY][3]));
+        float least_time = INFINITY;
+#pragma unroll
+        for (int k = 0; k < TRY; ++k) {
+            const float n = (float)(made[k][0] + made[k][1] + made[k][2] + made[k][3]);
+            const float ns = (float)(split_made[k][0] + split_made[k][1] + split_made[k][2] + split_made[k][3]);
+            const float item = (float)(min(candidate(k), longest) + kd.overhead);
+            const float load = ((float)sum + (float)kd.overhead * (n + ns)) * (float)a.KVH / (float)kd.target;
+            const float time = n * (float)a.KVH <= (float)kd.target ? item : fmaxf(item, load + 0.75f * item);
+            if (time < least_time) {
+                least_time = time;
+                C = candidate(k);
+            }
+        }
+    }
+    // Pieces in order of their size, in quarters of the largest, that first (and a tile's neighbours
     // beside it, whose keys are the same): what is dealt out last fills the gaps.
     __shared__ int count[4];
     if (tid < 4) count[tid] = 0;
     __syncthreads();
-    auto pieces = [&](int nv) { return (nv + C - 1) / C; };
-    auto rank = [&](int nv, int S) { return 3 - min(3, 4 * (nv / S) / C); };
+    auto pieces = [&](int nv) { return (nv - 1) / C + 1; };
+    const int top = min(C, longest);
+    auto rank = [&](int nv, int S) { return 3 - min(3, (int)(4 * (int64_t)(nv / S) / top)); };
     for (int i = tid; i < tiles; i += 256) {
         const int nv = tile(i).nv, S = pieces(nv);
         atomicAdd(&count[rank(nv, S)], S);
@@ -437,19 +487,22 @@ __device__ __forceinline__ void split_q(const f32x8& v, u32x4 (&p)[Parts<T>::Q])
     }
 }
 
-// 8 weights -> their parts.  f16: the first part cut off (a mask, exact in f16 but below 2^-14),
-// what is left of up to 2^-10 rounded: 2^-22 of the weight, in either direction, for three
-// instructions a weight where two roundings take four.
+// 8 weights -> their parts.  f16: the first part cut off, what is left of up to 2^-10 rounded:
+// 2^-22 of the weight, in either direction (one conversion a pair, one mixed-precision
+// multiply-add a weight that takes the f16 back out, one conversion a pair).
 template <class T>
 __device__ __forceinline__ void split_w(const f32x8& v, u32x4 (&p)[Parts<T>::Q]) {
     if constexpr (std::is_same_v<T, f16_t>) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float a = __uint_as_float(__float_as_uint(v[2 * j]) & 0xFFFFE000u);
-            const float b = __uint_as_float(__float_as_uint(v[2 * j + 1]) & 0xFFFFE000u);
-            p[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-            p[1][j] = __builtin_bit_cast(
-                uint32_t, __builtin_convertvector(f32x2{v[2 * j] - a, v[2 * j + 1] - b}, f16x2));
+            const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v[2 * j], v[2 * j + 1]));
+            f32x2 lo;  // v - hi, exactly
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]"
+                : "=v"(lo[0]) : "v"(hi), "v"(v[2 * j]));
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+                : "=v"(lo[1]) : "v"(hi), "v"(v[2 * j + 1]));
+            p[0][j] = hi;
+            p[1][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(lo, f16x2));
         }
     } else {
         split_q<T>(v, p);
@@ -1470,9 +1523,9 @@ struct Layout {
     size_t head_at[2], items_at[2], splits_at[2], turn_at, ms_at, po_at, count_at, redo_at, bytes;
 };
 
-// Pieces a kind's work is dealt out in: narrow, four workgroups of four waves for every CU; wide,
+// Pieces a kind's work is dealt out in: narrow, three workgroups of four waves for every CU; wide,
 // the one of eight waves (of four at hd 256) that a CU holds.
-int target_pieces(int kind) { return (kind == kNarrow ? 4 : 1) * device_info().cu_count; }
+int target_pieces(int kind) { return (kind == kNarrow ? 3 : 1) * device_info().cu_count; }
 
 int tile_rows(int kind, int64_t D) { return kind == kNarrow ? kTileRows : D < 256 ? 256 : 128; }
 
@@ -1568,7 +1621,7 @@ hipError_t launch_paged_attention(const PagedKv& c, const unillm_page_table& t, 
            reinterpret_cast<float*>(w + l.po_at), reinterpret_cast<int*>(w + l.count_at),
            reinterpret_cast<int*>(w + l.redo_at), {}};
     for (int k = 0; k < 2; ++k)
-        a.kind[k] = {tile_rows(k, c.head_dim), target_pieces(k), k == kNarrow ? 4 : 2, k == kNarrow ? 0 : (int)l.rows[0], reinterpret_cast<int*>(w + l.head_at[k]),
+        a.kind[k] = {tile_rows(k, c.head_dim), target_pieces(k), k == kNarrow ? 4 : 2, 5, k == kNarrow ? 0 : (int)l.rows[0], reinterpret_cast<int*>(w + l.head_at[k]),
                      reinterpret_cast<Item*>(w + l.items_at[k]),
                      reinterpret_cast<Split*>(w + l.splits_at[k])};
     if (c.type == UNILLM_QTYPE_F32) return launch_type<float>(c, t, a, l, s);
