@@ -211,53 +211,67 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     sum = part[0] + part[1] + part[2] + part[3];
     // The lists' and the partial rows' room is what this C can need, and a larger one needs less.
     const int C0 = max(kd.least, (int)((sum * a.KVH + kd.target - 1) / kd.target));
-    // Wide: of C0, 5 / 4, 3 / 2 and 2 C0 and whole tiles the one of the shortest time, in visits: an
-    // item's own time is `overhead` visits, and as much again where its sums go through memory;
-    // items that all have a place take the largest one's time, others the mean place's load
-    // and 3 / 4 of an item more (three chunks among 24 sequences: 155 us with pieces for 3 / 4 of the
-    // places, 188 with a few more pieces than places).
+    // Wide, few tiles: of C0, 5 / 4, 3 / 2 and 2 C0 and whole tiles the one of the shortest time, in
+    // visits.  An item's own time is `overhead` visits, and as much again where its sums go
+    // through memory.  Up to as many items as places take the largest one's time; up to twice as
+    // many, the sum of an item's and of one that follows it, the sizes sorted: the last to find a
+    // place of its own and the next, or the largest that is followed and the smallest; more, the
+    // mean place's load and half an item.  (Three chunks among 24 sequences, bf16: 152 us with
+    // pieces of 18 visits, 272 for 256 places, whose small ones pair up; 190 with pieces of 30, 216.)
     int C = C0, longest = INT_MAX;
-    if (kind == kWide && tiles > 0) {
-        constexpr int TRY = 5;
-        __shared__ int made[TRY + 1][4], split_made[TRY][4];
+    if (kind == kWide && tiles > 0 && (int64_t)tiles * a.KVH <= 4 * (int64_t)kd.target) {
+        constexpr int TRY = 5, BINS = 32;
+        __shared__ int hist[TRY][BINS], split_made[TRY], top;
+        __shared__ float times[TRY];
+        for (int i = tid; i < TRY * BINS; i += 256) hist[i / BINS][i % BINS] = 0;
+        if (tid < TRY) split_made[tid] = 0;
+        if (tid == 0) top = 0;
+        __syncthreads();
         auto candidate = [&](int k) { return k == 0 ? C0 : k == 1 ? C0 + C0 / 4 : k == 2 ? C0 + C0 / 2 : k == 3 ? 2 * C0 : INT_MAX / 2; };
-        int m[TRY + 1] = {}, sp[TRY] = {};
+        for (int i = tid; i < tiles; i += 256) atomicMax(&top, tile(i).nv);
+        __syncthreads();
+        longest = top;
         for (int i = tid; i < tiles; i += 256) {
             const int nv = tile(i).nv;
-            m[TRY] = max(m[TRY], nv);
-#pragma unroll
             for (int k = 0; k < TRY; ++k) {
                 const int S = (nv - 1) / candidate(k) + 1;
-                m[k] += S;
-                sp[k] += S > 1 ? S : 0;
+                atomicAdd(&hist[k][(int)((int64_t)(nv / S) * (BINS - 1) / longest)], S);
+                if (S > 1) atomicAdd(&split_made[k], S);
             }
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            m[TRY] = max(m[TRY], __shfl_xor(m[TRY], o, 64));
-#pragma unroll
-            for (int k = 0; k < TRY; ++k) m[k] += __shfl_xor(m[k], o, 64), sp[k] += __shfl_xor(sp[k], o, 64);
-        }
-        if ((tid & 63) == 0) {
-            made[TRY][tid >> 6] = m[TRY];
-#pragma unroll
-            for (int k = 0; k < TRY; ++k) made[k][tid >> 6] = m[k], split_made[k][tid >> 6] = sp[k];
         }
         __syncthreads();
-        longest = max(max(made[TRY][0], made[TRY][1]), max(made[TRY][2], made[TRY][3]));
-        float least_time = INFINITY;
+        if (tid < TRY) {
+            const int places = max(1, kd.target / a.KVH);
+            int n = 0;
+            for (int e = 0; e < BINS; ++e) n += hist[tid][e];
+            const float ov = (float)kd.overhead * (1.0f + (float)split_made[tid] / (float)n);
+            const float item = (float)min(candidate(tid), longest) + ov;
+            float time = item;
+            if (n > 2 * places) {
+                time = fmaxf(item, ((float)sum + ov * (float)n) / (float)places + 0.5f * item);
+            } else if (n > places) {
+                // sizes at these ranks, the largest first
+                const int want[4] = {places - 1, places, 2 * places - n, n - 1};
+                float size[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                int seen = 0;
+                for (int e = BINS - 1; e >= 0; --e) {
+                    const int upto = seen + hist[tid][e];
 #pragma unroll
-        for (int k = 0; k < TRY; ++k) {
-            const float n = (float)(made[k][0] + made[k][1] + made[k][2] + made[k][3]);
-            const float ns = (float)(split_made[k][0] + split_made[k][1] + split_made[k][2] + split_made[k][3]);
-            const float item = (float)(min(candidate(k), longest) + kd.overhead);
-            const float load = ((float)sum + (float)kd.overhead * (n + ns)) * (float)a.KVH / (float)kd.target;
-            const float time = n * (float)a.KVH <= (float)kd.target ? item : fmaxf(item, load + 0.75f * item);
-            if (time < least_time) {
-                least_time = time;
+                    for (int q = 0; q < 4; ++q)
+                        if (want[q] >= seen && want[q] < upto) size[q] = (float)e * (float)longest / (float)(BINS - 1);
+                    seen = upto;
+                }
+                time = fmaxf(item, 2.0f * ov + fmaxf(size[0] + size[1], size[2] + size[3]));
+            }
+            times[tid] = time;
+        }
+        __syncthreads();
+        float least_time = INFINITY;
+        for (int k = 0; k < TRY; ++k)
+            if (times[k] < least_time) {
+                least_time = times[k];
                 C = candidate(k);
             }
-        }
     }
     // Pieces in order of their size, in quarters of the largest, that first (and a tile's neighbours
     // beside it, whose keys are the same): what is dealt out last fills the gaps.

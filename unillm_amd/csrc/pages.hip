@@ -33,20 +33,32 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Inclusive sums of two ints over the workgroup (tmp: 2 ints a wave).
-__device__ __forceinline__ int2 block_scan2(int2 v, int2* tmp) {
+// a + b of counts that are at most `cap`, cut off just past it: what a call has no room for stays
+// so, and no sum wraps.
+__device__ __forceinline__ int2 add_capped(int2 a, int2 b, int2 cap) {
+    return make_int2(min(a.x + b.x, cap.x + 1), min(a.y + b.y, cap.y + 1));
+}
+
+// Sums of two counts over the workgroup's threads before this one, and all (tmp: 2 ints a wave).
+__device__ __forceinline__ int2 block_scan2(int2 v, int2 cap, int2* tmp, int2* all) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int2 s = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int a = __shfl_up(v.x, o, 64), b = __shfl_up(v.y, o, 64);
-        if (lane >= o) v.x += a, v.y += b;
+        const int2 up = make_int2(__shfl_up(s.x, o, 64), __shfl_up(s.y, o, 64));
+        if (lane >= o) s = add_capped(s, up, cap);
     }
-    if (lane == 63) tmp[w] = v;
+    if (lane == 63) tmp[w] = s;
+    const int2 left = make_int2(__shfl_up(s.x, 1, 64), __shfl_up(s.y, 1, 64));
     __syncthreads();
-    int2 base = make_int2(0, 0);
-    for (int i = 0; i < w; ++i) base.x += tmp[i].x, base.y += tmp[i].y;
-    __syncthreads();
-    return make_int2(v.x + base.x, v.y + base.y);
+    int2 base = make_int2(0, 0), sum = base;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) {
+        if (i < w) base = add_capped(base, tmp[i], cap);
+        sum = add_capped(sum, tmp[i], cap);
+    }
+    *all = sum;
+    return lane > 0 ? add_capped(base, left, cap) : base;
 }
 
 // The last workgroup of the launch to call this gets true (and clears the ticket).
@@ -75,8 +87,8 @@ __device__ __forceinline__ int bisect(const int* key, int n, int x) {
 }
 
 // Both calls' first part: each entry's id (-1: a padding entry) and old length into LDS, the
-// checks, and the prefix sums ca[0 .. B], cb[0 .. B] of a (tokens) and b (pages).  Returns the
-// largest error code found (full: the code of more pages than the pool has).
+// checks, and the prefix sums ca[0 .. B], cb[0 .. B] of tokens and pages.  Returns an error code
+// (full: that of more pages than the pool has).
 struct Entries {
     int* id;
     int* len;
@@ -84,58 +96,65 @@ struct Entries {
     int* cb;
 };
 
+// A thread takes neighbouring entries, 8 at a time with their loads in flight together, and the
+// threads' sums are scanned once.
 template <class F>
-__device__ int scan_entries(const Entries& e, int B, const PageTable& t, const int* ids, F&& counts,
-                            int* seen, int2* tmp, int* error, int full) {
+__device__ int scan_entries(const Entries& e, int B, const PageTable& t, const int* ids, const int* lens,
+                            F&& counts, int* seen, int2* tmp, int* error, int full) {
     const int words = (t.max_seqs + 31) / 32;
     for (int i = threadIdx.x; i < words; i += kThreads) seen[i] = 0;
-    if (threadIdx.x == 0) {
-        *error = 0;
-        e.ca[0] = 0;
-        e.cb[0] = 0;
-    }
+    if (threadIdx.x == 0) *error = 0;
+    const int each = (B + kThreads - 1) / kThreads, b0 = (int)threadIdx.x * each, b1 = min(B, b0 + each);
     __syncthreads();
     const int top = t.max_pages * t.page_size;
-    int2 carry = make_int2(0, 0);
-    for (int b0 = 0; b0 < B; b0 += kThreads) {
-        const int b = b0 + (int)threadIdx.x;
-        int2 v = make_int2(0, 0);
-        int bad = 0;
-        if (b < B) {
-            const int id = ids[b];
-            int len = 0;
-            if (id >= t.max_seqs) {
-                bad = kPagesBadId;
-            } else if (id >= 0) {
-                if (atomicOr(&seen[id / 32], 1 << (id % 32)) >> (id % 32) & 1) bad = kPagesBadId;
-                len = t.lens[id];
-                if (len < 0 || len > top) bad = kPagesBadState;
-                else if (!bad) bad = counts(b, len, v);
+    const int2 cap = make_int2(t.max_tokens, t.n_pages);
+    int2 sum = make_int2(0, 0);
+    int worst = 0;
+    for (int c = b0; c < b1; c += 8) {
+        int id[8], n[8], len[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            id[i] = c + i < b1 ? ids[c + i] : -1;
+            n[i] = c + i < b1 && lens ? lens[c + i] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) len[i] = id[i] >= 0 && id[i] < t.max_seqs ? t.lens[id[i]] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (c + i >= b1) break;
+            int2 v = make_int2(0, 0);
+            int bad = 0;
+            if (id[i] >= t.max_seqs) bad = kPagesBadId;
+            else if (id[i] >= 0) {
+                if (atomicOr(&seen[id[i] / 32], 1 << (id[i] % 32)) >> (id[i] % 32) & 1) bad = kPagesBadId;
+                if (len[i] < 0 || len[i] > top) bad = kPagesBadState;
+                else if (!bad) bad = counts(n[i], len[i], v);
             }
-            e.id[b] = id < t.max_seqs ? max(id, -1) : -1;
-            e.len[b] = len;
-        }
-        if (bad) {
-            v = make_int2(0, 0);
-            atomicMax(error, bad);
-        }
-        const int2 s = block_scan2(v, tmp);
-        if (b < B) {
-            e.ca[b + 1] = carry.x + s.x;
-            e.cb[b + 1] = carry.y + s.y;
-        }
-        __syncthreads();
-        const int n = min(B - b0, kThreads);
-        carry = make_int2(e.ca[b0 + n], e.cb[b0 + n]);
-        // 256 entries' sums stay below 2^31 (an entry's tokens and pages below 2^22); what is
-        // past the step's room or the pool fails here, before more can wrap them
-        if (carry.x > t.max_tokens || carry.y > t.n_pages) {
-            if (threadIdx.x == 0) atomicMax(error, carry.x > t.max_tokens ? kPagesStepFull : full);
-            carry = make_int2(0, 0);
+            worst = max(worst, bad);
+            if (bad) v = make_int2(0, 0);
+            e.id[c + i] = id[i] < t.max_seqs ? max(id[i], -1) : -1;
+            e.len[c + i] = len[i];
+            e.ca[c + i] = v.x;
+            e.cb[c + i] = v.y;
+            sum = add_capped(sum, v, cap);
         }
     }
+    if (worst) atomicMax(error, worst);
+    int2 all;
+    int2 at = block_scan2(sum, cap, tmp, &all);
+    for (int b = b0; b < b1; ++b) {  // counts to sums before
+        const int2 v = make_int2(e.ca[b], e.cb[b]);
+        e.ca[b] = at.x;
+        e.cb[b] = at.y;
+        at = add_capped(at, v, cap);
+    }
+    if (threadIdx.x == 0) {
+        e.ca[B] = all.x;
+        e.cb[B] = all.y;
+    }
     __syncthreads();
-    return *error;
+    const int err = *error;
+    return err ? err : all.x > t.max_tokens ? kPagesStepFull : all.y > t.n_pages ? full : 0;
 }
 
 // dynamic LDS: id[B] | len[B] | ca[B + 1] | cb[B + 1] | seen[ceil(max_seqs / 32)]
@@ -162,8 +181,7 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(PageTable t, const int
     const Entries e = entries_in(sm, B, &seen);
     const int ps = t.page_size, shift = t.page_shift;
     const int n_free = t.counts[kPagesFree];
-    int err = scan_entries(e, B, t, ids, [&](int b, int len, int2& v) {
-        const int n = news[b];
+    int err = scan_entries(e, B, t, ids, news, [&](int n, int len, int2& v) {
         if (n < 0) return kPagesBadLength;
         if (n > t.max_pages * ps - len) return kPagesSeqFull;
         if (n > t.max_tokens) return kPagesStepFull;
@@ -179,24 +197,35 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(PageTable t, const int
         const int stride = (int)gridDim.x * kThreads * 4;
         for (int r0 = ((int)blockIdx.x * kThreads + (int)threadIdx.x) * 4; r0 < total; r0 += stride) {
             int b = bisect(e.ca, B, r0);
-            const int r1 = min(r0 + 4, total);
-            for (int r = r0; r < r1; ++r) {
+            int4 at, page;
+            int* pos = &at.x;
+            int* pg = &page.x;
+            bool fresh[4];
+            int* entry[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = min(r0 + i, total - 1);
                 while (r >= e.ca[b + 1]) ++b;
-                const int id = e.id[b], len = e.len[b], pos = len + r - e.ca[b];
-                const int col = pos >> shift, held = (len + ps - 1) >> shift;
-                int* entry = t.table + (int64_t)id * t.max_pages + col;
-                int page;
-                if (col < held) {
-                    page = *entry;
-                } else {
-                    page = t.free_pages[n_free - 1 - (e.cb[b] + col - held)];
-                    if ((pos & (ps - 1)) == 0) *entry = page;  // (the page's first token)
-                }
+                const int len = e.len[b];
+                pos[i] = len + r - e.ca[b];
+                const int col = pos[i] >> shift, held = (len + ps - 1) >> shift;
+                entry[i] = t.table + (int64_t)e.id[b] * t.max_pages + col;
+                fresh[i] = col >= held;
+                pg[i] = *(fresh[i] ? t.free_pages + (n_free - 1 - (e.cb[b] + col - held)) : entry[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (fresh[i] && (pos[i] & (ps - 1)) == 0) *entry[i] = pg[i];  // (the page's first token)
                 // a page of a restored state that the pool does not have: the token has no slot
-                const bool good = (unsigned)page < (unsigned)t.n_pages;
+                const bool good = (unsigned)pg[i] < (unsigned)t.n_pages;
                 if (!good) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
-                t.slots[r] = good ? page * ps + (pos & (ps - 1)) : -1;
-                t.positions[r] = pos;
+                pg[i] = good ? pg[i] * ps + (pos[i] & (ps - 1)) : -1;
+            }
+            if (r0 + 4 <= total) {
+                *reinterpret_cast<int4*>(t.slots + r0) = page;
+                *reinterpret_cast<int4*>(t.positions + r0) = at;
+            } else {
+                for (int i = 0; r0 + i < total; ++i) t.slots[r0 + i] = pg[i], t.positions[r0 + i] = pos[i];
             }
         }
     }
@@ -226,8 +255,7 @@ __global__ __launch_bounds__(kThreads) void truncate_kernel(PageTable t, const i
     const Entries e = entries_in(sm, B, &seen);
     const int ps = t.page_size, shift = t.page_shift;
     const int n_free = t.counts[kPagesFree];
-    int err = scan_entries(e, B, t, ids, [&](int b, int len, int2& v) {
-        const int n = news ? news[b] : 0;
+    int err = scan_entries(e, B, t, ids, news, [&](int n, int len, int2& v) {
         if (n < 0 || n > len) return kPagesBadLength;
         v.x = 0;
         v.y = ((len + ps - 1) >> shift) - ((n + ps - 1) >> shift);
