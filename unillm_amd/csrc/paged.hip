@@ -140,50 +140,63 @@ struct Visits {
     __device__ int key(int v) const { return (v < sink_blocks ? v : first + v - sink_blocks) * U; }
 };
 
-// Inclusive sums of two ints over 256 threads (tmp: [4]).
-__device__ __forceinline__ int2 block_scan2(int2 v, int2* tmp) {
+// Inclusive sums of two values over 256 threads, and all (tmp: [4]).
+__device__ __forceinline__ ulong2 block_scan(ulong2 v, ulong2* tmp, ulong2* all) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(v.x, o, 64), y = __shfl_up(v.y, o, 64);
+        const uint64_t x = __shfl_up(v.x, o, 64), y = __shfl_up(v.y, o, 64);
         if (lane >= o) v.x += x, v.y += y;
     }
     if (lane == 63) tmp[w] = v;
     __syncthreads();
-    int2 base = make_int2(0, 0);
-    for (int i = 0; i < w; ++i) base.x += tmp[i].x, base.y += tmp[i].y;
+    ulong2 base = {0, 0}, sum = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const ulong2 x = tmp[i];
+        if (i < w) base.x += x.x, base.y += x.y;
+        sum.x += x.x;
+        sum.y += x.y;
+    }
     __syncthreads();
-    return make_int2(v.x + base.x, v.y + base.y);
+    *all = sum;
+    return ulong2{v.x + base.x, v.y + base.y};
 }
 
 // Deals one kind's work out (one workgroup): every entry's rows in equal tiles, every tile's visits of
 // U keys in equal pieces of at most C, where C makes the kind's target of pieces over all kv
 // heads.
-// sm: LDS, tp[B + 1] (tiles before each entry) | m[B] | ctx[B].
+// sm: LDS, for max_seqs entries each: tp (tiles before each entry, and all) | m | ctx.
 template <int U>
 __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
-    __shared__ int2 tmp[4];
+    __shared__ ulong2 tmp[4];
     __shared__ long long part[4];
-    __shared__ int off[257], info[256][7], last[6];
+    __shared__ int off[257], info[256][7];
     const Call::Kind& kd = a.kind[kind];
-    const int tid = threadIdx.x, B = t.counts[kPagesEntries], TR = kd.tile_rows;
-    int *tp = sm, *ms = tp + B + 1, *ctxs = ms + B;
+    const int tid = threadIdx.x, TR = kd.tile_rows;
+    int *tp = sm, *ms = tp + t.max_seqs + 1, *ctxs = ms + t.max_seqs;
+    // (entries' facts are requested with their number: the arrays hold max_seqs)
+    const int b_first = min(tid, t.max_seqs - 1);
+    int c0 = t.cu[b_first], c1 = t.cu[b_first + 1], held = t.step_lens[b_first];
+    const int B = t.counts[kPagesEntries];
     int tiles = 0;
     if (tid == 0) tp[0] = 0;
     for (int b0 = 0; b0 < B; b0 += 256) {
         const int b = b0 + tid;
         int n = 0;
         if (b < B) {
-            const int m = t.cu[b + 1] - t.cu[b], rows = m * a.G;
+            if (b0 > 0) c0 = t.cu[b], c1 = t.cu[b + 1], held = t.step_lens[b];
+            const int m = c1 - c0, rows = m * a.G;
             ms[b] = m;
-            ctxs[b] = t.step_lens[b] - m;
+            ctxs[b] = held - m;
             if ((rows <= kNarrowRows) == (kind == kNarrow)) n = (rows + TR - 1) / TR;
         }
-        const int2 s = block_scan2(make_int2(n, 0), tmp);
-        if (b < B) tp[b + 1] = tiles + s.x;
-        __syncthreads();
-        tiles = tp[min(b0 + 256, B)];
+        ulong2 all;
+        const ulong2 s = block_scan(ulong2{(uint64_t)n, 0}, tmp, &all);
+        if (b < B) tp[b + 1] = tiles + (int)s.x;
+        tiles += (int)all.x;
     }
+    __syncthreads();
     struct Tile {
         int b, row0, rows, nv;
     };
@@ -202,8 +215,10 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         x.nv = Visits<U>(ctxs[lo] + x.row0 / a.G, ctxs[lo] + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks).count;
         return x;
     };
-    long long sum = 0;
-    for (int i = tid; i < tiles; i += 256) sum += tile(i).nv;
+    Tile mine{0, 0, 0, 0};  // the thread's first
+    if (tid < tiles) mine = tile(tid);
+    long long sum = mine.nv;
+    for (int i = tid + 256; i < tiles; i += 256) sum += tile(i).nv;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if ((tid & 63) == 0) part[tid >> 6] = sum;
@@ -274,74 +289,79 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
             }
     }
     // Pieces in order of their size, in quarters of the largest, that first (and a tile's neighbours
-    // beside it, whose keys are the same): what is dealt out last fills the gaps.
-    __shared__ int count[4];
-    if (tid < 4) count[tid] = 0;
-    __syncthreads();
+    // beside it, whose keys are the same): what is dealt out last fills the gaps.  The four
+    // ranks' numbers are 16 bits each of a scan's first value: pieces are at most target + tiles.
+    const int largest = min(C, longest);
     auto pieces = [&](int nv) { return (nv - 1) / C + 1; };
-    const int top = min(C, longest);
-    auto rank = [&](int nv, int S) { return 3 - min(3, (int)(4 * (int64_t)(nv / S) / top)); };
-    for (int i = tid; i < tiles; i += 256) {
-        const int nv = tile(i).nv, S = pieces(nv);
-        atomicAdd(&count[rank(nv, S)], S);
+    auto rank = [&](int nv, int S) { return 3 - min(3, (int)(4 * (int64_t)(nv / S) / largest)); };
+    int fill[4] = {0, 0, 0, 0};
+    if (tiles > 256) {
+        __shared__ int count[4];
+        if (tid < 4) count[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < tiles; i += 256) {
+            const int nv = tile(i).nv, S = pieces(nv);
+            atomicAdd(&count[rank(nv, S)], S);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 1; e < 4; ++e) fill[e] = fill[e - 1] + count[e - 1];
     }
-    __syncthreads();
-    int fill[4] = {0, count[0], count[0] + count[1], count[0] + count[1] + count[2]};
-    if (tid == 0) kd.head[0] = fill[3] + count[3];
-    int splits = 0, rows = 0;
+    int items = 0, splits = 0, rows = 0;
     for (int i0 = 0; i0 < tiles; i0 += 256) {
         const int i = i0 + tid;
-        Tile x{0, 0, 0, 0};
-        int S = 0;
-        if (i < tiles) {
-            x = tile(i);
-            S = pieces(x.nv);
-        }
+        Tile x = mine;
+        if (i0 > 0 && i < tiles) x = tile(i);
+        const int S = i < tiles ? pieces(x.nv) : 0, rk = S > 0 ? rank(x.nv, S) : 0;
         const int want = S > 1 ? S * a.KVH * x.rows : 0;
-        const int2 r = block_scan2(make_int2(want, S > 1 ? 1 : 0), tmp);
-        const int2 n = block_scan2(make_int2(S, 0), tmp);
-        const int rk = S > 0 ? rank(x.nv, S) : 0;
-        const int2 n01 = block_scan2(make_int2(rk == 0 ? S : 0, rk == 1 ? S : 0), tmp);
-        const int2 n23 = block_scan2(make_int2(rk == 2 ? S : 0, rk == 3 ? S : 0), tmp);
-        const int upto[4] = {n01.x, n01.y, n23.x, n23.y};
-        int at = 0;
+        const int first = S > 0 ? t.cu[x.b] : 0, id = S > 0 ? t.step_ids[x.b] : 0;
+        ulong2 all;
+        const ulong2 n = block_scan(ulong2{(uint64_t)S << (16 * rk), (uint64_t)want << 16 | (S > 1 ? 1 : 0)}, tmp, &all);
+        auto field = [](uint64_t v, int e) { return (int)(v >> (16 * e) & 0xFFFF); };
+        if (tiles <= 256)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (rk == e) at = fill[e] + upto[e] - S;
-        const int base = rows + r.x - want;
-        off[tid + 1] = n.x;
-        if (tid == 0) off[0] = 0;
-        if (tid == 255) {
-            last[0] = r.y;
-            last[1] = r.x;
+            for (int e = 1; e < 4; ++e) fill[e] = fill[e - 1] + field(all.x, e - 1);
+        int at = 0, upto = 0, made = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) last[2 + e] = upto[e];
+        for (int e = 0; e < 4; ++e) {
+            if (rk == e) at = fill[e] + field(n.x, e) - S;
+            upto += field(n.x, e);
+            made += field(all.x, e);
+            fill[e] += field(all.x, e);
         }
-        const int v[7] = {x.b, x.row0, x.rows, x.nv, kd.row0 + base, S, at};
+        const int base = kd.row0 + rows + (int)(n.y >> 16) - want;
+        off[tid + 1] = upto;
+        if (tid == 0) off[0] = 0;
+        const int v[7] = {x.b, x.row0, x.rows, x.nv, base, S, at};
 #pragma unroll
         for (int e = 0; e < 7; ++e) info[tid][e] = v[e];
-        if (want) kd.splits[splits + r.y - 1] = {t.cu[x.b], x.row0, x.rows, kd.row0 + base, S, {}};
+        if (want) kd.splits[splits + (int)(n.y & 0xFFFF) - 1] = {first, x.row0, x.rows, base, S, {}};
+        if (S == 1) kd.items[at] = {first, ctxs[x.b], ctxs[x.b] + ms[x.b], id, x.row0, x.rows, 0, x.nv, base, 0, 1, 0};
         __syncthreads();
-        for (int k = tid; k < off[256]; k += 256) {
-            int lo = 0, hi = 256;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (off[mid] <= k) lo = mid;
-                else hi = mid;
+        if ((all.y & 0xFFFF) != 0)
+            for (int k = tid; k < made; k += 256) {  // tiles in pieces: a thread a piece
+                int lo = 0, hi = 256;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if (off[mid] <= k) lo = mid;
+                    else hi = mid;
+                }
+                const int* w = info[lo];
+                const int s = k - off[lo], nv = w[3], Sw = w[5];
+                if (Sw < 2) continue;
+                const int v0 = (int)((int64_t)s * nv / Sw), v1 = (int)((int64_t)(s + 1) * nv / Sw);
+                const int b = w[0], ctx = ctxs[b];
+                kd.items[w[6] + s] = {t.cu[b], ctx, ctx + ms[b], t.step_ids[b], w[1], w[2], v0, v1 - v0, w[4], s, Sw, 0};
             }
-            const int* w = info[lo];
-            const int s = k - off[lo], nv = w[3], Sw = w[5];
-            const int v0 = (int)((int64_t)s * nv / Sw), v1 = (int)((int64_t)(s + 1) * nv / Sw);
-            const int b = w[0], ctx = ctxs[b];
-            kd.items[w[6] + s] = {t.cu[b], ctx, ctx + ms[b], t.step_ids[b], w[1], w[2], v0, v1 - v0, w[4], s, Sw, 0};
-        }
-        splits += last[0];
-        rows += last[1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) fill[e] += last[2 + e];
+        items += made;
+        splits += (int)(all.y & 0xFFFF);
+        rows += (int)(all.y >> 16);
         __syncthreads();
     }
-    if (tid == 0) kd.head[1] = splits;
+    if (tid == 0) {
+        kd.head[0] = items;
+        kd.head[1] = splits;
+    }
 }
 
 // The first kernel of a call.  Workgroups 0 and 1 deal the work out; each other one takes 16 rows
