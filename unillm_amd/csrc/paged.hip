@@ -364,8 +364,8 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     }
 }
 
-// The first kernel of a call.  Workgroups 0 and 1 deal the work out; each other one takes 16 rows
-// of the step and `heads` kv heads: the rows' rotations (kept in f32 for the queries), their
+// The first kernel of a call.  Workgroups 0 and 1 deal the work out; each other one takes nr rows
+// of the step (16, or 4 of a short one) and `heads` kv heads: the rows' rotations (kept in f32 for the queries), their
 // keys rotated and stored, their values stored.  A V page runs along the keys, so where 8 rows
 // are 8 neighbouring slots of a page, aligned (a prompt's rows, but for its ends), a thread
 // stores a dimension's 8 values at once; other rows value by value.  (2048 rows of 32 heads of
@@ -373,21 +373,21 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
 constexpr int kAppendRows = 16;
 
 template <class T, int D>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable t, Call a, int heads) {
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable t, Call a, int nr, int heads) {
     constexpr int HALF = D / 2, Q4 = HALF / 4, NR = kAppendRows;
     __shared__ double2 turn[NR][HALF];
     __shared__ int slots[NR + 14];  // of the rows from 7 before the workgroup's to 7 after
     extern __shared__ int plan_lds[];
     const int tid = threadIdx.x;
     const int bx = (int)blockIdx.x - 2, groups = (a.KVH + heads - 1) / heads;
-    const int row0 = bx / groups * NR, g0 = bx % groups * heads;
+    const int row0 = bx / groups * nr, g0 = bx % groups * heads;
     // (rows' slots and positions are requested with the plan's header: both arrays hold max_tokens)
     int slot = -1, pos = 0;
-    if (bx >= 0 && tid < NR + 14) {
+    if (bx >= 0 && tid < nr + 14) {
         const int row = row0 + tid - 7;
         if (row >= 0 && row < t.max_tokens) slot = t.slots[row];
     }
-    if (bx >= 0 && tid < NR && row0 + tid < t.max_tokens) pos = t.positions[row0 + tid];
+    if (bx >= 0 && tid < nr && row0 + tid < t.max_tokens) pos = t.positions[row0 + tid];
     if (!step_fits(t, a.n)) {
         if (blockIdx.x < 2 && tid < 2) a.kind[blockIdx.x].head[tid] = 0;
         if (blockIdx.x == 0 && tid == 0) *a.redo_count = 0;
@@ -399,11 +399,23 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable 
     if (blockIdx.x == 1) return plan<kWideUnit<T, D>>(t, a, kWide, plan_lds);
     const int total = t.counts[kPagesTokens];
     if (row0 >= total) return;
-    const int rows = min(NR, total - row0);
+    const int rows = min(nr, total - row0);
     __shared__ int at[NR];
-    if (tid < NR + 14) slots[tid] = row0 + tid - 7 < total ? slot : -1;
-    if (tid < NR) at[tid] = pos;
+    if (tid < nr + 14) slots[tid] = row0 + tid - 7 < total ? slot : -1;
+    if (tid < nr) at[tid] = pos;
     __syncthreads();
+    // Row r is in a run of 8 if the row r - slot % 8 and the one 7 after it are 7 slots apart; the
+    // runs that begin here and the rows in none, listed.
+    __shared__ int list[2], run_rows[NR], one_rows[NR];
+    if (tid < 64) {
+        const int sl = tid < rows ? slots[tid + 7] : -1, s0 = tid - (sl & 7);
+        const bool run = sl >= 0 && s0 >= -7 && s0 < nr && slots[s0 + 7] == (sl & ~7) && slots[s0 + 14] == (sl | 7);
+        const uint64_t begins = __ballot(run && (sl & 7) == 0), ones = __ballot(sl >= 0 && !run);
+        const uint64_t before = (1ull << tid) - 1;
+        if (begins >> tid & 1) run_rows[__popcll(begins & before)] = tid;
+        if (ones >> tid & 1) one_rows[__popcll(ones & before)] = tid;
+        if (tid == 0) list[0] = __popcll(begins), list[1] = __popcll(ones);
+    }
     for (int i = tid; i < rows * HALF; i += 256) {
         const int r = i / HALF, p = i % HALF;
         double sn, cs;
@@ -439,35 +451,41 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable 
         *reinterpret_cast<Four*>(dst) = lo;
         *reinterpret_cast<Four*>(dst + HALF) = hi;
     }
-    // values: a wave a task of 64 dimensions; row r is in a run of 8 if the row r - slot % 8 and
-    // the one 7 after it are 7 slots apart
+    // values: a wave a task of 64 dimensions of a run or of a single row
     const int lane = tid & 63;
     constexpr int DG = D / 64;
-    auto runs = [&](int r) {  // r from -7 on
-        const int sl = slots[r + 7], s0 = r - (sl & 7);
-        return sl >= 0 && s0 >= -7 && s0 + 7 < NR + 7 && slots[s0 + 7] == (sl & ~7) &&
-               slots[s0 + 14] == (sl | 7);
-    };
-    for (int i = __builtin_amdgcn_readfirstlane(tid >> 6); i < (g1 - g0) * rows * DG; i += 4) {
-        const int g = g0 + i / (rows * DG), r = i / DG % rows, d = i % DG * 64 + lane;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n_runs = list[0], n_ones = list[1];
+    for (int i = wv; i < (g1 - g0) * n_runs * DG; i += 4) {
+        const int g = g0 + i / (n_runs * DG), r = run_rows[i / DG % n_runs], d = i % DG * 64 + lane;
         const int sl = slots[r + 7];
-        if (sl < 0) continue;
-        const bool run = runs(r);
-        if (run && (sl & 7) != 0) continue;  // (stored with the run's first row)
         T* dst = static_cast<T*>(c.v) + (((((int64_t)(sl >> shift) * KVH + g) * D + d) << shift) + (sl & (ps - 1)));
         const float* x = xv + r * a.qstride + (int64_t)g * D + d;
-        if (run) {
-            struct alignas(16) Eight {
-                T v[8];
-            } y;
-            float f[8];
+        struct alignas(16) Eight {
+            T v[8];
+        } y;
+        float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = x[e * a.qstride];
+        for (int e = 0; e < 8; ++e) f[e] = x[e * a.qstride];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y.v[e] = narrow<T>(f[e]);
-            *reinterpret_cast<Eight*>(dst) = y;
-        } else {
-            *dst = narrow<T>(*x);
+        for (int e = 0; e < 8; ++e) y.v[e] = narrow<T>(f[e]);
+        *reinterpret_cast<Eight*>(dst) = y;
+    }
+    const int tasks = (g1 - g0) * n_ones * DG;
+    for (int i0 = wv; i0 < tasks; i0 += 16) {
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // (four tasks' loads in flight)
+            const int i = min(i0 + 4 * k, tasks - 1), g = g0 + i / (n_ones * DG), r = one_rows[i / DG % n_ones];
+            x[k] = xv[r * a.qstride + (int64_t)g * D + i % DG * 64 + lane];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = i0 + 4 * k;
+            if (i >= tasks) break;
+            const int g = g0 + i / (n_ones * DG), d = i % DG * 64 + lane;
+            const int sl = slots[one_rows[i / DG % n_ones] + 7];
+            static_cast<T*>(c.v)[((((int64_t)(sl >> shift) * KVH + g) * D + d) << shift) + (sl & (ps - 1))] = narrow<T>(x[k]);
         }
     }
 }
@@ -1610,10 +1628,11 @@ hipError_t launch_typed(const PagedKv& c, const unillm_page_table& t, const Call
     // (the plan keeps three ints an entry in LDS)
     const size_t plan_lds = (size_t)(3 * t.st.max_seqs + 1) * sizeof(int);
     // kv heads a workgroup: one, or what makes four workgroups a CU
-    const int64_t blocks = (a.n + kAppendRows - 1) / kAppendRows, most = 4 * device_info().cu_count;
+    const int nr = a.n <= 512 ? 4 : kAppendRows;
+    const int64_t blocks = (a.n + nr - 1) / nr, most = 4 * device_info().cu_count;
     const int heads = (int)std::min<int64_t>(a.KVH, std::max<int64_t>(1, blocks * a.KVH / most));
     const int64_t append = blocks * ((a.KVH + heads - 1) / heads);
-    paged_append_kernel<T, D><<<(unsigned)(2 + append), 256, plan_lds, s>>>(c, t.st, a, heads);
+    paged_append_kernel<T, D><<<(unsigned)(2 + append), 256, plan_lds, s>>>(c, t.st, a, nr, heads);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (l.items[kWide] > 0) {
