@@ -234,7 +234,18 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     // mean place's load and half an item.  (Three chunks among 24 sequences, bf16: 152 us with
     // pieces of 18 visits, 272 for 256 places, whose small ones pair up; 190 with pieces of 30, 216.)
     int C = C0, longest = INT_MAX;
-    if (kind == kWide && tiles > 0 && (int64_t)tiles * a.KVH <= 4 * (int64_t)kd.target) {
+    bool search = false;  // (as many places as items of C0: no C is better)
+    if (kind == kWide && (int64_t)tiles * a.KVH <= 4 * (int64_t)kd.target) {
+        __shared__ int made;
+        if (tid == 0) made = 0;
+        __syncthreads();
+        int n = mine.nv > 0 ? (mine.nv - 1) / C0 + 1 : 0;
+        for (int i = tid + 256; i < tiles; i += 256) n += (tile(i).nv - 1) / C0 + 1;
+        if (n > 0) atomicAdd(&made, n);
+        __syncthreads();
+        search = (int64_t)made * a.KVH > kd.target;
+    }
+    if (search) {
         constexpr int TRY = 5, BINS = 32;
         __shared__ int hist[TRY][BINS], split_made[TRY], top;
         __shared__ float times[TRY];
@@ -243,42 +254,45 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         if (tid == 0) top = 0;
         __syncthreads();
         auto candidate = [&](int k) { return k == 0 ? C0 : k == 1 ? C0 + C0 / 4 : k == 2 ? C0 + C0 / 2 : k == 3 ? 2 * C0 : INT_MAX / 2; };
-        for (int i = tid; i < tiles; i += 256) atomicMax(&top, tile(i).nv);
+        int my_top = mine.nv;
+        for (int i = tid + 256; i < tiles; i += 256) my_top = max(my_top, tile(i).nv);
+        if (my_top > 0) atomicMax(&top, my_top);
         __syncthreads();
         longest = top;
+        const float bin = (float)(BINS - 1) / (float)longest;
         for (int i = tid; i < tiles; i += 256) {
-            const int nv = tile(i).nv;
+            const int nv = i < 256 ? mine.nv : tile(i).nv;
+#pragma unroll
             for (int k = 0; k < TRY; ++k) {
                 const int S = (nv - 1) / candidate(k) + 1;
-                atomicAdd(&hist[k][(int)((int64_t)(nv / S) * (BINS - 1) / longest)], S);
+                atomicAdd(&hist[k][min(BINS - 1, (int)((float)nv / (float)S * bin))], S);
                 if (S > 1) atomicAdd(&split_made[k], S);
             }
         }
         __syncthreads();
-        if (tid < TRY) {
-            const int places = max(1, kd.target / a.KVH);
-            int n = 0;
-            for (int e = 0; e < BINS; ++e) n += hist[tid][e];
-            const float ov = (float)kd.overhead * (1.0f + (float)split_made[tid] / (float)n);
-            const float item = (float)min(candidate(tid), longest) + ov;
+        const int lane = tid & 63;
+        for (int k = tid >> 6; k < TRY; k += 4) {  // a wave a candidate, a lane a bin
+            const int places = max(1, kd.target / a.KVH), h = lane < BINS ? hist[k][lane] : 0;
+            int upto = h;  // items of this size and larger
+#pragma unroll
+            for (int o = 1; o < BINS; o <<= 1) {
+                const int x = __shfl_down(upto, o, 64);
+                if (lane + o < BINS) upto += x;
+            }
+            const int n = __shfl(upto, 0, 64);
+            const float ov = (float)kd.overhead * (1.0f + (float)split_made[k] / (float)n);
+            const float item = (float)min(candidate(k), longest) + ov;
             float time = item;
             if (n > 2 * places) {
                 time = fmaxf(item, ((float)sum + ov * (float)n) / (float)places + 0.5f * item);
             } else if (n > places) {
-                // sizes at these ranks, the largest first
-                const int want[4] = {places - 1, places, 2 * places - n, n - 1};
-                float size[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                int seen = 0;
-                for (int e = BINS - 1; e >= 0; --e) {
-                    const int upto = seen + hist[tid][e];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (want[q] >= seen && want[q] < upto) size[q] = (float)e * (float)longest / (float)(BINS - 1);
-                    seen = upto;
-                }
-                time = fmaxf(item, 2.0f * ov + fmaxf(size[0] + size[1], size[2] + size[3]));
+                auto size = [&](int rank) {  // of the item at this rank, the largest first
+                    const uint64_t here = __ballot(lane < BINS && rank >= upto - h && rank < upto);
+                    return (float)__builtin_ctzll(here | 1ull << 63) / bin;
+                };
+                time = fmaxf(item, 2.0f * ov + fmaxf(size(places - 1) + size(places), size(2 * places - n) + size(n - 1)));
             }
-            times[tid] = time;
+            if (lane == 0) times[k] = time;
         }
         __syncthreads();
         float least_time = INFINITY;
