@@ -12,7 +12,7 @@ torch = pytest.importorskip("torch")
 
 from paged_oracle import attend, rotate  # noqa: E402
 from unillm_amd import HipError, PagedKvCache, PageTable  # noqa: E402
-from unillm_amd._capi import ERR_INVALID_ARG  # noqa: E402
+from unillm_amd._capi import ERR_INVALID_ARG, ERR_UNSUPPORTED  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -131,6 +131,67 @@ def test_long_sequences(dtype, hd, window, sinks):
     s.check(s.call(window, sinks), window, sinks)
 
 
+# query rows of an entry on both sides of the tiles' sizes: 16 (narrow), 64 (the last narrow
+# entry), waves of 32 and tiles of 128 and 256 (wide)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_row_counts(dtype, hd):
+    new = [15, 16, 17, 63, 64, 65, 95, 97, 128, 129, 255, 256, 257, 290]
+    s = Step(dtype, 1, 1, hd, 16, [0, 3, 20, 0, 1, 0, 40, 9, 0, 2, 0, 31, 0, 64], new, seed=hd)
+    s.check(s.call())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,KVH,hd,new", [(7, 1, 64, 41), (6, 2, 128, 130), (5, 1, 256, 60), (16, 1, 64, 20)])
+def test_groups_that_divide_no_tile(dtype, H, KVH, hd, new):
+    s = Step(dtype, H, KVH, hd, 32, [100, 0, 517], [new, new + 3, 7], seed=new)
+    s.check(s.call())
+    s.check(s.call(77, 5), 77, 5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (256, 256)])
+def test_chunks_behind_long_prefixes(dtype, hd, page):
+    # the keys of a tile in pieces, on more pages than one read of page ids
+    s = Step(dtype, 2, 1, hd, page, [20011, 0, 9000], [70, 1, 3], seed=page)
+    s.check(s.call())
+    s.check(s.call(5000, 100), 5000, 100)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_tiles_than_one_scan(dtype):
+    # 300 entries of 70 rows (wide) and 300 of one, the plan's lists past 256 of each
+    r = np.random.RandomState(5)
+    new = [70 if i % 2 else 1 for i in range(600)]
+    s = Step(dtype, 1, 1, 64, 16, [int(c) for c in r.randint(0, 90, 600)], new, seed=6)
+    s.check(s.call(), seqs={0, 1, 255, 256, 257, 511, 513, 598, 599})
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+def test_the_most_sequences(hd):
+    # 8192 entries, the most of a table, in an order of their own
+    g = torch.Generator().manual_seed(2)
+    n, page = 8192, 16
+    table = PageTable(n, 2, 2 * n, page, 3 * n)
+    cache = PagedKvCache(1, hd, 2 * n, page, torch.bfloat16)
+    ids = torch.randperm(n, generator=g).to(torch.int32).cuda()
+    one = torch.ones(n, dtype=torch.int32, device="cuda")
+    qkv = [torch.randn(n, 3 * hd, generator=g).cuda() for _ in range(3)]
+    for x in qkv:
+        table.extend(ids, one)
+        out = cache.attention(table, x, 1)
+    table.check()
+    assert (table.seq_lens == 3).all()
+    rows = [x.double().cpu().numpy().reshape(n, 3, hd) for x in qkv]
+    for b in range(0, n, 1000):
+        k = np.stack([torch.from_numpy(rotate(x[b:b + 1, 1:2], [t], 10000.0)).bfloat16().double().numpy()[0]
+                      for t, x in enumerate(rows)])
+        v = np.stack([torch.from_numpy(x[b, 2:3]).bfloat16().double().numpy() for x in rows])
+        ref, bound = attend(rotate(rows[2][b:b + 1, :1], [2], 10000.0), k, v, [2])
+        # (a key on a rounding boundary may be a unit off: 2^-8 of the scores' terms)
+        assert (np.abs(out[b].double().cpu().numpy() - ref[0, 0]) <= bound[0, 0] + 2.0 ** -8).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_many_sequences(dtype):
     r = np.random.RandomState(3)
@@ -197,6 +258,24 @@ def test_infinite_and_nan_keys_and_values_that_are_seen(dtype, new):
     mask = torch.ones_like(o, dtype=torch.bool)
     mask[new:, 2:, 5] = False
     assert ((o - c).abs()[mask] <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [3, 90])
+def test_non_finite_values_where_keys_are_in_pieces(dtype, new):
+    # a sequence long enough to be dealt out: NaN and infinities in its first page are seen without
+    # a window and hidden behind one; both ways every piece's rows are right
+    s = Step(dtype, 4, 2, 64, 16, [6000, 10], [new, new], seed=12)
+    whole, windowed = s.call().clone(), s.call(300, 2).clone()
+    page = int(s.table.block_table[int(s.ids[0]), 0])
+    s.cache.v[page, 0, 7, 3] = float("inf")   # key 3, kv head 0, dimension 7
+    s.cache.k[page, 1, 5, 9] = float("nan")   # key 5, kv head 1
+    out = s.call().view(-1, 4, 64)
+    assert (out[:new, :2, 7] == float("inf")).all() and torch.isnan(out[:new, 2:]).all()
+    assert torch.isfinite(out[new:]).all()
+    tol = 4096 * 2.0 ** -24
+    assert (out[:new, :2, :7] - whole.view(-1, 4, 64)[:new, :2, :7]).abs().max() <= tol
+    assert (s.call(300, 2) - windowed).abs().max() <= tol
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -304,6 +383,9 @@ def test_arguments_are_checked():
     with pytest.raises(HipError, match="pages of"):
         other.attention(s.table, s.qkv, 4)
     assert a(s.table, s.qkv[:0], 4).shape == (0, 256)
+    many = PageTable(1, 1, s.n_pages, 16, 1 << 20)
+    with pytest.raises(HipError, match="2\\^30"):
+        s.cache.reserve(many, 1 << 20, 1024)
     with pytest.raises(RuntimeError):
         PagedKvCache(2, 64, 4, 16, torch.float64)
     with pytest.raises(RuntimeError):
@@ -357,8 +439,30 @@ def test_captured_steps_replay_at_other_lengths(dtype, heads, hd, rows):
     eager_table.check()
 
 
-def test_capture_needs_a_reserved_workspace_or_none():
-    # a call that would allocate under capture is refused, and the stream's next calls work
+def test_capture_refuses_to_grow_the_workspace():
+    # (250000 rows of head_dim 256 keep 256 MB of cosines and sines: more than other tests leave)
+    n = 250000
+    table, cache = PageTable(1, 1, 2, 16, n), PagedKvCache(1, 256, 2, 16)
+    qkv, out = torch.zeros(n, 768, device="cuda"), torch.zeros(n, 256, device="cuda")
+    ids, one = ints([0]), ints([1])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        table.extend(ids, one)
+        with pytest.raises(HipError) as e:
+            cache.attention(table, qkv, 1, out=out)
+        assert e.value.status == ERR_UNSUPPORTED
+        with pytest.raises(HipError, match="captured") as e:
+            table.check()
+        assert e.value.status == ERR_UNSUPPORTED
+    graph.replay()
+    torch.cuda.synchronize()
+    table.check()
+    assert table.seq_lens[0].item() == 1
+
+
+def test_captured_attention_reads_the_current_plan():
     s = Step(torch.float16, 32, 4, 128, 16, [9000, 3], [1, 1], seed=3)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

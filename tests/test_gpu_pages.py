@@ -41,7 +41,7 @@ def extend(table, model, ids, news):
 # one entry to thousands (more than one scan of 256), one token to more than a workgroup's share
 @pytest.mark.parametrize("page,max_seqs,most,steps", [
     (16, 1, 40, 6), (16, 7, 1, 40), (32, 300, 9, 6), (64, 300, 70, 4), (128, 5, 3000, 4),
-    (256, 64, 300, 4), (16, 2500, 20, 3)])
+    (256, 64, 300, 4), (16, 2500, 20, 3), (16, 8192, 5, 2)])
 def test_random_steps_equal_the_restatement(page, max_seqs, most, steps):
     r = random.Random(page * max_seqs + most)
     max_pages = -(-most * steps // page) + 1

@@ -105,7 +105,9 @@ def test_null_tables_and_caches_are_refused(lib):
     (dict(kv_type=_capi.Q8_0), _capi.ERR_UNSUPPORTED), (dict(kv_type=99), _capi.ERR_UNSUPPORTED),
     (dict(heads=0), None), (dict(hd=96), None), (dict(hd=0), None), (dict(n_pages=0), None),
     (dict(page=24), None), (dict(theta=0.0), None), (dict(theta=float("nan")), None),
-    (dict(theta=float("inf")), None), (dict(k=16), None), (dict(v=16), None), (dict(k=8, v=16), None)])
+    (dict(theta=float("inf")), None), (dict(k=16), None), (dict(v=16), None), (dict(k=8, v=16), None),
+    (dict(heads=65536), None), (dict(heads=40000, hd=256, page=256), None),
+    (dict(heads=60000, n_pages=60000), None), (dict(n_pages=1 << 28), None)])
 def test_pool_shapes_are_checked_on_the_host(lib, change, status):
     a = {**dict(kv_type=_capi.F16, heads=2, hd=64, n_pages=4, page=16, theta=1e4, k=None, v=None),
          **change}

@@ -1027,8 +1027,12 @@ int unillm_hip_page_table_check(unillm_page_table* t, void* stream) {
     hipStream_t s = static_cast<hipStream_t>(stream);
     int code = 0;
     const int none = 0;
-    hipError_t e = hipMemcpyAsync(&code, t->st.counts + kPagesError, sizeof(code),
-                                  hipMemcpyDeviceToHost, s);
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    hipError_t e = hipStreamIsCapturing(s, &cs);
+    if (e == hipSuccess && cs != hipStreamCaptureStatusNone)
+        return fail(UNILLM_ERR_UNSUPPORTED, "page table check: the stream is being captured");
+    if (e == hipSuccess)
+        e = hipMemcpyAsync(&code, t->st.counts + kPagesError, sizeof(code), hipMemcpyDeviceToHost, s);
     if (e == hipSuccess) e = hipStreamSynchronize(s);
     if (e == hipSuccess && code != 0) {
         e = hipMemcpyAsync(t->st.counts + kPagesError, &none, sizeof(none), hipMemcpyHostToDevice, s);

@@ -1688,7 +1688,8 @@ hipError_t launch_paged_attention(const PagedKv& c, const unillm_page_table& t, 
            reinterpret_cast<float*>(w + l.po_at), reinterpret_cast<int*>(w + l.count_at),
            reinterpret_cast<int*>(w + l.redo_at), {}};
     for (int k = 0; k < 2; ++k)
-        a.kind[k] = {tile_rows(k, c.head_dim), target_pieces(k), k == kNarrow ? 4 : 2, 5, k == kNarrow ? 0 : (int)l.rows[0], reinterpret_cast<int*>(w + l.head_at[k]),
+        a.kind[k] = {tile_rows(k, c.head_dim), target_pieces(k), k == kNarrow ? 4 : 2, 5,
+                     k == kNarrow ? 0 : (int)l.rows[0], reinterpret_cast<int*>(w + l.head_at[k]),
                      reinterpret_cast<Item*>(w + l.items_at[k]),
                      reinterpret_cast<Split*>(w + l.splits_at[k])};
     if (c.type == UNILLM_QTYPE_F32) return launch_type<float>(c, t, a, l, s);
