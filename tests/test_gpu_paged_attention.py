@@ -519,3 +519,17 @@ def test_positions_past_31_bits_of_bytes():
     table.extend(ints([1]), ints([1]))
     small_table.extend(ints([1]), ints([1]))
     assert torch.equal(cache.attention(table, qkv[:1], 8), small.attention(small_table, qkv[:1], 8))
+
+
+def test_results_of_a_side_stream_outlive_it():
+    # the output is the side stream's memory, used and freed on the current one
+    s = Step(torch.float16, 4, 2, 64, 16, [30, 5], [1, 9], seed=2)
+    want = s.call().clone()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        side.wait_stream(torch.cuda.current_stream())
+        out = s.cache.attention(s.table, s.qkv, 4, stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+        got = out + 0.0
+        del out
+        assert torch.equal(got, want)

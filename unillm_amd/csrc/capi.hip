@@ -901,6 +901,17 @@ int check_entries(const unillm_page_table* t, const void* ids, const void* lens,
     return UNILLM_OK;
 }
 
+// Memory that is known to be another device's than the library's.
+bool elsewhere(const void* p) {
+    hipPointerAttribute_t a{};
+    if (!p) return false;
+    if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return a.type == hipMemoryTypeDevice && a.device != g_device;
+}
+
 // What a paged attention call and its reserve check alike.
 int check_paged(const unillm_paged_kv* c, const unillm_page_table* t, int64_t n, int64_t n_heads,
                 const std::string& what) {
@@ -943,6 +954,8 @@ int unillm_hip_page_table_create(int64_t max_seqs, int64_t max_pages, int64_t n_
     if (((uintptr_t)storage_dev & 255u) != 0)
         return fail(UNILLM_ERR_INVALID_ARG, "page table: storage must be 256-byte aligned");
     if (int rc = ensure_init()) return rc;
+    if (elsewhere(storage_dev))
+        return fail(UNILLM_ERR_INVALID_ARG, "page table: storage on another device than the library's");
     unillm_page_table* t = new (std::nothrow) unillm_page_table{};
     if (!t) return fail(UNILLM_ERR_OUT_OF_MEMORY, "host allocation failed");
     hipError_t e = hipSuccess;
@@ -1089,6 +1102,8 @@ int unillm_hip_paged_kv_create(int kv_type, int64_t n_kv_heads, int64_t head_dim
         return fail(UNILLM_ERR_INVALID_ARG,
                     "paged KV cache: give both of k and v, 16-byte aligned, or neither");
     if (int rc = ensure_init()) return rc;
+    if (elsewhere(k_dev) || elsewhere(v_dev))
+        return fail(UNILLM_ERR_INVALID_ARG, "paged KV cache: k or v on another device than the library's");
     unillm_paged_kv* c = new (std::nothrow) unillm_paged_kv{};
     if (!c) return fail(UNILLM_ERR_OUT_OF_MEMORY, "host allocation failed");
     c->device = g_device;

@@ -1605,9 +1605,12 @@ Layout layout(const PagedKv& c, const unillm_page_table& t, int64_t n, int64_t H
         return here;
     };
     for (int k = 0; k < 2; ++k) {
-        // tiles: an entry's last may be ragged.  A tile of nv visits makes at most nv / C + 1
-        // pieces, and the nv / C add up to target / KVH; more than one piece, at most 2 nv / C.
-        const int64_t tiles = n * G / tile_rows(k, D) + std::min<int64_t>(n, t.st.max_seqs);
+        // tiles: an entry's last may be ragged (a wide entry has more than kNarrowRows rows).  A
+        // tile of nv visits makes at most nv / C + 1 pieces, and the nv / C add up to target /
+        // KVH; more than one piece, at most 2 nv / C.
+        const int64_t entries = std::min<int64_t>(k == kNarrow ? n : n * G / (kNarrowRows + 1),
+                                                  t.st.max_seqs);
+        const int64_t tiles = n * G / tile_rows(k, D) + entries;
         const bool some = k == kNarrow || n * G > kNarrowRows;
         l.items[k] = some ? tiles + target_pieces(k) / KVH + 1 : 0;
         l.rows[k] = some ? 2 * (int64_t)target_pieces(k) * std::min<int64_t>(tile_rows(k, D), n * G) : 0;

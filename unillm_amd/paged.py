@@ -15,17 +15,24 @@ import torch
 
 from . import _capi
 from ._capi import HipError
-from .attention import _stream_ptr
 
 _KV_TYPES = {torch.float32: _capi.F32, torch.float16: _capi.F16, torch.bfloat16: _capi.BF16}
 
 
+def _stream_ptr(stream: torch.cuda.Stream | None, device: torch.device) -> int:
+    """The stream given, or the device's current one (read as the handle alone: 0.1 us, where
+    making a Stream object takes 3 of a table call's 8)."""
+    if stream is not None:
+        return stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _hold(stream: torch.cuda.Stream | None, *tensors: torch.Tensor | None) -> None:
     """Tensors used on a stream other than the current one are not reused before it is done."""
-    if stream is None or stream == torch.cuda.current_stream():
+    if stream is None:
         return
     for t in tensors:
-        if t is not None:
+        if t is not None and stream != torch.cuda.current_stream(t.device):
             t.record_stream(stream)
 
 
@@ -51,7 +58,8 @@ class PageTable:
         _check(_capi.lib().unillm_hip_page_table_bytes(max_seqs, max_pages, n_pages, page_size,
                                                        max_tokens, ctypes.byref(n)))
         self._mem = torch.empty(n.value, dtype=torch.uint8, device=device or "cuda")
-        torch.cuda.current_stream(self._mem.device).synchronize()  # the storage is free to write
+        self._device = self._mem.device
+        torch.cuda.current_stream(self._device).synchronize()  # the storage is free to write
         h = ctypes.c_void_p()
         _check(_capi.lib().unillm_hip_page_table_create(max_seqs, max_pages, n_pages, page_size,
                                                         max_tokens, self._mem.data_ptr(),
@@ -78,10 +86,10 @@ class PageTable:
 
     def _entries(self, what: str, ids: torch.Tensor, lens: torch.Tensor | None) -> int:
         for name, t in (("seq_ids", ids), ("lengths", lens)):
-            if t is not None and (t.dtype != torch.int32 or t.device != self._mem.device
+            if t is not None and (t.dtype != torch.int32 or t.device != self._device
                                   or t.dim() != 1 or not t.is_contiguous()):
                 raise RuntimeError(f"{what}: {name} must be a contiguous int32 vector on "
-                                   f"{self._mem.device}")
+                                   f"{self._device}")
         if lens is not None and lens.numel() != ids.numel():
             raise RuntimeError(f"{what}: {ids.numel()} ids and {lens.numel()} lengths")
         return ids.numel()
@@ -93,8 +101,8 @@ class PageTable:
         device (no free page) leaves the table as it was, and ``check`` raises it."""
         n = self._entries("extend", seq_ids, new_lens)
         _hold(stream, seq_ids, new_lens, self._mem)
-        _check(_capi.lib().unillm_hip_page_table_extend(self._h, seq_ids.data_ptr(),
-                                                        new_lens.data_ptr(), n, _stream_ptr(stream)))
+        _check(_capi.lib().unillm_hip_page_table_extend(
+            self._h, seq_ids.data_ptr(), new_lens.data_ptr(), n, _stream_ptr(stream, self._device)))
 
     def truncate(self, seq_ids: torch.Tensor, lens: torch.Tensor,
                  stream: torch.cuda.Stream | None = None) -> None:
@@ -102,25 +110,25 @@ class PageTable:
         pages past them are free again, as before the extend that took them.  Ends the plan."""
         n = self._entries("truncate", seq_ids, lens)
         _hold(stream, seq_ids, lens, self._mem)
-        _check(_capi.lib().unillm_hip_page_table_truncate(self._h, seq_ids.data_ptr(),
-                                                          lens.data_ptr(), n, _stream_ptr(stream)))
+        _check(_capi.lib().unillm_hip_page_table_truncate(
+            self._h, seq_ids.data_ptr(), lens.data_ptr(), n, _stream_ptr(stream, self._device)))
 
     def release(self, seq_ids: torch.Tensor, stream: torch.cuda.Stream | None = None) -> None:
         """Finished requests: all their pages are free again."""
         n = self._entries("release", seq_ids, None)
         _hold(stream, seq_ids, self._mem)
-        _check(_capi.lib().unillm_hip_page_table_truncate(self._h, seq_ids.data_ptr(), None, n,
-                                                          _stream_ptr(stream)))
+        _check(_capi.lib().unillm_hip_page_table_truncate(
+            self._h, seq_ids.data_ptr(), None, n, _stream_ptr(stream, self._device)))
 
     def clear(self, stream: torch.cuda.Stream | None = None) -> None:
         """No sequence holds a token, every page is free."""
         _hold(stream, self._mem)
-        _check(_capi.lib().unillm_hip_page_table_clear(self._h, _stream_ptr(stream)))
+        _check(_capi.lib().unillm_hip_page_table_clear(self._h, _stream_ptr(stream, self._device)))
 
     def check(self, stream: torch.cuda.Stream | None = None) -> None:
         """Waits for the stream and raises the first call since the last check that failed on
         the device."""
-        _check(_capi.lib().unillm_hip_page_table_check(self._h, _stream_ptr(stream)))
+        _check(_capi.lib().unillm_hip_page_table_check(self._h, _stream_ptr(stream, self._device)))
 
     def close(self) -> None:
         if self._h is not None and self._h.value:
@@ -162,7 +170,7 @@ class PagedKvCache:
                                                       page_size, float(rope_theta), k.data_ptr(),
                                                       v.data_ptr(), ctypes.byref(h)))
         self._h = h
-        self.k, self.v, self.dtype = k, v, dtype
+        self.k, self.v, self.dtype, self._device = k, v, dtype, k.device
         self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
         self.n_pages, self.page_size = n_pages, page_size
 
@@ -171,7 +179,7 @@ class PagedKvCache:
         """Grow the stream's workspace for calls of up to n_tokens rows, so that they can be
         captured into a HIP graph."""
         _check(_capi.lib().unillm_hip_paged_attention_reserve(self._h, table._h, n_tokens, n_heads,
-                                                              _stream_ptr(stream)))
+                                                              _stream_ptr(stream, self._device)))
 
     def attention(self, table: PageTable, qkv: torch.Tensor, n_heads: int, window: int = 0,
                   sinks: int = 0, out: torch.Tensor | None = None,
@@ -183,25 +191,28 @@ class PagedKvCache:
         width, owidth = (n_heads + 2 * self.n_kv_heads) * self.head_dim, n_heads * self.head_dim
 
         def rows(t, w):
-            return (t.dtype == torch.float32 and t.device == self.k.device and t.dim() == 2
+            return (t.dtype == torch.float32 and t.device == self._device and t.dim() == 2
                     and t.shape[1] == w and (t.stride(1) == 1 or t.numel() == 0))
 
-        if table._mem.device != self.k.device:
+        if table._device != self._device:
             raise RuntimeError("paged attention: the table is on another device")
         if not rows(qkv, width):
             raise RuntimeError(f"paged attention: qkv must be an f32 [n, {width}] tensor on "
-                               f"{self.k.device} with contiguous rows")
+                               f"{self._device} with contiguous rows")
         n = qkv.shape[0]
-        if out is None:
-            out = torch.empty(n, owidth, dtype=torch.float32, device=qkv.device)
+        if out is None:  # (memory that `stream` may write at once: its own)
+            with torch.cuda.stream(stream):
+                out = torch.empty(n, owidth, dtype=torch.float32, device=self._device)
+            if stream is not None:
+                out.record_stream(torch.cuda.current_stream(self._device))
         elif not rows(out, owidth) or out.shape[0] != n:
             raise RuntimeError(f"paged attention: out must be an f32 [{n}, {owidth}] tensor on "
-                               f"{self.k.device} with contiguous rows")
+                               f"{self._device} with contiguous rows")
         _hold(stream, qkv, out, self.k, self.v, table._mem)
         one = n <= 1  # (a single row's stride means nothing)
         _check(_capi.lib().unillm_hip_paged_attention(
             self._h, table._h, qkv.data_ptr(), width if one else qkv.stride(0), n, n_heads, window,
-            sinks, out.data_ptr(), owidth if one else out.stride(0), _stream_ptr(stream)))
+            sinks, out.data_ptr(), owidth if one else out.stride(0), _stream_ptr(stream, self._device)))
         return out
 
     def close(self) -> None:
