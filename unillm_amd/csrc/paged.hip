@@ -90,7 +90,9 @@ struct Call {
     int* redo;
     struct Kind {
         int tile_rows;  // most query rows of a tile
-        int target;     // pieces to deal the kind's work out in, over all kv heads
+        int places;     // workgroups of the kind that the device holds
+        int target;     // most pieces to deal the kind's work out in, over all kv heads, but for
+                        // tiles' remainders; at least places
         int least;      // visits of the smallest piece
         int overhead;   // of a piece, in visits
         int row0;       // its first partial row
@@ -101,7 +103,10 @@ struct Call {
 };
 
 constexpr int kNarrow = 0, kWide = 1;
-constexpr int kNarrowRows = 64;  // most query rows of an entry (a kv head) for narrow tiles
+// Most query rows of an entry (a kv head) for narrow tiles.  (8 entries on 4000 keys, 8 kv heads of
+// 128, f16 / bf16 / f32, us: of 48 rows narrow 65 / 65 / 114, wide 80 / 125 / 180; of 128 rows 132 /
+// 133 / 250 and 82 / 124 / 188; of 96 rows 104 / 104 / 194 and 81 / 125 / 186.)
+constexpr int kNarrowRows = 64;
 constexpr int kTileRows = 16;    // query rows of a narrow tile
 constexpr int kUnit = 32;        // keys of a narrow tile's visit
 // Wide tiles: groups of four waves of 32 rows each (what the registers hold: two groups, one at
@@ -224,28 +229,45 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     if ((tid & 63) == 0) part[tid >> 6] = sum;
     __syncthreads();
     sum = part[0] + part[1] + part[2] + part[3];
+    // (In 32 bits where they hold it: 64-bit divisions are long.  No tile has more than 2^27
+    // visits: so large a C is whole tiles.)
+    const long long work = sum * a.KVH;
+    auto equal = [&](int n) {
+        const int C = work < 1 << 30 ? ((int)work + n - 1) / n
+                                     : (int)min<long long>(1 << 28, (work + n - 1) / n);
+        return max(kd.least, C);
+    };
+    auto pieces = [&](int nv, int C) { return (nv - 1) / C + 1; };
     // The lists' and the partial rows' room is what this C can need, and a larger one needs less.
-    const int C0 = max(kd.least, (int)((sum * a.KVH + kd.target - 1) / kd.target));
-    // Wide, few tiles: of C0, 5 / 4, 3 / 2 and 2 C0 and whole tiles the one of the shortest time, in
+    int C = equal(kd.target), longest = INT_MAX;
+    // A piece for every place the device has, if tiles' remainders make no more of them: no piece
+    // then waits for a place.  Otherwise (narrow) the larger number, whose second round is shorter.
+    // (16 rows on 32000 keys, hd 256, f32: 112 us, with 3 pieces a CU 133; 8 entries of 48 rows on
+    // 4000 keys, hd 128, f16, where 2 a CU make 576: 76 us, with 3 a CU 65.)
+    bool fit = false;
+    if ((kind == kWide || kd.places < kd.target) && (int64_t)tiles * a.KVH <= kd.places) {
+        const int one_each = equal(kd.places);
+        __shared__ int made;
+        if (tid == 0) made = 0;
+        __syncthreads();
+        int n = mine.nv > 0 ? pieces(mine.nv, one_each) : 0;
+        for (int i = tid + 256; i < tiles; i += 256) n += pieces(tile(i).nv, one_each);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+        if ((tid & 63) == 0 && n > 0) atomicAdd(&made, n);
+        __syncthreads();
+        fit = (int64_t)made * a.KVH <= kd.places;
+        if (fit) C = one_each;
+    }
+    // Else wide, few tiles: of C0 = C, 5 / 4, 3 / 2 and 2 C0 and whole tiles the one of the shortest time, in
     // visits.  An item's own time is `overhead` visits, and as much again where its sums go
     // through memory.  Up to as many items as places take the largest one's time; up to twice as
     // many, the sum of an item's and of one that follows it, the sizes sorted: the last to find a
     // place of its own and the next, or the largest that is followed and the smallest; more, the
     // mean place's load and half an item.  (Three chunks among 24 sequences, bf16: 152 us with
     // pieces of 18 visits, 272 for 256 places, whose small ones pair up; 190 with pieces of 30, 216.)
-    int C = C0, longest = INT_MAX;
-    bool search = false;  // (as many places as items of C0: no C is better)
-    if (kind == kWide && (int64_t)tiles * a.KVH <= 4 * (int64_t)kd.target) {
-        __shared__ int made;
-        if (tid == 0) made = 0;
-        __syncthreads();
-        int n = mine.nv > 0 ? (mine.nv - 1) / C0 + 1 : 0;
-        for (int i = tid + 256; i < tiles; i += 256) n += (tile(i).nv - 1) / C0 + 1;
-        if (n > 0) atomicAdd(&made, n);
-        __syncthreads();
-        search = (int64_t)made * a.KVH > kd.target;
-    }
-    if (search) {
+    if (!fit && kind == kWide && (int64_t)tiles * a.KVH <= 4 * (int64_t)kd.places) {
+        const int C0 = C;
         constexpr int TRY = 5, BINS = 32;
         __shared__ int hist[TRY][BINS], split_made[TRY], top;
         __shared__ float times[TRY];
@@ -264,7 +286,7 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
             const int nv = i < 256 ? mine.nv : tile(i).nv;
 #pragma unroll
             for (int k = 0; k < TRY; ++k) {
-                const int S = (nv - 1) / candidate(k) + 1;
+                const int S = pieces(nv, candidate(k));
                 atomicAdd(&hist[k][min(BINS - 1, (int)((float)nv / (float)S * bin))], S);
                 if (S > 1) atomicAdd(&split_made[k], S);
             }
@@ -272,7 +294,7 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         __syncthreads();
         const int lane = tid & 63;
         for (int k = tid >> 6; k < TRY; k += 4) {  // a wave a candidate, a lane a bin
-            const int places = max(1, kd.target / a.KVH), h = lane < BINS ? hist[k][lane] : 0;
+            const int places = max(1, kd.places / a.KVH), h = lane < BINS ? hist[k][lane] : 0;
             int upto = h;  // items of this size and larger
 #pragma unroll
             for (int o = 1; o < BINS; o <<= 1) {
@@ -306,7 +328,6 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     // beside it, whose keys are the same): what is dealt out last fills the gaps.  The four
     // ranks' numbers are 16 bits each of a scan's first value: pieces are at most target + tiles.
     const int largest = min(C, longest);
-    auto pieces = [&](int nv) { return (nv - 1) / C + 1; };
     auto rank = [&](int nv, int S) { return 3 - min(3, (int)(4 * (int64_t)(nv / S) / largest)); };
     int fill[4] = {0, 0, 0, 0};
     if (tiles > 256) {
@@ -314,7 +335,7 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         if (tid < 4) count[tid] = 0;
         __syncthreads();
         for (int i = tid; i < tiles; i += 256) {
-            const int nv = tile(i).nv, S = pieces(nv);
+            const int nv = tile(i).nv, S = pieces(nv, C);
             atomicAdd(&count[rank(nv, S)], S);
         }
         __syncthreads();
@@ -326,7 +347,7 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         const int i = i0 + tid;
         Tile x = mine;
         if (i0 > 0 && i < tiles) x = tile(i);
-        const int S = i < tiles ? pieces(x.nv) : 0, rk = S > 0 ? rank(x.nv, S) : 0;
+        const int S = i < tiles ? pieces(x.nv, C) : 0, rk = S > 0 ? rank(x.nv, S) : 0;
         const int want = S > 1 ? S * a.KVH * x.rows : 0;
         const int first = S > 0 ? t.cu[x.b] : 0, id = S > 0 ? t.step_ids[x.b] : 0;
         ulong2 all;
@@ -379,11 +400,15 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
 }
 
 // The first kernel of a call.  Workgroups 0 and 1 deal the work out; each other one takes nr rows
-// of the step (16, or 4 of a short one) and `heads` kv heads: the rows' rotations (kept in f32 for the queries), their
+// of the step and `heads` kv heads: the rows' rotations (kept in f32 for the queries), their
 // keys rotated and stored, their values stored.  A V page runs along the keys, so where 8 rows
 // are 8 neighbouring slots of a page, aligned (a prompt's rows, but for its ends), a thread
-// stores a dimension's 8 values at once; other rows value by value.  (2048 rows of 32 heads of
-// 128: 65 us with every value on its own, a row after the other.)
+// stores a dimension's 8 values at once; other rows value by value.
+// Bound by HBM where rows are many: 2048 rows of 32 kv heads of 128, f16, 100 MB in 21 us (65 with
+// every value on its own, a row after the other); by latency and by the plan where they are few:
+// 5 us for one row, 12 where three chunks of 24 entries are dealt out.
+// nr is 16, or 4 of a step of up to 512 rows, whose workgroups are too few otherwise (a whole call of
+// 512 such rows 44 us, 45 with 16 a workgroup; of 2048 rows 127 us, 142 with 4).
 constexpr int kAppendRows = 16;
 
 template <class T, int D>
@@ -659,7 +684,9 @@ __device__ __forceinline__ f32x8 rotated8(const Call& a, int first, int g, int r
 // one's are used, its values likewise, so each has the other's products to arrive in.
 // The reference that the weights' exponents are taken against follows a row's maximum only when
 // some score passes it by 2^8, so a visit needs no exchange between lanes; the sums of the
-// weights stay per lane until the end.  Bound by HBM: 4 D bytes of a 16-bit pool a key.
+// weights stay per lane until the end.  Bound by HBM: 4 D bytes of a 16-bit pool a key (one GB of f16
+// at hd 128, two sequences of up to 131040 keys: 178 us, 5.7 TB/s; 64 sequences, bf16, 596 MB: 109 us, 5.5 TB/s),
+// and for short sequences by latency (one, of 4000 keys: 8 us).
 template <class T, int D>
 struct NarrowLds {
     static constexpr int NB = D / 32, OT = D / 16;
@@ -948,12 +975,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
 // operand of the second product contracts.
 // Visit n is a matrix phase, p v of visit n - 1 and q k of visit n, and a vector phase, the
 // weights of visit n; a barrier ends each.  The two groups of four waves, a wave of each on every
-// SIMD, are a phase apart, so the matrix cores and the vector units are both at work: without
-// that the two workgroups of a CU ran their phases together (a 2048-token prompt of 32 heads of
-// 128, f16: matrix cores busy 20 % of the time, 142 us).  V of n - 1 and K of n share one of two
+// SIMD, are a phase apart, so the matrix cores and the vector units are both at work (as two
+// workgroups a CU they ran their phases together).  V of n - 1 and K of n share one of two
 // LDS buffers; each group stores its half of the next pair in its vector phase, requested one
 // visit before.
-// Bound by the matrix cores: Parts::N times the products of a 16-bit attention.
+// Bound by the matrix cores, with Parts::N times the products of a 16-bit attention, and at hd 64
+// by the vector units (a visit's weights 1400 to 1600 cycles, its products 1024).  At hd 128 in f16 a visit
+// takes 3000 cycles of matrix phase, 2048 of them MFMAs back to back, the rest reads of LDS and the
+// barriers.  A 2048-token prompt of 32 heads of 128, f16, 34 GFLOP in two parts: 101 us, 680 TFLOP/s
+// of f16 products, where a large library product reaches 1066.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <class T>
@@ -1589,8 +1619,11 @@ struct Layout {
     size_t head_at[2], items_at[2], splits_at[2], turn_at, ms_at, po_at, count_at, redo_at, bytes;
 };
 
-// Pieces a kind's work is dealt out in: narrow, three workgroups of four waves for every CU; wide,
-// the one of eight waves (of four at hd 256) that a CU holds.
+// Workgroups of a kind that the device holds: wide one a CU, narrow by its registers.
+int places(int kind, int64_t D) {
+    return (kind == kWide || D == 256 ? 1 : D == 128 ? 2 : 3) * device_info().cu_count;
+}
+// Pieces a kind's work is dealt out in at most.
 int target_pieces(int kind) { return (kind == kNarrow ? 3 : 1) * device_info().cu_count; }
 
 int tile_rows(int kind, int64_t D) { return kind == kNarrow ? kTileRows : D < 256 ? 256 : 128; }
@@ -1691,9 +1724,9 @@ hipError_t launch_paged_attention(const PagedKv& c, const unillm_page_table& t, 
            reinterpret_cast<float*>(w + l.po_at), reinterpret_cast<int*>(w + l.count_at),
            reinterpret_cast<int*>(w + l.redo_at), {}};
     for (int k = 0; k < 2; ++k)
-        a.kind[k] = {tile_rows(k, c.head_dim), target_pieces(k), k == kNarrow ? 4 : 2, 5,
-                     k == kNarrow ? 0 : (int)l.rows[0], reinterpret_cast<int*>(w + l.head_at[k]),
-                     reinterpret_cast<Item*>(w + l.items_at[k]),
+        a.kind[k] = {tile_rows(k, c.head_dim), places(k, c.head_dim), target_pieces(k),
+                     k == kNarrow ? 4 : 2, 5, k == kNarrow ? 0 : (int)l.rows[0],
+                     reinterpret_cast<int*>(w + l.head_at[k]), reinterpret_cast<Item*>(w + l.items_at[k]),
                      reinterpret_cast<Split*>(w + l.splits_at[k])};
     if (c.type == UNILLM_QTYPE_F32) return launch_type<float>(c, t, a, l, s);
     if (c.type == UNILLM_QTYPE_F16) return launch_type<f16_t>(c, t, a, l, s);

@@ -159,6 +159,7 @@ class PagedKvCache:
         shapes = ((n_pages, n_kv_heads, page_size, head_dim), (n_pages, n_kv_heads, head_dim, page_size))
         if k is None:
             k, v = (torch.zeros(s, dtype=dtype, device=device or "cuda") for s in shapes)
+            torch.cuda.current_stream(k.device).synchronize()  # zeroed for every stream
         for name, t, s in (("k", k, shapes[0]), ("v", v, shapes[1])):
             if tuple(t.shape) != s or t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
                 raise RuntimeError(f"PagedKvCache: {name} must be a contiguous {dtype} device "
