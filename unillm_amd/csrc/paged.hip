@@ -1014,11 +1014,15 @@ struct WideLds {
     static constexpr int KROW = 2 * D, VROW = 2 * U;
     static constexpr int PLANE = U * KROW;                  // of K, and of V^T
     static constexpr int K = 0, V = KPARTS * PLANE, PAIR = 2 * V;
-    static constexpr int QL = GR * PAIR;                    // q's last part, where registers lack
-    static constexpr bool kQl = sizeof(T) == 2 && D == 128;
+    // q's last part, where registers lack: held there the queries spill to memory (8 heads on one kv
+    // head, 2000 tokens behind 8000, us: f32 hd 64 241 -> 222, 128 434 -> 395, 256 1418 -> 963; bf16
+    // hd 256 740 -> 483, f16 428 -> 399)
+    static constexpr int QL = GR * PAIR;
+    static constexpr bool kQl = D >= 128 || sizeof(T) == 4;
+    static constexpr int QL0 = sizeof(T) == 4 && D >= 128 ? 1 : 0;    // from this block of 16 dimensions on (LDS is full)
     static constexpr int QREGS = Parts<T>::Q - (kQl ? 1 : 0);
     static constexpr int QROWS = 32 * D * 4;                // a wave's rows in f32, before and after
-    static constexpr int USED = QL + (kQl ? NT / 64 * (D / 16) * 1024 : 0), ROWS = NT / 64 * QROWS;
+    static constexpr int USED = QL + (kQl ? NT / 64 * (D / 16 - QL0) * 1024 : 0), ROWS = NT / 64 * QROWS;
     static constexpr int STAT = USED > ROWS ? USED : ROWS;  // whether a page is bad
     static constexpr int BYTES = STAT + 64;
     static constexpr int TASKS = U * D / 8 / NT;            // 8-element chunks of K (or V) a thread
@@ -1172,14 +1176,14 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
         fetch(0);
 
         u32x4 q[L::QREGS][NB];
-        u32x4* ql = reinterpret_cast<u32x4*>(lds + L::QL) + wv * NB * 64 + lane;
+        u32x4* ql = reinterpret_cast<u32x4*>(lds + L::QL) + (wv * (NB - L::QL0) - L::QL0) * 64 + lane;
         __syncthreads();  // (the item before is done with the LDS)
         if (tid == 0) flags[0] = 0;
         float inv = 1.0f;
         // The wave's rows of q and of their rotations come whole rows at a time and through its own
         // part of the LDS: a lane's operand is 32 bytes of a row, and loaded so every request would
         // touch 32 lines (22000 cycles an item at hd 128 before, of 115000).
-        u32x4 qlast[L::kQl ? NB : 1];
+        u32x4 qfirst;
         {
             // (opaque lane numbers here and at the end: no address of these is kept through the visits)
             int el = lane;
@@ -1187,15 +1191,23 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
             constexpr int CH = D / 4, N = 32 * CH / 64;  // 16-byte chunks of a row, requests of 32 rows
             f32x4* own = reinterpret_cast<f32x4*>(lds + wv * L::QROWS);
             auto slot = [&](int r, int ch) { return r * CH + (ch ^ (r & (CH - 1 < 31 ? CH - 1 : 31))); };
-            f32x4 x[N];
+            // (requests at once: with all 32 of hd 256 the compiler spills, tuples of four in two places,
+            // and reads one back wrong)
+            constexpr int NX = N < 16 ? N : 16;
             // (a lane's own row is `myrow`: its place is handed to the lanes that load it)
             auto rows = [&](const float* from, int64_t place) {
 #pragma unroll
-                for (int i = 0; i < N; ++i)
-                    x[i] = reinterpret_cast<const f32x4*>(from + __shfl(place, (i * 64 + el) / CH, 64))[el % CH];
-                __builtin_amdgcn_sched_barrier(0);
+                for (int i0 = 0; i0 < N; i0 += NX) {
+                    f32x4 x[NX];
 #pragma unroll
-                for (int i = 0; i < N; ++i) own[slot((i * 64 + el) / CH, el % CH)] = x[i];
+                    for (int i = 0; i < NX; ++i)
+                        x[i] = reinterpret_cast<const f32x4*>(
+                            from + __shfl(place, ((i0 + i) * 64 + el) / CH, 64))[el % CH];
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < NX; ++i) own[slot(((i0 + i) * 64 + el) / CH, el % CH)] = x[i];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 settle_wave();
             };
             f32x8 r[NB];
@@ -1236,6 +1248,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                 up = sc.x;
                 inv = sc.y;
             }
+            __syncthreads();  // (every wave is done with its rows: the buffers and q's last parts go there)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (std::is_same_v<T, f16_t>) r[b] *= up;
@@ -1243,13 +1256,10 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                 split_q<T>(r[b], p);
 #pragma unroll
                 for (int i = 0; i < L::QREGS; ++i) q[i][b] = p[i];
-                if (L::kQl) qlast[L::kQl ? b : 0] = p[P::Q - 1];
+                if (L::kQl && b < L::QL0) qfirst = p[P::Q - 1];
+                else if (L::kQl) ql[b * 64] = p[P::Q - 1];
             }
         }
-        __syncthreads();  // (every wave is done with its rows: the buffers and q's last parts go there)
-        if (L::kQl)
-#pragma unroll
-            for (int b = 0; b < (L::kQl ? NB : 0); ++b) ql[b * 64] = qlast[b];
         float ref = -INFINITY, l = 0.0f;
         f32x16 o[OT];
 #pragma unroll
@@ -1288,7 +1298,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                     for (int x = 0; x < P::K; ++x)
                         kp[b % 2][u][x] = *reinterpret_cast<const u32x4*>(
                             buf + L::K + x * L::PLANE + 32 * u * L::KROW + (ka ^ 32 * b));
-                if (L::kQl) qx[b % 2] = ql[b * 64];
+                if (L::kQl) qx[b % 2] = b < L::QL0 ? qfirst : ql[b * 64];
             };
             read(0);
 #pragma unroll
