@@ -973,7 +973,6 @@ int unillm_hip_page_table_create(int64_t max_seqs, int64_t max_pages, int64_t n_
              at(l.table), at(l.lens), at(l.free_pages), at(l.cu), at(l.ids), at(l.step_lens),
              at(l.slots), at(l.positions), at(l.counts)};
     t->device = g_device;
-    t->entries = 0;
     if ((e = launch_pages_clear(t->st, nullptr)) != hipSuccess ||
         (e = hipStreamSynchronize(nullptr)) != hipSuccess) {
         if (t->owned) (void)hipFree(t->storage);
@@ -1019,9 +1018,7 @@ int unillm_hip_page_table_extend(unillm_page_table* t, const int32_t* seq_ids_de
     if (int rc = ensure_init()) return rc;
     hipError_t e = launch_pages_extend(t->st, seq_ids_dev, new_lens_dev, n_seqs,
                                        static_cast<hipStream_t>(stream));
-    if (e != hipSuccess) return fail_hip(e, "page table extend");
-    t->entries = n_seqs;
-    return UNILLM_OK;
+    return e == hipSuccess ? UNILLM_OK : fail_hip(e, "page table extend");
 }
 
 int unillm_hip_page_table_truncate(unillm_page_table* t, const int32_t* seq_ids_dev,

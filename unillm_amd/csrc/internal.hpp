@@ -94,14 +94,12 @@ struct unillm_page_state {
     int* counts;      // [kPagesCounts], below
 };
 
-// The opaque page-table handle.  entries: the batch of the last extend (what an attention
-// call sizes its grid for; its kernels take the device's own count).
+// The opaque page-table handle.
 struct unillm_page_table {
     unillm_page_state st;
     int device;
     void* storage;
     bool owned;
-    int64_t entries;
 };
 
 // The opaque handle of one layer's pool of KV pages: K [n_pages][n_kv_heads][page_size][hd],
