@@ -217,7 +217,8 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         const int each = kind == kNarrow ? TR : ((rows + n - 1) / n + 31) / 32 * 32;
         Tile x{lo, (tp[lo + 1] - 1 - i) * each, 0, 0};  // (an entry's last, which sees the most keys, first)
         x.rows = min(each, rows - x.row0);
-        x.nv = Visits<U>(ctxs[lo] + x.row0 / a.G, ctxs[lo] + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks).count;
+        const int last = x.row0 + x.rows - 1;
+        x.nv = Visits<U>(ctxs[lo] + x.row0 / a.G, ctxs[lo] + last / a.G, a.window, a.sinks).count;
         return x;
     };
     Tile mine{0, 0, 0, 0};  // the thread's first
@@ -275,7 +276,9 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         if (tid < TRY) split_made[tid] = 0;
         if (tid == 0) top = 0;
         __syncthreads();
-        auto candidate = [&](int k) { return k == 0 ? C0 : k == 1 ? C0 + C0 / 4 : k == 2 ? C0 + C0 / 2 : k == 3 ? 2 * C0 : INT_MAX / 2; };
+        auto candidate = [&](int k) {
+            return k == 0 ? C0 : k == 1 ? C0 + C0 / 4 : k == 2 ? C0 + C0 / 2 : k == 3 ? 2 * C0 : INT_MAX / 2;
+        };
         int my_top = mine.nv;
         for (int i = tid + 256; i < tiles; i += 256) my_top = max(my_top, tile(i).nv);
         if (my_top > 0) atomicMax(&top, my_top);
@@ -312,7 +315,8 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
                     const uint64_t here = __ballot(lane < BINS && rank >= upto - h && rank < upto);
                     return (float)__builtin_ctzll(here | 1ull << 63) / bin;
                 };
-                time = fmaxf(item, 2.0f * ov + fmaxf(size(places - 1) + size(places), size(2 * places - n) + size(n - 1)));
+                time = fmaxf(item, 2.0f * ov + fmaxf(size(places - 1) + size(places),
+                                                     size(2 * places - n) + size(n - 1)));
             }
             if (lane == 0) times[k] = time;
         }
@@ -351,7 +355,8 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
         const int want = S > 1 ? S * a.KVH * x.rows : 0;
         const int first = S > 0 ? t.cu[x.b] : 0, id = S > 0 ? t.step_ids[x.b] : 0;
         ulong2 all;
-        const ulong2 n = block_scan(ulong2{(uint64_t)S << (16 * rk), (uint64_t)want << 16 | (S > 1 ? 1 : 0)}, tmp, &all);
+        const ulong2 n = block_scan(
+            ulong2{(uint64_t)S << (16 * rk), (uint64_t)want << 16 | (S > 1 ? 1 : 0)}, tmp, &all);
         auto field = [](uint64_t v, int e) { return (int)(v >> (16 * e) & 0xFFFF); };
         if (tiles <= 256)
 #pragma unroll
@@ -371,7 +376,8 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
 #pragma unroll
         for (int e = 0; e < 7; ++e) info[tid][e] = v[e];
         if (want) kd.splits[splits + (int)(n.y & 0xFFFF) - 1] = {first, x.row0, x.rows, base, S, {}};
-        if (S == 1) kd.items[at] = {first, ctxs[x.b], ctxs[x.b] + ms[x.b], id, x.row0, x.rows, 0, x.nv, base, 0, 1, 0};
+        if (S == 1)
+            kd.items[at] = {first, ctxs[x.b], ctxs[x.b] + ms[x.b], id, x.row0, x.rows, 0, x.nv, base, 0, 1, 0};
         __syncthreads();
         if ((all.y & 0xFFFF) != 0)
             for (int k = tid; k < made; k += 256) {  // tiles in pieces: a thread a piece
@@ -386,7 +392,8 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
                 if (Sw < 2) continue;
                 const int v0 = (int)((int64_t)s * nv / Sw), v1 = (int)((int64_t)(s + 1) * nv / Sw);
                 const int b = w[0], ctx = ctxs[b];
-                kd.items[w[6] + s] = {t.cu[b], ctx, ctx + ms[b], t.step_ids[b], w[1], w[2], v0, v1 - v0, w[4], s, Sw, 0};
+                kd.items[w[6] + s] = {t.cu[b], ctx, ctx + ms[b], t.step_ids[b], w[1], w[2],
+                                      v0, v1 - v0, w[4], s, Sw, 0};
             }
         items += made;
         splits += (int)(all.y & 0xFFFF);
@@ -448,7 +455,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable 
     __shared__ int list[2], run_rows[NR], one_rows[NR];
     if (tid < 64) {
         const int sl = tid < rows ? slots[tid + 7] : -1, s0 = tid - (sl & 7);
-        const bool run = sl >= 0 && s0 >= -7 && s0 < nr && slots[s0 + 7] == (sl & ~7) && slots[s0 + 14] == (sl | 7);
+        const bool run = sl >= 0 && s0 >= -7 && s0 < nr && slots[s0 + 7] == (sl & ~7) &&
+                         slots[s0 + 14] == (sl | 7);
         const uint64_t begins = __ballot(run && (sl & 7) == 0), ones = __ballot(sl >= 0 && !run);
         const uint64_t before = (1ull << tid) - 1;
         if (begins >> tid & 1) run_rows[__popcll(begins & before)] = tid;
@@ -498,7 +506,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable 
     for (int i = wv; i < (g1 - g0) * n_runs * DG; i += 4) {
         const int g = g0 + i / (n_runs * DG), r = run_rows[i / DG % n_runs], d = i % DG * 64 + lane;
         const int sl = slots[r + 7];
-        T* dst = static_cast<T*>(c.v) + (((((int64_t)(sl >> shift) * KVH + g) * D + d) << shift) + (sl & (ps - 1)));
+        T* dst = static_cast<T*>(c.v) +
+                 (((((int64_t)(sl >> shift) * KVH + g) * D + d) << shift) + (sl & (ps - 1)));
         const float* x = xv + r * a.qstride + (int64_t)g * D + d;
         struct alignas(16) Eight {
             T v[8];
@@ -524,7 +533,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable 
             if (i >= tasks) break;
             const int g = g0 + i / (n_ones * DG), d = i % DG * 64 + lane;
             const int sl = slots[one_rows[i / DG % n_ones] + 7];
-            static_cast<T*>(c.v)[((((int64_t)(sl >> shift) * KVH + g) * D + d) << shift) + (sl & (ps - 1))] = narrow<T>(x[k]);
+            T* page = static_cast<T*>(c.v) + ((((int64_t)(sl >> shift) * KVH + g) * D + d) << shift);
+            page[sl & (ps - 1)] = narrow<T>(x[k]);
         }
     }
 }
@@ -689,7 +699,8 @@ __device__ __forceinline__ f32x8 rotated8(const Call& a, int first, int g, int r
 // The reference that the weights' exponents are taken against follows a row's maximum only when
 // some score passes it by 2^8, so a visit needs no exchange between lanes; the sums of the
 // weights stay per lane until the end.  Bound by HBM: 4 D bytes of a 16-bit pool a key (one GB of f16
-// at hd 128, two sequences of up to 131040 keys: 178 us, 5.7 TB/s; 64 sequences, bf16, 596 MB: 109 us, 5.5 TB/s),
+// at hd 128, two sequences of up to 131040 keys: 177 us, 5.8 TB/s; 64 sequences, bf16, 596 MB: 109 us,
+// 5.5 TB/s),
 // and for short sequences by latency (one, of 4000 keys: 8 us).
 template <class T, int D>
 struct NarrowLds {
@@ -962,7 +973,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
                         bad_page ? f32x4(__builtin_nanf("")) : res[i];
             if (wv == 0 && qd == 0) {
                 if (again) redo_row(a, row, h);
-                if (!whole) a.ms[piece] = make_float2(top - P::shift, again || bad_page ? __builtin_nanf("") : sum);
+                if (!whole)
+                    a.ms[piece] = make_float2(top - P::shift, again || bad_page ? __builtin_nanf("") : sum);
             }
         }
     }
@@ -1019,7 +1031,8 @@ struct WideLds {
     // hd 256 740 -> 483, f16 428 -> 399)
     static constexpr int QL = GR * PAIR;
     static constexpr bool kQl = D >= 128 || sizeof(T) == 4;
-    static constexpr int QL0 = sizeof(T) == 4 && D >= 128 ? 1 : 0;    // from this block of 16 dimensions on (LDS is full)
+    // (from this block of 16 dimensions on: LDS is full)
+    static constexpr int QL0 = sizeof(T) == 4 && D >= 128 ? 1 : 0;
     static constexpr int QREGS = Parts<T>::Q - (kQl ? 1 : 0);
     static constexpr int QROWS = 32 * D * 4;                // a wave's rows in f32, before and after
     static constexpr int USED = QL + (kQl ? NT / 64 * (D / 16 - QL0) * 1024 : 0), ROWS = NT / 64 * QROWS;
@@ -1035,7 +1048,8 @@ struct WideLds {
 };
 
 template <class T, int D>
-__global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void paged_wide_kernel(PagedKv c, PageTable t, Call a) {
+__global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void paged_wide_kernel(
+    PagedKv c, PageTable t, Call a) {
     using L = WideLds<T, D>;
     using P = Parts<T>;
     constexpr int U = L::U, NB = D / 16, OT = D / 32, NG = U / 32, GR = L::GR, NT = L::NT;
@@ -1045,7 +1059,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
     // A buffer's pair m - 2 was last read in the second group's matrix phase m - 2, so either group may
     // store its share of pair m in the two phases after: its matrix phase m - 1, or the vector
     // phase m - 1 (m - 2 in the second group).  The stores go with the shorter phase (f16: at hd 128
-    // a matrix phase takes 2330 cycles, the weights 1290; at hd 64 1350 and 1600).
+    // a matrix phase takes 3000 cycles, the weights 1470; at hd 64 1350 and 1600).
     constexpr bool kStoreEarly = GR == 2 && D == 64 && sizeof(T) == 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
@@ -1435,7 +1449,8 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
         if (mine && hf == 0) {
             const int rr = it.row0 + w0 + col;
             if (again) redo_row(a, first + rr / G, g * G + rr % G);
-            if (!whole) a.ms[piece + w0 + col] = make_float2(ref - P::shift, again || bad_page ? __builtin_nanf("") : l);
+            if (!whole)
+                a.ms[piece + w0 + col] = make_float2(ref - P::shift, again || bad_page ? __builtin_nanf("") : l);
         }
         // whole rows out, through the wave's part of the LDS (a row with a bad page is NaN, whatever its
         // other pieces hold)
@@ -1553,8 +1568,8 @@ __device__ void attend_row(const PagedKv& c, const Call& a, const int* pages, in
     for (int i = 0; i < D / 64; ++i) acc[i] = l != l ? l : acc[i] / l;
 }
 
-// The last kernel of a call.  The pieces of a tile dealt out, joined: out = sum_s 2^(M_s - M) o_s / sum_s 2^(M_s - M) l_s over the
-// pieces' (M_s, l_s, o_s); a piece in which a row sees no key has M_s = -inf, weight 0.  A
+// The last kernel of a call.  The pieces of a tile dealt out, joined: out = sum_s 2^(M_s - M) o_s /
+// sum_s 2^(M_s - M) l_s over the pieces' (M_s, l_s, o_s); a piece in which a row sees no key has M_s = -inf, weight 0.  A
 // workgroup per (16 rows of a tile, kv head), D / 4 threads to a row; where there are fewer rows
 // than such groups, several share a row's pieces and meet in LDS.  A row with a piece of NaN sum
 // is left: its output is written (a bad page), or it is one of the rows listed to be done again,
