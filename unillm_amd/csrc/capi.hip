@@ -1124,8 +1124,9 @@ int unillm_hip_paged_kv_create(int kv_type, int64_t n_kv_heads, int64_t head_dim
     if (e == hipSuccess)
         e = hipMemcpy(f, freq.data(), freq.size() * sizeof(double), hipMemcpyHostToDevice);
     if (c->owned && e == hipSuccess && (e = hipMalloc(&c->k, bytes)) == hipSuccess &&
-        (e = hipMalloc(&c->v, bytes)) == hipSuccess && (e = hipMemset(c->k, 0, bytes)) == hipSuccess)
-        e = hipMemset(c->v, 0, bytes);
+        (e = hipMalloc(&c->v, bytes)) == hipSuccess && (e = hipMemset(c->k, 0, bytes)) == hipSuccess &&
+        (e = hipMemset(c->v, 0, bytes)) == hipSuccess)
+        e = hipStreamSynchronize(nullptr);  // (zeroed for every stream: a memset may return before it ends)
     if (e != hipSuccess) {
         (void)hipFree(f);
         if (c->owned) {
