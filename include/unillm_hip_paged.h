@@ -87,7 +87,8 @@ int unillm_hip_paged_kv_buffers(const unillm_paged_kv* c, void** k, void** v, si
  * RoPE; the angles p theta^(-2 i / hd) are formed in f64, where unillm_hip_attention_decode
  * takes them in f32), k and v rounded once to the pool's type into the row's slot, and out =
  * softmax(q k^T / sqrt(hd)) v over the positions j <= p of its sequence, at f32's precision
- * whatever the pool's type.  window > 0: only j > p - window, and j < sinks (sliding window
+ * whatever the pool's type (f16: a chunk's row may be off by 2^-16 of its largest output besides,
+ * where keys of almost no value take almost all of its weight).  window > 0: only j > p - window, and j < sinks (sliding window
  * with attention sinks; the reference's masks, crates/runtime/src/tensor_core.rs:1761-1781);
  * window 0: all, sinks 0.  What masked keys and values hold does not matter.
  * Rows past the step's last are left as they were; if the table has no plan, or one of more

@@ -58,6 +58,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -545,28 +546,39 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedKv c, PageTable 
 // single part.  f32 values are sums of parts: against bf16 (and f32, itself three bf16 parts) three
 // bf16 ones, all 24 bits; against f16 two f16 ones, 22 bits, where a power of two per query
 // row brings q into range (its largest magnitude in [2^14, 2^15)) and the weights, at most
-// 2^8 above their reference (below), are taken times 2^7: parts down to 2^-24 then reach
-// 2^-38 of a row's largest element and 2^-31 of the reference weight.
+// 2^slack above their reference (below), are taken times 2^shift: parts down to 2^-24 then reach
+// 2^-38 of a row's largest element and 2^-35 of the reference weight.  A weight is then off by
+// 2^-36 of the reference's at most, and that is too much where the large weights' values are nothing
+// (a key that takes all the attention, of value 0: with the others 16 nats below it the outputs
+// were 1e-3 off).  Narrow tiles multiply a visit with a weight so small by bf16 parts, wide ones
+// look at what came of them (below).
 template <class T>
 struct Parts;
 template <>
 struct Parts<f16_t> {
     static constexpr int K = 1, Q = 2, N = 2;
     static constexpr int ki[N] = {0, 0}, qi[N] = {1, 0};  // products, the large one last
-    static constexpr float shift = 7.0f;
+    static constexpr float shift = 11.0f, slack = 4.0f;
 };
 template <>
 struct Parts<bf16_t> {
     static constexpr int K = 1, Q = 3, N = 3;
     static constexpr int ki[N] = {0, 0, 0}, qi[N] = {2, 1, 0};
-    static constexpr float shift = 0.0f;
+    static constexpr float shift = 0.0f, slack = 8.0f;
 };
 template <>
 struct Parts<float> {
     static constexpr int K = 3, Q = 3, N = 6;
     static constexpr int ki[N] = {2, 0, 1, 1, 0, 0}, qi[N] = {0, 2, 1, 0, 1, 0};
-    static constexpr float shift = 0.0f;
+    static constexpr float shift = 0.0f, slack = 8.0f;
 };
+// How far below a row's reference (log2) a weight held in two parts of f16 may be in a narrow tile's
+// visit: 2^-20 of it is lost at most.  (32 sequences of 8192 keys, scores that make half of the visits
+// and all of them such: 210 and 205 us, 201 with none.)
+constexpr float kSpread = 16.0f;
+// What a wide tile's row may lose by them, of its largest sum.  (Five products a visit would be 7 for 4 in
+// all, and most visits are such where scores spread; few rows' values cancel so far.)
+constexpr float kLoss = 0x1p-16f;
 
 // 8 f32 -> the parts of a q or weight operand
 template <class T>
@@ -642,6 +654,16 @@ __device__ __forceinline__ void split_k(const Raw<T>& r, u32x4 (&p)[Parts<T>::K]
     }
 }
 
+// 8 f16 values -> their two bf16 parts, exactly: 8 of the 11 bits and the rest
+__device__ __forceinline__ void widen_f16(u32x4 r, u32x4 (&p)[2]) {
+    const f32x8 v = __builtin_convertvector(__builtin_bit_cast(f16x8, r), f32x8);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        p[0][j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        p[1][j] = pack_bf16(v[2 * j] - bf16_lo(p[0][j]), v[2 * j + 1] - bf16_hi(p[0][j]));
+    }
+}
+
 template <class T>
 __device__ __forceinline__ f32x4 mfma16(u32x4 x, u32x4 y, f32x4 z) {
     if constexpr (std::is_same_v<T, f16_t>)
@@ -697,7 +719,7 @@ __device__ __forceinline__ f32x8 rotated8(const Call& a, int first, int g, int r
 // A page id per 16 keys is read ahead into LDS; the next visit's keys are requested once this
 // one's are used, its values likewise, so each has the other's products to arrive in.
 // The reference that the weights' exponents are taken against follows a row's maximum only when
-// some score passes it by 2^8, so a visit needs no exchange between lanes; the sums of the
+// some score passes it by 2^slack, so a visit needs no exchange between lanes; the sums of the
 // weights stay per lane until the end.  Bound by HBM: 4 D bytes of a 16-bit pool a key (one GB of f16
 // at hd 128, two sequences of up to 131040 keys: 177 us, 5.8 TB/s; 64 sequences, bf16, 596 MB: 109 us,
 // 5.5 TB/s),
@@ -856,6 +878,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
                 }
                 if (v + 4 < nseg) load_k(v + 4);
                 if (std::is_same_v<T, f16_t>) s *= inv;
+                float low = s[0];  // (hidden keys' among them: their visit only takes longer)
+#pragma unroll
+                for (int r = 1; r < 8; ++r) low = fminf(low, s[r]);
                 // masks, where some row of the tile does not see the whole visit
                 const bool whole = j0 + kUnit - 1 <= pmin &&
                                    (a.window == 0 || j0 > pmax - a.window || j0 + kUnit <= a.sinks);
@@ -871,7 +896,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
                 float top = s[0];
 #pragma unroll
                 for (int r = 1; r < 8; ++r) top = fmaxf(top, s[r]);
-                if (__any(top > ref + 8.0f)) {
+                if (__any(top > ref + P::slack)) {
                     top = fmaxf(top, __shfl_xor(top, 16, 64));
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
                     const float up = fmaxf(ref, top);
@@ -887,8 +912,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
                     s[r] = __builtin_amdgcn_exp2f(s[r] - from);
                     l += s[r];
                 }
-                u32x4 p[P::Q];
-                split_q<T>(s, p);
                 if (j0 + kUnit > len) {  // past the sequence's end a page holds anything
 #pragma unroll
                     for (int i = 0; i < OT; ++i) {
@@ -902,6 +925,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
                             }
                     }
                 }
+                if (std::is_same_v<T, f16_t> && __any(low < ref - kSpread)) {
+                    // weights of any size: five products of three bf16 parts and two (and none is left below)
+                    u32x4 p[3];
+                    split_q<bf16_t>(s, p);
+#pragma unroll
+                    for (int i = 0; i < OT; ++i) {
+                        u32x4 vp[2];
+                        widen_f16(vr[i].w[0], vp);
+                        o[i] = mfma16<bf16_t>(vp[1], p[1], o[i]);
+                        o[i] = mfma16<bf16_t>(vp[0], p[2], o[i]);
+                        o[i] = mfma16<bf16_t>(vp[1], p[0], o[i]);
+                        o[i] = mfma16<bf16_t>(vp[0], p[1], o[i]);
+                        o[i] = mfma16<bf16_t>(vp[0], p[0], o[i]);
+                    }
+                    s = 0.0f;
+                }
+                u32x4 p[P::Q];
+                split_q<T>(s, p);
 #pragma unroll
                 for (int i = 0; i < OT; ++i) {
                     u32x4 vp[P::K];
@@ -1036,8 +1077,8 @@ struct WideLds {
     static constexpr int QREGS = Parts<T>::Q - (kQl ? 1 : 0);
     static constexpr int QROWS = 32 * D * 4;                // a wave's rows in f32, before and after
     static constexpr int USED = QL + (kQl ? NT / 64 * (D / 16 - QL0) * 1024 : 0), ROWS = NT / 64 * QROWS;
-    static constexpr int STAT = USED > ROWS ? USED : ROWS;  // whether a page is bad
-    static constexpr int BYTES = STAT + 64;
+    static constexpr int STAT = USED > ROWS ? USED : ROWS;  // whether a page is bad, V's largest
+    static constexpr int BYTES = STAT + 64 + 256;
     static constexpr int TASKS = U * D / 8 / NT;            // 8-element chunks of K (or V) a thread
     __device__ static uint32_t kslot(uint32_t r, uint32_t c) {
         return D >= 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
@@ -1063,6 +1104,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
     constexpr bool kStoreEarly = GR == 2 && D == 64 && sizeof(T) == 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
+    int* vtop = flags + 16;  // f16: [64] V's largest magnitudes (as bits), by lanes that staged them
     const int tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = wv / 4;
@@ -1177,6 +1219,15 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                         w = e >= mine ? w & keep : w;
                     }
             }
+            if constexpr (std::is_same_v<T, f16_t>) {
+                u16x2 top = 0;
+#pragma unroll
+                for (int i = 0; i < L::TASKS; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, sv[i].w[0][j] & 0x7FFF7FFFu));
+                atomicMax(&vtop[lane], max((int)top[0], (int)top[1]));
+            }
 #pragma unroll
             for (int i = 0; i < L::TASKS; ++i) {
                 u32x4 p[P::K];
@@ -1193,6 +1244,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
         u32x4* ql = reinterpret_cast<u32x4*>(lds + L::QL) + (wv * (NB - L::QL0) - L::QL0) * 64 + lane;
         __syncthreads();  // (the item before is done with the LDS)
         if (tid == 0) flags[0] = 0;
+        if (std::is_same_v<T, f16_t> && tid < 64) vtop[tid] = 0;
         float inv = 1.0f;
         // The wave's rows of q and of their rotations come whole rows at a time and through its own
         // part of the LDS: a lane's operand is 32 bytes of a row, and loaded so every request would
@@ -1357,7 +1409,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                     for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
                 }
                 if (std::is_same_v<T, f16_t>) top *= inv;  // (a power of two)
-                if (__any(top > ref + 8.0f)) {
+                if (__any(top > ref + P::slack)) {
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
                     const float to = fmaxf(ref, top);
                     const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
@@ -1431,6 +1483,18 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
         l += __shfl_xor(l, 32, 64);
         const float inv_l = 1.0f / l;
         float chk = l * 0.0f;
+        if constexpr (std::is_same_v<T, f16_t>) {
+            // Weights in two parts are off by up to 2^-25, and a row's sums by that times the item's keys and
+            // V's largest magnitude: a row whose largest sum may have lost too much is done again.
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < OT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(o[i][e]));
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            const float vmax = wave_max((float)__builtin_bit_cast(f16_t, (uint16_t)vtop[lane]));
+            if (l > 0.0f && most * kLoss < vmax * ((float)(it.nv * U) * 0x1p-25f)) chk = 1.0f;
+        }
 #pragma unroll
         for (int i = 0; i < OT; ++i)
 #pragma unroll
@@ -1483,7 +1547,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 }
 
 // One row and head by a wave, in plain f32: for rows whose products of parts came out non-finite
-// (an infinity times a part that is 0, also where a mask hides it).  Bound by the latency of its
+// (an infinity times a part that is 0, also where a mask hides it) or lost too much.  Bound by the latency of its
 // loads: all rows of a 2048-token prompt of 32 heads of 128, f16, 4.4 ms (an infinite value in the
 // first position; 0.35 where a NaN key ends each row early).  qf: LDS [D], the query;
 // sc: LDS [64].  Lane el gets dimensions el + 64 i of out.
