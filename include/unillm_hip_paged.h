@@ -55,7 +55,9 @@ int unillm_hip_page_table_clear(unillm_page_table* t, void* stream);
  * max_seqs, and the step's plan: pages from the top of the free stack, entries in order, the
  * step's rows entry after entry.  A sequence may be in a batch once; an entry with a negative
  * id is padding (no tokens, its length not read).  Rows of slots and positions past the
- * step's last are left as they were. */
+ * step's last are left as they were.  A restored free_pages with an id that is no page among those
+ * to be taken fails the call like a pool that ran out, and its rows' slots become -1; such an id in a
+ * sequence's own row of block_table is the attention's to find. */
 int unillm_hip_page_table_extend(unillm_page_table* t, const int32_t* seq_ids_dev,
                                  const int32_t* new_lens_dev, int64_t n_seqs, void* stream);
 /* Sequence seq_ids_dev[b] keeps its first lens_dev[b] tokens (0 <= lens_dev[b] <= its length;

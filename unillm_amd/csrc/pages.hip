@@ -10,9 +10,11 @@
 //     lies at row cu_b + t, position len + t, slot page * ps + position % ps.
 //   truncate: the pages past the new length go back as free[n_free + F - 1 - (off_b + i)],
 //     F of them in all, so a truncate to the old lengths undoes an extend exactly.
-// Everything a call checks (ids in range and distinct, lengths, free pages, room) it checks
-// before it writes, and a failing call leaves the state as it was: the step it leaves is
-// empty and the first error is kept for unillm_hip_page_table_check.
+// Everything a call checks (ids in range and distinct, lengths, room, free pages and whether what it
+// takes of them are pages) it checks before it writes, and a failing call leaves the state as it
+// was: the step it leaves is empty and the first error is kept for unillm_hip_page_table_check.
+// (The ids in sequences' own rows of a restored table are the attention's to check: a truncate puts
+// them on the stack as they are, and no extend takes one that is no page.)
 //
 // One launch a call.  Every workgroup reads all entries and forms both prefix sums itself, in
 // LDS, and then serves its share of the step's tokens (or freed pages): a thread finds its
@@ -157,6 +159,40 @@ __device__ int scan_entries(const Entries& e, int B, const PageTable& t, const i
     return err ? err : all.x > t.max_tokens ? kPagesStepFull : all.y > t.n_pages ? full : 0;
 }
 
+// Page ids from the stack's top: four a load (past n_free within the part's 256 bytes), each thread its
+// group of four of every 1024 downwards.  The first is requested before the entries are read.
+struct Popped {
+    int4 first;
+    int at;
+    __device__ static int4 load(const PageTable& t, int i) {
+        return i >= 0 ? *reinterpret_cast<const int4*>(t.free_pages + i) : make_int4(0, 0, 0, 0);
+    }
+    __device__ Popped(const PageTable& t, int n_free) {
+        at = n_free > 0 && n_free <= t.n_pages ? ((n_free - 1) & ~3) - 4 * (int)threadIdx.x : -4;
+        first = load(t, at);
+    }
+    // whether one of free_pages[lo .. n_free - 1] that this thread reads is no page
+    __device__ bool bad(const PageTable& t, int lo, int n_free) const {
+        auto none = [&](int4 x, int i) {
+            const int id[4] = {x.x, x.y, x.z, x.w};
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                any |= i + j >= lo && i + j < n_free && (unsigned)id[j] >= (unsigned)t.n_pages;
+            return any;
+        };
+        bool any = none(first, at);
+        for (int i = at - 4 * kThreads; i + 3 >= lo; i -= 16 * kThreads) {  // (four loads in flight)
+            int4 x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = load(t, i - 4 * kThreads * k);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) any |= none(x[k], i - 4 * kThreads * k);
+        }
+        return any;
+    }
+};
+
 // dynamic LDS: id[B] | len[B] | ca[B + 1] | cb[B + 1] | seen[ceil(max_seqs / 32)]
 __device__ __forceinline__ Entries entries_in(int* sm, int B, int** seen) {
     Entries e;
@@ -176,11 +212,13 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(PageTable t, const int
                                                           const int* __restrict__ news, int B) {
     extern __shared__ int sm[];
     __shared__ int2 tmp[kThreads / 64];
-    __shared__ int error;
+    __shared__ int error, no_page;
     int* seen;
     const Entries e = entries_in(sm, B, &seen);
     const int ps = t.page_size, shift = t.page_shift;
     const int n_free = t.counts[kPagesFree];
+    if (threadIdx.x == 0) no_page = 0;
+    Popped popped(t, n_free);
     int err = scan_entries(e, B, t, ids, news, [&](int n, int len, int2& v) {
         if (n < 0) return kPagesBadLength;
         if (n > t.max_pages * ps - len) return kPagesSeqFull;
@@ -192,6 +230,14 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(PageTable t, const int
     const int total = e.ca[B], pages = e.cb[B];
     if (!err && (n_free < 0 || n_free > t.n_pages)) err = kPagesBadState;
     if (!err && pages > n_free) err = kPagesNoPages;
+    if (!err && pages > 0) {
+        if (popped.bad(t, n_free - pages, n_free)) no_page = 1;
+        __syncthreads();
+        if (no_page) err = kPagesBadState;
+    }
+    if (no_page)  // (no slots for its rows)
+        for (int r = (int)blockIdx.x * kThreads + (int)threadIdx.x; r < total; r += (int)gridDim.x * kThreads)
+            t.slots[r] = -1;
     if (!err) {
         // four rows a thread at a time: a row's entry is the one before's or a later one
         const int stride = (int)gridDim.x * kThreads * 4;
@@ -216,10 +262,8 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(PageTable t, const int
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (fresh[i] && (pos[i] & (ps - 1)) == 0) *entry[i] = pg[i];  // (the page's first token)
-                // a page of a restored state that the pool does not have: the token has no slot
-                const bool good = (unsigned)pg[i] < (unsigned)t.n_pages;
-                if (!good) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
-                pg[i] = good ? pg[i] * ps + (pos[i] & (ps - 1)) : -1;
+                // (a sequence's own page that is none: no slot, and the attention reports it)
+                pg[i] = (unsigned)pg[i] < (unsigned)t.n_pages ? pg[i] * ps + (pos[i] & (ps - 1)) : -1;
             }
             if (r0 + 4 <= total) {
                 *reinterpret_cast<int4*>(t.slots + r0) = page;
