@@ -43,6 +43,7 @@ int unillm_hip_page_table_destroy(unillm_page_table* t);
 /* The table's parts in device memory (any out-pointer may be NULL).  block_table[max_seqs]
  * [max_pages] page ids (-1: none), seq_lens[max_seqs], free_pages[n_pages] (a stack, its top
  * at n_free - 1) and n_free[1] are its state: copied out and back they save and restore it.
+ * (Of these only seq_lens may itself be passed to extend or truncate.)
  * The last extend's plan, to be read only: cu_tokens[max_seqs + 1] (entry b's rows are
  * cu_tokens[b] .. cu_tokens[b + 1] - 1), and per row slots (page * page_size + offset) and
  * positions. */

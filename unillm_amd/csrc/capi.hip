@@ -898,6 +898,15 @@ int check_entries(const unillm_page_table* t, const void* ids, const void* lens,
     if (((uintptr_t)ids & 3u) != 0 || ((uintptr_t)lens & 3u) != 0)
         return fail(UNILLM_ERR_INVALID_ARG,
                     std::string(what) + ": ids and lengths must be 4-byte aligned (int32)");
+    // A call's workgroups read them while others write the table; its lengths alone are written last.
+    for (const void* p : {ids, lens}) {
+        const uintptr_t at = (uintptr_t)p, end = at + (uintptr_t)n * sizeof(int);
+        const uintptr_t own = (uintptr_t)t->storage, seq = (uintptr_t)t->st.lens;
+        if (p && at < own + t->bytes && end > own &&
+            !(at >= seq && end <= seq + (uintptr_t)t->st.max_seqs * sizeof(int)))
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        std::string(what) + ": ids and lengths must not lie in the table, but for seq_lens");
+    }
     return UNILLM_OK;
 }
 
@@ -961,6 +970,7 @@ int unillm_hip_page_table_create(int64_t max_seqs, int64_t max_pages, int64_t n_
     hipError_t e = hipSuccess;
     t->owned = storage_dev == nullptr;
     t->storage = storage_dev;
+    t->bytes = l.bytes;
     if (t->owned && (e = hipMalloc(&t->storage, l.bytes)) != hipSuccess) {
         delete t;
         return e == hipErrorOutOfMemory ? fail(UNILLM_ERR_OUT_OF_MEMORY, "page table allocation")

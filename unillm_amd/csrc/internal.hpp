@@ -99,6 +99,7 @@ struct unillm_page_table {
     unillm_page_state st;
     int device;
     void* storage;
+    size_t bytes;
     bool owned;
 };
 

@@ -208,8 +208,7 @@ size_t entries_bytes(const PageTable& t, int64_t B) {
     return (size_t)(4 * B + 2 + (t.max_seqs + 31) / 32) * sizeof(int);
 }
 
-__global__ __launch_bounds__(kThreads) void extend_kernel(PageTable t, const int* __restrict__ ids,
-                                                          const int* __restrict__ news, int B) {
+__global__ __launch_bounds__(kThreads) void extend_kernel(PageTable t, const int* ids, const int* news, int B) {
     extern __shared__ int sm[];
     __shared__ int2 tmp[kThreads / 64];
     __shared__ int error, no_page;
@@ -290,8 +289,8 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(PageTable t, const int
     }
 }
 
-__global__ __launch_bounds__(kThreads) void truncate_kernel(PageTable t, const int* __restrict__ ids,
-                                                            const int* __restrict__ news, int B) {
+__global__ __launch_bounds__(kThreads) void truncate_kernel(PageTable t, const int* ids, const int* news,
+                                                            int B) {
     extern __shared__ int sm[];
     __shared__ int2 tmp[kThreads / 64];
     __shared__ int error;
@@ -318,9 +317,12 @@ __global__ __launch_bounds__(kThreads) void truncate_kernel(PageTable t, const i
         }
     }
     if (!last_to_arrive(&t.counts[kPagesTicket])) return;
+    // (the new lengths may lie among the table's own: all are read before one is written)
+    for (int b = threadIdx.x; b < B; b += kThreads) e.len[b] = news ? news[b] : 0;
+    __syncthreads();
     if (!err)
         for (int b = threadIdx.x; b < B; b += kThreads)
-            if (e.id[b] >= 0) t.lens[e.id[b]] = news ? news[b] : 0;
+            if (e.id[b] >= 0) t.lens[e.id[b]] = e.len[b];
     if (threadIdx.x == 0) {
         if (!err) t.counts[kPagesFree] = n_free + freed;
         else atomicCAS(&t.counts[kPagesError], 0, err);
