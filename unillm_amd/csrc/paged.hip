@@ -1219,15 +1219,6 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                         w = e >= mine ? w & keep : w;
                     }
             }
-            if constexpr (std::is_same_v<T, f16_t>) {
-                u16x2 top = 0;
-#pragma unroll
-                for (int i = 0; i < L::TASKS; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, sv[i].w[0][j] & 0x7FFF7FFFu));
-                atomicMax(&vtop[lane], max((int)top[0], (int)top[1]));
-            }
 #pragma unroll
             for (int i = 0; i < L::TASKS; ++i) {
                 u32x4 p[P::K];
@@ -1235,6 +1226,14 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 #pragma unroll
                 for (int x = 0; x < P::K; ++x)
                     *reinterpret_cast<u32x4*>(buf + L::V + x * L::PLANE + vto + 32 * i * L::VROW) = p[x];
+                if constexpr (std::is_same_v<T, f16_t>) {
+                    // (a chunk at a time behind its store: all before the stores costs hd 256 3 %, hd 64 3 % more)
+                    u16x2 top = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, p[0][j] & 0x7FFF7FFFu));
+                    atomicMax(&vtop[lane], max((int)top[0], (int)top[1]));
+                }
             }
         };
         read_pages(k1, k0);
