@@ -74,7 +74,7 @@ int unillm_hip_page_table_check(unillm_page_table* t, void* stream);
 /* One layer's pool: K [n_pages][n_kv_heads][page_size][head_dim] and V [n_pages][n_kv_heads]
  * [head_dim][page_size] (keys contiguous) of kv_type UNILLM_QTYPE_F32, _F16 or _BF16;
  * head_dim 64, 128 or 256; n_kv_heads page_size head_dim and n_pages n_kv_heads below 2^31.
- * k_dev, v_dev: such buffers of the caller's, 16-byte aligned,
+ * k_dev, v_dev: such buffers of the caller's, 16-byte aligned, not overlapping,
  * which must outlive the handle; both NULL: the library allocates them (zeroed). */
 int unillm_hip_paged_kv_create(int kv_type, int64_t n_kv_heads, int64_t head_dim, int64_t n_pages,
                                int64_t page_size, float rope_theta, void* k_dev, void* v_dev,
@@ -86,7 +86,7 @@ int unillm_hip_paged_kv_buffers(const unillm_paged_kv* c, void** k, void** v, si
 /* The attention of one layer for the rows of t's plan.  qkv_dev: n_tokens rows of (n_heads +
  * 2 n_kv_heads) head_dim f32 (q, k, v projections), qkv_stride floats apart; out_dev: n_tokens
  * rows of n_heads head_dim, out_stride apart (strides multiples of 4 floats, both 16-byte
- * aligned, not overlapping); n_tokens n_heads below 2^30.  Each row's q and k are rotated at its position p (half-split
+ * aligned, overlapping neither each other nor the pool; out_dev not the table); n_tokens n_heads below 2^30.  Each row's q and k are rotated at its position p (half-split
  * RoPE; the angles p theta^(-2 i / hd) are formed in f64, where unillm_hip_attention_decode
  * takes them in f32), k and v rounded once to the pool's type into the row's slot, and out =
  * softmax(q k^T / sqrt(hd)) v over the positions j <= p of its sequence, at f32's precision

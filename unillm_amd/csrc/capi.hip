@@ -910,6 +910,16 @@ int check_entries(const unillm_page_table* t, const void* ids, const void* lens,
     return UNILLM_OK;
 }
 
+// Whether two stretches of memory have a byte in common.
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
+// Bytes of a pool's K (and of its V).
+size_t pool_bytes(int type, int64_t n_kv_heads, int64_t head_dim, int64_t n_pages, int64_t page_size) {
+    return (size_t)(n_pages * page_size) * (size_t)(n_kv_heads * head_dim) * (size_t)dense_elem_bytes(type);
+}
+
 // Memory that is known to be another device's than the library's.
 bool elsewhere(const void* p) {
     hipPointerAttribute_t a{};
@@ -1108,6 +1118,9 @@ int unillm_hip_paged_kv_create(int kv_type, int64_t n_kv_heads, int64_t head_dim
     if ((k_dev == nullptr) != (v_dev == nullptr) || !aligned16(k_dev) || !aligned16(v_dev))
         return fail(UNILLM_ERR_INVALID_ARG,
                     "paged KV cache: give both of k and v, 16-byte aligned, or neither");
+    const size_t bytes = pool_bytes(kv_type, n_kv_heads, head_dim, n_pages, page_size);
+    if (k_dev && overlap(k_dev, bytes, v_dev, bytes))
+        return fail(UNILLM_ERR_INVALID_ARG, "paged KV cache: k and v must not share memory");
     if (int rc = ensure_init()) return rc;
     if (elsewhere(k_dev) || elsewhere(v_dev))
         return fail(UNILLM_ERR_INVALID_ARG, "paged KV cache: k or v on another device than the library's");
@@ -1127,8 +1140,6 @@ int unillm_hip_paged_kv_create(int kv_type, int64_t n_kv_heads, int64_t head_dim
     std::vector<double> freq((size_t)head_dim / 2);
     for (size_t i = 0; i < freq.size(); ++i)
         freq[i] = pow((double)rope_theta, -2.0 * (double)i / (double)head_dim) / M_PI;
-    const size_t bytes = (size_t)(n_pages * page_size) * (size_t)(n_kv_heads * head_dim) *
-                         (size_t)dense_elem_bytes(kv_type);
     void* f = nullptr;
     hipError_t e = hipMalloc(&f, freq.size() * sizeof(double));
     if (e == hipSuccess)
@@ -1168,9 +1179,7 @@ int unillm_hip_paged_kv_buffers(const unillm_paged_kv* c, void** k, void** v, si
     if (!c) return fail(UNILLM_ERR_INVALID_ARG, "cache is NULL");
     if (k) *k = c->k;
     if (v) *v = c->v;
-    if (bytes)
-        *bytes = (size_t)(c->n_pages * c->page_size) * (size_t)(c->n_kv_heads * c->head_dim) *
-                 (size_t)dense_elem_bytes(c->type);
+    if (bytes) *bytes = pool_bytes(c->type, c->n_kv_heads, c->head_dim, c->n_pages, c->page_size);
     return UNILLM_OK;
 }
 
@@ -1194,11 +1203,16 @@ int unillm_hip_paged_attention(unillm_paged_kv* c, const unillm_page_table* t,
     if (!qkv_dev || !out_dev) return fail(UNILLM_ERR_INVALID_ARG, what + ": qkv or out is NULL");
     if (!aligned16(qkv_dev) || !aligned16(out_dev))
         return fail(UNILLM_ERR_INVALID_ARG, what + ": qkv and out must be 16-byte aligned");
-    const uintptr_t q0 = (uintptr_t)qkv_dev, o0 = (uintptr_t)out_dev;
-    const uintptr_t q1 = q0 + (uintptr_t)((n_tokens - 1) * qkv_stride + width) * sizeof(float),
-                    o1 = o0 + (uintptr_t)((n_tokens - 1) * out_stride + owidth) * sizeof(float);
-    if (q0 < o1 && o0 < q1)
+    const size_t qn = (size_t)((n_tokens - 1) * qkv_stride + width) * sizeof(float),
+                 on = (size_t)((n_tokens - 1) * out_stride + owidth) * sizeof(float),
+                 pn = pool_bytes(c->type, c->n_kv_heads, c->head_dim, c->n_pages, c->page_size);
+    if (overlap(qkv_dev, qn, out_dev, on))
         return fail(UNILLM_ERR_INVALID_ARG, what + ": out must not share memory with qkv");
+    for (const void* p : {c->k, c->v})
+        if (overlap(qkv_dev, qn, p, pn) || overlap(out_dev, on, p, pn))
+            return fail(UNILLM_ERR_INVALID_ARG, what + ": qkv and out must not share memory with the pool");
+    if (overlap(out_dev, on, t->storage, t->bytes))
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": out must not share memory with the table");
     if (int rc = ensure_init()) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const std::unique_lock<std::mutex> order = stream_order(s);
