@@ -86,14 +86,16 @@ int unillm_hip_paged_kv_buffers(const unillm_paged_kv* c, void** k, void** v, si
 /* The attention of one layer for the rows of t's plan.  qkv_dev: n_tokens rows of (n_heads +
  * 2 n_kv_heads) head_dim f32 (q, k, v projections), qkv_stride floats apart; out_dev: n_tokens
  * rows of n_heads head_dim, out_stride apart (strides multiples of 4 floats, both 16-byte
- * aligned, overlapping neither each other nor the pool; out_dev not the table); n_tokens n_heads below 2^30.  Each row's q and k are rotated at its position p (half-split
- * RoPE; the angles p theta^(-2 i / hd) are formed in f64, where unillm_hip_attention_decode
- * takes them in f32), k and v rounded once to the pool's type into the row's slot, and out =
- * softmax(q k^T / sqrt(hd)) v over the positions j <= p of its sequence, at f32's precision
- * whatever the pool's type (f16: a chunk's row may be off by 2^-16 of its largest output besides,
- * where keys of almost no value take almost all of its weight).  window > 0: only j > p - window, and j < sinks (sliding window
- * with attention sinks; the reference's masks, crates/runtime/src/tensor_core.rs:1761-1781);
- * window 0: all, sinks 0.  What masked keys and values hold does not matter.
+ * aligned, overlapping neither each other nor the pool, out_dev nor the table); n_tokens n_heads
+ * below 2^30.  Each row's q and k are rotated at its position p (half-split RoPE; the angles
+ * p theta^(-2 i / hd) are formed in f64, where unillm_hip_attention_decode takes them in f32), k
+ * and v rounded once to the pool's type into the row's slot, and out = softmax(q k^T / sqrt(hd)) v
+ * over the positions j <= p of its sequence, at f32's precision whatever the pool's type.  (f16:
+ * q is held to 22 bits, an element 2^-17 below its row's largest to fewer, 2^-39 of that one; a
+ * chunk's row may be off by 2^-16 of its largest output besides, 2^-27 a key where it sees more
+ * than 2048, if keys of almost no value take almost all of its weight.)  window > 0: only j > p - window, and j < sinks (sliding window with
+ * attention sinks; the reference's masks, crates/runtime/src/tensor_core.rs:1761-1781); window 0:
+ * all, sinks 0.  What masked keys and values hold does not matter.
  * Rows past the step's last are left as they were; if the table has no plan, or one of more
  * than n_tokens rows, nothing is appended, all n_tokens rows become NaN, and the check reports
  * it.  A call may be made again on the same plan (each layer does). */

@@ -576,9 +576,12 @@ struct Parts<float> {
 // visit: 2^-20 of it is lost at most.  (32 sequences of 8192 keys, scores that make half of the visits
 // and all of them such: 210 and 205 us, 201 with none.)
 constexpr float kSpread = 16.0f;
-// What a wide tile's row may lose by them, of its largest sum.  (Five products a visit would be 7 for 4 in
-// all, and most visits are such where scores spread; few rows' values cancel so far.)
+// What a wide tile's row may lose by them, of its largest sum: 2^-16 over up to 2048 keys, 2^-27 a key
+// over more (an f32 sum of as many terms may be off by 2^-24 a term).  A row loses so much where
+// keys of values below 1/512 of V's largest have all but 1/512 of the weight.  (Five products a visit
+// would be 7 for 4 in all, and most visits are such where scores spread; few rows are.)
 constexpr float kLoss = 0x1p-16f;
+constexpr int kLossKeys = 2048;
 
 // 8 f32 -> the parts of a q or weight operand
 template <class T>
@@ -1492,7 +1495,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
                 for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(o[i][e]));
             most = fmaxf(most, __shfl_xor(most, 32, 64));
             const float vmax = wave_max((float)__builtin_bit_cast(f16_t, (uint16_t)vtop[lane]));
-            if (l > 0.0f && most * kLoss < vmax * ((float)(it.nv * U) * 0x1p-25f)) chk = 1.0f;
+            if (l > 0.0f && most * kLoss < vmax * ((float)min(it.nv * U, kLossKeys) * 0x1p-25f)) chk = 1.0f;
         }
 #pragma unroll
         for (int i = 0; i < OT; ++i)
