@@ -104,9 +104,11 @@ struct Call {
 };
 
 constexpr int kNarrow = 0, kWide = 1;
-// Most query rows of an entry (a kv head) for narrow tiles.  (8 entries on 4000 keys, 8 kv heads of
-// 128, f16 / bf16 / f32, us: of 48 rows narrow 65 / 65 / 114, wide 80 / 125 / 180; of 128 rows 132 /
-// 133 / 250 and 82 / 124 / 188; of 96 rows 104 / 104 / 194 and 81 / 125 / 186.)
+// Most query rows of an entry (a kv head) for narrow tiles.  (8 entries on 4000 keys, 8 kv heads of 128,
+// f16 / bf16 / f32, us: of 48 rows narrow 66 / 66 / 114, wide 84 / 123 / 159; of 80 rows 97 / 97 / 178
+// and 82 / 125 / 162; of 112 rows 133 / 133 / 250 and 83 / 125 / 166.  One number for all types and
+// widths: bf16 entries of 65 to about 100 rows are up to a fourth slower for it at hd 128, a tenth at
+// hd 64 (68 rows: 64, narrow 56); at hd 256 wide is right from there on for each, 87 and 137.)
 constexpr int kNarrowRows = 64;
 constexpr int kTileRows = 16;    // query rows of a narrow tile
 constexpr int kUnit = 32;        // keys of a narrow tile's visit
@@ -244,8 +246,10 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     int C = equal(kd.target), longest = INT_MAX;
     // A piece for every place the device has, if tiles' remainders make no more of them: no piece
     // then waits for a place.  Otherwise (narrow) the larger number, whose second round is shorter.
-    // (16 rows on 32000 keys, hd 256, f32: 112 us, with 3 pieces a CU 133; 8 entries of 48 rows on
-    // 4000 keys, hd 128, f16, where 2 a CU make 576: 76 us, with 3 a CU 65.)
+    // (One token on 8192 keys, 8 kv heads of 128, f16: 25 us, with 3 pieces a CU 28; 32 sequences on 4096, hd
+    // 256, f16: 114, 128; 8 entries of 48 rows on 4000 keys, hd 128, f16, where 2 a CU make 576: 77 us,
+    // with 3 a CU 66.  Wide: 500 tokens behind 777, 8 heads on one of 256, f32, 223 pieces of 5 visits 83
+    // us, by the search below 91; 145 of 8 visits 96, 117 of 10 105, 85 of 15 131.)
     bool fit = false;
     if ((kind == kWide || kd.places < kd.target) && (int64_t)tiles * a.KVH <= kd.places) {
         const int one_each = equal(kd.places);
@@ -266,8 +270,9 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     // through memory.  Up to as many items as places take the largest one's time; up to twice as
     // many, the sum of an item's and of one that follows it, the sizes sorted: the last to find a
     // place of its own and the next, or the largest that is followed and the smallest; more, the
-    // mean place's load and half an item.  (Three chunks among 24 sequences, bf16: 152 us with
-    // pieces of 18 visits, 272 for 256 places, whose small ones pair up; 190 with pieces of 30, 216.)
+    // mean place's load and half an item.  (Three chunks among 24 sequences, bf16: 165 us with pieces of 18
+    // visits, 272 for 256 places, whose small ones pair up; 195 with 15, 328 pieces; 191 with 22, 264; 207
+    // with 30, 216.)
     if (!fit && kind == kWide && (int64_t)tiles * a.KVH <= 4 * (int64_t)kd.places) {
         const int C0 = C;
         constexpr int TRY = 5, BINS = 32;
@@ -414,9 +419,9 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
 // stores a dimension's 8 values at once; other rows value by value.
 // Bound by HBM where rows are many: 2048 rows of 32 kv heads of 128, f16, 100 MB in 21 us (65 with
 // every value on its own, a row after the other); by latency and by the plan where they are few:
-// 5 us for one row, 12 where three chunks of 24 entries are dealt out.
+// 6 us for one row, 12 where three chunks of 24 entries are dealt out.
 // nr is 16, or 4 of a step of up to 512 rows, whose workgroups are too few otherwise (a whole call of
-// 512 such rows 44 us, 45 with 16 a workgroup; of 2048 rows 127 us, 142 with 4).
+// 512 such rows 45 us, 46 with 16 a workgroup; of 2048 rows 129 us, 145 with 4).
 constexpr int kAppendRows = 16;
 
 template <class T, int D>
@@ -1042,7 +1047,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
 // Bound by the matrix cores, with Parts::N times the products of a 16-bit attention, and at hd 64
 // by the vector units (a visit's weights 1400 to 1600 cycles, its products 1024).  At hd 128 in f16 a visit
 // takes 3000 cycles of matrix phase, 2048 of them MFMAs back to back, the rest reads of LDS and the
-// barriers.  A 2048-token prompt of 32 heads of 128, f16, 34 GFLOP in two parts: 101 us, 680 TFLOP/s
+// barriers.  A 2048-token prompt of 32 heads of 128, f16, 34 GFLOP in two parts: 100 us, 690 TFLOP/s
 // of f16 products, where a large library product reaches 1066.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -1072,7 +1077,7 @@ struct WideLds {
     static constexpr int K = 0, V = KPARTS * PLANE, PAIR = 2 * V;
     // q's last part, where registers lack: held there the queries spill to memory (8 heads on one kv
     // head, 2000 tokens behind 8000, us: f32 hd 64 241 -> 222, 128 434 -> 395, 256 1418 -> 963; bf16
-    // hd 256 740 -> 483, f16 428 -> 399)
+    // hd 256 740 -> 483, f16 428 -> 399, and 415 since V's magnitudes are looked at)
     static constexpr int QL = GR * PAIR;
     static constexpr bool kQl = D >= 128 || sizeof(T) == 4;
     // (from this block of 16 dimensions on: LDS is full)
@@ -1437,7 +1442,7 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
             if (!kStoreEarly) store(n + 1 + grp);
             __syncthreads();  // the vector phase ends
             // (where the matrix phase is the longer one, its wave goes first on the SIMD: three chunks
-            // among 24 sequences, bf16, 175 us against 181; at hd 64, 225 against 205)
+            // among 24 sequences, bf16, 169 us against 175; at hd 64, f16, 233 against 224)
             if (!kStoreEarly) __builtin_amdgcn_s_setprio(1);
             {
                 // o += p v of visit n.  Step i: dimensions 32 (i % OT) .., keys of MFMA i / OT
@@ -1549,9 +1554,9 @@ __global__ __launch_bounds__((256 * kGroups<T, D>), (D == 256 ? 1 : 2)) void pag
 }
 
 // One row and head by a wave, in plain f32: for rows whose products of parts came out non-finite
-// (an infinity times a part that is 0, also where a mask hides it) or lost too much.  Bound by the latency of its
-// loads: all rows of a 2048-token prompt of 32 heads of 128, f16, 4.4 ms (an infinite value in the
-// first position; 0.35 where a NaN key ends each row early).  qf: LDS [D], the query;
+// (an infinity times a part that is 0, also where a mask hides it) or lost too much.  Bound by the
+// latency of its loads: all rows of a 2048-token prompt of 32 heads of 128, f16, 5.0 ms (an infinite
+// value in the first position; 0.37 where a NaN key ends each row early).  qf: LDS [D], the query;
 // sc: LDS [64].  Lane el gets dimensions el + 64 i of out.
 template <class T, int D>
 __device__ void attend_row(const PagedKv& c, const Call& a, const int* pages, int row, int h, int p,
