@@ -86,8 +86,8 @@ int unillm_hip_paged_kv_buffers(const unillm_paged_kv* c, void** k, void** v, si
 /* The attention of one layer for the rows of t's plan.  qkv_dev: n_tokens rows of (n_heads +
  * 2 n_kv_heads) head_dim f32 (q, k, v projections), qkv_stride floats apart; out_dev: n_tokens
  * rows of n_heads head_dim, out_stride apart (strides multiples of 4 floats, both 16-byte
- * aligned, overlapping neither each other nor the pool, out_dev nor the table); n_tokens n_heads
- * below 2^30.  Each row's q and k are rotated at its position p (half-split RoPE; the angles
+ * aligned, overlapping neither each other nor the pool, out_dev nor the table); n_tokens at most
+ * t's max_tokens, n_heads a multiple of n_kv_heads below 2^16, n_tokens n_heads below 2^30.  Each row's q and k are rotated at its position p (half-split RoPE; the angles
  * p theta^(-2 i / hd) are formed in f64, where unillm_hip_attention_decode takes them in f32), k
  * and v rounded once to the pool's type into the row's slot, and out = softmax(q k^T / sqrt(hd)) v
  * over the positions j <= p of its sequence, at f32's precision whatever the pool's type.  (f16:
