@@ -160,7 +160,9 @@ __device__ int scan_entries(const Entries& e, int B, const PageTable& t, const i
 }
 
 // Page ids from the stack's top: four a load (past n_free within the part's 256 bytes), each thread its
-// group of four of every 1024 downwards.  The first is requested before the entries are read.
+// group of four of every 1024 downwards.  The first is requested before the entries are read.  (The look
+// at them takes 0.4 us of 5.0 for 8 entries, 1.5 of 13.2 where 2048 entries take 4200 pages; four
+// groups a thread requested ahead, 1.1 and 2.3.)
 struct Popped {
     int4 first;
     int at;
