@@ -313,5 +313,7 @@ int unillm_hip_graph_destroy(unillm_graph* g);
 
 /* Many sequences on one pool of KV pages: page tables and attention over them. */
 #include "unillm_hip_paged.h"
+/* Rotary positions, and paged KV caches held in 8 bits. */
+#include "unillm_hip_kv8.h"
 
 #endif /* UNILLM_HIP_H */

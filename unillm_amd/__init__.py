@@ -16,7 +16,7 @@ __all__ = [
     "Q4_0", "Q4_K", "Q5_0", "Q5_K", "Q6_K", "Q8_0",
     "HipError",
     "QuantLinear", "quantize_blocks", "lm_head_forward", "KvCache",
-    "PageTable", "PagedKvCache",
+    "PageTable", "PagedKvCache", "Rope", "PagedKvCache8",
 ]
 
 
@@ -31,4 +31,10 @@ def __getattr__(name):
     if name in ("PageTable", "PagedKvCache"):
         from . import paged
         return getattr(paged, name)
+    if name == "Rope":
+        from . import rope
+        return rope.Rope
+    if name == "PagedKvCache8":
+        from . import paged8
+        return paged8.PagedKvCache8
     raise AttributeError(name)

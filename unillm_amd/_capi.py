@@ -11,6 +11,7 @@ import re
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libunillm_hip.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "unillm_hip.h")
+KV8_HEADER = os.path.join(os.path.dirname(HERE), "include", "unillm_hip_kv8.h")
 PAGED_HEADER = os.path.join(os.path.dirname(HERE), "include", "unillm_hip_paged.h")
 
 Q4_0 = 2
@@ -29,6 +30,10 @@ QK = 32
 # block of one)
 BLOCK_ELEMS = {Q4_0: 32, Q5_0: 32, Q8_0: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256, F32: 1, F16: 1, BF16: 1}
 BLOCK_BYTES = {Q4_0: 18, Q5_0: 22, Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210, F32: 4, F16: 2, BF16: 2}
+
+# codes of an 8-bit paged KV cache
+KV8_INT8 = 1
+KV8_E4M3 = 2
 
 PATH_AUTO = 0
 PATH_GEMV = 1
@@ -120,6 +125,27 @@ PAGED_SIGNATURES = {
 }
 
 
+# include/unillm_hip_kv8.h
+F64 = ctypes.c_double
+KV8_SIGNATURES = {
+    "unillm_hip_rope_create": (
+        [I64, I64, ctypes.c_int, F64, ctypes.c_int, F64, F64, F64, I64, ctypes.POINTER(F64), F64,
+         ctypes.POINTER(P)], ctypes.c_int),
+    "unillm_hip_rope_destroy": ([P], ctypes.c_int),
+    "unillm_hip_rope_apply": ([P, ctypes.c_int, P, I64, I64, I64, P, P, I64, P], ctypes.c_int),
+    "unillm_hip_paged_kv8_create": (
+        [ctypes.c_int, I64, I64, I64, I64, P, P, P, P, P, ctypes.POINTER(P)], ctypes.c_int),
+    "unillm_hip_paged_kv8_destroy": ([P], ctypes.c_int),
+    "unillm_hip_paged_kv8_buffers": (
+        [P] + [ctypes.POINTER(P)] * 4 + [ctypes.POINTER(ctypes.c_size_t)] * 2, ctypes.c_int),
+    "unillm_hip_paged_kv8_append": ([P, P, P, I64, I64, P], ctypes.c_int),
+    "unillm_hip_paged_kv8_attention": (
+        [P, P, P, I64, I64, I64, ctypes.c_int, I64, I64, P, I64, P], ctypes.c_int),
+    "unillm_hip_paged_kv8_reserve": ([P, P, I64, I64, P], ctypes.c_int),
+    "unillm_hip_paged_kv8_read": ([P, P, P, P, P, I64, I64, ctypes.c_int, P, P, I64, P], ctypes.c_int),
+}
+
+
 def header_symbols(header: str = HEADER) -> list[str]:
     """Every function a public header declares."""
     with open(header) as f:
@@ -135,7 +161,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -m unillm_amd.build` "
                 "(the HIP library is required; there is no CPU fallback)")
         l = ctypes.CDLL(LIB_PATH)
-        for name, (args, res) in {**SIGNATURES, **PAGED_SIGNATURES}.items():
+        for name, (args, res) in {**SIGNATURES, **PAGED_SIGNATURES, **KV8_SIGNATURES}.items():
             fn = getattr(l, name)
             fn.argtypes = args
             fn.restype = res

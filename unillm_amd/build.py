@@ -24,7 +24,7 @@ LIB = os.path.join(HERE, "libunillm_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["capi.hip", "weights.hip", "gemv.hip", "decode.hip", "prefill.hip", "attention.hip",
-           "dense.hip", "pages.hip", "paged.hip"]
+           "dense.hip", "pages.hip", "paged.hip", "rope.hip", "paged8.hip"]
 LIBS = []  # libraries the link adds besides HIP's own
 HOST_SOURCES = ["gguf.cpp", "unillm_host.cpp"]
 HOST_LIB = os.path.join(HERE, "libunillm_host.so")

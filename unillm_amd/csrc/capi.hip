@@ -403,7 +403,7 @@ int fail_launch(hipError_t e, const std::string& what) {
                         std::to_string(g_ws_capture_need) +
                         " bytes, which cannot happen while the stream is being captured; "
                         "reserve it before capture (unillm_hip_qmatmul_reserve / "
-                        "unillm_hip_attention_reserve / unillm_hip_paged_attention_reserve) or make the same call once eagerly");
+                        "unillm_hip_attention_reserve / unillm_hip_paged_attention_reserve / unillm_hip_paged_kv8_reserve) or make the same call once eagerly");
     return fail_hip(e, what.c_str());
 }
 
@@ -1090,6 +1090,14 @@ int unillm_hip_page_table_check(unillm_page_table* t, void* stream) {
         case kPagesRows:
             return fail(UNILLM_ERR_INVALID_ARG,
                         what + "attention on fewer rows than the step's plan has");
+        case kPagesNotFinite:
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + "a key or value for an 8-bit cache that is not finite (held as the largest "
+                               "code, NaN as 0)");
+        case kPagesBadRead:
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + "a read of positions that their sequence does not hold, of an id past max_seqs, "
+                               "or on a page id out of range");
         default:
             return fail(UNILLM_ERR_INVALID_ARG,
                         what + "its state is not one that its calls leave (a length, n_free or a "
@@ -1230,6 +1238,348 @@ int unillm_hip_paged_attention_reserve(const unillm_paged_kv* c, const unillm_pa
     void* p = nullptr;
     hipError_t e = stream_workspace(static_cast<hipStream_t>(stream),
                                     paged_workspace_bytes(*c, *t, n_tokens, n_heads), &p, kPagedSlot);
+    return e == hipSuccess ? UNILLM_OK : fail_launch(e, what);
+}
+
+// ---- rotary positions and 8-bit paged caches --------------------------------------------------
+
+int unillm_hip_rope_create(int64_t head_dim, int64_t rotary_dim, int layout, double theta, int scaling,
+                           double factor, double low, double high, int64_t original,
+                           const double* freq_factors, double magnitude, unillm_rope** out) {
+    if (!out) return fail(UNILLM_ERR_INVALID_ARG, "out is NULL");
+    *out = nullptr;
+    const std::string what = "rope: ";
+    if (head_dim < 2 || head_dim > 512 || rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 != 0)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + "need head_dim in [2, 512] and an even rotary_dim in [2, head_dim]");
+    if (layout != UNILLM_ROPE_HALF && layout != UNILLM_ROPE_INTERLEAVED)
+        return fail(UNILLM_ERR_UNSUPPORTED, what + "unknown layout " + std::to_string(layout));
+    if (scaling < UNILLM_ROPE_SCALE_NONE || scaling > UNILLM_ROPE_SCALE_YARN)
+        return fail(UNILLM_ERR_UNSUPPORTED, what + "unknown scaling " + std::to_string(scaling));
+    if (!(theta > 1.0) || !isfinite(theta) || !isfinite(magnitude))
+        return fail(UNILLM_ERR_INVALID_ARG, what + "need a finite theta > 1 and a finite magnitude");
+    if (scaling != UNILLM_ROPE_SCALE_NONE && (!(factor >= 1.0) || !isfinite(factor)))
+        return fail(UNILLM_ERR_INVALID_ARG, what + "need a finite factor >= 1");
+    const bool ramp = scaling == UNILLM_ROPE_SCALE_LLAMA3 || scaling == UNILLM_ROPE_SCALE_YARN;
+    if (ramp && (!(low > 0.0) || !(high > low) || !isfinite(high) || original < 1))
+        return fail(UNILLM_ERR_INVALID_ARG, what + "need 0 < low < high (turns) and original >= 1");
+    const int pairs = (int)rotary_dim / 2;
+    for (int i = 0; freq_factors && i < pairs; ++i)
+        if (!(freq_factors[i] > 0.0) || !isfinite(freq_factors[i]))
+            return fail(UNILLM_ERR_INVALID_ARG, what + "freq_factors must be positive and finite");
+    if (int rc = ensure_init()) return rc;
+    const double R = (double)rotary_dim, context = (double)original;
+    double first = 0.0, last = 0.0;  // YARN's ramp, by the pair's number
+    if (scaling == UNILLM_ROPE_SCALE_YARN) {
+        auto number = [&](double turns) { return R * log(context / (2.0 * M_PI * turns)) / (2.0 * log(theta)); };
+        first = std::min(std::max(floor(number(high)), 0.0), R - 1.0);
+        last = std::max(std::min(ceil(number(low)), R - 1.0), 0.0);
+        if (magnitude == 0.0) magnitude = 0.1 * log(factor) + 1.0;
+    }
+    if (magnitude == 0.0) magnitude = 1.0;
+    double half_turns[256];
+    for (int i = 0; i < pairs; ++i) {
+        double f = pow(theta, -2.0 * i / R);
+        if (freq_factors) f /= freq_factors[i];
+        double r = 1.0;  // of the frequency as it is
+        if (scaling == UNILLM_ROPE_SCALE_LINEAR) r = 0.0;
+        if (scaling == UNILLM_ROPE_SCALE_LLAMA3) r = (context * f / (2.0 * M_PI) - low) / (high - low);
+        if (scaling == UNILLM_ROPE_SCALE_YARN) r = 1.0 - (i - first) / std::max(last - first, 0.001);
+        r = std::min(std::max(r, 0.0), 1.0);
+        if (scaling != UNILLM_ROPE_SCALE_NONE) f *= r + (1.0 - r) / factor;
+        half_turns[i] = f / M_PI;
+    }
+    unillm_rope* h = new (std::nothrow) unillm_rope{};
+    if (!h) return fail(UNILLM_ERR_OUT_OF_MEMORY, "host allocation failed");
+    *h = {g_device, layout, head_dim, rotary_dim, magnitude, nullptr};
+    void* f = nullptr;
+    hipError_t e = hipMalloc(&f, pairs * sizeof(double));
+    if (e == hipSuccess) e = hipMemcpy(f, half_turns, pairs * sizeof(double), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        (void)hipFree(f);
+        delete h;
+        return e == hipErrorOutOfMemory ? fail(UNILLM_ERR_OUT_OF_MEMORY, "rope allocation")
+                                        : fail_hip(e, "rope allocation");
+    }
+    h->freq = static_cast<double*>(f);
+    *out = h;
+    return UNILLM_OK;
+}
+
+int unillm_hip_rope_destroy(unillm_rope* r) {
+    if (!r) return UNILLM_OK;
+    const hipError_t e = hipFree(r->freq);
+    delete r;
+    return e == hipSuccess ? UNILLM_OK : fail_hip(e, "hipFree (rope)");
+}
+
+int unillm_hip_rope_apply(const unillm_rope* r, int type, const void* x_dev, int64_t x_stride, int64_t n,
+                          int64_t n_heads, const int32_t* positions_dev, void* out_dev,
+                          int64_t out_stride, void* stream) {
+    const std::string what = "rope: ";
+    if (!r) return fail(UNILLM_ERR_INVALID_ARG, what + "handle is NULL");
+    if (!is_dense(type))
+        return fail(UNILLM_ERR_UNSUPPORTED, what + "unsupported type " + std::to_string(type) +
+                                                " (want 0 = F32, 1 = F16, 30 = BF16)");
+    if (n < 0 || n > (int64_t)INT32_MAX || n_heads < 1 || n_heads > 65535)
+        return fail(UNILLM_ERR_INVALID_ARG, what + "need n in [0, 2^31) and n_heads in [1, 65535]");
+    const int64_t width = n_heads * r->head_dim, far = (int64_t)1 << 31;
+    if (x_stride < width || out_stride < width || x_stride > far || out_stride > far)
+        return fail(UNILLM_ERR_INVALID_ARG, what + "row strides must be at least " + std::to_string(width));
+    if (n == 0) return UNILLM_OK;
+    if (!x_dev || !out_dev || !positions_dev)
+        return fail(UNILLM_ERR_INVALID_ARG, what + "x, out or positions is NULL");
+    const size_t size = (size_t)dense_elem_bytes(type);
+    if ((uintptr_t)x_dev % size != 0 || (uintptr_t)out_dev % size != 0 || ((uintptr_t)positions_dev & 3u) != 0)
+        return fail(UNILLM_ERR_INVALID_ARG, what + "pointers must be aligned to their elements");
+    const size_t xn = (size_t)((n - 1) * x_stride + width) * size, on = (size_t)((n - 1) * out_stride + width) * size;
+    if (x_dev == out_dev ? x_stride != out_stride : overlap(x_dev, xn, out_dev, on))
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + "out must be x, with its stride, or not share memory with it");
+    if (overlap(out_dev, on, positions_dev, (size_t)n * sizeof(int32_t)))
+        return fail(UNILLM_ERR_INVALID_ARG, what + "out must not share memory with positions");
+    if (int rc = ensure_init()) return rc;
+    const hipError_t e = launch_rope(*r, type, x_dev, x_stride, n, n_heads, positions_dev, out_dev, out_stride,
+                                     static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? UNILLM_OK : fail_hip(e, "rope launch");
+}
+
+namespace {
+
+// Bytes of an 8-bit pool's K codes (and of its V), and of either's exponents.
+size_t kv8_bytes(const unillm_paged_kv8& c) { return (size_t)(c.n_pages * c.page_size) * (size_t)(c.n_kv_heads * c.head_dim); }
+size_t kv8_exp_bytes(const unillm_paged_kv8& c) { return (size_t)(c.n_pages * (c.page_size / 16)) * (size_t)c.n_kv_heads; }
+
+// Whether [p, p + n) has a byte in common with the pool.
+bool in_pool(const unillm_paged_kv8& c, const void* p, size_t n) {
+    return overlap(p, n, c.k, kv8_bytes(c)) || overlap(p, n, c.v, kv8_bytes(c)) ||
+           overlap(p, n, c.k_exp, kv8_exp_bytes(c)) || overlap(p, n, c.v_exp, kv8_exp_bytes(c));
+}
+
+// What the calls on an 8-bit cache and a table check alike.
+int check_kv8(const unillm_paged_kv8* c, const unillm_page_table* t, int64_t n, const std::string& what) {
+    if (!c || !t) return fail(UNILLM_ERR_INVALID_ARG, what + ": cache or table is NULL");
+    if (c->n_pages != t->st.n_pages || c->page_size != t->st.page_size)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + ": the cache has " + std::to_string(c->n_pages) + " pages of " +
+                        std::to_string(c->page_size) + ", the table " +
+                        std::to_string(t->st.n_pages) + " of " + std::to_string(t->st.page_size));
+    if (n < 0 || n > t->st.max_tokens)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": n_tokens " + std::to_string(n) +
+                                                " outside [0, " + std::to_string(t->st.max_tokens) +
+                                                "]");
+    return UNILLM_OK;
+}
+int check_kv8_heads(const unillm_paged_kv8* c, int64_t n, int64_t n_heads, const std::string& what) {
+    if (n_heads < c->n_kv_heads || n_heads % c->n_kv_heads != 0 || n_heads > 65535)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": need n_heads a multiple of n_kv_heads");
+    if (n * n_heads > (int64_t)INT32_MAX / 2)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": n_tokens * n_heads must be below 2^30");
+    return UNILLM_OK;
+}
+
+// Rows of f32 that a call reads.
+int check_rows(const float* p, int64_t stride, int64_t width, const std::string& what, const char* name) {
+    if (stride < width || stride % 4 != 0 || stride > (int64_t)1 << 40)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": row strides must be multiples of 4 floats, of at least " +
+                                                std::to_string(width) + " (" + name + ")");
+    if (!p) return fail(UNILLM_ERR_INVALID_ARG, what + ": " + name + " is NULL");
+    if (!aligned16(p)) return fail(UNILLM_ERR_INVALID_ARG, what + ": " + name + " must be 16-byte aligned");
+    return UNILLM_OK;
+}
+
+}  // namespace
+
+int unillm_hip_paged_kv8_create(int kv_type, int64_t n_kv_heads, int64_t head_dim, int64_t n_pages,
+                                int64_t page_size, const unillm_rope* rope, void* k_dev, void* v_dev,
+                                void* k_exp_dev, void* v_exp_dev, unillm_paged_kv8** out) {
+    if (!out) return fail(UNILLM_ERR_INVALID_ARG, "out is NULL");
+    *out = nullptr;
+    const std::string what = "8-bit paged KV cache: ";
+    if (kv_type != UNILLM_KV8_INT8 && kv_type != UNILLM_KV8_E4M3)
+        return fail(UNILLM_ERR_UNSUPPORTED, what + "unsupported type " + std::to_string(kv_type) +
+                                                " (want 1 = INT8, 2 = E4M3)");
+    PageLayout l;
+    if (n_kv_heads < 1 || n_kv_heads > 65535 || !(head_dim == 64 || head_dim == 128 || head_dim == 256))
+        return fail(UNILLM_ERR_INVALID_ARG, what + "need n_kv_heads in [1, 65535], head_dim 64 / 128 / 256");
+    if (int rc = page_layout(1, 1, n_pages, page_size, 1, &l)) return rc;
+    if (n_kv_heads * page_size * head_dim > (int64_t)INT32_MAX || n_pages * n_kv_heads > (int64_t)INT32_MAX)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + "need n_kv_heads * page_size * head_dim and n_pages * n_kv_heads below 2^31");
+    if (rope && (rope->head_dim != head_dim || rope->rotary_dim % 8 != 0))
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + "rope must be of this head_dim, its rotary_dim a multiple of 8");
+    void* const parts[4] = {k_dev, v_dev, k_exp_dev, v_exp_dev};
+    for (void* p : parts)
+        if ((p == nullptr) != (k_dev == nullptr) || !aligned16(p))
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + "give all of k, v and their exponents, 16-byte aligned, or none");
+    unillm_paged_kv8 c{};
+    c.type = kv_type;
+    c.n_kv_heads = n_kv_heads;
+    c.head_dim = head_dim;
+    c.n_pages = n_pages;
+    c.page_size = page_size;
+    while (((int64_t)1 << c.page_shift) < page_size) ++c.page_shift;
+    const size_t sizes[4] = {kv8_bytes(c), kv8_bytes(c), kv8_exp_bytes(c), kv8_exp_bytes(c)};
+    for (int i = 0; k_dev && i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(parts[i], sizes[i], parts[j], sizes[j]))
+                return fail(UNILLM_ERR_INVALID_ARG, what + "its buffers must not share memory");
+    if (int rc = ensure_init()) return rc;
+    for (void* p : parts)
+        if (elsewhere(p))
+            return fail(UNILLM_ERR_INVALID_ARG, what + "a buffer on another device than the library's");
+    c.device = g_device;
+    c.owned = k_dev == nullptr;
+    uint8_t** const at[4] = {&c.k, &c.v, &c.k_exp, &c.v_exp};
+    for (int i = 0; i < 4; ++i) *at[i] = static_cast<uint8_t*>(parts[i]);
+    hipError_t e = hipSuccess;
+    if (rope) {
+        c.layout = rope->layout;
+        c.rotary_dim = (int)rope->rotary_dim;
+        c.magnitude = rope->magnitude;
+        const size_t n = (size_t)rope->rotary_dim / 2 * sizeof(double);
+        if ((e = hipMalloc(reinterpret_cast<void**>(&c.freq), n)) == hipSuccess)
+            e = hipMemcpy(c.freq, rope->freq, n, hipMemcpyDeviceToDevice);
+    }
+    for (int i = 0; c.owned && i < 4 && e == hipSuccess; ++i)
+        if ((e = hipMalloc(reinterpret_cast<void**>(at[i]), sizes[i])) == hipSuccess)
+            e = hipMemset(*at[i], 0, sizes[i]);
+    if (e == hipSuccess) e = hipStreamSynchronize(nullptr);  // (for every stream)
+    unillm_paged_kv8* h = e == hipSuccess ? new (std::nothrow) unillm_paged_kv8(c) : nullptr;
+    if (!h) {
+        (void)hipFree(c.freq);
+        for (int i = 0; c.owned && i < 4; ++i) (void)hipFree(*at[i]);
+        if (e == hipSuccess) return fail(UNILLM_ERR_OUT_OF_MEMORY, "host allocation failed");
+        return e == hipErrorOutOfMemory ? fail(UNILLM_ERR_OUT_OF_MEMORY, what + "allocation")
+                                        : fail_hip(e, "8-bit paged KV cache allocation");
+    }
+    *out = h;
+    return UNILLM_OK;
+}
+
+int unillm_hip_paged_kv8_destroy(unillm_paged_kv8* c) {
+    if (!c) return UNILLM_OK;
+    hipError_t e = hipFree(c->freq);
+    for (void* p : {c->k, c->v, c->k_exp, c->v_exp})
+        if (c->owned) {
+            const hipError_t e2 = hipFree(p);
+            if (e == hipSuccess) e = e2;
+        }
+    delete c;
+    return e == hipSuccess ? UNILLM_OK : fail_hip(e, "hipFree (8-bit paged KV cache)");
+}
+
+int unillm_hip_paged_kv8_buffers(const unillm_paged_kv8* c, void** k, void** v, void** k_exp,
+                                 void** v_exp, size_t* bytes, size_t* exp_bytes) {
+    if (!c) return fail(UNILLM_ERR_INVALID_ARG, "cache is NULL");
+    if (k) *k = c->k;
+    if (v) *v = c->v;
+    if (k_exp) *k_exp = c->k_exp;
+    if (v_exp) *v_exp = c->v_exp;
+    if (bytes) *bytes = kv8_bytes(*c);
+    if (exp_bytes) *exp_bytes = kv8_exp_bytes(*c);
+    return UNILLM_OK;
+}
+
+int unillm_hip_paged_kv8_append(unillm_paged_kv8* c, const unillm_page_table* t, const float* kv_dev,
+                                int64_t kv_stride, int64_t n_tokens, void* stream) {
+    const std::string what = "8-bit paged append";
+    if (int rc = check_kv8(c, t, n_tokens, what)) return rc;
+    if (n_tokens == 0) return UNILLM_OK;
+    const int64_t width = 2 * c->n_kv_heads * c->head_dim;
+    if (int rc = check_rows(kv_dev, kv_stride, width, what, "kv")) return rc;
+    const size_t n = (size_t)((n_tokens - 1) * kv_stride + width) * sizeof(float);
+    if (in_pool(*c, kv_dev, n)) return fail(UNILLM_ERR_INVALID_ARG, what + ": kv must not share memory with the pool");
+    if (overlap(kv_dev, n, t->storage, t->bytes))
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": kv must not share memory with the table");
+    if (int rc = ensure_init()) return rc;
+    const hipError_t e = launch_kv8_append(*c, *t, kv_dev, kv_stride, n_tokens, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? UNILLM_OK : fail_launch(e, what);
+}
+
+int unillm_hip_paged_kv8_attention(unillm_paged_kv8* c, const unillm_page_table* t,
+                                   const float* qkv_dev, int64_t qkv_stride, int64_t n_tokens,
+                                   int64_t n_heads, int append, int64_t window, int64_t sinks,
+                                   float* out_dev, int64_t out_stride, void* stream) {
+    const std::string what = "8-bit paged attention";
+    if (int rc = check_kv8(c, t, n_tokens, what)) return rc;
+    if (int rc = check_kv8_heads(c, n_tokens, n_heads, what)) return rc;
+    if (append != 0 && append != 1) return fail(UNILLM_ERR_INVALID_ARG, what + ": append must be 0 or 1");
+    if (window < 0 || sinks < 0 || (window == 0 && sinks != 0))
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + ": need window >= 0 and sinks >= 0 (0 without a window)");
+    if (n_tokens == 0) return UNILLM_OK;
+    const int64_t owidth = n_heads * c->head_dim, width = owidth + (append ? 2 * c->n_kv_heads * c->head_dim : 0);
+    if (int rc = check_rows(qkv_dev, qkv_stride, width, what, "qkv")) return rc;
+    if (int rc = check_rows(out_dev, out_stride, owidth, what, "out")) return rc;
+    const size_t qn = (size_t)((n_tokens - 1) * qkv_stride + width) * sizeof(float),
+                 on = (size_t)((n_tokens - 1) * out_stride + owidth) * sizeof(float);
+    if (overlap(qkv_dev, qn, out_dev, on))
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": out must not share memory with qkv");
+    if (in_pool(*c, qkv_dev, qn) || in_pool(*c, out_dev, on))
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": qkv and out must not share memory with the pool");
+    if (overlap(out_dev, on, t->storage, t->bytes) || overlap(qkv_dev, qn, t->storage, t->bytes))
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": qkv and out must not share memory with the table");
+    if (int rc = ensure_init()) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const std::unique_lock<std::mutex> order = stream_order(s);
+    const hipError_t e = launch_kv8_attention(*c, *t, qkv_dev, qkv_stride, n_tokens, n_heads, append != 0, window,
+                                              sinks, out_dev, out_stride, s);
+    return e == hipSuccess ? UNILLM_OK : fail_launch(e, what);
+}
+
+int unillm_hip_paged_kv8_reserve(const unillm_paged_kv8* c, const unillm_page_table* t,
+                                 int64_t n_tokens, int64_t n_heads, void* stream) {
+    const std::string what = "8-bit paged attention reserve";
+    if (int rc = check_kv8(c, t, n_tokens, what)) return rc;
+    if (int rc = check_kv8_heads(c, n_tokens, n_heads, what)) return rc;
+    if (n_tokens == 0) return UNILLM_OK;
+    if (int rc = ensure_init()) return rc;
+    void* p = nullptr;
+    const hipError_t e = stream_workspace(static_cast<hipStream_t>(stream),
+                                          kv8_workspace_bytes(*c, *t, n_tokens, n_heads), &p, kPagedSlot);
+    return e == hipSuccess ? UNILLM_OK : fail_launch(e, what);
+}
+
+int unillm_hip_paged_kv8_read(const unillm_paged_kv8* c, const unillm_page_table* t,
+                              const int32_t* seq_ids_dev, const int32_t* starts_dev,
+                              const int32_t* cu_rows_dev, int64_t n_seqs, int64_t n_rows, int out_type,
+                              void* k_out_dev, void* v_out_dev, int64_t out_stride, void* stream) {
+    const std::string what = "8-bit paged read";
+    if (int rc = check_kv8(c, t, 0, what)) return rc;
+    if (!is_dense(out_type))
+        return fail(UNILLM_ERR_UNSUPPORTED, what + ": unsupported type " + std::to_string(out_type) +
+                                                " (want 0 = F32, 1 = F16, 30 = BF16)");
+    if (n_seqs < 0 || n_seqs > (int64_t)1 << 22 || n_rows < 0 || n_rows > (int64_t)1 << 26)
+        return fail(UNILLM_ERR_INVALID_ARG, what + ": need n_seqs in [0, 2^22] and n_rows in [0, 2^26]");
+    const int64_t width = c->n_kv_heads * c->head_dim;
+    const size_t size = (size_t)dense_elem_bytes(out_type);
+    if (out_stride < width || out_stride > (int64_t)1 << 40 || (size_t)out_stride * size % 16 != 0)
+        return fail(UNILLM_ERR_INVALID_ARG,
+                    what + ": out_stride must be at least " + std::to_string(width) + ", a multiple of 16 bytes");
+    if (n_seqs == 0 || n_rows == 0) return UNILLM_OK;
+    const void* const entries[3] = {seq_ids_dev, starts_dev, cu_rows_dev};
+    for (const void* p : entries)
+        if (!p || ((uintptr_t)p & 3u) != 0)
+            return fail(UNILLM_ERR_INVALID_ARG,
+                        what + ": seq_ids, starts or cu_rows is NULL or not 4-byte aligned (int32)");
+    void* const outs[2] = {k_out_dev, v_out_dev};
+    const size_t on = (size_t)((n_rows - 1) * out_stride + width) * size;
+    for (int i = 0; i < 2; ++i) {
+        const void* p = outs[i];
+        if (!aligned16(p)) return fail(UNILLM_ERR_INVALID_ARG, what + ": k_out and v_out must be 16-byte aligned");
+        if (!p) continue;
+        bool shared = in_pool(*c, p, on) || overlap(p, on, t->storage, t->bytes) ||
+                      (i == 0 && v_out_dev && overlap(p, on, v_out_dev, on));
+        for (int j = 0; j < 3; ++j) shared |= overlap(p, on, entries[j], (size_t)(n_seqs + (j == 2)) * sizeof(int32_t));
+        if (shared) return fail(UNILLM_ERR_INVALID_ARG, what + ": k_out and v_out must share no memory with the call's others");
+    }
+    if (!k_out_dev && !v_out_dev) return UNILLM_OK;
+    if (int rc = ensure_init()) return rc;
+    const hipError_t e = launch_kv8_read(*c, *t, seq_ids_dev, starts_dev, cu_rows_dev, n_seqs, n_rows, out_type,
+                                         k_out_dev, v_out_dev, out_stride, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? UNILLM_OK : fail_launch(e, what);
 }
 

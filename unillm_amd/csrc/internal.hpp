@@ -117,6 +117,29 @@ struct unillm_paged_kv {
     bool owned;
 };
 
+// The opaque handle of rotary positions (rope.hip).
+struct unillm_rope {
+    int device;
+    int layout;
+    int64_t head_dim, rotary_dim;
+    double magnitude;
+    double* freq;  // [rotary_dim / 2] half turns a position of each pair, in device memory
+};
+
+// The opaque handle of one layer's pool in 8 bits (paged8.hip): the shapes of unillm_paged_kv, codes of
+// a byte, and a byte b for each 16 positions and kv head: codes times 2^(b - 127).
+struct unillm_paged_kv8 {
+    int device;
+    int type;  // UNILLM_KV8_INT8 or _E4M3
+    int64_t n_kv_heads, head_dim, n_pages, page_size;
+    int page_shift;
+    int layout, rotary_dim;  // of q and k (rotary_dim 0: they come rotated)
+    double magnitude;
+    double* freq;
+    uint8_t *k, *v, *k_exp, *v_exp;
+    bool owned;
+};
+
 namespace unillm {
 
 constexpr int QK = 32;  // weights per block
@@ -322,7 +345,8 @@ using PageTable = ::unillm_page_state;
 constexpr int kPagesFree = 0, kPagesStep = 1, kPagesTokens = 2, kPagesEntries = 3, kPagesTicket = 32,
               kPagesError = 64, kPagesCounts = 96;
 constexpr int kPagesBadId = 1, kPagesBadLength = 2, kPagesSeqFull = 3, kPagesStepFull = 4,
-              kPagesNoPages = 5, kPagesBadState = 6, kPagesNoPlan = 7, kPagesRows = 8;
+              kPagesNoPages = 5, kPagesBadState = 6, kPagesNoPlan = 7, kPagesRows = 8,
+              kPagesNotFinite = 9, kPagesBadRead = 10;
 constexpr int64_t kPagesMaxSeqs = 8192;       // (a call's entries are scanned in LDS)
 constexpr int64_t kPagesMaxEach = 1 << 22;    // max_tokens, max_pages
 hipError_t launch_pages_clear(const PageTable& t, hipStream_t s);
@@ -341,6 +365,24 @@ hipError_t launch_paged_attention(const PagedKv& c, const unillm_page_table& t, 
                                   int64_t sinks, float* out, int64_t ostride, hipStream_t s);
 // Workspace (slot kPagedSlot) of such a call of up to n rows.
 size_t paged_workspace_bytes(const PagedKv& c, const unillm_page_table& t, int64_t n, int64_t H);
+
+// Rotary positions (rope.hip): n rows of `heads` heads of type F32, F16 or BF16; x == out: in place.
+hipError_t launch_rope(const unillm_rope& r, int type, const void* x, int64_t xstride, int64_t n,
+                       int64_t heads, const int* positions, void* out, int64_t ostride, hipStream_t s);
+
+// Paged caches in 8 bits (paged8.hip).  The step's keys and values, rows of 2 KVH hd, into their blocks.
+using PagedKv8 = ::unillm_paged_kv8;
+hipError_t launch_kv8_append(const PagedKv8& c, const unillm_page_table& t, const float* kv,
+                             int64_t kvstride, int64_t n, hipStream_t s);
+// As launch_paged_attention; append: the rows are q, k and v, else q alone.
+hipError_t launch_kv8_attention(const PagedKv8& c, const unillm_page_table& t, const float* qkv,
+                                int64_t qstride, int64_t n, int64_t H, bool append, int64_t window,
+                                int64_t sinks, float* out, int64_t ostride, hipStream_t s);
+size_t kv8_workspace_bytes(const PagedKv8& c, const unillm_page_table& t, int64_t n, int64_t H);  // (kPagedSlot)
+// Values of stretches of sequences into k_out and v_out (either may be null), of type F32, F16 or BF16.
+hipError_t launch_kv8_read(const PagedKv8& c, const unillm_page_table& t, const int* ids,
+                           const int* starts, const int* cu, int64_t n_seqs, int64_t n, int type,
+                           void* k_out, void* v_out, int64_t ostride, hipStream_t s);
 
 constexpr int64_t kGemvMaxM = 4;
 constexpr int64_t kDecodeMaxM = 64;

@@ -1,0 +1,162 @@
+// rope.hip -- rotary positions of rows of heads (unillm_hip_rope_apply).
+//
+// A pair (x, y) of a head, in a row at position p, becomes m (x cos a - y sin a), m (x sin a + y
+// cos a) with a = p f_i, i the pair's number: dimensions i and i + R / 2 (half-split) or 2 i and
+// 2 i + 1 (interleaved) of the first R; the dimensions past R stay as they are.  Angles are formed
+// and reduced in f64, in half turns (at position 100000 their f32 forms are 0.003 off), and the
+// products are f64 as well: a row's own type is rounded to once.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "internal.hpp"
+#include "split.hpp"
+
+namespace unillm {
+namespace {
+
+typedef _Float16 rope_f16;
+struct rope_bf16 {
+    uint16_t bits;
+};
+__device__ __forceinline__ float rope_widen(float v) { return v; }
+__device__ __forceinline__ float rope_widen(rope_f16 v) { return (float)v; }
+__device__ __forceinline__ float rope_widen(rope_bf16 v) { return __uint_as_float((uint32_t)v.bits << 16); }
+template <class T>
+__device__ __forceinline__ T rope_narrow(double v);
+template <>
+__device__ __forceinline__ float rope_narrow<float>(double v) { return (float)v; }
+template <>
+__device__ __forceinline__ rope_f16 rope_narrow<rope_f16>(double v) { return (rope_f16)(float)v; }
+template <>
+__device__ __forceinline__ rope_bf16 rope_narrow<rope_bf16>(double v) {
+    return rope_bf16{(uint16_t)(pack_bf16((float)v, 0.0f) & 0xFFFF)};
+}
+
+// V neighbouring elements; W: that many are aligned together.
+template <class T, int V, int W>
+struct alignas(W * sizeof(T)) Some {
+    T v[V];
+};
+
+struct RopeCall {
+    const void* x;
+    void* out;
+    const int* positions;
+    const double* freq;  // half turns a position of each pair
+    double magnitude;
+    int64_t xstride, ostride;
+    int n, heads, hd, rot, copy;
+};
+
+// A workgroup takes `rows` rows: their cosines and sines into LDS, then a thread takes the same V
+// elements (half-split: and their partners) of every so many heads.
+// Bound by HBM where rows are many, by latency for one.
+template <class T, int V, int W, bool HALF>
+__global__ __launch_bounds__(256) void rope_kernel(RopeCall a, int rows) {
+    extern __shared__ double2 turn[];  // [rows][rot / 2]
+    const int tid = threadIdx.x, pairs = a.rot / 2;
+    const int64_t row0 = (int64_t)blockIdx.x * rows;
+    const int n = (int)min((int64_t)rows, a.n - row0);
+    for (int i = tid; i < n * pairs; i += 256) {
+        double sn, cs;
+        sincospi((double)a.positions[row0 + i / pairs] * a.freq[i % pairs], &sn, &cs);
+        turn[i] = make_double2(cs * a.magnitude, sn * a.magnitude);
+    }
+    __syncthreads();
+    // units of a head: those that turn first, then those that are copied
+    const int turning = (HALF ? pairs : a.rot) / V, units = turning + (a.copy ? (a.hd - a.rot) / V : 0);
+    const int across = min(units, 256), side = tid / across, sides = 256 / across;
+    if (side >= sides) return;
+    using S = Some<T, V, W>;
+    for (int u = tid % across; u < units; u += across)
+        for (int r = 0; r < n; ++r) {
+            const T* x = static_cast<const T*>(a.x) + (row0 + r) * a.xstride;
+            T* out = static_cast<T*>(a.out) + (row0 + r) * a.ostride;
+            if (u >= turning) {
+                const int d = a.rot + (u - turning) * V;
+#pragma unroll 4
+                for (int h = side; h < a.heads; h += sides)
+                    *reinterpret_cast<S*>(out + h * a.hd + d) = *reinterpret_cast<const S*>(x + h * a.hd + d);
+            } else if (HALF) {
+                const int d = u * V;
+                double2 z[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) z[e] = turn[r * pairs + d + e];
+#pragma unroll 4
+                for (int h = side; h < a.heads; h += sides) {
+                    S lo = *reinterpret_cast<const S*>(x + h * a.hd + d);
+                    S hi = *reinterpret_cast<const S*>(x + h * a.hd + d + pairs);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const double p = rope_widen(lo.v[e]), q = rope_widen(hi.v[e]);
+                        lo.v[e] = rope_narrow<T>(p * z[e].x - q * z[e].y);
+                        hi.v[e] = rope_narrow<T>(p * z[e].y + q * z[e].x);
+                    }
+                    *reinterpret_cast<S*>(out + h * a.hd + d) = lo;
+                    *reinterpret_cast<S*>(out + h * a.hd + d + pairs) = hi;
+                }
+            } else {
+                const int d = u * V;
+                double2 z[V / 2 > 0 ? V / 2 : 1];
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) z[e] = turn[r * pairs + d / 2 + e];
+#pragma unroll 4
+                for (int h = side; h < a.heads; h += sides) {
+                    S w = *reinterpret_cast<const S*>(x + h * a.hd + d);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) {
+                        const double p = rope_widen(w.v[2 * e]), q = rope_widen(w.v[2 * e + 1]);
+                        w.v[2 * e] = rope_narrow<T>(p * z[e].x - q * z[e].y);
+                        w.v[2 * e + 1] = rope_narrow<T>(p * z[e].y + q * z[e].x);
+                    }
+                    *reinterpret_cast<S*>(out + h * a.hd + d) = w;
+                }
+            }
+        }
+}
+
+template <class T, int V, int W, bool HALF>
+hipError_t launch_width(const RopeCall& a, hipStream_t s) {
+    // rows a workgroup: one, or what leaves 4096 workgroups; their turns in 32 KiB
+    const int pairs = a.rot / 2;
+    const int most = std::max(1, 2048 / pairs);
+    const int rows = (int)std::min<int64_t>(most, std::max<int64_t>(1, a.n / 4096));
+    const unsigned grid = (unsigned)((a.n + rows - 1) / rows);
+    rope_kernel<T, V, W, HALF><<<grid, 256, (size_t)rows * pairs * sizeof(double2), s>>>(a, rows);
+    return hipGetLastError();
+}
+
+template <class T, bool HALF>
+hipError_t launch_type(const RopeCall& a, hipStream_t s) {
+    // elements a lane moves at once: as many, up to 16 bytes, as divide everything
+    auto fits = [&](int v) {
+        const int64_t bytes = v * (int64_t)sizeof(T);
+        return a.hd % v == 0 && (HALF ? a.rot / 2 : a.rot) % v == 0 && a.xstride % v == 0 &&
+               a.ostride % v == 0 && (uintptr_t)a.x % bytes == 0 && (uintptr_t)a.out % bytes == 0;
+    };
+    if constexpr (sizeof(T) == 2)
+        if (fits(8)) return launch_width<T, 8, 8, HALF>(a, s);
+    if (fits(4)) return launch_width<T, 4, 4, HALF>(a, s);
+    if (fits(2)) return launch_width<T, 2, 2, HALF>(a, s);
+    return launch_width<T, HALF ? 1 : 2, 1, HALF>(a, s);
+}
+
+template <class T>
+hipError_t launch_rope_type(bool interleaved, const RopeCall& a, hipStream_t s) {
+    return interleaved ? launch_type<T, false>(a, s) : launch_type<T, true>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_rope(const unillm_rope& r, int type, const void* x, int64_t xstride, int64_t n,
+                       int64_t heads, const int* positions, void* out, int64_t ostride, hipStream_t s) {
+    const RopeCall a{x, out, positions, r.freq, r.magnitude, xstride, ostride, (int)n, (int)heads,
+                     (int)r.head_dim, (int)r.rotary_dim, x != out};
+    const bool inter = r.layout == UNILLM_ROPE_INTERLEAVED;
+    if (type == UNILLM_QTYPE_F32) return launch_rope_type<float>(inter, a, s);
+    if (type == UNILLM_QTYPE_F16) return launch_rope_type<rope_f16>(inter, a, s);
+    return launch_rope_type<rope_bf16>(inter, a, s);
+}
+
+}  // namespace unillm

@@ -21,6 +21,8 @@ const SOURCES: &[&str] = &[
     "dense.hip",
     "pages.hip",
     "paged.hip",
+    "rope.hip",
+    "paged8.hip",
 ];
 
 // Libraries the link adds besides HIP's own.  Keep in step with LIBS in unillm_amd/build.py.

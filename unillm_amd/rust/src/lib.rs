@@ -12,6 +12,7 @@
 //!   projections (llama.rs:1044-1150).
 //! * [`PageTable`] and [`PagedKvCache`] are many sequences on one pool of KV pages, the cache
 //!   that `crates/kv` declares without a device behind it (crates/kv/src/gpu_memory.rs:110).
+//! * [`kv8`] has rotary positions in other orders and scales, and that cache in 8 bits.
 //!
 //! No dependencies: errors are [`HipError`], which implements `std::error::Error`, so
 //! `?` turns it into the reference's `anyhow::Error`.  Its message is the library's
@@ -25,6 +26,8 @@
 use std::ffi::{c_int, c_void, CStr};
 use std::fmt;
 use std::ptr;
+
+pub mod kv8;
 
 /// The C ABI (`include/unillm_hip.h`).
 #[allow(non_camel_case_types)]
@@ -662,6 +665,10 @@ impl PageTable {
                                stream: *mut c_void) -> Result<()> {
         check(sys::unillm_hip_page_table_truncate(self.t, seq_ids, lens,
                                                   to_i64(n_seqs, "n_seqs")?, stream))
+    }
+
+    pub(crate) fn as_ptr(&self) -> *const sys::unillm_page_table {
+        self.t
     }
 
     /// Waits for `stream`; the first call since the last check that failed on the device.
