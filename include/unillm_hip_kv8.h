@@ -65,7 +65,7 @@ int unillm_hip_rope_apply(const unillm_rope* r, int type_, const void* x_dev, in
 /* One layer's pool in 8 bits: K codes [n_pages][n_kv_heads][page_size][head_dim], V codes [n_pages]
  * [n_kv_heads][head_dim][page_size] (keys contiguous), and for each block of 16 positions and kv head a
  * power of two, k_exp and v_exp [n_pages][n_kv_heads][page_size / 16]: a code c of a block with byte
- * b stands for c 2^(min(b, 254) - 127) (b 0: for 0).  Shapes as unillm_hip_paged_kv_create's.  rope:
+ * b stands for c 2^(b - 127) (b 0 and 255, which no append leaves, count as 1 and 254).  Shapes as unillm_hip_paged_kv_create's.  rope:
  * how q and k are rotated, of this head_dim and a rotary_dim that is a multiple of 8 (copied, need not
  * outlive the call), or NULL: not at all (they come rotated).  The four buffers are the caller's,
  * 16-byte aligned, not overlapping, and outlive the handle; all NULL: the library allocates them

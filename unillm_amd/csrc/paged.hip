@@ -630,18 +630,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_narrow_kernel(Pag
 // takes 3000 cycles of matrix phase, 2048 of them MFMAs back to back, the rest reads of LDS and the
 // barriers.  A 2048-token prompt of 32 heads of 128, f16, 34 GFLOP in two parts: 100 us, 690 TFLOP/s
 // of f16 products, where a large library product reaches 1066.
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-template <class T>
-__device__ __forceinline__ f32x16 mfma32(u32x4 x, u32x4 y, f32x16 z) {
-    if constexpr (std::is_same_v<T, f16_t>)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x),
-                                                      __builtin_bit_cast(f16x8, y), z, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
-                                                       __builtin_bit_cast(bf16x8, y), z, 0, 0, 0);
-}
-
 template <class T, int D>
 struct WideLds {
     static constexpr int GR = kGroups<T, D>, NT = 256 * GR;

@@ -51,6 +51,7 @@ __device__ __forceinline__ float wave_add(float v) {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -427,6 +428,18 @@ __device__ __forceinline__ float2 row_scale(float amax) {
 
 __device__ __forceinline__ void redo_row(const Call& a, int64_t row, int h) {
     a.redo[atomicAdd(a.redo_count, 1)] = (int)row * a.H + h;
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <class T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 x, u32x4 y, f32x16 z) {
+    if constexpr (std::is_same_v<T, f16_t>)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x),
+                                                      __builtin_bit_cast(f16x8, y), z, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
+                                                       __builtin_bit_cast(bf16x8, y), z, 0, 0, 0);
 }
 
 // the wave's LDS stores before its reads after them

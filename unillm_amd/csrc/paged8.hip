@@ -26,6 +26,8 @@ namespace unillm {
 namespace {
 
 constexpr int kBlock = 16;  // positions to an exponent
+// Most query rows of an entry (a kv head) for narrow tiles.
+constexpr int kNarrowRows8 = 64;
 struct Int8 {
     static constexpr float top = 127.0f, room = 127.0f / 128.0f;  // top = room 2^bits
     static constexpr int bits = 7;
@@ -42,8 +44,8 @@ __device__ __forceinline__ int least_exponent(float top) {
     const int e = __builtin_amdgcn_frexp_expf(top) - C::bits + (__builtin_amdgcn_frexp_mantf(top) > C::room ? 1 : 0);
     return max(1, e + 127);
 }
-// 2^(b - 127), of b in [1, 254] (0: 0; 255, which no block is given, as 254)
-__device__ __forceinline__ float power(int b) { return __uint_as_float((uint32_t)min(b, 254) << 23); }
+// 2^(b - 127), of b in [1, 254] (0 and 255, which no block is given, as those)
+__device__ __forceinline__ float power(int b) { return __uint_as_float((uint32_t)min(max(b, 1), 254) << 23); }
 
 // Four values, in steps, as codes: to nearest even, infinities to the largest code, NaN to 0.
 template <class C>
@@ -283,9 +285,8 @@ __global__ __launch_bounds__(256) void kv8_prepare_kernel(PagedKv8 c, PageTable 
     int bx = (int)blockIdx.x;
     if (bx < p.plan) {
         if (bx == 0 && tid == 0) *a.redo_count = 0;
-        if (bx == 0) return plan<64, INT_MAX>(t, a, kNarrow, reinterpret_cast<int*>(lds));
-        if (tid < 2) a.kind[kWide].head[tid] = 0;
-        return;
+        if (bx == 0) return plan<64, kNarrowRows8>(t, a, kNarrow, reinterpret_cast<int*>(lds));
+        return plan<D == 256 ? 32 : 64, kNarrowRows8>(t, a, kWide, reinterpret_cast<int*>(lds));
     }
     bx -= p.plan;
     const int total = t.counts[kPagesTokens];
@@ -385,6 +386,26 @@ __device__ __forceinline__ u32x4 codes_bf16(uint32_t lo, uint32_t hi) {
         r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
         r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
         r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+    }
+    return r;
+}
+
+// the same times a power of two
+template <class C>
+__device__ __forceinline__ u32x4 values_bf16(uint32_t lo, uint32_t hi, float step) {
+    u32x4 r;
+    if constexpr (std::is_same_v<C, Int8>) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = i < 2 ? lo : hi;
+            const float a = i % 2 ? decode<C, 2>(w) : decode<C, 0>(w), b = i % 2 ? decode<C, 3>(w) : decode<C, 1>(w);
+            r[i] = __builtin_amdgcn_perm(__float_as_uint(b * step), __float_as_uint(a * step), 0x07060302u);
+        }
+    } else {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, step, false));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, step, true));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, step, false));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, step, true));
     }
     return r;
 }
@@ -677,6 +698,451 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
     }
 }
 
+// ---- many query rows: tiles of keys shared through LDS -----------------------------------------
+//
+// The wide kernel of paged.hip on codes: an item of a tile of up to 256 query rows of a kv head (128 at
+// hd 256), 32 to each wave (32x32x16 MFMAs), U keys at a time through LDS; two groups of four waves a phase
+// apart, so that one's products run beside the other's softmax.  Codes are widened on their way into the
+// LDS, K's to f16 as they are, V's to bf16 times their block's power of two; K's powers of two go beside
+// them, for the scores.
+template <int D>
+struct Wide8Lds {
+    static constexpr int GR = D < 256 ? 2 : 1, NT = 256 * GR;
+    static constexpr int U = D == 256 ? 32 : 64;
+    static constexpr int KROW = 2 * D, VROW = 2 * U;
+    static constexpr int PLANE = U * KROW;                  // of K, and of V^T
+    static constexpr int K = 0, V = PLANE, PAIR = 2 * PLANE;
+    static constexpr int QL = GR * PAIR;                    // q's second part, where registers lack
+    static constexpr bool kQl = D >= 128;
+    static constexpr int QREGS = kQl ? 1 : 2;
+    static constexpr int QROWS = 32 * D * 4;                // a wave's rows in f32, before and after
+    static constexpr int USED = QL + (kQl ? NT / 64 * (D / 16) * 1024 : 0), ROWS = NT / 64 * QROWS;
+    static constexpr int STAT = USED > ROWS ? USED : ROWS;  // whether a page is bad, K's powers of two
+    static constexpr int BYTES = STAT + 64 + 64;
+    static constexpr int TASKS = U * D / 8 / NT;            // 8-code chunks of K (or V) a thread
+    __device__ static uint32_t kslot(uint32_t r, uint32_t c) {
+        return D >= 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
+    }
+    __device__ static uint32_t vslot(uint32_t d, uint32_t c) {
+        return U == 64 ? c ^ ((d >> 1) & 7) : c ^ ((d >> 2) & 3);
+    }
+};
+
+template <class C, int D>
+__global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void kv8_wide_kernel(
+    PagedKv8 c, PageTable t, Call a) {
+    using L = Wide8Lds<D>;
+    constexpr int U = L::U, NB = D / 16, OT = D / 32, NG = U / 32, GR = L::GR, NT = L::NT;
+    constexpr int LOG_D = D == 64 ? 6 : D == 128 ? 7 : 8;
+    constexpr int KSTEP = NT * 8 / D, KROWS = 512 / D;  // keys between a thread's chunks, keys of a wave's
+    constexpr int VGROUPS = U / 16;
+    // A buffer's pair m - 2 was last read in the second group's matrix phase m - 2, so either group may
+    // store its share of pair m in the two phases after: its matrix phase m - 1, or the vector
+    // phase m - 1 (m - 2 in the second group).  The stores go with the shorter phase (f16: at hd 128
+    // a matrix phase takes 3000 cycles, the weights 1470; at hd 64 1350 and 1600).
+    constexpr bool kStoreEarly = GR == 2 && D == 64;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
+    float* steps = reinterpret_cast<float*>(lds + L::STAT + 64);  // [4][4] K's powers of two, by visit and block
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wv / 4;
+    const int col = lane & 31, hf = lane >> 5;
+    const int ps = (int)c.page_size, shift = c.page_shift;
+    const int KVH = a.KVH, G = a.G;
+    const int kread = ((col & 16) | (col & 4) << 1 | (col & 8) >> 1 | (col & 3));  // operand row's key
+    // where the lane's operand rows begin, chunk hf
+    const uint32_t kat = kread * L::KROW + L::kslot(kread, hf) * 16;
+    const uint32_t vat = col * L::VROW + L::vslot(col, hf) * 16;
+    // its staging: offsets of its chunks of K and V from their group's first, and in a buffer
+    const int kr0 = tid / (D / 8), vgroup = wv % VGROUPS;
+    const uint32_t vd0 = wv / VGROUPS * (32 * L::TASKS) + lane / 2;
+    const uint32_t klane = (uint32_t)(kr0 % 16 * D + tid % (D / 8) * 8);
+    const uint32_t vlane = (vd0 << shift) + 8 * (lane & 1);
+    const uint32_t kto = kr0 * L::KROW + L::kslot(kr0, tid % (D / 8)) * 16;
+    const uint32_t vto = vd0 * L::VROW + L::vslot(vd0, 2 * vgroup + (lane & 1)) * 16;
+    const int total = a.kind[kWide].head[0] * KVH;
+    for (int idx = blockIdx.x; idx < total; idx += gridDim.x) {
+        const Item it = a.kind[kWide].items[idx / KVH];
+        const int g = idx % KVH;
+        const int first = it.first, len = it.len, ctx = it.ctx;
+        const int* pages = t.table + (int64_t)it.id * t.max_pages;
+        const Visits<U> vis(ctx + it.row0 / G, ctx + (it.row0 + it.rows - 1) / G, a.window, a.sinks);
+        // the wave's rows and their positions
+        const int w0 = 32 * wv;
+        const int wmin = ctx + (it.row0 + min(w0, it.rows - 1)) / G;
+        const int wmax = ctx + (it.row0 + min(w0 + 31, it.rows - 1)) / G;
+        const int myrow = it.row0 + min(w0 + col, it.rows - 1);  // (rows past the tile repeat its last)
+        const int ppos = ctx + myrow / G;
+
+        // Staging.  A wave's chunks of K are 8 dimensions of keys kr0 + i KSTEP of the visit each, of V 8
+        // keys of dimensions vd0 + 32 i, all chunk i of one group of 16 keys and so of one page:
+        // addresses are a uniform base and the lane's fixed offset.  A page id is read a pair ahead
+        // of its request, that a pair ahead of its store.  Past the item's ends the nearest visit is
+        // staged again, unused: with no branch around a load the waits count only what they need.
+        u32x2 sk[L::TASKS], sv[L::TASKS];
+        int ke[L::TASKS], ve;  // their blocks' exponents
+        int pk[L::TASKS], pv;
+        bool bad_id = false;
+        auto key_of = [&](int n) { return vis.key(it.v0 + max(0, min(n, it.nv - 1))); };
+        // the keys of visits m - 1, m and m + 1 where pair m (V of m - 1, K of m) is fetched next, and
+        // of V's visit in the pair fetched last
+        int k0 = key_of(-1), k1 = key_of(0), k2 = key_of(1), kstored = k0;
+        // (past the sequence: the visit's first group again)
+        auto group_key = [&](int j0, int grp16) { return j0 + 16 * grp16 < len ? j0 + 16 * grp16 : j0; };
+        auto sound = [&](int page) {  // (looked at when it is used: its load has a pair to arrive in)
+            const uint32_t pg = (uint32_t)__builtin_amdgcn_readfirstlane(page);
+            bad_id |= pg >= (uint32_t)c.n_pages;
+            return min(pg, (uint32_t)c.n_pages - 1);
+        };
+        auto kgroup = [&](int i) { return (wv * KROWS + i * KSTEP) / 16; };
+        const uint8_t* kbase = c.k + ((int64_t)g << (shift + LOG_D));
+        const uint8_t* vbase = c.v + ((int64_t)g << (shift + LOG_D));
+        const uint32_t page_elems = (uint32_t)KVH << (shift + LOG_D);
+        auto read_pages = [&](int jk, int jv) {
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) pk[i] = pages[group_key(jk, kgroup(i)) >> shift];
+            pv = pages[group_key(jv, vgroup) >> shift];
+        };
+        auto fetch_k = [&](int i) {
+            const uint32_t at = (uint32_t)group_key(k1, kgroup(i)) & (uint32_t)(ps - 1);
+            const uint64_t page = sound(pk[i]);
+            sk[i] = *reinterpret_cast<const u32x2*>(kbase + (page * page_elems + (at << LOG_D)) +
+                                                    (klane + (KSTEP == 8 ? i % 2 * 8 * D : 0)));
+            ke[i] = c.k_exp[((page * KVH + g) << (shift - 4)) + at / kBlock];
+        };
+        auto fetch_v = [&] {
+            const uint32_t at = (uint32_t)group_key(k0, vgroup) & (uint32_t)(ps - 1);
+            const uint64_t page = sound(pv);
+            const uint8_t* from = vbase + (page * page_elems + at);
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) sv[i] = *reinterpret_cast<const u32x2*>(from + (32 * i << shift) + vlane);
+            ve = c.v_exp[((page * KVH + g) << (shift - 4)) + at / kBlock];
+        };
+        auto fetch_pages = [&](int m) {  // of pair m + 1, after pair m's requests
+            read_pages(k2, k1);
+            kstored = k0;
+            k0 = k1;
+            k1 = k2;
+            k2 = key_of(m + 2);
+        };
+        // pair m in four pieces, to go between MFMAs
+        auto fetch_piece = [&](int m, int piece) {
+            constexpr int HALF_T = (L::TASKS + 1) / 2;
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i)
+                if (piece == (i < HALF_T ? 0 : 1)) fetch_k(i);
+            if (piece == 2) fetch_v();
+            if (piece == 3) fetch_pages(m);
+        };
+        auto fetch = [&](int m) {
+#pragma unroll
+            for (int piece = 0; piece < 4; ++piece) fetch_piece(m, piece);
+        };
+        auto store = [&](int m) {
+            uint8_t* buf = lds + m % GR * L::PAIR;
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i) {
+                // (a chunk step of 8 rows turns bit 3 of the slot)
+                const uint32_t at = (KSTEP == 8 && i % 2 ? kto ^ 128 : kto) + i * KSTEP * L::KROW;
+                *reinterpret_cast<u32x4*>(buf + L::K + at) = codes_f16<C>(sk[i][0], sk[i][1]);
+                if (lane == 0) steps[m % 4 * 4 + kgroup(i)] = power(ke[i]);
+            }
+            const int left = len - kstored;  // keys of V's visit and on
+            if (left < U) {                  // past the sequence's end a page holds anything
+                const int mine = left - 16 * vgroup - 8 * (lane & 1);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const int n = min(max(mine - 4 * w, 0), 4);
+                    const uint32_t keep = n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1;
+#pragma unroll
+                    for (int i = 0; i < L::TASKS; ++i) sv[i][w] &= keep;
+                }
+            }
+            const float step = power(ve);
+#pragma unroll
+            for (int i = 0; i < L::TASKS; ++i)
+                *reinterpret_cast<u32x4*>(buf + L::V + vto + 32 * i * L::VROW) = values_bf16<C>(sv[i][0], sv[i][1], step);
+        };
+        read_pages(k1, k0);
+        fetch(0);
+
+        u32x4 q[L::QREGS][NB];
+        u32x4* ql = reinterpret_cast<u32x4*>(lds + L::QL) + wv * NB * 64 + lane;
+        __syncthreads();  // (the item before is done with the LDS)
+        if (tid == 0) flags[0] = 0;
+        float inv = 1.0f;
+        // The wave's rows of q and of their rotations come whole rows at a time and through its own
+        // part of the LDS: a lane's operand is 32 bytes of a row, and loaded so every request would
+        // touch 32 lines (22000 cycles an item at hd 128 before, of 115000).
+        {
+            // (opaque lane numbers here and at the end: no address of these is kept through the visits)
+            int el = lane;
+            asm volatile("" : "+v"(el));
+            constexpr int CH = D / 4, N = 32 * CH / 64;  // 16-byte chunks of a row, requests of 32 rows
+            f32x4* own = reinterpret_cast<f32x4*>(lds + wv * L::QROWS);
+            auto slot = [&](int r, int ch) { return r * CH + (ch ^ (r & (CH - 1 < 31 ? CH - 1 : 31))); };
+            // (requests at once: with all 32 of hd 256 the compiler spills, tuples of four in two places,
+            // and reads one back wrong)
+            constexpr int NX = N < 16 ? N : 16;
+            // (a lane's own row is `myrow`: its place is handed to the lanes that load it)
+            auto rows = [&](const float* from, int64_t place) {
+#pragma unroll
+                for (int i0 = 0; i0 < N; i0 += NX) {
+                    f32x4 x[NX];
+#pragma unroll
+                    for (int i = 0; i < NX; ++i)
+                        x[i] = reinterpret_cast<const f32x4*>(
+                            from + __shfl(place, ((i0 + i) * 64 + el) / CH, 64))[el % CH];
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < NX; ++i) own[slot(((i0 + i) * 64 + el) / CH, el % CH)] = x[i];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                settle_wave();
+            };
+            f32x8 r[NB];
+            const int64_t myq = first + myrow / G;
+            rows(a.qkv, myq * a.qstride + (int64_t)(g * G + myrow % G) * D);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const f32x4 v = own[slot(el % 32, 4 * b + 2 * (el / 32) + k)];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) r[b][4 * k + j] = v[j];
+                }
+            float up = 1.0f;
+            {
+                float amax = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(r[b][j]));
+                amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+                const float2 sc = row_scale(amax);
+                up = sc.x;
+                inv = sc.y;
+            }
+            __syncthreads();  // (every wave is done with its rows: the buffers and q's last parts go there)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                r[b] *= up;
+                u32x4 p[2];
+                parts_f16(r[b], p);
+#pragma unroll
+                for (int i = 0; i < L::QREGS; ++i) q[i][b] = p[i];
+                if (L::kQl) ql[b * 64] = p[1];
+            }
+        }
+        float ref = -INFINITY, l = 0.0f;
+        f32x16 o[OT];
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+
+        store(0);
+        fetch(1);
+        __syncthreads();
+        if (grp == 1) {  // (a phase behind)
+            if (!kStoreEarly) {
+                store(1);
+                fetch(2);
+            }
+            __syncthreads();
+        }
+        // s = q k of visit n: operands read ahead of the MFMAs of the block before (chunk 2 b + hf of a
+        // row: the swizzle is an XOR, so b's bits can be turned last).  Every wave forms all its
+        // products, seen or not: the phase lasts as long as the longest wave's.
+        f32x16 s[NG];
+        auto scores = [&](int n) {
+            const uint8_t* buf = lds + n % GR * L::PAIR;
+            uint32_t ka = kat;  // (opaque: no address is kept across visits, nor 32 zeros)
+            float zero = 0.0f;
+            asm volatile("" : "+v"(ka), "+v"(zero));
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[u][e] = zero;
+            u32x4 kp[2][NG], qx[2];
+            auto read = [&](int b) {
+#pragma unroll
+                for (int u = 0; u < NG; ++u)
+                    kp[b % 2][u] = *reinterpret_cast<const u32x4*>(buf + L::K + 32 * u * L::KROW + (ka ^ 32 * b));
+                if (L::kQl) qx[b % 2] = ql[b * 64];
+            };
+            read(0);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (b + 1 < NB) read(b + 1);
+                if (kStoreEarly && b % (NB / 4) == 0) fetch_piece(n + 2, b / (NB / 4));
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 1; x >= 0; --x)
+#pragma unroll
+                    for (int u = 0; u < NG; ++u)
+                        s[u] = mfma32<f16_t>(kp[b % 2][u], x < L::QREGS ? q[x < L::QREGS ? x : 0][b] : qx[b % 2], s[u]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        if (kStoreEarly) store(1);
+        scores(0);
+        __syncthreads();  // the first matrix phase ends
+        for (int n = 0;; ++n) {
+            const int j0 = vis.key(it.v0 + n);
+            u32x4 p[NG][2][3];
+            {
+                float top = -INFINITY, times[NG][2];
+#pragma unroll
+                for (int u = 0; u < NG; ++u)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) times[u][x] = inv * steps[n % 4 * 4 + 2 * u + x];
+#pragma unroll
+                for (int u = 0; u < NG; ++u) {
+                    const int ju = j0 + 32 * u;
+                    const bool all = ju + 31 <= wmin &&
+                                     (a.window == 0 || ju > wmax - a.window || ju + 32 <= a.sinks);
+                    if (!all) {
+                        const int at = ppos - ju - 8 * hf, far = a.window > 0 ? at - a.window : INT_MIN;
+                        const int sk0 = a.sinks - ju - 8 * hf;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int j = 16 * (e / 8) + e % 8;
+                            const bool hidden = (j > at) | ((j <= far) & (j >= sk0));
+                            s[u][e] = hidden ? -INFINITY : s[u][e];
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float most = s[u][8 * x];
+#pragma unroll
+                        for (int e = 1; e < 8; ++e) most = fmaxf(most, s[u][8 * x + e]);
+                        top = fmaxf(top, most * times[u][x]);  // (a power of two)
+                    }
+                }
+                if (__any(top > ref + kSlack)) {
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float to = fmaxf(ref, top);
+                    const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+                    l *= f;
+#pragma unroll
+                    for (int i = 0; i < OT; ++i) o[i] *= f;
+                    ref = to;
+                }
+                const float from = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+                for (int u = 0; u < NG; ++u)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        f32x8 w;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            w[e] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * k + e], times[u][k], -from));
+                            l += w[e];
+                        }
+                        parts_bf16(w, p[u][k]);
+                    }
+            }
+            if (!kStoreEarly) store(n + 1 + grp);
+            __syncthreads();  // the vector phase ends
+            // (where the matrix phase is the longer one, its wave goes first on the SIMD: three chunks
+            // among 24 sequences, bf16, 169 us against 175; at hd 64, f16, 233 against 224)
+            if (!kStoreEarly) __builtin_amdgcn_s_setprio(1);
+            {
+                // o += p v of visit n.  Step i: dimensions 32 (i % OT) .., keys of MFMA i / OT
+                const uint8_t* buf = lds + (n + 1) % GR * L::PAIR;
+                uint32_t va = vat;
+                asm volatile("" : "+v"(va));
+                u32x4 vp[2];
+                auto read = [&](int i) {
+                    vp[i % 2] = *reinterpret_cast<const u32x4*>(buf + L::V + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
+                };
+                read(0);
+#pragma unroll
+                for (int i = 0; i < 2 * NG * OT; ++i) {
+                    if (i + 1 < 2 * NG * OT) read(i + 1);
+                    // (what is stored next is requested between the first MFMAs after the stores before)
+                    if (!kStoreEarly && i % (NG * OT / 2) == 0) fetch_piece(n + 2 + grp, i / (NG * OT / 2));
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int x = 2; x >= 0; --x)
+                        o[i % OT] = mfma32<bf16_t>(vp[i % 2], p[i / OT / 2][i / OT % 2][x], o[i % OT]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (n + 1 == it.nv) {
+                __builtin_amdgcn_s_setprio(0);
+                break;
+            }
+            if (kStoreEarly) store(n + 2);
+            scores(n + 1);
+            if (!kStoreEarly) __builtin_amdgcn_s_setprio(0);
+            __syncthreads();  // the matrix phase ends
+        }
+        if (GR == 2) {  // (both groups pass 2 nv + 2 barriers from the first pair on)
+            __syncthreads();
+            if (grp == 0) __syncthreads();
+        }
+        if (bad_id) flags[0] = 1;
+        __syncthreads();
+
+        const bool whole = it.S == 1;
+        const bool mine = w0 + col < it.rows;
+        l += __shfl_xor(l, 32, 64);
+        const float inv_l = 1.0f / l;
+        float chk = l * 0.0f;
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                // the quotient: the rounded product, corrected by its remainder
+                const float y = o[i][e] * inv_l;
+                if (whole) o[i][e] = fmaf(fmaf(-y, l, o[i][e]), inv_l, y);
+                chk = fmaf(o[i][e], 0.0f, chk);
+            }
+        bool bad = mine && chk != 0.0f;
+        bad |= (bool)__shfl_xor((int)bad, 32, 64);  // (both halves of a row)
+        const bool bad_page = flags[0] != 0;
+        if (bad_page && tid == 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadState);
+        const bool again = mine && !bad_page && bad;
+        const int64_t piece = (int64_t)it.base + ((int64_t)g * it.S + it.s) * it.rows;
+        if (mine && hf == 0) {
+            const int rr = it.row0 + w0 + col;
+            if (again) redo_row(a, first + rr / G, g * G + rr % G);
+            if (!whole)
+                a.ms[piece + w0 + col] = make_float2(ref, again || bad_page ? __builtin_nanf("") : l);
+        }
+        // whole rows out, through the wave's part of the LDS (a row with a bad page is NaN, whatever its
+        // other pieces hold)
+        const uint32_t skip = (uint32_t)__ballot(again);
+        constexpr int CH = D / 4, N = 32 * CH / 64;
+        int el = lane;
+        asm volatile("" : "+v"(el));
+        f32x4* own = reinterpret_cast<f32x4*>(lds + wv * L::QROWS);
+        auto slot = [&](int r, int ch) { return r * CH + (ch ^ (r & (CH - 1 < 31 ? CH - 1 : 31))); };
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                own[slot(el % 32, 8 * i + 2 * u + el / 32)] =
+                    f32x4{o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]};
+        settle_wave();
+        const bool direct = whole || bad_page;
+        float* to = direct ? a.out : a.po;
+        const int64_t place = direct ? (int64_t)(first + myrow / G) * a.ostride + (int64_t)(g * G + myrow % G) * D
+                                     : (piece + w0 + col) * D;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = (i * 64 + el) / CH;
+            float* dst = to + __shfl(place, r, 64) + el % CH * 4;
+            const f32x4 v = own[slot(r, el % CH)];
+            if (w0 + r < it.rows && !(skip >> r & 1))
+                *reinterpret_cast<f32x4*>(dst) = bad_page ? f32x4(__builtin_nanf("")) : v;
+        }
+    }
+}
+
 // One row and head by a wave, in plain f32: for rows whose products of parts came out non-finite (an
 // infinite query, or scores past f32's range).  qf: LDS [D], the query; sc: LDS [64].  Lane el gets
 // dimensions el + 64 i of out.
@@ -901,13 +1367,16 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, 
 
 // ---- launches ---------------------------------------------------------------------------------
 
-// Workgroups of the narrow kernel that the device holds, and pieces to deal its work out in at most.
-int places(int64_t D) { return (D == 256 ? 1 : 2) * device_info().cu_count; }
-int target_pieces() { return 3 * device_info().cu_count; }
+// Workgroups of a kind that the device holds: wide one a CU, narrow by its registers.
+int places(int kind, int64_t D) { return (kind == kWide || D == 256 ? 1 : 2) * device_info().cu_count; }
+// Pieces a kind's work is dealt out in at most.
+int target_pieces(int kind) { return (kind == kNarrow ? 3 : 1) * device_info().cu_count; }
+
+int tile_rows(int kind, int64_t D) { return kind == kNarrow ? kTileRows : D < 256 ? 256 : 128; }
 
 struct Layout {
-    int64_t items, rows;
-    size_t head_at[2], items_at, splits_at, q_at, ms_at, po_at, count_at, redo_at, bytes;
+    int64_t items[2], rows[2];
+    size_t head_at[2], items_at[2], splits_at[2], q_at, ms_at, po_at, count_at, redo_at, bytes;
 };
 
 Layout layout(const PagedKv8& c, const unillm_page_table& t, int64_t n, int64_t H) {
@@ -919,20 +1388,25 @@ Layout layout(const PagedKv8& c, const unillm_page_table& t, int64_t n, int64_t 
         at += ((size_t)bytes + 255) & ~(size_t)255;
         return here;
     };
-    // tiles: an entry's last may be ragged.  A tile of nv visits makes at most nv / C + 1 pieces, and
-    // the nv / C add up to target / KVH; more than one piece, at most 2 nv / C.
-    const int64_t tiles = n * G / kTileRows + std::min<int64_t>(n, t.st.max_seqs);
-    l.items = tiles + target_pieces() / KVH + 1;
-    l.rows = 2 * (int64_t)target_pieces() * std::min<int64_t>(kTileRows, n * G);
-    for (int k = 0; k < 2; ++k) l.head_at[k] = take(2 * sizeof(int));
-    l.items_at = take(l.items * (int64_t)sizeof(Item));
-    l.splits_at = take(tiles * (int64_t)sizeof(Split));
+    for (int k = 0; k < 2; ++k) {
+        // tiles: an entry's last may be ragged (a wide entry has more than kNarrowRows8 rows).  A
+        // tile of nv visits makes at most nv / C + 1 pieces, and the nv / C add up to target /
+        // KVH; more than one piece, at most 2 nv / C.
+        const int64_t entries = std::min<int64_t>(k == kNarrow ? n : n * G / (kNarrowRows8 + 1), t.st.max_seqs);
+        const int64_t tiles = n * G / tile_rows(k, D) + entries;
+        const bool some = k == kNarrow || n * G > kNarrowRows8;
+        l.items[k] = some ? tiles + target_pieces(k) / KVH + 1 : 0;
+        l.rows[k] = some ? 2 * (int64_t)target_pieces(k) * std::min<int64_t>(tile_rows(k, D), n * G) : 0;
+        l.head_at[k] = take(2 * sizeof(int));
+        l.items_at[k] = take(l.items[k] * (int64_t)sizeof(Item));
+        l.splits_at[k] = take(tiles * (int64_t)sizeof(Split));
+    }
     l.q_at = take(n * H * D * (int64_t)sizeof(float));
-    l.ms_at = take(l.rows * (int64_t)sizeof(float2));
-    l.po_at = take(l.rows * D * (int64_t)sizeof(float));
+    l.ms_at = take((l.rows[0] + l.rows[1]) * (int64_t)sizeof(float2));
+    l.po_at = take((l.rows[0] + l.rows[1]) * D * (int64_t)sizeof(float));
     // rows to do again: every (row, head), and again for each piece
     l.count_at = take(sizeof(int));
-    l.redo_at = take((n * H + l.rows) * (int64_t)sizeof(int));
+    l.redo_at = take((n * H + l.rows[0] + l.rows[1]) * (int64_t)sizeof(int));
     l.bytes = at;
     return l;
 }
@@ -972,13 +1446,22 @@ hipError_t launch_typed(const PagedKv8& c, const unillm_page_table& t, const Cal
     hipError_t e = launch_prepare<C, D>(c, t, a, p, writes, s);
     if (e != hipSuccess) return e;
     using N = Narrow8Lds<D>;
-    static const bool attr = hipFuncSetAttribute((const void*)kv8_narrow_kernel<C, D>,
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, N::BYTES) == hipSuccess;
+    using W = Wide8Lds<D>;
+    static const bool attr =
+        hipFuncSetAttribute((const void*)kv8_narrow_kernel<C, D>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            N::BYTES) == hipSuccess &&
+        hipFuncSetAttribute((const void*)kv8_wide_kernel<C, D>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            W::BYTES) == hipSuccess;
     if (!attr) return hipErrorInvalidValue;
     const int64_t most = 4 * device_info().cu_count;
-    kv8_narrow_kernel<C, D><<<(unsigned)std::min<int64_t>(l.items * a.KVH, most), 256, N::BYTES, s>>>(c, t.st, a);
+    auto grid = [&](int64_t n, int64_t limit) { return (unsigned)std::min(n, limit); };
+    if (l.items[kWide] > 0) {
+        kv8_wide_kernel<C, D><<<grid(l.items[kWide] * a.KVH, 4 * most), W::NT, W::BYTES, s>>>(c, t.st, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    kv8_narrow_kernel<C, D><<<grid(l.items[kNarrow] * a.KVH, most), 256, N::BYTES, s>>>(c, t.st, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    kv8_merge_kernel<C, D><<<(unsigned)std::min<int64_t>(l.rows / 2, most), 256, 0, s>>>(c, t.st, a);
+    kv8_merge_kernel<C, D><<<grid((l.rows[0] + l.rows[1]) / 2, most), 256, 0, s>>>(c, t.st, a);
     return hipGetLastError();
 }
 
@@ -1021,9 +1504,10 @@ hipError_t launch_kv8_attention(const PagedKv8& c, const unillm_page_table& t, c
            (int)std::min(window, far), (int)std::min(sinks, far), nullptr,
            reinterpret_cast<float2*>(w + l.ms_at), reinterpret_cast<float*>(w + l.po_at),
            reinterpret_cast<int*>(w + l.count_at), reinterpret_cast<int*>(w + l.redo_at), {}};
-    a.kind[kNarrow] = {kTileRows, places(D), target_pieces(), 4, 5, 0, reinterpret_cast<int*>(w + l.head_at[0]),
-                       reinterpret_cast<Item*>(w + l.items_at), reinterpret_cast<Split*>(w + l.splits_at)};
-    a.kind[kWide] = {16, 1, 1, 1, 1, 0, reinterpret_cast<int*>(w + l.head_at[1]), nullptr, nullptr};
+    for (int k = 0; k < 2; ++k)
+        a.kind[k] = {tile_rows(k, D), places(k, D), target_pieces(k), k == kNarrow ? 4 : 2, 5,
+                     k == kNarrow ? 0 : (int)l.rows[0], reinterpret_cast<int*>(w + l.head_at[k]),
+                     reinterpret_cast<Item*>(w + l.items_at[k]), reinterpret_cast<Split*>(w + l.splits_at[k])};
     Prepare p{qkv, qkv + H * D, qstride, q, 2, 0, 0, 0, 0, 0};
     p.q_rows = n <= 512 ? 4 : 16;
     const int64_t blocks = (n + p.q_rows - 1) / p.q_rows;
