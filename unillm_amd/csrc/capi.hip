@@ -1277,7 +1277,7 @@ int unillm_hip_rope_create(int64_t head_dim, int64_t rotary_dim, int layout, dou
         if (magnitude == 0.0) magnitude = 0.1 * log(factor) + 1.0;
     }
     if (magnitude == 0.0) magnitude = 1.0;
-    double half_turns[256];
+    double turns[3 * 256];  // half turns a position, then the turn of one position
     for (int i = 0; i < pairs; ++i) {
         double f = pow(theta, -2.0 * i / R);
         if (freq_factors) f /= freq_factors[i];
@@ -1287,14 +1287,16 @@ int unillm_hip_rope_create(int64_t head_dim, int64_t rotary_dim, int layout, dou
         if (scaling == UNILLM_ROPE_SCALE_YARN) r = 1.0 - (i - first) / std::max(last - first, 0.001);
         r = std::min(std::max(r, 0.0), 1.0);
         if (scaling != UNILLM_ROPE_SCALE_NONE) f *= r + (1.0 - r) / factor;
-        half_turns[i] = f / M_PI;
+        turns[i] = f / M_PI;
+        turns[pairs + 2 * i] = cos(f);
+        turns[pairs + 2 * i + 1] = sin(f);
     }
     unillm_rope* h = new (std::nothrow) unillm_rope{};
     if (!h) return fail(UNILLM_ERR_OUT_OF_MEMORY, "host allocation failed");
     *h = {g_device, layout, head_dim, rotary_dim, magnitude, nullptr};
     void* f = nullptr;
-    hipError_t e = hipMalloc(&f, pairs * sizeof(double));
-    if (e == hipSuccess) e = hipMemcpy(f, half_turns, pairs * sizeof(double), hipMemcpyHostToDevice);
+    hipError_t e = hipMalloc(&f, 3 * pairs * sizeof(double));
+    if (e == hipSuccess) e = hipMemcpy(f, turns, 3 * pairs * sizeof(double), hipMemcpyHostToDevice);
     if (e != hipSuccess) {
         (void)hipFree(f);
         delete h;
@@ -1439,7 +1441,7 @@ int unillm_hip_paged_kv8_create(int kv_type, int64_t n_kv_heads, int64_t head_di
         c.layout = rope->layout;
         c.rotary_dim = (int)rope->rotary_dim;
         c.magnitude = rope->magnitude;
-        const size_t n = (size_t)rope->rotary_dim / 2 * sizeof(double);
+        const size_t n = 3 * (size_t)rope->rotary_dim / 2 * sizeof(double);
         if ((e = hipMalloc(reinterpret_cast<void**>(&c.freq), n)) == hipSuccess)
             e = hipMemcpy(c.freq, rope->freq, n, hipMemcpyDeviceToDevice);
     }

@@ -123,7 +123,8 @@ struct unillm_rope {
     int layout;
     int64_t head_dim, rotary_dim;
     double magnitude;
-    double* freq;  // [rotary_dim / 2] half turns a position of each pair, in device memory
+    double* freq;  // [rotary_dim / 2] half turns a position of each pair, then [rotary_dim / 2][2] the cosine and
+                   // sine of one position's, in device memory
 };
 
 // The opaque handle of one layer's pool in 8 bits (paged8.hip): the shapes of unillm_paged_kv, codes of

@@ -83,8 +83,8 @@ constexpr int kWriteRows = 16;  // rows of a workgroup whose runs it takes, at m
 
 struct Runs {
     int slots[2 * kWriteRows];  // of row row0 - 1 + i, -1: none
-    int first[kWriteRows], count[kWriteRows];
-    int n, end;  // runs; rows from row0 on that they take in
+    int first[kWriteRows], count[kWriteRows];  // those of several rows first
+    int n, many, end;  // runs, those of several rows; rows from row0 on that they take in
 };
 
 // The runs that begin in rows row0 .. row0 + nr - 1 (slot: of row row0 - 1 + threadIdx.x, up to nr + 16 of
@@ -97,55 +97,92 @@ __device__ __forceinline__ void find_runs(Runs& r, int slot, int nr) {
     if (tid < 64) {
         const int sl = tid < nr ? r.slots[tid + 1] : -1;
         const bool begins = sl >= 0 && (r.slots[tid] + 1 != sl || sl % kBlock == 0);
-        const uint64_t all = __ballot(begins);
-        if (begins) {
-            int n = 1;
+        int n = begins ? 1 : 0;
+        if (begins)
             while (sl % kBlock + n < kBlock && tid + 1 + n < nr + 16 && r.slots[tid + 1 + n] == sl + n) ++n;
-            const int at = __popcll(all & ((1ull << tid) - 1));
+        const uint64_t many = __ballot(n > 1), ones = __ballot(n == 1), before = (1ull << tid) - 1;
+        if (begins) {
+            const int at = n > 1 ? __popcll(many & before) : __popcll(many) + __popcll(ones & before);
             r.first[at] = tid;
             r.count[at] = n;
             atomicMax(&r.end, tid + n);
         }
-        if (tid == 0) r.n = __popcll(all);
+        if (tid == 0) r.many = __popcll(many), r.n = __popcll(many | ones);
     }
     __syncthreads();
 }
 
-// The cosines and sines of rows row0 .. row0 + rows - 1, [rows][R / 2].  All threads of the workgroup.
-__device__ __forceinline__ void turns(const PagedKv8& c, const PageTable& t, int row0, int rows, double2* turn) {
+// The cosines and sines of `rows` rows (positions at: LDS), in turn [rows][R / 2], a row's pair p at (p % 4) R /
+// 8 + p / 4: what lanes read together lies together.  A thread takes a pair of several rows; a position
+// that follows the one before is that one's turn times a position's (f64, up to 7 times in a row: an angle off
+// by 2^-50, where the position's product with the frequency has 2^-53 of itself; f64's sines are
+// a third of a prompt's append otherwise: 4000 rows of 32 kv heads of 128, 61 us, 47 with no
+// rotation at all).  All threads of the workgroup.
+__device__ __forceinline__ void turns(const PagedKv8& c, const int* at, int rows, double2* turn) {
     const int pairs = c.rotary_dim / 2;
-    for (int i = threadIdx.x; i < rows * pairs; i += 256) {
-        double sn, cs;
-        sincospi((double)t.positions[row0 + i / pairs] * c.freq[i % pairs], &sn, &cs);
-        turn[i] = make_double2(cs * c.magnitude, sn * c.magnitude);
+    if (pairs == 0) return;
+    const int each = min(8, max(1, rows * pairs / 256)), sets = (rows + each - 1) / each;
+    const double2* unit = reinterpret_cast<const double2*>(c.freq + pairs);
+    for (int i = threadIdx.x; i < sets * pairs; i += 256) {
+        const int p = i % pairs, r0 = i / pairs * each, to = p % 4 * (pairs / 4) + p / 4;
+        const double f = c.freq[p];
+        const double2 w = unit[p];
+        double cs = 0.0, sn = 0.0;
+        for (int r = r0; r < min(r0 + each, rows); ++r) {
+            if (r > r0 && at[r] == at[r - 1] + 1) {
+                const double x = cs * w.x - sn * w.y;
+                sn = cs * w.y + sn * w.x;
+                cs = x;
+            } else {
+                sincospi((double)at[r] * f, &sn, &cs);
+            }
+            turn[r * pairs + to] = make_double2(cs * c.magnitude, sn * c.magnitude);
+        }
     }
     __syncthreads();
 }
 
-// Dimensions d .. d + 3 (d a multiple of 4) of the head at x, rotated.
-__device__ __forceinline__ f32x4 rotated4(const PagedKv8& c, const float* x, int d, const double2* turn) {
-    f32x4 v = *reinterpret_cast<const f32x4*>(x + d);
-    const int R = c.rotary_dim, half = R / 2;
-    if (d >= R) return v;
+// Eight dimensions of a head, four at d0 and four at d1, that turn among themselves: unit u of D / 8.
+struct Octet {
+    f32x4 lo, hi;
+};
+__device__ __forceinline__ int2 octet_at(const PagedKv8& c, int u) {
+    const int R = c.rotary_dim;
+    if (c.layout == UNILLM_ROPE_HALF && 8 * u < R) return make_int2(4 * u, 4 * u + R / 2);
+    return make_int2(8 * u, 8 * u + 4);
+}
+__device__ __forceinline__ Octet octet(const float* x, int2 d) {
+    return Octet{*reinterpret_cast<const f32x4*>(x + d.x), *reinterpret_cast<const f32x4*>(x + d.y)};
+}
+// It rotated, in f64, to f32.
+__device__ __forceinline__ void rotate(const PagedKv8& c, Octet& o, int u, const double2* turn) {
+    const int R = c.rotary_dim;
+    if (8 * u >= R) return;
+    double2 z[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = turn[e * (R / 8) + u];
+    auto pair = [](float& a, float& b, const double2& w) {
+        const double x = a, y = b;
+        a = (float)(x * w.x - y * w.y);
+        b = (float)(x * w.y + y * w.x);
+    };
+    float a[4], b[4];
     if (c.layout == UNILLM_ROPE_HALF) {
-        const bool lo = d < half;
-        const f32x4 w = *reinterpret_cast<const f32x4*>(x + (lo ? d + half : d - half));
-        const double2* z = turn + (lo ? d : d - half);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const double a = v[e], b = w[e];
-            v[e] = (float)(lo ? a * z[e].x - b * z[e].y : b * z[e].y + a * z[e].x);
+            a[e] = o.lo[e], b[e] = o.hi[e];
+            pair(a[e], b[e], z[e]);
         }
     } else {
-        const double2* z = turn + d / 2;
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            const double a = v[e], b = v[e + 1];
-            v[e] = (float)(a * z[e / 2].x - b * z[e / 2].y);
-            v[e + 1] = (float)(a * z[e / 2].y + b * z[e / 2].x);
-        }
+        for (int e = 0; e < 4; ++e) a[e] = o.lo[e], b[e] = o.hi[e];
+        pair(a[0], a[1], z[0]);
+        pair(a[2], a[3], z[1]);
+        pair(b[0], b[1], z[2]);
+        pair(b[2], b[3], z[3]);
     }
-    return v;
+    o.lo = f32x4{a[0], a[1], a[2], a[3]};
+    o.hi = f32x4{b[0], b[1], b[2], b[3]};
 }
 
 // A value's magnitude where it is finite, else 0 (and `odd` is set).
@@ -156,93 +193,101 @@ __device__ __forceinline__ float magnitude(float v, bool& odd) {
     return 0.0f;
 }
 
-// Byte of a run's block: what its values need, and what it has if it holds positions before them.
-template <class C>
-__device__ __forceinline__ int grow(uint8_t* exps, int64_t at, float top, bool held, int& had) {
-    const int need = least_exponent<C>(wave_max(top));
-    had = held ? min((int)exps[at], 254) : 0;
-    const int b = max(need, had);
-    if ((threadIdx.x & 63) == 0) exps[at] = (uint8_t)b;
-    return b;
-}
-
-// A run's keys of kv head g: rows row .. row + n - 1 of kv (a head's keys at x), into slots sl ..
+// A run's keys of kv head g (its first row's at x), into slots sl ..
 template <class C, int D>
-__device__ void write_keys(const PagedKv8& c, const float* x, int64_t stride, int n, int sl, int g,
-                           const double2* turn, bool& odd) {
-    constexpr int CH = D / 4, RP = 64 / CH, N = kBlock / RP;  // lanes a row, rows and passes
-    const int lane = threadIdx.x & 63, d = lane % CH * 4, sub = lane / CH;
+__device__ __forceinline__ void write_keys(const PagedKv8& c, const float* x, int64_t stride, int n, int sl, int g,
+                                           const double2* turn, bool& odd) {
+    constexpr int CH = D / 8, RP = 64 / CH, N = kBlock / RP;  // lanes a row, rows and passes
+    const int lane = threadIdx.x & 63, u = lane % CH, sub = lane / CH;
     const int pairs = c.rotary_dim / 2, off = sl % kBlock;
     const int in_page = sl & ((int)c.page_size - 1);
     const int64_t head = (int64_t)(sl >> c.page_shift) * c.n_kv_heads + g;
-    uint8_t* dst = c.k + ((head << c.page_shift) + in_page) * D + d;
-    f32x4 v[N];
+    uint8_t* dst = c.k + ((head << c.page_shift) + in_page) * D;
+    uint8_t* exps = c.k_exp + ((head << c.page_shift >> 4) + in_page / kBlock);
+    const int had = off > 0 ? min((int)*exps, 254) : 0;
+    const int2 d = octet_at(c, u);
+    Octet v[N];
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        v[i] = 0.0f;
+        v[i].lo = v[i].hi = 0.0f;
         const int r = i * RP + sub;
-        if (r < n) v[i] = rotated4(c, x + r * stride, d, turn + r * pairs);
+        if (r < n) v[i] = octet(x + r * stride, d);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+        const int r = i * RP + sub;
+        if (r < n) rotate(c, v[i], u, turn + r * pairs);
         // (opaque: the keys are rows of f32 first, and rounded from there)
-        asm volatile("" : "+v"(v[i]));
+        asm volatile("" : "+v"(v[i].lo), "+v"(v[i].hi));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, magnitude(v[i][e], odd));
+        for (int e = 0; e < 4; ++e) {
+            top = fmaxf(top, magnitude(v[i].lo[e], odd));
+            top = fmaxf(top, magnitude(v[i].hi[e], odd));
+        }
     }
-    int had;
-    const int b = grow<C>(c.k_exp, (head << c.page_shift >> 4) + in_page / kBlock, top, off > 0, had);
+    const int b = max(least_exponent<C>(wave_max(top)), had);
+    if (lane == 0) *exps = (uint8_t)b;
     const float inv = power(254 - b);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int r = i * RP + sub;
-        if (r < n)
-            *reinterpret_cast<uint32_t*>(dst + r * D) =
-                encode4<C>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+        if (r < n) {
+            const f32x4 lo = v[i].lo * inv, hi = v[i].hi * inv;
+            *reinterpret_cast<uint32_t*>(dst + r * D + d.x) = encode4<C>(lo[0], lo[1], lo[2], lo[3]);
+            *reinterpret_cast<uint32_t*>(dst + r * D + d.y) = encode4<C>(hi[0], hi[1], hi[2], hi[3]);
+        }
     }
     if (off > 0 && b > had) {
-        const float f = power(max(127 + had - b, 1));
-        uint32_t* old = reinterpret_cast<uint32_t*>(dst - d - off * D);
-        for (int i = lane; i < off * CH; i += 64) old[i] = again4<C>(old[i], f);
+        const float f = power(127 + had - b);
+        uint32_t* old = reinterpret_cast<uint32_t*>(dst - off * D);
+        for (int i = lane; i < off * (D / 4); i += 64) old[i] = again4<C>(old[i], f);
     }
 }
 
 // A run's values.
 template <class C, int D>
-__device__ void write_values(const PagedKv8& c, const float* x, int64_t stride, int n, int sl, int g, bool& odd) {
-    constexpr int N = D / 64;
+__device__ __forceinline__ void write_values(const PagedKv8& c, const float* x, int64_t stride, int n, int sl, int g,
+                                             bool& odd) {
+    constexpr int N = D / 64;  // neighbouring dimensions a lane
+    struct alignas(4 * N) Dims {
+        float v[N];
+    };
     const int lane = threadIdx.x & 63, off = sl % kBlock;
     const int in_page = sl & ((int)c.page_size - 1);
     const int64_t head = (int64_t)(sl >> c.page_shift) * c.n_kv_heads + g;
-    uint8_t* dst = c.v + ((head * D + lane) << c.page_shift) + in_page / kBlock * kBlock;
-    float v[N][kBlock], top = 0.0f;  // by position of the block
+    uint8_t* dst = c.v + ((head * D + N * lane) << c.page_shift) + in_page / kBlock * kBlock;
+    uint8_t* exps = c.v_exp + ((head << c.page_shift >> 4) + in_page / kBlock);
+    const int had = off > 0 ? min((int)*exps, 254) : 0;
+    u32x4 old[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        old[j] = 0u;
+        if (n < kBlock) old[j] = *reinterpret_cast<const u32x4*>(dst + ((int64_t)j << c.page_shift));
+    }
+    Dims v[kBlock];  // by position of the block
+    float top = 0.0f;
 #pragma unroll
     for (int p = 0; p < kBlock; ++p) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j][p] = 0.0f;
-        if (p >= off && p < off + n)
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j][p] = x[(p - off) * stride + 64 * j + lane];
+        for (int j = 0; j < N; ++j) v[p].v[j] = 0.0f;
+        if (p >= off && p < off + n) v[p] = *reinterpret_cast<const Dims*>(x + (p - off) * stride + N * lane);
     }
 #pragma unroll
     for (int p = 0; p < kBlock; ++p)
 #pragma unroll
-        for (int j = 0; j < N; ++j) top = fmaxf(top, magnitude(v[j][p], odd));
-    int had;
-    const int b = grow<C>(c.v_exp, (head << c.page_shift >> 4) + in_page / kBlock, top, off > 0, had);
-    const float inv = power(254 - b), f = power(max(127 + had - b, 1));
+        for (int j = 0; j < N; ++j) top = fmaxf(top, magnitude(v[p].v[j], odd));
+    const int b = max(least_exponent<C>(wave_max(top)), had);
+    if (lane == 0) *exps = (uint8_t)b;
+    const float inv = power(254 - b), f = power(127 + had - b);
     const bool anew = off > 0 && b > had;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        u32x4* to = reinterpret_cast<u32x4*>(dst + ((int64_t)(64 * j) << c.page_shift));
-        u32x4 w = 0u;
-        if (n < kBlock) w = *to;
+        u32x4 w;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t fresh = encode4<C>(v[j][4 * i] * inv, v[j][4 * i + 1] * inv, v[j][4 * i + 2] * inv,
-                                              v[j][4 * i + 3] * inv);
-            const uint32_t old = anew ? again4<C>(w[i], f) : w[i];
+            const uint32_t fresh = encode4<C>(v[4 * i].v[j] * inv, v[4 * i + 1].v[j] * inv, v[4 * i + 2].v[j] * inv,
+                                              v[4 * i + 3].v[j] * inv);
             uint32_t is_old = 0, is_new = 0;  // bytes of the word
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -250,11 +295,102 @@ __device__ void write_values(const PagedKv8& c, const float* x, int64_t stride, 
                 if (p < off) is_old |= 0xFFu << (8 * e);
                 else if (p < off + n) is_new |= 0xFFu << (8 * e);
             }
-            w[i] = (fresh & is_new) | (old & is_old) | (w[i] & ~(is_new | is_old));
+            const uint32_t kept = anew && is_old != 0 ? (again4<C>(old[j][i], f) & is_old) | (old[j][i] & ~is_old) : old[j][i];
+            w[i] = (fresh & is_new) | (kept & ~is_new);
         }
-        *to = w;
+        *reinterpret_cast<u32x4*>(dst + ((int64_t)j << c.page_shift)) = w;
     }
 }
+
+// Several runs of one row each (decoding requests'): their keys, each by the lanes of one row.
+template <class C, int D>
+__device__ __forceinline__ void write_one_keys(const PagedKv8& c, const float* kv, int64_t stride, const Runs& runs,
+                                               int from, int n, int g, const double2* turn, bool& odd) {
+    constexpr int CH = D / 8;  // lanes a row
+    const int lane = threadIdx.x & 63, u = lane % CH;
+    const int row = runs.first[from + min(lane / CH, n - 1)], sl = runs.slots[row + 1];
+    const bool live = lane / CH < n;
+    const int off = sl % kBlock, in_page = sl & ((int)c.page_size - 1);
+    const int64_t head = (int64_t)(sl >> c.page_shift) * c.n_kv_heads + g;
+    uint8_t* dst = c.k + ((head << c.page_shift) + in_page) * D;
+    uint8_t* exps = c.k_exp + ((head << c.page_shift >> 4) + in_page / kBlock);
+    const int2 d = octet_at(c, u);
+    Octet v = octet(kv + row * stride + (int64_t)g * D, d);
+    const int had = off > 0 ? min((int)*exps, 254) : 0;
+    rotate(c, v, u, turn + row * (c.rotary_dim / 2));
+    asm volatile("" : "+v"(v.lo), "+v"(v.hi));  // (rows of f32 first)
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        top = fmaxf(top, magnitude(v.lo[e], odd));
+        top = fmaxf(top, magnitude(v.hi[e], odd));
+    }
+#pragma unroll
+    for (int o = CH / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const int b = max(least_exponent<C>(top), had);
+    if (!live) return;
+    if (u == 0) *exps = (uint8_t)b;
+    const float inv = power(254 - b);
+    const f32x4 lo = v.lo * inv, hi = v.hi * inv;
+    *reinterpret_cast<uint32_t*>(dst + d.x) = encode4<C>(lo[0], lo[1], lo[2], lo[3]);
+    *reinterpret_cast<uint32_t*>(dst + d.y) = encode4<C>(hi[0], hi[1], hi[2], hi[3]);
+    if (off > 0 && b > had) {
+        const float f = power(127 + had - b);
+        uint32_t* old = reinterpret_cast<uint32_t*>(dst - off * D);
+        for (int i = u; i < off * (D / 4); i += CH) old[i] = again4<C>(old[i], f);
+    }
+}
+
+// The values of up to B of them.
+template <class C, int D, int B>
+__device__ __forceinline__ void write_one_values(const PagedKv8& c, const float* kv, int64_t stride, const Runs& runs,
+                                                 int from, int n, int g, bool& odd) {
+    constexpr int N = D / 64;  // neighbouring dimensions a lane
+    struct alignas(4 * N) Dims {
+        float v[N];
+    };
+    const int lane = threadIdx.x & 63;
+    Dims v[B];
+    int sl[B], had[B];
+    int64_t head[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        const int row = __builtin_amdgcn_readfirstlane(runs.first[from + min(i, n - 1)]);
+        sl[i] = __builtin_amdgcn_readfirstlane(runs.slots[row + 1]);
+        head[i] = (int64_t)(sl[i] >> c.page_shift) * c.n_kv_heads + g;
+        v[i] = *reinterpret_cast<const Dims*>(kv + row * stride + (int64_t)(c.n_kv_heads + g) * D + N * lane);
+        had[i] = c.v_exp[(head[i] << c.page_shift >> 4) + (sl[i] & ((int)c.page_size - 1)) / kBlock];
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        if (i >= n) break;
+        const int off = sl[i] % kBlock, in_page = sl[i] & ((int)c.page_size - 1);
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) top = fmaxf(top, magnitude(v[i].v[j], odd));
+        const int was = off > 0 ? min(had[i], 254) : 0;
+        const int b = max(least_exponent<C>(wave_max(top)), was);
+        if (lane == 0) c.v_exp[(head[i] << c.page_shift >> 4) + in_page / kBlock] = (uint8_t)b;
+        uint8_t* dst = c.v + ((head[i] * D + N * lane) << c.page_shift) + in_page - off;
+        const float inv = power(254 - b);
+        if (off > 0 && b > was) {  // (the codes before it, in the row's first words)
+            const float f = power(127 + was - b);
+            for (int j = 0; j < N; ++j)
+                for (int w = 0; 4 * w < off; ++w) {
+                    uint32_t* to = reinterpret_cast<uint32_t*>(dst + ((int64_t)j << c.page_shift)) + w;
+                    const uint32_t x = *to, keep = off - 4 * w >= 4 ? 0xFFFFFFFFu : (1u << (8 * (off - 4 * w))) - 1;
+                    *to = (again4<C>(x, f) & keep) | (x & ~keep);
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            dst[((int64_t)j << c.page_shift) + off] = (uint8_t)encode4<C>(v[i].v[j] * inv, 0.0f, 0.0f, 0.0f);
+    }
+}
+
+// Consecutive numbers to workgroups of one XCD, which takes every eighth: neighbours share lines of a V page
+// (1/8 of a line each at a page of 128), which each XCD's cache fetches for itself.
+__device__ __forceinline__ int by_xcd(int i, int n) { return i % 8 * (n / 8) + i / 8; }
 
 // What a call's first kernel does: `plan` workgroups deal the work out; then q_groups take q_rows query
 // rows and q_heads heads each (rotated, times log2 e / sqrt(hd), f32, into q_out); the rest write the runs
@@ -263,14 +399,27 @@ struct Prepare {
     const float *q, *kv;
     int64_t stride;  // of both
     float* q_out;
-    int plan, q_groups, q_rows, q_heads, rows, heads;
+    int plan, q_groups, q_rows, q_heads, rows, heads, writes;  // writes: its workgroups, a multiple of 8
 };
 
 template <class C, int D>
-__global__ __launch_bounds__(256) void kv8_prepare_kernel(PagedKv8 c, PageTable t, Call a, Prepare p) {
+__global__ __launch_bounds__(256, D == 256 ? 3 : 4) void kv8_prepare_kernel(PagedKv8 c, PageTable t, Call a, Prepare p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ int at[2 * kWriteRows];
     double2* turn = reinterpret_cast<double2*>(lds);
     const int tid = threadIdx.x;
+    const int KVH = (int)c.n_kv_heads, bx = (int)blockIdx.x - p.plan;
+    const bool writes = bx >= p.q_groups;
+    // the workgroup's rows and heads
+    const int of = writes ? KVH : a.H, nr = writes ? p.rows : p.q_rows, each = writes ? p.heads : p.q_heads;
+    const int groups = (of + each - 1) / each, wx = writes ? by_xcd(bx - p.q_groups, p.writes) : bx;
+    const int row0 = wx / groups * nr, h0 = wx % groups * each, heads = min(each, of - h0);
+    // (slots and positions are requested with the plan's header: both arrays hold max_tokens)
+    int slot = -1, pos = 0;
+    if (bx >= 0 && tid < nr + 16) {
+        if (writes && row0 - 1 + tid >= 0 && row0 - 1 + tid < t.max_tokens) slot = t.slots[row0 - 1 + tid];
+        if (row0 + tid < t.max_tokens) pos = t.positions[row0 + tid];
+    }
     if (!step_fits(t, a.n)) {
         if (p.plan == 0) {
             if (blockIdx.x == 0 && tid == 0)
@@ -282,48 +431,60 @@ __global__ __launch_bounds__(256) void kv8_prepare_kernel(PagedKv8 c, PageTable 
         fail_call(t, a, D, blockIdx.x, gridDim.x);
         return;
     }
-    int bx = (int)blockIdx.x;
-    if (bx < p.plan) {
-        if (bx == 0 && tid == 0) *a.redo_count = 0;
-        if (bx == 0) return plan<64, kNarrowRows8>(t, a, kNarrow, reinterpret_cast<int*>(lds));
+    if (bx < 0) {
+        if (blockIdx.x == 0 && tid == 0) *a.redo_count = 0;
+        if (blockIdx.x == 0) return plan<64, kNarrowRows8>(t, a, kNarrow, reinterpret_cast<int*>(lds));
         return plan<D == 256 ? 32 : 64, kNarrowRows8>(t, a, kWide, reinterpret_cast<int*>(lds));
     }
-    bx -= p.plan;
     const int total = t.counts[kPagesTokens];
-    if (bx < p.q_groups) {
-        const int groups = (a.H + p.q_heads - 1) / p.q_heads;
-        const int row0 = bx / groups * p.q_rows, h0 = bx % groups * p.q_heads;
-        const int rows = min(p.q_rows, total - row0), heads = min(p.q_heads, a.H - h0);
-        if (rows <= 0) return;
-        turns(c, t, row0, rows, turn);
+    if (row0 >= total) return;
+    if (tid < nr + 16) at[tid] = pos;
+    const int pairs = c.rotary_dim / 2;
+    if (!writes) {
+        const int rows = min(nr, total - row0);
+        __syncthreads();
+        turns(c, at, rows, turn);
         const float scale = kLog2e / sqrtf((float)D);
-        constexpr int CH = D / 4;
+        constexpr int CH = D / 8;
+#pragma unroll 2
         for (int i = tid; i < rows * heads * CH; i += 256) {
-            const int d = i % CH * 4, h = h0 + i / CH % heads, r = i / CH / heads;
-            const f32x4 v = rotated4(c, p.q + (row0 + r) * p.stride + (int64_t)h * D, d, turn + r * (c.rotary_dim / 2));
-            *reinterpret_cast<f32x4*>(p.q_out + ((int64_t)(row0 + r) * a.H + h) * D + d) = v * scale;
+            const int u = i % CH, h = h0 + i / CH % heads, r = i / CH / heads;
+            const int2 d = octet_at(c, u);
+            Octet o = octet(p.q + (row0 + r) * p.stride + (int64_t)h * D, d);
+            rotate(c, o, u, turn + r * pairs);
+            float* to = p.q_out + ((int64_t)(row0 + r) * a.H + h) * D;
+            *reinterpret_cast<f32x4*>(to + d.x) = o.lo * scale;
+            *reinterpret_cast<f32x4*>(to + d.y) = o.hi * scale;
         }
         return;
     }
-    bx -= p.q_groups;
     __shared__ Runs runs;
-    const int KVH = (int)c.n_kv_heads, groups = (KVH + p.heads - 1) / p.heads;
-    const int row0 = bx / groups * p.rows, g0 = bx % groups * p.heads, heads = min(p.heads, KVH - g0);
-    if (row0 >= total) return;
-    const int row = row0 - 1 + tid;
-    find_runs(runs, tid < p.rows + 16 && row >= 0 && row < total ? t.slots[row] : -1, p.rows);
+    find_runs(runs, row0 - 1 + tid < total ? slot : -1, nr);
     if (runs.n == 0) return;
-    turns(c, t, row0, runs.end, turn);
+    turns(c, at, runs.end, turn);
     bool odd = false;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    for (int i = wv; i < runs.n * heads * 2; i += 4) {
-        const int g = g0 + i / 2 % heads, run = i / 2 / heads;
-        const int r = __builtin_amdgcn_readfirstlane(runs.first[run]);
-        const int n = __builtin_amdgcn_readfirstlane(runs.count[run]);
-        const int sl = __builtin_amdgcn_readfirstlane(runs.slots[r + 1]);
-        const float* x = p.kv + (row0 + r) * p.stride + (int64_t)g * D;
-        if (i % 2 == 0) write_keys<C, D>(c, x, p.stride, n, sl, g, turn + r * (c.rotary_dim / 2), odd);
-        else write_values<C, D>(c, x + (int64_t)KVH * D, p.stride, n, sl, g, odd);
+    const float* kv = p.kv + row0 * p.stride;
+    constexpr int RP = 512 / D;  // one-row runs of a task of keys
+    const int many = runs.many, ones = runs.n - many, batch = ones > 4 ? 4 : 1;
+    const int k_tasks = (ones + RP - 1) / RP, tasks = 2 * many + k_tasks + (ones + batch - 1) / batch;
+    for (int i = wv; i < tasks * heads; i += 4) {
+        const int g = h0 + i % heads, task = i / heads;
+        if (task < 2 * many) {
+            const int r = __builtin_amdgcn_readfirstlane(runs.first[task / 2]);
+            const int n = __builtin_amdgcn_readfirstlane(runs.count[task / 2]);
+            const int sl = __builtin_amdgcn_readfirstlane(runs.slots[r + 1]);
+            const float* x = kv + r * p.stride + (int64_t)g * D;
+            if (task % 2 == 0) write_keys<C, D>(c, x, p.stride, n, sl, g, turn + r * pairs, odd);
+            else write_values<C, D>(c, x + (int64_t)KVH * D, p.stride, n, sl, g, odd);
+        } else if (task < 2 * many + k_tasks) {
+            const int from = (task - 2 * many) * RP;
+            write_one_keys<C, D>(c, kv, p.stride, runs, many + from, min(RP, ones - from), g, turn, odd);
+        } else {
+            const int from = (task - 2 * many - k_tasks) * batch;
+            if (batch == 4) write_one_values<C, D, 4>(c, kv, p.stride, runs, many + from, min(4, ones - from), g, odd);
+            else write_one_values<C, D, 1>(c, kv, p.stride, runs, many + from, 1, g, odd);
+        }
     }
     if (__any(odd) && (tid & 63) == 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesNotFinite);
 }
@@ -341,7 +502,7 @@ template <int D>
 struct Narrow8Lds {
     static constexpr int NB = D / 32, OT = D / 16;
     static constexpr int IDS = 0;                          // page ids of 256 visits, 4 each
-    static constexpr int STAT = IDS + 4096;                // row scales, maxima, sums, flags
+    static constexpr int STAT = IDS + 4096;                // maxima, sums, flags
     static constexpr int Q = STAT + 1024;                  // q's parts [2][NB][64][16 B]
     static constexpr int QBYTES = 2 * NB * 1024;
     static constexpr int O = Q;                            // later the waves' sums [4][OT][64][16 B]
@@ -437,8 +598,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
     constexpr int NB = L::NB, OT = L::OT, KB = D / 64, U = 64;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int* ids = reinterpret_cast<int*>(lds + L::IDS);               // [256][4]
-    float* rowmax = reinterpret_cast<float*>(lds + L::STAT);       // [16]
-    float* wm = rowmax + 16;                                        // [4][16]
+    float* wm = reinterpret_cast<float*>(lds + L::STAT);           // [4][16]
     float* wl = wm + 64;                                            // [4][16]
     int* flags = reinterpret_cast<int*>(wl + 64);                  // [0] a bad page, [1] rows to redo
     u32x4* qp = reinterpret_cast<u32x4*>(lds + L::Q);
@@ -455,13 +615,55 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
         const int* pages = t.table + (int64_t)it.id * t.max_pages;
         const int pmin = ctx + it.row0 / G, pmax = ctx + (it.row0 + it.rows - 1) / G;
         const Visits<U> vis(pmin, pmax, a.window, a.sinks);
-        // q's parts: task (product, lane) as the B operand takes it
+        bool bad = false;
+        auto read_ids = [&](int seg) {  // the page of each block of up to 256 visits
+            for (int i = tid; i < 4 * min(256, it.nv - seg); i += 256) {
+                int j = vis.key(it.v0 + seg + i / 4);
+                if (j + i % 4 * kBlock < len) j += i % 4 * kBlock;  // (past the sequence: the visit's first again)
+                int pg = pages[j >> shift];
+                if ((unsigned)pg >= (unsigned)c.n_pages) {
+                    pg = 0;
+                    bad = true;
+                }
+                ids[i] = pg;
+            }
+        };
+        // block x of visit v of a segment: its page and head, and its first key's place in the page
+        auto block = [&](int seg, int v, int x, int64_t& head, int& off) {
+            const int j = vis.key(it.v0 + seg + v);
+            head = (int64_t)ids[4 * v + x] * KVH + g;
+            off = (j + (j + x * kBlock < len ? x * kBlock : 0)) & (ps - 1);
+        };
+        u32x4 kr[4][KB], vr[OT];
+        int ke = 0, ve = 0;
+        auto load_k = [&](int seg, int v) {
+            int64_t head;
+            int off;
+            block(seg, v, col / 4, head, off);
+            const uint8_t* k = c.k + ((head << shift) + off + col % 4) * D + 16 * qd;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int b = 0; b < KB; ++b) kr[s][b] = *reinterpret_cast<const u32x4*>(k + 4 * s * D + 64 * b);
+            block(seg, v, qd, head, off);
+            ke = c.k_exp[(head << shift >> 4) + off / kBlock];
+        };
+        auto load_v = [&](int seg, int v) {
+            int64_t head;
+            int off;
+            block(seg, v, qd, head, off);
+            const uint8_t* x = c.v + ((head * D + col) << shift) + off;
+#pragma unroll
+            for (int i = 0; i < OT; ++i) vr[i] = *reinterpret_cast<const u32x4*>(x + ((16 * i) << shift));
+            ve = c.v_exp[(head << shift >> 4) + off / kBlock];
+        };
+        // q's parts: task (product, lane) as the B operand takes it.  (Its requests and the page ids' go out
+        // together, the first keys' and values' before its parts are formed.)
         constexpr int TASKS = (NB * 64 + 255) / 256;
         f32x8 qv[TASKS];
+        float mx = 0.0f;
         __syncthreads();  // (the item before is done with the LDS)
-        if (tid < 16) rowmax[tid] = 0.0f;
         if (tid < 2) flags[tid] = 0;
-        __syncthreads();
 #pragma unroll
         for (int i = 0; i < TASKS; ++i) {
             const int f = i * 256 + tid, r = f % 16, b = f / 64, d = b / 2 * 64 + f / 16 % 4 * 16 + b % 2 * 8;
@@ -471,86 +673,57 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
                 const f32x4* x = reinterpret_cast<const f32x4*>(
                     a.qkv + (first + rr / G) * a.qstride + (int64_t)(g * G + rr % G) * D + d);
                 const f32x4 lo = x[0], hi = x[1];
-                float mx = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    qv[i][j] = j < 4 ? lo[j % 4] : hi[j % 4];
-                    mx = fmaxf(mx, fabsf(qv[i][j]));
-                }
-                atomicMax(reinterpret_cast<int*>(rowmax) + r, __float_as_int(mx));  // (magnitudes order as their bits)
+                for (int j = 0; j < 8; ++j) qv[i][j] = j < 4 ? lo[j % 4] : hi[j % 4];
             }
         }
+        read_ids(0);
+#pragma unroll
+        for (int i = 0; i < TASKS; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(qv[i][j]));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (lane < 16) wm[wv * 16 + lane] = mx;
         __syncthreads();
-        const float inv = row_scale(rowmax[col]).y;  // of this lane's row
+        if (wv < min(256, it.nv)) {
+            load_k(0, wv);
+            load_v(0, wv);
+        }
+        const float2 size = row_scale(fmaxf(fmaxf(wm[col], wm[16 + col]), fmaxf(wm[32 + col], wm[48 + col])));
+        const float inv = size.y;  // of this lane's row (and tasks': f % 16 is lane % 16)
 #pragma unroll
         for (int i = 0; i < TASKS; ++i) {
             const int f = i * 256 + tid;
             if (f < NB * 64) {
-                qv[i] *= row_scale(rowmax[f % 16]).x;
                 u32x4 p[2];
-                parts_f16(qv[i], p);
+                parts_f16(qv[i] * size.x, p);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) qp[q * NB * 64 + f] = p[q];
             }
         }
+        __syncthreads();
+        u32x4 q[2][NB];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) q[i][b] = qp[(i * NB + b) * 64 + lane];
         const int ppos = ctx + min(it.row0 + col, it.row0 + it.rows - 1) / G;  // the lane's row's position
 
         float ref = -INFINITY, l = 0.0f;
         f32x4 o[OT];
 #pragma unroll
         for (int i = 0; i < OT; ++i) o[i] = 0.0f;
-        u32x4 q[2][NB];
-        u32x4 kr[4][KB], vr[OT];
-        int ke = 0, ve = 0;
         for (int seg = 0; seg < it.nv; seg += 256) {
             const int nseg = min(256, it.nv - seg);
-            __syncthreads();
-            for (int i = tid; i < 4 * nseg; i += 256) {  // the page of each block
-                int j = vis.key(it.v0 + seg + i / 4);
-                if (j + i % 4 * kBlock < len) j += i % 4 * kBlock;  // (past the sequence: the visit's first again)
-                int pg = pages[j >> shift];
-                if ((unsigned)pg >= (unsigned)c.n_pages) {
-                    pg = 0;
-                    flags[0] = 1;
+            if (seg > 0) {
+                __syncthreads();
+                read_ids(seg);
+                __syncthreads();
+                if (wv < nseg) {
+                    load_k(seg, wv);
+                    load_v(seg, wv);
                 }
-                ids[i] = pg;
-            }
-            __syncthreads();
-            if (seg == 0)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) q[i][b] = qp[(i * NB + b) * 64 + lane];
-            // block x of visit v: its page and head, and its first key's place in the page
-            auto block = [&](int v, int x, int64_t& head, int& off) {
-                const int j = vis.key(it.v0 + seg + v);
-                head = (int64_t)ids[4 * v + x] * KVH + g;
-                off = (j + (j + x * kBlock < len ? x * kBlock : 0)) & (ps - 1);
-            };
-            auto load_k = [&](int v) {
-                int64_t head;
-                int off;
-                block(v, col / 4, head, off);
-                const uint8_t* k = c.k + ((head << shift) + off + col % 4) * D + 16 * qd;
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int b = 0; b < KB; ++b) kr[s][b] = *reinterpret_cast<const u32x4*>(k + 4 * s * D + 64 * b);
-                block(v, qd, head, off);
-                ke = c.k_exp[(head << shift >> 4) + off / kBlock];
-            };
-            auto load_v = [&](int v) {
-                int64_t head;
-                int off;
-                block(v, qd, head, off);
-                const uint8_t* x = c.v + ((head * D + col) << shift) + off;
-#pragma unroll
-                for (int i = 0; i < OT; ++i) vr[i] = *reinterpret_cast<const u32x4*>(x + ((16 * i) << shift));
-                ve = c.v_exp[(head << shift >> 4) + off / kBlock];
-            };
-            if (wv < nseg) {
-                load_k(wv);
-                load_v(wv);
             }
             for (int v = wv; v < nseg; v += 4) {
                 const int j0 = vis.key(it.v0 + seg + v);
@@ -569,7 +742,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[4 * u + r] = (hi[r] + lo[r]) * times;
                 }
-                if (v + 4 < nseg) load_k(v + 4);
+                if (v + 4 < nseg) load_k(seg, v + 4);
                 // masks, where some row of the tile does not see the whole visit
                 const bool whole = j0 + U - 1 <= pmin &&
                                    (a.window == 0 || j0 > pmax - a.window || j0 + U <= a.sinks);
@@ -628,13 +801,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
                         o[i] = mfma16<bf16_t>(x, p[0], o[i]);
                     }
                 }
-                if (v + 4 < nseg) load_v(v + 4);
+                if (v + 4 < nseg) load_v(seg, v + 4);
             }
         }
 
         // the four waves' sums: scaled to one reference, added through LDS
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
+        if (bad) flags[0] = 1;
         __syncthreads();  // (q's parts are read)
         if (lane < 16) {
             wm[wv * 16 + lane] = ref;
@@ -720,6 +894,9 @@ struct Wide8Lds {
     static constexpr int STAT = USED > ROWS ? USED : ROWS;  // whether a page is bad, K's powers of two
     static constexpr int BYTES = STAT + 64 + 64;
     static constexpr int TASKS = U * D / 8 / NT;            // 8-code chunks of K (or V) a thread
+    // Operands held: read so many products less one ahead.  (One wave a SIMD at hd 256: nothing else
+    // runs while it waits.)
+    static constexpr int AHEAD = D == 256 ? 4 : 2;
     __device__ static uint32_t kslot(uint32_t r, uint32_t c) {
         return D >= 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
     }
@@ -965,24 +1142,26 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
             for (int u = 0; u < NG; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[u][e] = zero;
-            u32x4 kp[2][NG], qx[2];
+            u32x4 kp[L::AHEAD][NG], qx[L::AHEAD];
             auto read = [&](int b) {
 #pragma unroll
                 for (int u = 0; u < NG; ++u)
-                    kp[b % 2][u] = *reinterpret_cast<const u32x4*>(buf + L::K + 32 * u * L::KROW + (ka ^ 32 * b));
-                if (L::kQl) qx[b % 2] = ql[b * 64];
+                    kp[b % L::AHEAD][u] = *reinterpret_cast<const u32x4*>(buf + L::K + 32 * u * L::KROW + (ka ^ 32 * b));
+                if (L::kQl) qx[b % L::AHEAD] = ql[b * 64];
             };
-            read(0);
+#pragma unroll
+            for (int b = 0; b < L::AHEAD - 1; ++b) read(b);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                if (b + 1 < NB) read(b + 1);
+                if (b + L::AHEAD - 1 < NB) read(b + L::AHEAD - 1);
                 if (kStoreEarly && b % (NB / 4) == 0) fetch_piece(n + 2, b / (NB / 4));
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int x = 1; x >= 0; --x)
 #pragma unroll
                     for (int u = 0; u < NG; ++u)
-                        s[u] = mfma32<f16_t>(kp[b % 2][u], x < L::QREGS ? q[x < L::QREGS ? x : 0][b] : qx[b % 2], s[u]);
+                        s[u] = mfma32<f16_t>(kp[b % L::AHEAD][u], x < L::QREGS ? q[x < L::QREGS ? x : 0][b] : qx[b % L::AHEAD],
+                                             s[u]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
@@ -1054,20 +1233,22 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                 const uint8_t* buf = lds + (n + 1) % GR * L::PAIR;
                 uint32_t va = vat;
                 asm volatile("" : "+v"(va));
-                u32x4 vp[2];
+                u32x4 vp[L::AHEAD];
                 auto read = [&](int i) {
-                    vp[i % 2] = *reinterpret_cast<const u32x4*>(buf + L::V + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
+                    vp[i % L::AHEAD] =
+                        *reinterpret_cast<const u32x4*>(buf + L::V + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
                 };
-                read(0);
+#pragma unroll
+                for (int i = 0; i < L::AHEAD - 1; ++i) read(i);
 #pragma unroll
                 for (int i = 0; i < 2 * NG * OT; ++i) {
-                    if (i + 1 < 2 * NG * OT) read(i + 1);
+                    if (i + L::AHEAD - 1 < 2 * NG * OT) read(i + L::AHEAD - 1);
                     // (what is stored next is requested between the first MFMAs after the stores before)
                     if (!kStoreEarly && i % (NG * OT / 2) == 0) fetch_piece(n + 2 + grp, i / (NG * OT / 2));
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int x = 2; x >= 0; --x)
-                        o[i % OT] = mfma32<bf16_t>(vp[i % 2], p[i / OT / 2][i / OT % 2][x], o[i % OT]);
+                        o[i % OT] = mfma32<bf16_t>(vp[i % L::AHEAD], p[i / OT / 2][i / OT % 2][x], o[i % OT]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -1256,7 +1437,7 @@ struct Read {
 };
 
 template <class O>
-struct alignas(16) Eight {
+struct alignas(16) Eight {  // (four, of f32)
     O v[16 / sizeof(O)];
 };
 
@@ -1264,13 +1445,19 @@ struct alignas(16) Eight {
 template <class C, class O, int D>
 __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, Read a) {
     constexpr int NR = kWriteRows;
+    constexpr int kHold = 1024;  // entries that are held, and searched, in LDS
     __shared__ Runs runs;
     __shared__ uint64_t bad_rows;
+    __shared__ int cu[kHold], ids[kHold], starts[kHold];
     const int tid = threadIdx.x, lane = tid & 63;
     const int KVH = (int)c.n_kv_heads, groups = (KVH + a.heads - 1) / a.heads;
-    const int row0 = (int)(blockIdx.x / groups) * NR, g0 = (int)(blockIdx.x % groups) * a.heads;
+    const int bx = by_xcd(blockIdx.x, gridDim.x), row0 = bx / groups * NR, g0 = bx % groups * a.heads;
     const int heads = min(a.heads, KVH - g0), end = min(a.n, a.cu[a.B]);
+    const bool in_lds = a.B <= kHold;
+    if (in_lds)
+        for (int i = tid; i < a.B; i += 256) cu[i] = a.cu[i], ids[i] = a.ids[i], starts[i] = a.starts[i];
     if (row0 >= end) return;
+    __syncthreads();
     int slot = -1;
     bool bad = false;
     const int row = row0 - 1 + tid;
@@ -1278,16 +1465,16 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, 
         int lo = 0, hi = a.B;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (a.cu[mid] <= row) lo = mid;
+            if ((in_lds ? cu[mid] : a.cu[mid]) <= row) lo = mid;
             else hi = mid;
         }
-        const int id = a.ids[lo];
-        const int64_t pos = (int64_t)a.starts[lo] + row - a.cu[lo];
+        const int id = in_lds ? ids[lo] : a.ids[lo];
+        const int64_t pos = (int64_t)(in_lds ? starts[lo] : a.starts[lo]) + row - (in_lds ? cu[lo] : a.cu[lo]);
         if (id >= 0) {
             bad = true;
-            if (id < t.max_seqs && pos >= 0 && pos < t.lens[id] && (pos >> c.page_shift) < t.max_pages) {
+            if (id < t.max_seqs && pos >= 0 && (pos >> c.page_shift) < t.max_pages) {
                 const int pg = t.table[(int64_t)id * t.max_pages + (pos >> c.page_shift)];
-                if ((unsigned)pg < (unsigned)c.n_pages) {
+                if (pos < t.lens[id] && (unsigned)pg < (unsigned)c.n_pages) {
                     slot = (pg << c.page_shift) + (int)(pos & (c.page_size - 1));
                     bad = false;
                 }
@@ -1323,23 +1510,23 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, 
         const float step = power((i % 2 ? c.v_exp : c.k_exp)[(head << c.page_shift >> 4) + in_page / kBlock]);
         out += (row0 + r0) * a.stride + (int64_t)g * D;
         if (i % 2 == 0) {
-            constexpr int CH = D / 16, RP = 64 / CH;  // lanes a row, rows at a time
-            const uint8_t* k = c.k + ((head << c.page_shift) + in_page) * D;
+            constexpr int E = 16 / sizeof(O);           // 16 bytes of the output a lane
+            constexpr int CH = D / E, RP = 64 / CH;     // lanes a row, rows at a time
+            const uint8_t* k = c.k + ((head << c.page_shift) + in_page) * D + lane % CH * E;
+            O* to = out + lane % CH * E;
+#pragma unroll 4
             for (int r = lane / CH; r < n; r += RP) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(k + r * D + lane % CH * 16);
-                O* to = out + r * a.stride + lane % CH * 16;
-                constexpr int E = 16 / sizeof(O);
+                uint32_t w[E / 4];
 #pragma unroll
-                for (int x = 0; x < 16 / E; ++x) {
-                    Eight<O> y;
+                for (int x = 0; x < E / 4; ++x) w[x] = reinterpret_cast<const uint32_t*>(k + r * D)[x];
+                Eight<O> y;
 #pragma unroll
-                    for (int e = 0; e < E; e += 4) {
-                        const f32x4 z = decode4<C>(w[(x * E + e) / 4]) * step;
+                for (int x = 0; x < E / 4; ++x) {
+                    const f32x4 z = decode4<C>(w[x]) * step;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) y.v[e + j] = (O)z[j];
-                    }
-                    *reinterpret_cast<Eight<O>*>(to + x * E) = y;
+                    for (int j = 0; j < 4; ++j) y.v[4 * x + j] = (O)z[j];
                 }
+                *reinterpret_cast<Eight<O>*>(to + r * a.stride) = y;
             }
         } else {
             // two dimensions a lane
@@ -1416,17 +1603,21 @@ int heads_each(int64_t blocks, int64_t heads) {
     return (int)std::min<int64_t>(heads, std::max<int64_t>(1, blocks * heads / (4 * device_info().cu_count)));
 }
 
-// The writes' part of a first kernel: its workgroups.
-int64_t plan_writes(const PagedKv8& c, int64_t n, Prepare& p) {
-    p.rows = n <= 512 ? 4 : kWriteRows;
+// The writes' part of a first kernel: rows and heads to a workgroup, so that few rows and heads still make
+// many workgroups (decoding requests begin a run a row, which a workgroup's waves take one after the other).
+void plan_writes(const PagedKv8& c, int64_t n, Prepare& p) {
+    p.rows = kWriteRows;
+    while (p.rows > 2 && n * c.n_kv_heads < 1024 * p.rows) p.rows /= 2;
     const int64_t blocks = (n + p.rows - 1) / p.rows;
     p.heads = heads_each(blocks, c.n_kv_heads);
-    return blocks * ((c.n_kv_heads + p.heads - 1) / p.heads);
+    // (a prompt's run is two tasks a head, for four waves)
+    if (p.rows == kWriteRows) p.heads = (int)std::min<int64_t>(c.n_kv_heads, std::max(p.heads, 2));
+    p.writes = (int)((blocks * ((c.n_kv_heads + p.heads - 1) / p.heads) + 7) / 8 * 8);
 }
 
 template <class C, int D>
 hipError_t launch_prepare(const PagedKv8& c, const unillm_page_table& t, const Call& a, const Prepare& p,
-                          int64_t writes, hipStream_t s) {
+                          hipStream_t s) {
     constexpr int kMost = (3 * kPagesMaxSeqs + 1) * (int)sizeof(int);
     static_assert(kMost >= (2 * kBlock - 1) * 128 * (int)sizeof(double2), "31 rows of 128 pairs");
     static const bool attr = hipFuncSetAttribute((const void*)kv8_prepare_kernel<C, D>,
@@ -1435,15 +1626,15 @@ hipError_t launch_prepare(const PagedKv8& c, const unillm_page_table& t, const C
     const size_t pairs = (size_t)c.rotary_dim / 2 * sizeof(double2);
     size_t lds = std::max((size_t)(p.rows + kBlock - 1) * pairs, (size_t)p.q_rows * pairs);
     if (p.plan) lds = std::max(lds, (size_t)(3 * t.st.max_seqs + 1) * sizeof(int));  // (three ints an entry)
-    const unsigned grid = (unsigned)(p.plan + p.q_groups + writes);
+    const unsigned grid = (unsigned)(p.plan + p.q_groups + p.writes);
     kv8_prepare_kernel<C, D><<<grid, 256, lds, s>>>(c, t.st, a, p);
     return hipGetLastError();
 }
 
 template <class C, int D>
 hipError_t launch_typed(const PagedKv8& c, const unillm_page_table& t, const Call& a, const Prepare& p,
-                        int64_t writes, const Layout& l, hipStream_t s) {
-    hipError_t e = launch_prepare<C, D>(c, t, a, p, writes, s);
+                        const Layout& l, hipStream_t s) {
+    hipError_t e = launch_prepare<C, D>(c, t, a, p, s);
     if (e != hipSuccess) return e;
     using N = Narrow8Lds<D>;
     using W = Wide8Lds<D>;
@@ -1482,10 +1673,10 @@ hipError_t launch_kv8_append(const PagedKv8& c, const unillm_page_table& t, cons
                              int64_t kvstride, int64_t n, hipStream_t s) {
     Call a{};
     a.n = (int)n;
-    Prepare p{nullptr, kv, kvstride, nullptr, 0, 0, 0, 1, 0, 0};
-    const int64_t writes = plan_writes(c, n, p);
+    Prepare p{nullptr, kv, kvstride, nullptr, 0, 0, 0, 1, 0, 0, 0};
+    plan_writes(c, n, p);
     return by_pool(c, [&](auto code, auto dim) {
-        return launch_prepare<decltype(code), decltype(dim)::value>(c, t, a, p, writes, s);
+        return launch_prepare<decltype(code), decltype(dim)::value>(c, t, a, p, s);
     });
 }
 
@@ -1508,14 +1699,14 @@ hipError_t launch_kv8_attention(const PagedKv8& c, const unillm_page_table& t, c
         a.kind[k] = {tile_rows(k, D), places(k, D), target_pieces(k), k == kNarrow ? 4 : 2, 5,
                      k == kNarrow ? 0 : (int)l.rows[0], reinterpret_cast<int*>(w + l.head_at[k]),
                      reinterpret_cast<Item*>(w + l.items_at[k]), reinterpret_cast<Split*>(w + l.splits_at[k])};
-    Prepare p{qkv, qkv + H * D, qstride, q, 2, 0, 0, 0, 0, 0};
+    Prepare p{qkv, qkv + H * D, qstride, q, 2, 0, 0, 0, 0, 1, 0};
     p.q_rows = n <= 512 ? 4 : 16;
     const int64_t blocks = (n + p.q_rows - 1) / p.q_rows;
     p.q_heads = heads_each(blocks, H);
     p.q_groups = (int)(blocks * ((H + p.q_heads - 1) / p.q_heads));
-    const int64_t writes = append ? plan_writes(c, n, p) : (p.heads = 1, p.rows = 0, 0);
+    if (append) plan_writes(c, n, p);
     return by_pool(c, [&](auto code, auto dim) {
-        return launch_typed<decltype(code), decltype(dim)::value>(c, t, a, p, writes, l, s);
+        return launch_typed<decltype(code), decltype(dim)::value>(c, t, a, p, l, s);
     });
 }
 
@@ -1528,7 +1719,7 @@ hipError_t launch_kv8_read(const PagedKv8& c, const unillm_page_table& t, const 
                            void* k_out, void* v_out, int64_t ostride, hipStream_t s) {
     const int64_t blocks = (n + kWriteRows - 1) / kWriteRows;
     Read a{ids, starts, cu, (int)n_seqs, (int)n, k_out, v_out, ostride, heads_each(blocks, c.n_kv_heads)};
-    const unsigned grid = (unsigned)(blocks * ((c.n_kv_heads + a.heads - 1) / a.heads));
+    const unsigned grid = (unsigned)((blocks * ((c.n_kv_heads + a.heads - 1) / a.heads) + 7) / 8 * 8);
     return by_pool(c, [&](auto code, auto dim) {
         using C = decltype(code);
         constexpr int D = decltype(dim)::value;

@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.hpp"
 #include "split.hpp"
@@ -22,15 +23,19 @@ struct rope_bf16 {
 __device__ __forceinline__ float rope_widen(float v) { return v; }
 __device__ __forceinline__ float rope_widen(rope_f16 v) { return (float)v; }
 __device__ __forceinline__ float rope_widen(rope_bf16 v) { return __uint_as_float((uint32_t)v.bits << 16); }
+// An f64 value to a row's type, the 16-bit ones through f32, which is off by 2^-24 at most.  (Opaque between: the
+// compiler would fold the two conversions into one from f64, some 30 instructions; 4096 rows of 32 heads
+// of 128 took 28 us.)
 template <class T>
-__device__ __forceinline__ T rope_narrow(double v);
-template <>
-__device__ __forceinline__ float rope_narrow<float>(double v) { return (float)v; }
-template <>
-__device__ __forceinline__ rope_f16 rope_narrow<rope_f16>(double v) { return (rope_f16)(float)v; }
-template <>
-__device__ __forceinline__ rope_bf16 rope_narrow<rope_bf16>(double v) {
-    return rope_bf16{(uint16_t)(pack_bf16((float)v, 0.0f) & 0xFFFF)};
+__device__ __forceinline__ T rope_narrow(double v) {
+    float f = (float)v;
+    if constexpr (sizeof(T) == 4) {
+        return f;
+    } else {
+        asm volatile("" : "+v"(f));
+        if constexpr (std::is_same_v<T, rope_f16>) return (rope_f16)f;
+        else return rope_bf16{(uint16_t)(pack_bf16(f, 0.0f) & 0xFFFF)};
+    }
 }
 
 // V neighbouring elements; W: that many are aligned together.
@@ -49,71 +54,87 @@ struct RopeCall {
     int n, heads, hd, rot, copy;
 };
 
-// A workgroup takes `rows` rows: their cosines and sines into LDS, then a thread takes the same V
-// elements (half-split: and their partners) of every so many heads.
-// Bound by HBM where rows are many, by latency for one.
+// A workgroup takes `rows` rows: a thread has a unit of a head, V elements (half-split: and their partners),
+// of every so many of their heads, four at a time, the first four requested before the rows' cosines and
+// sines are formed (in LDS).
+// Bound by HBM where rows are many, by latency for few.
 template <class T, int V, int W, bool HALF>
 __global__ __launch_bounds__(256) void rope_kernel(RopeCall a, int rows) {
-    extern __shared__ double2 turn[];  // [rows][rot / 2]
-    const int tid = threadIdx.x, pairs = a.rot / 2;
+    using S = Some<T, V, W>;
+    constexpr int B = 4, P = HALF ? V : V / 2;  // items at a time, pairs of a unit
+    // [rows][rot / 2], pair p at p % P rot / 2 P + p / P: what lanes read together lies together
+    extern __shared__ double2 turn[];
+    const int tid = threadIdx.x, pairs = a.rot / 2, sets = pairs / P;
     const int64_t row0 = (int64_t)blockIdx.x * rows;
     const int n = (int)min((int64_t)rows, a.n - row0);
-    for (int i = tid; i < n * pairs; i += 256) {
-        double sn, cs;
-        sincospi((double)a.positions[row0 + i / pairs] * a.freq[i % pairs], &sn, &cs);
-        turn[i] = make_double2(cs * a.magnitude, sn * a.magnitude);
-    }
-    __syncthreads();
     // units of a head: those that turn first, then those that are copied
     const int turning = (HALF ? pairs : a.rot) / V, units = turning + (a.copy ? (a.hd - a.rot) / V : 0);
     const int across = min(units, 256), side = tid / across, sides = 256 / across;
-    if (side >= sides) return;
-    using S = Some<T, V, W>;
-    for (int u = tid % across; u < units; u += across)
-        for (int r = 0; r < n; ++r) {
-            const T* x = static_cast<const T*>(a.x) + (row0 + r) * a.xstride;
-            T* out = static_cast<T*>(a.out) + (row0 + r) * a.ostride;
-            if (u >= turning) {
-                const int d = a.rot + (u - turning) * V;
-#pragma unroll 4
-                for (int h = side; h < a.heads; h += sides)
-                    *reinterpret_cast<S*>(out + h * a.hd + d) = *reinterpret_cast<const S*>(x + h * a.hd + d);
-            } else if (HALF) {
-                const int d = u * V;
-                double2 z[V];
+    const int dr = sides / a.heads, dh = sides % a.heads;
+    int u = side < sides ? tid % across : units;
+    // the thread's place among the rows and heads, of unit u
+    int r = 0, h = 0;
+    auto begin = [&] {
+        r = side / a.heads;
+        h = side % a.heads;
+    };
+    auto next = [&] {
+        r += dr;
+        h += dh;
+        if (h >= a.heads) h -= a.heads, ++r;
+    };
+    S lo[B], hi[B];
+    int rr[B], hh[B];
+    auto load = [&] {
+        const int d = u < turning ? u * V : a.rot + (u - turning) * V;
 #pragma unroll
-                for (int e = 0; e < V; ++e) z[e] = turn[r * pairs + d + e];
-#pragma unroll 4
-                for (int h = side; h < a.heads; h += sides) {
-                    S lo = *reinterpret_cast<const S*>(x + h * a.hd + d);
-                    S hi = *reinterpret_cast<const S*>(x + h * a.hd + d + pairs);
+        for (int i = 0; i < B; ++i) {
+            rr[i] = r;
+            hh[i] = h;
+            if (u < units && r < n) {
+                const T* x = static_cast<const T*>(a.x) + (row0 + r) * a.xstride + h * a.hd + d;
+                lo[i] = *reinterpret_cast<const S*>(x);
+                if (HALF && u < turning) hi[i] = *reinterpret_cast<const S*>(x + pairs);
+            }
+            next();
+        }
+    };
+    begin();
+    load();
+    for (int i = tid; i < n * pairs; i += 256) {
+        double sn, cs;
+        sincospi((double)a.positions[row0 + i / pairs] * a.freq[i % pairs], &sn, &cs);
+        turn[i / pairs * pairs + i % pairs % P * sets + i % pairs / P] = make_double2(cs * a.magnitude, sn * a.magnitude);
+    }
+    __syncthreads();
+    for (; u < units; u += across, begin(), load()) {
+        const int d = u < turning ? u * V : a.rot + (u - turning) * V;
+        for (; rr[0] < n; load())
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                if (rr[i] >= n) break;
+                T* out = static_cast<T*>(a.out) + (row0 + rr[i]) * a.ostride + hh[i] * a.hd + d;
+                if (u < turning && HALF) {
+                    const double2* z = turn + rr[i] * pairs + u;
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        const double p = rope_widen(lo.v[e]), q = rope_widen(hi.v[e]);
-                        lo.v[e] = rope_narrow<T>(p * z[e].x - q * z[e].y);
-                        hi.v[e] = rope_narrow<T>(p * z[e].y + q * z[e].x);
+                        const double p = rope_widen(lo[i].v[e]), q = rope_widen(hi[i].v[e]);
+                        lo[i].v[e] = rope_narrow<T>(p * z[e * sets].x - q * z[e * sets].y);
+                        hi[i].v[e] = rope_narrow<T>(p * z[e * sets].y + q * z[e * sets].x);
                     }
-                    *reinterpret_cast<S*>(out + h * a.hd + d) = lo;
-                    *reinterpret_cast<S*>(out + h * a.hd + d + pairs) = hi;
-                }
-            } else {
-                const int d = u * V;
-                double2 z[V / 2 > 0 ? V / 2 : 1];
-#pragma unroll
-                for (int e = 0; e < V / 2; ++e) z[e] = turn[r * pairs + d / 2 + e];
-#pragma unroll 4
-                for (int h = side; h < a.heads; h += sides) {
-                    S w = *reinterpret_cast<const S*>(x + h * a.hd + d);
+                    *reinterpret_cast<S*>(out + pairs) = hi[i];
+                } else if (u < turning) {
+                    const double2* z = turn + rr[i] * pairs + u;
 #pragma unroll
                     for (int e = 0; e < V / 2; ++e) {
-                        const double p = rope_widen(w.v[2 * e]), q = rope_widen(w.v[2 * e + 1]);
-                        w.v[2 * e] = rope_narrow<T>(p * z[e].x - q * z[e].y);
-                        w.v[2 * e + 1] = rope_narrow<T>(p * z[e].y + q * z[e].x);
+                        const double p = rope_widen(lo[i].v[2 * e]), q = rope_widen(lo[i].v[2 * e + 1]);
+                        lo[i].v[2 * e] = rope_narrow<T>(p * z[e * sets].x - q * z[e * sets].y);
+                        lo[i].v[2 * e + 1] = rope_narrow<T>(p * z[e * sets].y + q * z[e * sets].x);
                     }
-                    *reinterpret_cast<S*>(out + h * a.hd + d) = w;
                 }
+                *reinterpret_cast<S*>(out) = lo[i];
             }
-        }
+    }
 }
 
 template <class T, int V, int W, bool HALF>

@@ -11,7 +11,7 @@ import torch
 
 from . import _capi
 from .paged import PageTable, _check, _hold, _stream_ptr
-from .rope import Rope
+from .rope import Rope, _empty
 
 _KV8_TYPES = {torch.int8: _capi.KV8_INT8, torch.float8_e4m3fn: _capi.KV8_E4M3}
 _OUT_TYPES = {torch.float32: _capi.F32, torch.float16: _capi.F16, torch.bfloat16: _capi.BF16}
@@ -99,11 +99,8 @@ class PagedKvCache8:
         self._on(what, table)
         width = self._rows(what, "qkv", qkv, owidth + 2 * self.n_kv_heads * self.head_dim, owidth)
         n = qkv.shape[0]
-        if out is None:  # (memory that `stream` may write at once: its own)
-            with torch.cuda.stream(stream):
-                out = torch.empty(n, owidth, dtype=torch.float32, device=self._device)
-            if stream is not None:
-                out.record_stream(torch.cuda.current_stream(self._device))
+        if out is None:
+            out = _empty((n, owidth), torch.float32, self._device, stream)
         else:
             self._rows(what, "out", out, owidth)
             if out.shape[0] != n:
@@ -135,11 +132,7 @@ class PagedKvCache8:
         if n_rows < 0:
             raise RuntimeError(f"{what}: n_rows {n_rows}")
         shape = (n_rows, self.n_kv_heads, self.head_dim)
-        with torch.cuda.stream(stream):  # (memory that `stream` may write at once: its own)
-            k, v = (torch.empty(shape, dtype=dtype, device=self._device) for _ in range(2))
-        if stream is not None:
-            for t in (k, v):
-                t.record_stream(torch.cuda.current_stream(self._device))
+        k, v = _empty(shape, dtype, self._device, stream), _empty(shape, dtype, self._device, stream)
         _hold(stream, seq_ids, starts, cu_rows, self.k, self.v, self.k_exp, self.v_exp, table._mem)
         _check(_capi.lib().unillm_hip_paged_kv8_read(
             self._h, table._h, seq_ids.data_ptr(), starts.data_ptr(), cu_rows.data_ptr(), seq_ids.numel(), n_rows,

@@ -18,6 +18,17 @@ _TYPES = {torch.float32: _capi.F32, torch.float16: _capi.F16, torch.bfloat16: _c
 _SCALINGS = {None: 0, "linear": 1, "llama3": 2, "yarn": 3}
 
 
+def _empty(shape: tuple, dtype: torch.dtype, device: torch.device, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """An output's memory, that `stream` may write at once: its own.  (The current stream's without a
+    context around it, which takes 2 us.)"""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        out = torch.empty(shape, dtype=dtype, device=device)
+    out.record_stream(torch.cuda.current_stream(device))
+    return out
+
+
 class Rope:
     """Frequencies f_i = theta^(-2 i / rotary_dim) / freq_factors[i] of the pairs of a head's first
     rotary_dim dimensions: i and i + rotary_dim / 2, or interleaved 2 i and 2 i + 1.
@@ -68,11 +79,8 @@ class Rope:
         if (positions.dtype != torch.int32 or positions.device != self._device or positions.dim() != 1
                 or positions.numel() != n or not positions.is_contiguous()):
             raise RuntimeError(f"Rope.apply: positions must be {n} contiguous int32 on {self._device}")
-        if out is None:  # (memory that `stream` may write at once: its own)
-            with torch.cuda.stream(stream):
-                out = torch.empty(n, heads, self.head_dim, dtype=x.dtype, device=self._device)
-            if stream is not None:
-                out.record_stream(torch.cuda.current_stream(self._device))
+        if out is None:
+            out = _empty((n, heads, self.head_dim), x.dtype, self._device, stream)
         elif out.dtype != x.dtype or out.shape != x.shape or not rows(out):
             raise RuntimeError("Rope.apply: out must be as x, with contiguous heads")
         if x.numel() == 0:
