@@ -11,6 +11,12 @@ To it comes f32's range: a weight is e^(s - top) against the largest, 1, and bel
 number, 2^-126, it (or one of its parts) may be 0 in any f32 evaluation, so that an output whose large
 weights' values are all 0 may lose 2^-126 of the largest value for each key (scores 87 and more below the
 largest; the first run of the exponents' test found a true output of 1e-83 there).
+
+And, for entries of more than 64 query rows a kv head, the loss that the header states: their weights
+(times a power of two) are held in two f16 parts, against 2^11 for the row's largest, so each is off by
+2^-25 at most beyond 2^-22 of itself, and a sum over K keys of codes up to C by K C 2^-25.  A row whose
+largest sum is below min(K, 2048) C 2^-9 is done again in f32; the others' loss is thus at most 2^-16 max(1,
+K / 2048) of a piece's largest sum, which is at most the row's largest sum of |weight x value|.
 """
 import numpy as np
 import pytest
@@ -55,6 +61,9 @@ def expect(cache, table, q, H, entries, freq=None, interleaved=False, window=0, 
             x = rotate(x, pos, freq, interleaved)
         k, v = values(cache, rows[i], lens[i])
         o, b = attend(x, k, v, pos, window, sinks)
+        if n * (H // cache.n_kv_heads) > 64:
+            sums = attend(x, k, np.abs(v), pos, window, sinks)[0].max(-1, keepdims=True)
+            b = b + 2.0 ** -16 * max(1, len(v) / 2048) * sums
         outs.append(o)
         bounds.append(b + len(v) * 2.0 ** -126 * np.abs(v).max())
         at += n

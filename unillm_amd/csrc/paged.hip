@@ -211,26 +211,11 @@ __device__ __forceinline__ void split_q(const f32x8& v, u32x4 (&p)[Parts<T>::Q])
     }
 }
 
-// 8 weights -> their parts.  f16: the first part cut off, what is left of up to 2^-10 rounded:
-// 2^-22 of the weight, in either direction (one conversion a pair, one mixed-precision
-// multiply-add a weight that takes the f16 back out, one conversion a pair).
+// 8 weights -> their parts
 template <class T>
 __device__ __forceinline__ void split_w(const f32x8& v, u32x4 (&p)[Parts<T>::Q]) {
-    if constexpr (std::is_same_v<T, f16_t>) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v[2 * j], v[2 * j + 1]));
-            f32x2 lo;  // v - hi, exactly
-            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]"
-                : "=v"(lo[0]) : "v"(hi), "v"(v[2 * j]));
-            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-                : "=v"(lo[1]) : "v"(hi), "v"(v[2 * j + 1]));
-            p[0][j] = hi;
-            p[1][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(lo, f16x2));
-        }
-    } else {
-        split_q<T>(v, p);
-    }
+    if constexpr (std::is_same_v<T, f16_t>) halve_weights(v, p);
+    else split_q<T>(v, p);
 }
 
 // 8 elements of the pool as loaded, and as an operand's parts

@@ -408,6 +408,23 @@ __device__ void plan(const PageTable& t, const Call& a, int kind, int* sm) {
     }
 }
 
+// 8 weights -> two f16 parts: the first cut off, what is left of up to 2^-10 rounded: 2^-22 of the weight, in
+// either direction, and 2^-25 where that is more (one conversion a pair, one mixed-precision multiply-add a
+// weight that takes the f16 back out, one conversion a pair).
+__device__ __forceinline__ void halve_weights(const f32x8& v, u32x4 (&p)[2]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v[2 * j], v[2 * j + 1]));
+        f32x2 lo;  // v - hi, exactly
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]"
+            : "=v"(lo[0]) : "v"(hi), "v"(v[2 * j]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+            : "=v"(lo[1]) : "v"(hi), "v"(v[2 * j + 1]));
+        p[0][j] = hi;
+        p[1][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(lo, f16x2));
+    }
+}
+
 template <class T>
 __device__ __forceinline__ f32x4 mfma16(u32x4 x, u32x4 y, f32x4 z) {
     if constexpr (std::is_same_v<T, f16_t>)

@@ -551,26 +551,6 @@ __device__ __forceinline__ u32x4 codes_bf16(uint32_t lo, uint32_t hi) {
     return r;
 }
 
-// the same times a power of two
-template <class C>
-__device__ __forceinline__ u32x4 values_bf16(uint32_t lo, uint32_t hi, float step) {
-    u32x4 r;
-    if constexpr (std::is_same_v<C, Int8>) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t w = i < 2 ? lo : hi;
-            const float a = i % 2 ? decode<C, 2>(w) : decode<C, 0>(w), b = i % 2 ? decode<C, 3>(w) : decode<C, 1>(w);
-            r[i] = __builtin_amdgcn_perm(__float_as_uint(b * step), __float_as_uint(a * step), 0x07060302u);
-        }
-    } else {
-        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, step, false));
-        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, step, true));
-        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, step, false));
-        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, step, true));
-    }
-    return r;
-}
-
 // 8 f32 -> two f16 parts (22 bits), or three bf16 ones (all)
 __device__ __forceinline__ void parts_f16(const f32x8& v, u32x4 (&p)[2]) {
     const f16x8 hi = __builtin_convertvector(v, f16x8);
@@ -876,9 +856,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
 //
 // The wide kernel of paged.hip on codes: an item of a tile of up to 256 query rows of a kv head (128 at
 // hd 256), 32 to each wave (32x32x16 MFMAs), U keys at a time through LDS; two groups of four waves a phase
-// apart, so that one's products run beside the other's softmax.  Codes are widened on their way into the
-// LDS, K's to f16 as they are, V's to bf16 times their block's power of two; K's powers of two go beside
-// them, for the scores.
+// apart, so that one's products run beside the other's softmax.  Codes are widened to f16 on their way into the
+// LDS; their blocks' powers of two go beside them, K's for the scores, V's for the weights.
+// A weight times its block's power of two is held in two f16 parts (four products a visit in all, where three
+// bf16 parts make five: a prompt of 3001 tokens, 32 heads on 8 of 128, 200 us with those), taken against
+// the row's largest weight times power of two so far, as 2^11: parts down to 2^-24 reach 2^-35 of it.  (A
+// whole power of two apart from the weights' own reference, so that sums and weights are scaled alike, to the
+// bit.)  What that may lose is looked at in the end.
+constexpr int kWideShift = 11;
+constexpr float kWideSlack = 4.0f;
+// What a row may lose by the weights' parts, of its largest sum: 2^-16 over up to 2048 keys, 2^-27 a key over
+// more (an f32 sum of as many terms may be off by 2^-24 a term).  A row loses so much where keys whose values
+// are almost nothing in their blocks have all but 1/512 of the weight (an attention sink of value 0).
+constexpr float kWideLoss = 0x1p-16f;
+constexpr int kWideLossKeys = 2048;
+
 template <int D>
 struct Wide8Lds {
     static constexpr int GR = D < 256 ? 2 : 1, NT = 256 * GR;
@@ -892,7 +884,7 @@ struct Wide8Lds {
     static constexpr int QROWS = 32 * D * 4;                // a wave's rows in f32, before and after
     static constexpr int USED = QL + (kQl ? NT / 64 * (D / 16) * 1024 : 0), ROWS = NT / 64 * QROWS;
     static constexpr int STAT = USED > ROWS ? USED : ROWS;  // whether a page is bad, K's powers of two
-    static constexpr int BYTES = STAT + 64 + 64;
+    static constexpr int BYTES = STAT + 64 + 128;
     static constexpr int TASKS = U * D / 8 / NT;            // 8-code chunks of K (or V) a thread
     // Operands held: read so many products less one ahead.  (One wave a SIMD at hd 256: nothing else
     // runs while it waits.)
@@ -920,7 +912,9 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
     constexpr bool kStoreEarly = GR == 2 && D == 64;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
-    float* steps = reinterpret_cast<float*>(lds + L::STAT + 64);  // [4][4] K's powers of two, by visit and block
+    // [4][4], by visit and block: K's powers of two, V's exponents
+    float* steps = reinterpret_cast<float*>(lds + L::STAT + 64);
+    int* vexps = reinterpret_cast<int*>(steps + 16);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = wv / 4;
@@ -958,7 +952,7 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
         // of its request, that a pair ahead of its store.  Past the item's ends the nearest visit is
         // staged again, unused: with no branch around a load the waits count only what they need.
         u32x2 sk[L::TASKS], sv[L::TASKS];
-        int ke[L::TASKS], ve;  // their blocks' exponents
+        int ke[L::TASKS], ve[L::TASKS];  // K's chunks' blocks' exponents, and those of V there
         int pk[L::TASKS], pv;
         bool bad_id = false;
         auto key_of = [&](int n) { return vis.key(it.v0 + max(0, min(n, it.nv - 1))); };
@@ -986,7 +980,9 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
             const uint64_t page = sound(pk[i]);
             sk[i] = *reinterpret_cast<const u32x2*>(kbase + (page * page_elems + (at << LOG_D)) +
                                                     (klane + (KSTEP == 8 ? i % 2 * 8 * D : 0)));
-            ke[i] = c.k_exp[((page * KVH + g) << (shift - 4)) + at / kBlock];
+            const uint64_t block = ((page * KVH + g) << (shift - 4)) + at / kBlock;
+            ke[i] = c.k_exp[block];
+            ve[i] = c.v_exp[block];
         };
         auto fetch_v = [&] {
             const uint32_t at = (uint32_t)group_key(k0, vgroup) & (uint32_t)(ps - 1);
@@ -994,7 +990,6 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
             const uint8_t* from = vbase + (page * page_elems + at);
 #pragma unroll
             for (int i = 0; i < L::TASKS; ++i) sv[i] = *reinterpret_cast<const u32x2*>(from + (32 * i << shift) + vlane);
-            ve = c.v_exp[((page * KVH + g) << (shift - 4)) + at / kBlock];
         };
         auto fetch_pages = [&](int m) {  // of pair m + 1, after pair m's requests
             read_pages(k2, k1);
@@ -1023,7 +1018,10 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                 // (a chunk step of 8 rows turns bit 3 of the slot)
                 const uint32_t at = (KSTEP == 8 && i % 2 ? kto ^ 128 : kto) + i * KSTEP * L::KROW;
                 *reinterpret_cast<u32x4*>(buf + L::K + at) = codes_f16<C>(sk[i][0], sk[i][1]);
-                if (lane == 0) steps[m % 4 * 4 + kgroup(i)] = power(ke[i]);
+                if (lane == 0) {
+                    steps[m % 4 * 4 + kgroup(i)] = power(ke[i]);
+                    vexps[m % 4 * 4 + kgroup(i)] = min(max(ve[i], 1), 254) - 127;
+                }
             }
             const int left = len - kstored;  // keys of V's visit and on
             if (left < U) {                  // past the sequence's end a page holds anything
@@ -1036,10 +1034,9 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                     for (int i = 0; i < L::TASKS; ++i) sv[i][w] &= keep;
                 }
             }
-            const float step = power(ve);
 #pragma unroll
             for (int i = 0; i < L::TASKS; ++i)
-                *reinterpret_cast<u32x4*>(buf + L::V + vto + 32 * i * L::VROW) = values_bf16<C>(sv[i][0], sv[i][1], step);
+                *reinterpret_cast<u32x4*>(buf + L::V + vto + 32 * i * L::VROW) = codes_f16<C>(sv[i][0], sv[i][1]);
         };
         read_pages(k1, k0);
         fetch(0);
@@ -1112,7 +1109,10 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                 if (L::kQl) ql[b * 64] = p[1];
             }
         }
-        float ref = -INFINITY, l = 0.0f;
+        // the weights' reference; the row's largest weight times power of two, against which (as a whole power of
+        // two: `rise` above the weights') the products' weights are taken
+        float ref = -INFINITY, peak = -INFINITY, l = 0.0f;
+        int rise = 0;
         f32x16 o[OT];
 #pragma unroll
         for (int i = 0; i < OT; ++i)
@@ -1170,13 +1170,17 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
         __syncthreads();  // the first matrix phase ends
         for (int n = 0;; ++n) {
             const int j0 = vis.key(it.v0 + n);
-            u32x4 p[NG][2][3];
+            u32x4 p[NG][2][2];
             {
-                float top = -INFINITY, times[NG][2];
+                float top = -INFINITY, high = -INFINITY, times[NG][2];
+                int ve[NG][2];
 #pragma unroll
                 for (int u = 0; u < NG; ++u)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) times[u][x] = inv * steps[n % 4 * 4 + 2 * u + x];
+                    for (int x = 0; x < 2; ++x) {
+                        times[u][x] = inv * steps[n % 4 * 4 + 2 * u + x];
+                        ve[u][x] = vexps[n % 4 * 4 + 2 * u + x];
+                    }
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
                     const int ju = j0 + 32 * u;
@@ -1197,30 +1201,40 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                         float most = s[u][8 * x];
 #pragma unroll
                         for (int e = 1; e < 8; ++e) most = fmaxf(most, s[u][8 * x + e]);
-                        top = fmaxf(top, most * times[u][x]);  // (a power of two)
+                        most *= times[u][x];  // (a power of two)
+                        top = fmaxf(top, most);
+                        high = fmaxf(high, most + (float)ve[u][x]);
                     }
                 }
-                if (__any(top > ref + kSlack)) {
+                if (__any((top > ref + kWideSlack) | (high > ref + (float)rise + kWideSlack))) {
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    high = fmaxf(high, __shfl_xor(high, 32, 64));
                     const float to = fmaxf(ref, top);
-                    const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+                    peak = fmaxf(peak, high);
+                    const int up = to == -INFINITY ? 0 : (int)ceilf(fminf(fmaxf(peak - to, -1000.0f), 1000.0f));
+                    const float f = ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+                    const float fo = __builtin_amdgcn_ldexpf(f, rise - up);
                     l *= f;
 #pragma unroll
-                    for (int i = 0; i < OT; ++i) o[i] *= f;
+                    for (int i = 0; i < OT; ++i) o[i] *= fo;
                     ref = to;
+                    rise = up;
                 }
                 const float from = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll
                 for (int u = 0; u < NG; ++u)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
+                        // (a weight of 0 stays one: of a block that no row sees the exponent may be any)
+                        const float step = __builtin_amdgcn_ldexpf(1.0f, min(ve[u][k] - rise + kWideShift, 126));
                         f32x8 w;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             w[e] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * k + e], times[u][k], -from));
                             l += w[e];
+                            w[e] *= step;
                         }
-                        parts_bf16(w, p[u][k]);
+                        halve_weights(w, p[u][k]);
                     }
             }
             if (!kStoreEarly) store(n + 1 + grp);
@@ -1247,8 +1261,8 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                     if (!kStoreEarly && i % (NG * OT / 2) == 0) fetch_piece(n + 2 + grp, i / (NG * OT / 2));
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int x = 2; x >= 0; --x)
-                        o[i % OT] = mfma32<bf16_t>(vp[i % L::AHEAD], p[i / OT / 2][i / OT % 2][x], o[i % OT]);
+                    for (int x = 1; x >= 0; --x)
+                        o[i % OT] = mfma32<f16_t>(vp[i % L::AHEAD], p[i / OT / 2][i / OT % 2][x], o[i % OT]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -1272,7 +1286,22 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
         const bool mine = w0 + col < it.rows;
         l += __shfl_xor(l, 32, 64);
         const float inv_l = 1.0f / l;
-        float chk = l * 0.0f;
+        float chk = l * 0.0f, most = 0.0f;
+        // Weights in two parts are off by up to 2^-25, and a row's sums by that times the item's keys and the
+        // largest code: a row whose largest sum may have lost too much is done again (but where all values are
+        // 0, or next to it: their blocks' exponents are the least).
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(o[i][e]));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        if (l > 0.0f && rise > -100 &&
+            most * kWideLoss < C::top * ((float)min(it.nv * U, kWideLossKeys) * 0x1p-25f)) chk = 1.0f;
+        // the sums against the weights' reference
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] = __builtin_amdgcn_ldexpf(o[i][e], rise - kWideShift);
 #pragma unroll
         for (int i = 0; i < OT; ++i)
 #pragma unroll

@@ -54,14 +54,15 @@ class PagedKvCache8:
             *[p.data_ptr() for p in parts], ctypes.byref(h)))
         self._h = h
         self.k, self.v, self.k_exp, self.v_exp = parts
+        self._lib = _capi.lib()
         self.dtype, self._device = dtype, parts[0].device
         self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
         self.n_pages, self.page_size = n_pages, page_size
 
     def _rows(self, what: str, name: str, t: torch.Tensor, *widths: int) -> int:
         """The width of t, f32 rows of one of these on the cache's device."""
-        if (t.dtype != torch.float32 or t.device != self._device or t.dim() != 2 or t.shape[1] not in widths
-                or not (t.stride(1) == 1 or t.numel() == 0)):
+        if (t.dtype != torch.float32 or t.get_device() != self._device.index or t.dim() != 2
+                or t.shape[1] not in widths or not (t.stride(1) == 1 or t.numel() == 0)):
             raise RuntimeError(f"{what}: {name} must be an f32 [n, {' or '.join(map(str, widths))}] tensor on "
                                f"{self._device} with contiguous rows")
         return t.shape[1]
@@ -69,6 +70,10 @@ class PagedKvCache8:
     def _on(self, what: str, table: PageTable) -> None:
         if table._device != self._device:
             raise RuntimeError(f"{what}: the table is on another device")
+
+    def _held(self, stream: torch.cuda.Stream | None, table: PageTable, *tensors: torch.Tensor) -> None:
+        if stream is not None:
+            _hold(stream, *tensors, self.k, self.v, self.k_exp, self.v_exp, table._mem)
 
     def reserve(self, table: PageTable, n_tokens: int, n_heads: int,
                 stream: torch.cuda.Stream | None = None) -> None:
@@ -83,10 +88,10 @@ class PagedKvCache8:
         self._on("8-bit paged append", table)
         width = self._rows("8-bit paged append", "kv", kv, 2 * self.n_kv_heads * self.head_dim)
         n = kv.shape[0]
-        _hold(stream, kv, self.k, self.v, self.k_exp, self.v_exp, table._mem)
-        _check(_capi.lib().unillm_hip_paged_kv8_append(self._h, table._h, kv.data_ptr(),
-                                                       width if n <= 1 else kv.stride(0), n,
-                                                       _stream_ptr(stream, self._device)))
+        self._held(stream, table, kv)
+        _check(self._lib.unillm_hip_paged_kv8_append(self._h, table._h, kv.data_ptr(),
+                                                     width if n <= 1 else kv.stride(0), n,
+                                                     _stream_ptr(stream, self._device)))
 
     def attention(self, table: PageTable, qkv: torch.Tensor, n_heads: int, window: int = 0,
                   sinks: int = 0, out: torch.Tensor | None = None,
@@ -105,9 +110,9 @@ class PagedKvCache8:
             self._rows(what, "out", out, owidth)
             if out.shape[0] != n:
                 raise RuntimeError(f"{what}: out must have {n} rows")
-        _hold(stream, qkv, out, self.k, self.v, self.k_exp, self.v_exp, table._mem)
+        self._held(stream, table, qkv, out)
         one = n <= 1  # (a single row's stride means nothing)
-        _check(_capi.lib().unillm_hip_paged_kv8_attention(
+        _check(self._lib.unillm_hip_paged_kv8_attention(
             self._h, table._h, qkv.data_ptr(), width if one else qkv.stride(0), n, n_heads, int(width != owidth),
             window, sinks, out.data_ptr(), owidth if one else out.stride(0), _stream_ptr(stream, self._device)))
         return out
@@ -124,18 +129,18 @@ class PagedKvCache8:
         self._on(what, table)
         if dtype not in _OUT_TYPES:
             raise RuntimeError(f"{what}: dtype {dtype} (want float32, float16 or bfloat16)")
-        for name, t, more in (("seq_ids", seq_ids, 0), ("starts", starts, 0), ("cu_rows", cu_rows, 1)):
-            if (t.dtype != torch.int32 or t.device != self._device or t.dim() != 1 or not t.is_contiguous()
-                    or t.numel() != seq_ids.numel() + more):
-                raise RuntimeError(f"{what}: {name} must be {seq_ids.numel() + more} contiguous int32 on "
-                                   f"{self._device}")
+        B = seq_ids.numel()
+        for name, t, size in (("seq_ids", seq_ids, B), ("starts", starts, B), ("cu_rows", cu_rows, B + 1)):
+            if (t.dtype != torch.int32 or t.get_device() != self._device.index or t.shape != (size,)
+                    or not t.is_contiguous()):
+                raise RuntimeError(f"{what}: {name} must be {size} contiguous int32 on {self._device}")
         if n_rows < 0:
             raise RuntimeError(f"{what}: n_rows {n_rows}")
         shape = (n_rows, self.n_kv_heads, self.head_dim)
         k, v = _empty(shape, dtype, self._device, stream), _empty(shape, dtype, self._device, stream)
-        _hold(stream, seq_ids, starts, cu_rows, self.k, self.v, self.k_exp, self.v_exp, table._mem)
-        _check(_capi.lib().unillm_hip_paged_kv8_read(
-            self._h, table._h, seq_ids.data_ptr(), starts.data_ptr(), cu_rows.data_ptr(), seq_ids.numel(), n_rows,
+        self._held(stream, table, seq_ids, starts, cu_rows)
+        _check(self._lib.unillm_hip_paged_kv8_read(
+            self._h, table._h, seq_ids.data_ptr(), starts.data_ptr(), cu_rows.data_ptr(), B, n_rows,
             _OUT_TYPES[dtype], k.data_ptr(), v.data_ptr(), self.n_kv_heads * self.head_dim,
             _stream_ptr(stream, self._device)))
         return k, v

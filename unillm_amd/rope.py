@@ -58,6 +58,7 @@ class Rope:
                                                   _SCALINGS[scaling], float(factor), float(low), float(high),
                                                   original, factors, float(magnitude or 0.0), ctypes.byref(h)))
         self._h = h
+        self._apply = _capi.lib().unillm_hip_rope_apply
         self._device = torch.device("cuda", torch.cuda.current_device())  # (the library's, made current)
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, interleaved
 
@@ -67,32 +68,38 @@ class Rope:
         projections is fine), turned at int32 positions [n] -> out, a new tensor, one given, or x
         itself (in place).  A negative position turns back, if the magnitude is 1."""
 
-        def rows(t):
-            return (t.dim() == 3 and t.device == self._device and t.shape[2] == self.head_dim
-                    and (t.numel() == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == self.head_dim)
-                                            and (t.shape[0] == 1 or t.stride(0) >= t.shape[1] * self.head_dim))))
-
-        if x.dtype not in _TYPES or not rows(x):
+        kind = _TYPES.get(x.dtype)
+        if kind is None or not self._rows(x):
             raise RuntimeError(f"Rope.apply: x must be an f32, f16 or bf16 [n, heads, {self.head_dim}] tensor on "
                                f"{self._device} with contiguous heads")
-        n, heads = x.shape[0], x.shape[1]
-        if (positions.dtype != torch.int32 or positions.device != self._device or positions.dim() != 1
-                or positions.numel() != n or not positions.is_contiguous()):
+        n, heads, _ = x.shape
+        if (positions.dtype != torch.int32 or positions.get_device() != self._device.index
+                or positions.shape != (n,) or not positions.is_contiguous()):
             raise RuntimeError(f"Rope.apply: positions must be {n} contiguous int32 on {self._device}")
         if out is None:
             out = _empty((n, heads, self.head_dim), x.dtype, self._device, stream)
-        elif out.dtype != x.dtype or out.shape != x.shape or not rows(out):
+        elif out.dtype != x.dtype or out.shape != x.shape or not self._rows(out):
             raise RuntimeError("Rope.apply: out must be as x, with contiguous heads")
-        if x.numel() == 0:
+        if n == 0 or heads == 0:
             return out
-        _hold(stream, x, positions, out)
+        if stream is not None:
+            _hold(stream, x, positions, out)
         width = heads * self.head_dim
-        one = n <= 1  # (a single row's stride means nothing)
-        _check(_capi.lib().unillm_hip_rope_apply(
-            self._h, _TYPES[x.dtype], x.data_ptr(), width if one else x.stride(0), n, heads,
-            positions.data_ptr(), out.data_ptr(), width if one else out.stride(0),
-            _stream_ptr(stream, self._device)))
+        one = n == 1  # (a single row's stride means nothing)
+        status = self._apply(self._h, kind, x.data_ptr(), width if one else x.stride(0), n, heads,
+                             positions.data_ptr(), out.data_ptr(), width if one else out.stride(0),
+                             _stream_ptr(stream, self._device))
+        if status:
+            _check(status)
         return out
+
+    def _rows(self, t: torch.Tensor) -> bool:
+        """Whether t is rows of contiguous heads, apart by what they take at least."""
+        if t.dim() != 3 or t.get_device() != self._device.index:
+            return False
+        (n, heads, hd), (a, b, c) = t.shape, t.stride()
+        return hd == self.head_dim and (n == 0 or heads == 0 or (
+            c == 1 and (heads == 1 or b == hd) and (n == 1 or a >= heads * hd)))
 
     def close(self) -> None:
         if self._h is not None and self._h.value:
