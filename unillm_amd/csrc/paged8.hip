@@ -886,9 +886,6 @@ struct Wide8Lds {
     static constexpr int STAT = USED > ROWS ? USED : ROWS;  // whether a page is bad, K's powers of two
     static constexpr int BYTES = STAT + 64 + 128;
     static constexpr int TASKS = U * D / 8 / NT;            // 8-code chunks of K (or V) a thread
-    // Operands held: read so many products less one ahead.  (One wave a SIMD at hd 256: nothing else
-    // runs while it waits.)
-    static constexpr int AHEAD = D == 256 ? 4 : 2;
     __device__ static uint32_t kslot(uint32_t r, uint32_t c) {
         return D >= 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
     }
@@ -1142,25 +1139,24 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
             for (int u = 0; u < NG; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[u][e] = zero;
-            u32x4 kp[L::AHEAD][NG], qx[L::AHEAD];
+            u32x4 kp[2][NG], qx[2];
             auto read = [&](int b) {
 #pragma unroll
                 for (int u = 0; u < NG; ++u)
-                    kp[b % L::AHEAD][u] = *reinterpret_cast<const u32x4*>(buf + L::K + 32 * u * L::KROW + (ka ^ 32 * b));
-                if (L::kQl) qx[b % L::AHEAD] = ql[b * 64];
+                    kp[b % 2][u] = *reinterpret_cast<const u32x4*>(buf + L::K + 32 * u * L::KROW + (ka ^ 32 * b));
+                if (L::kQl) qx[b % 2] = ql[b * 64];
             };
-#pragma unroll
-            for (int b = 0; b < L::AHEAD - 1; ++b) read(b);
+            read(0);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                if (b + L::AHEAD - 1 < NB) read(b + L::AHEAD - 1);
+                if (b + 1 < NB) read(b + 1);
                 if (kStoreEarly && b % (NB / 4) == 0) fetch_piece(n + 2, b / (NB / 4));
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int x = 1; x >= 0; --x)
 #pragma unroll
                     for (int u = 0; u < NG; ++u)
-                        s[u] = mfma32<f16_t>(kp[b % L::AHEAD][u], x < L::QREGS ? q[x < L::QREGS ? x : 0][b] : qx[b % L::AHEAD],
+                        s[u] = mfma32<f16_t>(kp[b % 2][u], x < L::QREGS ? q[x < L::QREGS ? x : 0][b] : qx[b % 2],
                                              s[u]);
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -1247,22 +1243,21 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                 const uint8_t* buf = lds + (n + 1) % GR * L::PAIR;
                 uint32_t va = vat;
                 asm volatile("" : "+v"(va));
-                u32x4 vp[L::AHEAD];
+                u32x4 vp[2];
                 auto read = [&](int i) {
-                    vp[i % L::AHEAD] =
+                    vp[i % 2] =
                         *reinterpret_cast<const u32x4*>(buf + L::V + 32 * (i % OT) * L::VROW + (va ^ 32 * (i / OT)));
                 };
-#pragma unroll
-                for (int i = 0; i < L::AHEAD - 1; ++i) read(i);
+                read(0);
 #pragma unroll
                 for (int i = 0; i < 2 * NG * OT; ++i) {
-                    if (i + L::AHEAD - 1 < 2 * NG * OT) read(i + L::AHEAD - 1);
+                    if (i + 1 < 2 * NG * OT) read(i + 1);
                     // (what is stored next is requested between the first MFMAs after the stores before)
                     if (!kStoreEarly && i % (NG * OT / 2) == 0) fetch_piece(n + 2 + grp, i / (NG * OT / 2));
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int x = 1; x >= 0; --x)
-                        o[i % OT] = mfma32<f16_t>(vp[i % L::AHEAD], p[i / OT / 2][i / OT % 2][x], o[i % OT]);
+                        o[i % OT] = mfma32<f16_t>(vp[i % 2], p[i / OT / 2][i / OT % 2][x], o[i % OT]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
