@@ -81,15 +81,18 @@ __device__ __forceinline__ uint32_t again4(uint32_t w, float f) {
 // values, whole, so no two waves meet in a block, and an exponent's byte is its own.
 constexpr int kWriteRows = 16;  // rows of a workgroup whose runs it takes, at most
 
+template <int ROWS>
 struct Runs {
-    int slots[2 * kWriteRows];  // of row row0 - 1 + i, -1: none
-    int first[kWriteRows], count[kWriteRows];  // those of several rows first
+    int slots[ROWS + 16];  // of row row0 - 1 + i, -1: none
+    int first[ROWS], count[ROWS];  // those of several rows first
     int n, many, end;  // runs, those of several rows; rows from row0 on that they take in
 };
 
-// The runs that begin in rows row0 .. row0 + nr - 1 (slot: of row row0 - 1 + threadIdx.x, up to nr + 16 of
-// them).  All threads of the workgroup.
-__device__ __forceinline__ void find_runs(Runs& r, int slot, int nr) {
+// The runs that begin in rows row0 .. row0 + nr - 1, 64 at most (slot: of row row0 - 1 + threadIdx.x, up to nr +
+// 16 of them).  All threads of the workgroup.
+template <int ROWS>
+__device__ __forceinline__ void find_runs(Runs<ROWS>& r, int slot, int nr) {
+    static_assert(ROWS <= 64, "a wave looks at all");
     const int tid = threadIdx.x;
     if (tid < nr + 16) r.slots[tid] = slot;
     if (tid == 0) r.end = 0;
@@ -304,7 +307,7 @@ __device__ __forceinline__ void write_values(const PagedKv8& c, const float* x, 
 
 // Several runs of one row each (decoding requests'): their keys, each by the lanes of one row.
 template <class C, int D>
-__device__ __forceinline__ void write_one_keys(const PagedKv8& c, const float* kv, int64_t stride, const Runs& runs,
+__device__ __forceinline__ void write_one_keys(const PagedKv8& c, const float* kv, int64_t stride, const Runs<kWriteRows>& runs,
                                                int from, int n, int g, const double2* turn, bool& odd) {
     constexpr int CH = D / 8;  // lanes a row
     const int lane = threadIdx.x & 63, u = lane % CH;
@@ -343,7 +346,7 @@ __device__ __forceinline__ void write_one_keys(const PagedKv8& c, const float* k
 
 // The values of up to B of them.
 template <class C, int D, int B>
-__device__ __forceinline__ void write_one_values(const PagedKv8& c, const float* kv, int64_t stride, const Runs& runs,
+__device__ __forceinline__ void write_one_values(const PagedKv8& c, const float* kv, int64_t stride, const Runs<kWriteRows>& runs,
                                                  int from, int n, int g, bool& odd) {
     constexpr int N = D / 64;  // neighbouring dimensions a lane
     struct alignas(4 * N) Dims {
@@ -458,7 +461,7 @@ __global__ __launch_bounds__(256, D == 256 ? 3 : 4) void kv8_prepare_kernel(Page
         }
         return;
     }
-    __shared__ Runs runs;
+    __shared__ Runs<kWriteRows> runs;
     find_runs(runs, row0 - 1 + tid < total ? slot : -1, nr);
     if (runs.n == 0) return;
     turns(c, at, runs.end, turn);
@@ -509,6 +512,16 @@ struct Narrow8Lds {
     static constexpr int OBYTES = 4 * OT * 1024;
     static constexpr int BYTES = Q + (QBYTES > OBYTES ? QBYTES : OBYTES);
 };
+
+// A load of what no one else reads: it takes no place in the caches.  (32 sequences of 8192 keys, 8 kv heads of
+// 128, pages of 32: 115 us a call, 139 with ordinary loads.  ONCE, below: whether V comes so.  A visit's 64 keys
+// are half a line of V where a page is 128 positions or more, and the next wave reads the other half: on three
+// sequences of 70001 to 100000 a call takes 117 us with ordinary loads of V there, 124 with these, 225 with
+// these and neighbouring visits in one wave.  As two kernels: a branch around the loads costs 5 %.)
+template <class V>
+__device__ __forceinline__ V once(const V* p) {
+    return __builtin_nontemporal_load(p);
+}
 
 // 8 codes -> f16 or bf16, exactly
 template <class C>
@@ -572,7 +585,7 @@ __device__ __forceinline__ void parts_bf16(const f32x8& v, u32x4 (&p)[3]) {
 // How far above the reference a weight may come before the reference follows (log2).
 constexpr float kSlack = 8.0f;
 
-template <class C, int D>
+template <class C, int D, bool ONCE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(PagedKv8 c, PageTable t, Call a) {
     using L = Narrow8Lds<D>;
     constexpr int NB = L::NB, OT = L::OT, KB = D / 64, U = 64;
@@ -624,7 +637,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int b = 0; b < KB; ++b) kr[s][b] = *reinterpret_cast<const u32x4*>(k + 4 * s * D + 64 * b);
+                for (int b = 0; b < KB; ++b) kr[s][b] = once(reinterpret_cast<const u32x4*>(k + 4 * s * D + 64 * b));
             block(seg, v, qd, head, off);
             ke = c.k_exp[(head << shift >> 4) + off / kBlock];
         };
@@ -634,7 +647,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
             block(seg, v, qd, head, off);
             const uint8_t* x = c.v + ((head * D + col) << shift) + off;
 #pragma unroll
-            for (int i = 0; i < OT; ++i) vr[i] = *reinterpret_cast<const u32x4*>(x + ((16 * i) << shift));
+            for (int i = 0; i < OT; ++i) {
+                const u32x4* from = reinterpret_cast<const u32x4*>(x + ((16 * i) << shift));
+                vr[i] = ONCE ? once(from) : *from;
+            }
             ve = c.v_exp[(head << shift >> 4) + off / kBlock];
         };
         // q's parts: task (product, lane) as the B operand takes it.  (Its requests and the page ids' go out
@@ -1452,6 +1468,7 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(PagedKv8 c, PageTable t,
 }
 
 // ---- values read back -------------------------------------------------------------------------
+constexpr int kReadRows = 16;  // rows of a workgroup
 struct Read {
     const int *ids, *starts, *cu;
     int B, n;
@@ -1468,13 +1485,13 @@ struct alignas(16) Eight {  // (four, of f32)
 // The mirror of the writes: runs of rows in one block, a wave a run of one kv head's keys or values.
 template <class C, class O, int D>
 __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, Read a) {
-    constexpr int NR = kWriteRows;
     constexpr int kHold = 1024;  // entries that are held, and searched, in LDS
-    __shared__ Runs runs;
+    __shared__ Runs<kReadRows> runs;
     __shared__ uint64_t bad_rows;
     __shared__ int cu[kHold], ids[kHold], starts[kHold];
     const int tid = threadIdx.x, lane = tid & 63;
     const int KVH = (int)c.n_kv_heads, groups = (KVH + a.heads - 1) / a.heads;
+    constexpr int NR = kReadRows;
     const int bx = by_xcd(blockIdx.x, gridDim.x), row0 = bx / groups * NR, g0 = bx % groups * a.heads;
     const int heads = min(a.heads, KVH - g0), end = min(a.n, a.cu[a.B]);
     const bool in_lds = a.B <= kHold;
@@ -1522,57 +1539,66 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, 
                     if (outs[w])
                         for (int d = lane; d < heads * D; d += 64)
                             outs[w][(row0 + r) * a.stride + (int64_t)g0 * D + d] = (O)__builtin_nanf("");
-    for (int i = wv; i < runs.n * heads * 2; i += 4) {
-        const int g = g0 + i / 2 % heads, run = i / 2 / heads;
-        O* out = outs[i % 2];
-        if (!out) continue;
+    // a task: a run's keys and values of a head, all requested before the first is stored
+    constexpr int E = 16 / sizeof(O), CH = D / E, RP = 64 / CH, KN = kBlock / RP;  // K: 16 bytes of the output a lane
+    constexpr int VN = D / 128 > 0 ? D / 128 : 1;                                 // V: two dimensions a lane
+    struct alignas(2 * sizeof(O)) Two {
+        O v[2];
+    };
+    using Raw = std::conditional_t<sizeof(O) == 4, uint64_t, uint32_t>;
+    for (int i = wv; i < runs.n * heads; i += 4) {
+        const int g = g0 + i % heads, run = i / heads;
         const int r0 = __builtin_amdgcn_readfirstlane(runs.first[run]);
         const int n = __builtin_amdgcn_readfirstlane(runs.count[run]);
         const int sl = __builtin_amdgcn_readfirstlane(runs.slots[r0 + 1]);
         const int in_page = sl & ((int)c.page_size - 1), off = sl % kBlock;
         const int64_t head = (int64_t)(sl >> c.page_shift) * KVH + g;
-        const float step = power((i % 2 ? c.v_exp : c.k_exp)[(head << c.page_shift >> 4) + in_page / kBlock]);
-        out += (row0 + r0) * a.stride + (int64_t)g * D;
-        if (i % 2 == 0) {
-            constexpr int E = 16 / sizeof(O);           // 16 bytes of the output a lane
-            constexpr int CH = D / E, RP = 64 / CH;     // lanes a row, rows at a time
-            const uint8_t* k = c.k + ((head << c.page_shift) + in_page) * D + lane % CH * E;
-            O* to = out + lane % CH * E;
-#pragma unroll 4
-            for (int r = lane / CH; r < n; r += RP) {
-                uint32_t w[E / 4];
+        const int64_t block = (head << c.page_shift >> 4) + in_page / kBlock;
+        const uint8_t* k = c.k + ((head << c.page_shift) + in_page) * D + lane % CH * E;
+        const uint8_t* v = c.v + ((head * D + 2 * lane) << c.page_shift) + in_page - off;
+        const float k_step = power(c.k_exp[block]), v_step = power(c.v_exp[block]);
+        const int64_t at = (row0 + r0) * a.stride + (int64_t)g * D;
+        uint32_t kw[KN][E / 4];
+        u32x4 vw[VN][2];
 #pragma unroll
-                for (int x = 0; x < E / 4; ++x) w[x] = reinterpret_cast<const uint32_t*>(k + r * D)[x];
+        for (int x = 0; x < KN; ++x)
+            if (a.k && lane / CH + x * RP < n)
+#pragma unroll
+                for (int e = 0; e < E / 4; ++e) kw[x][e] = once(reinterpret_cast<const uint32_t*>(k + (lane / CH + x * RP) * D) + e);
+#pragma unroll
+        for (int x = 0; x < VN; ++x)
+            if (a.v && 2 * lane + 128 * x < D)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    vw[x][e] = *reinterpret_cast<const u32x4*>(v + ((int64_t)(128 * x + e) << c.page_shift));
+#pragma unroll
+        for (int x = 0; x < KN; ++x)
+            if (a.k && lane / CH + x * RP < n) {
                 Eight<O> y;
 #pragma unroll
-                for (int x = 0; x < E / 4; ++x) {
-                    const f32x4 z = decode4<C>(w[x]) * step;
+                for (int e = 0; e < E / 4; ++e) {
+                    const f32x4 z = decode4<C>(kw[x][e]) * k_step;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) y.v[4 * x + j] = (O)z[j];
+                    for (int j = 0; j < 4; ++j) y.v[4 * e + j] = (O)z[j];
                 }
-                *reinterpret_cast<Eight<O>*>(to + r * a.stride) = y;
+                O* to = static_cast<O*>(a.k) + at + (lane / CH + x * RP) * a.stride + lane % CH * E;
+                __builtin_nontemporal_store(__builtin_bit_cast(u32x4, y), reinterpret_cast<u32x4*>(to));
             }
-        } else {
-            // two dimensions a lane
-            struct alignas(2 * sizeof(O)) Two {
-                O v[2];
-            };
-            const uint8_t* v = c.v + ((head * D) << c.page_shift) + in_page - off;
-            for (int d = 2 * lane; d < D; d += 128) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(v + ((int64_t)d << c.page_shift));
-                const u32x4 y = *reinterpret_cast<const u32x4*>(v + ((int64_t)(d + 1) << c.page_shift));
+#pragma unroll
+        for (int x = 0; x < VN; ++x)
+            if (a.v && 2 * lane + 128 * x < D)
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const f32x4 p = decode4<C>(x[w]) * step, q = decode4<C>(y[w]) * step;
+                    const f32x4 p = decode4<C>(vw[x][0][w]) * v_step, q = decode4<C>(vw[x][1][w]) * v_step;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = 4 * w + e - off;
+                        O* to = static_cast<O*>(a.v) + at + r * a.stride + 128 * x + 2 * lane;
                         if (r >= 0 && r < n)
-                            *reinterpret_cast<Two*>(out + r * a.stride + d) = Two{{(O)p[e], (O)q[e]}};
+                            __builtin_nontemporal_store(__builtin_bit_cast(Raw, Two{{(O)p[e], (O)q[e]}}),
+                                                        reinterpret_cast<Raw*>(to));
                     }
                 }
-            }
-        }
     }
 }
 
@@ -1663,7 +1689,9 @@ hipError_t launch_typed(const PagedKv8& c, const unillm_page_table& t, const Cal
     using N = Narrow8Lds<D>;
     using W = Wide8Lds<D>;
     static const bool attr =
-        hipFuncSetAttribute((const void*)kv8_narrow_kernel<C, D>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        hipFuncSetAttribute((const void*)kv8_narrow_kernel<C, D, true>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            N::BYTES) == hipSuccess &&
+        hipFuncSetAttribute((const void*)kv8_narrow_kernel<C, D, false>, hipFuncAttributeMaxDynamicSharedMemorySize,
                             N::BYTES) == hipSuccess &&
         hipFuncSetAttribute((const void*)kv8_wide_kernel<C, D>, hipFuncAttributeMaxDynamicSharedMemorySize,
                             W::BYTES) == hipSuccess;
@@ -1674,7 +1702,9 @@ hipError_t launch_typed(const PagedKv8& c, const unillm_page_table& t, const Cal
         kv8_wide_kernel<C, D><<<grid(l.items[kWide] * a.KVH, 4 * most), W::NT, W::BYTES, s>>>(c, t.st, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    kv8_narrow_kernel<C, D><<<grid(l.items[kNarrow] * a.KVH, most), 256, N::BYTES, s>>>(c, t.st, a);
+    const unsigned narrow = grid(l.items[kNarrow] * a.KVH, most);
+    if (c.page_size <= 64) kv8_narrow_kernel<C, D, true><<<narrow, 256, N::BYTES, s>>>(c, t.st, a);
+    else kv8_narrow_kernel<C, D, false><<<narrow, 256, N::BYTES, s>>>(c, t.st, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     kv8_merge_kernel<C, D><<<grid((l.rows[0] + l.rows[1]) / 2, most), 256, 0, s>>>(c, t.st, a);
     return hipGetLastError();
@@ -1741,7 +1771,7 @@ size_t kv8_workspace_bytes(const PagedKv8& c, const unillm_page_table& t, int64_
 hipError_t launch_kv8_read(const PagedKv8& c, const unillm_page_table& t, const int* ids,
                            const int* starts, const int* cu, int64_t n_seqs, int64_t n, int type,
                            void* k_out, void* v_out, int64_t ostride, hipStream_t s) {
-    const int64_t blocks = (n + kWriteRows - 1) / kWriteRows;
+    const int64_t blocks = (n + kReadRows - 1) / kReadRows;
     Read a{ids, starts, cu, (int)n_seqs, (int)n, k_out, v_out, ostride, heads_each(blocks, c.n_kv_heads)};
     const unsigned grid = (unsigned)((blocks * ((c.n_kv_heads + a.heads - 1) / a.heads) + 7) / 8 * 8);
     return by_pool(c, [&](auto code, auto dim) {
