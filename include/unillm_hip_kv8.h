@@ -52,7 +52,7 @@ int unillm_hip_rope_create(int64_t head_dim, int64_t rotary_dim, int layout, dou
                            const double* freq_factors, double magnitude, unillm_rope** out);
 int unillm_hip_rope_destroy(unillm_rope* r);
 /* n rows of n_heads heads each, of type UNILLM_QTYPE_F32, _F16 or _BF16, x_stride and out_stride
- * elements from row to row (at least n_heads head_dim): each turned at its position
+ * elements from row to row (at least n_heads head_dim, at most 2^27): each turned at its position
  * positions_dev[row], rounded once.  A negative position turns back (where the magnitude is 1).
  * Pointers aligned to their elements; faster where 16 bytes divide pointers, strides and
  * rotary_dim / 2 (interleaved: rotary_dim).  out_dev is x_dev (with the same stride: in place), or
@@ -107,8 +107,10 @@ int unillm_hip_paged_kv8_attention(unillm_paged_kv8* c, const unillm_page_table*
                                    const float* qkv_dev, int64_t qkv_stride, int64_t n_tokens,
                                    int64_t n_heads, int append, int64_t window, int64_t sinks,
                                    float* out_dev, int64_t out_stride, void* stream);
-/* Grow `stream`'s workspace to what such calls of up to n_tokens rows need on this table, so
- * they can be captured into a HIP graph (unillm_hip_attention_reserve).  (append and read need none.) */
+/* Grow `stream`'s workspace to what such calls of up to n_tokens rows need on this table (the queries' bytes
+ * once more, and some 100 MB at most), so they can be captured into a HIP graph
+ * (unillm_hip_attention_reserve).  Graphs captured on one stream share it, with each other and with
+ * eager calls there: replay them on that stream.  (append and read need none.) */
 int unillm_hip_paged_kv8_reserve(const unillm_paged_kv8* c, const unillm_page_table* t,
                                  int64_t n_tokens, int64_t n_heads, void* stream);
 

@@ -208,6 +208,51 @@ def test_long_sequences_dealt_out_in_pieces():
     close(out, *expect(cache, table, q, 4, entries))
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("hd,G,ctx,n", [(128, 2, 5000, 70), (64, 3, 3000, 130), (256, 1, 2500, 140)])
+def test_long_chunks_dealt_out_in_pieces(kind, hd, G, ctx, n):
+    table, cache, gen = make(kind, 1, hd, 64, [ctx, 9], max_tokens=4096, rope=Rope(hd))
+    entries = [(1, 1), (0, n)]
+    q, out = step(table, cache, gen, G, entries, True)
+    close(out, *expect(cache, table, q, G, entries, frequencies(hd)))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("n", [1, 90])
+def test_values_of_zero_and_a_few_that_are_not(kind, n):
+    """All values 0: outputs 0.  Then one block's are not, which few weights reach."""
+    table, cache, gen = make(kind, 1, 64, 16, [200])
+    table.truncate(ints([0]), ints([0]))
+    table.extend(ints([0]), ints([200]))
+    kv = torch.randn(200, 128, device="cuda", generator=gen)
+    kv[:, 64:] = 0.0
+    cache.append(table, kv)
+    table.extend(ints([0]), ints([n]))
+    qkv = torch.randn(n, 192, device="cuda", generator=gen)
+    qkv[:, 128:] = 0.0
+    assert not cache.attention(table, qkv, 1).any()
+    table.truncate(ints([0]), ints([200]))
+    table.extend(ints([0]), ints([n]))
+    qkv[0, 128:] = 1e-3 * torch.randn(64, device="cuda", generator=gen)
+    out = cache.attention(table, qkv, 1)
+    table.check()
+    close(out, *expect(cache, table, qkv[:, :64], 1, [(0, n)]))
+
+
+def test_a_step_on_a_table_of_8192_sequences():
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    table = PageTable(8192, 8, 9000, 16, 9000)
+    cache = PagedKvCache8(1, 64, 9000, 16, torch.float8_e4m3fn)
+    ids = torch.randperm(8192, device="cuda", generator=gen).to(torch.int32)
+    table.extend(ids, torch.ones_like(ids))
+    qkv = torch.randn(8192, 64 * 4, device="cuda", generator=gen)
+    out = cache.attention(table, qkv, 2)
+    table.check()
+    # a token alone has its own value
+    k, v = cache.read(table, ids, torch.zeros_like(ids), torch.arange(8193, device="cuda", dtype=torch.int32), 8192)
+    assert torch.equal(out.view(8192, 2, 64), v.expand(8192, 2, 64))
+
+
 def test_padding_rows_and_strides():
     table, cache, gen = make("int8", 2, 64, 16, [30, 50])
     table.extend(ints([1, -1, 0]), ints([2, 3, 1]))

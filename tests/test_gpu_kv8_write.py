@@ -95,6 +95,25 @@ def test_many_rows_in_one_step(kind):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("heads,hd", [(9, 64), (18, 64), (34, 64), (33, 128), (32, 256)])
+def test_decoding_rows_among_chunks(kind, heads, hd):
+    """Workgroups of 4, 8 and 16 rows (by rows times heads), each with runs of one row and of several."""
+    rope = Rope(hd, interleaved=True)
+    run = Run(kind, heads, hd, 16, n_pages=300, max_seqs=90, rope=rope, freq=frequencies(hd), interleaved=True, max_tokens=700)
+    small = [(i, 1 + (i * 7 % 11 == 0) * 2) for i in range(80)]
+    first = [(i, 1 + i % 5) for i in range(80)] + [(80, 200)]
+    mixed = small[:30] + [(80, 170)] + small[30:] + [(81, 250)]
+    steps(run, 11, [([i for i, _ in e], [n for _, n in e]) for e in (first, mixed, mixed)], spread=2.0)
+
+
+def test_a_table_of_8192_sequences():
+    """The plan's LDS is the largest there; entries in any order."""
+    run = Run("int8", 1, 64, 16, n_pages=600, max_seqs=8192, max_tokens=600)
+    ids = [(i * 37) % 8192 for i in range(500)]
+    steps(run, 12, [(ids, [1] * 500), (ids[::-1], [1] * 500)])
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
 def test_every_growth_of_an_exponent(kind):
     """A block whose positions each need twice the last one's step, and more; values on ties."""
     run = Run(kind, 1, 64, 16, n_pages=4)

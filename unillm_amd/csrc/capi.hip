@@ -1325,9 +1325,9 @@ int unillm_hip_rope_apply(const unillm_rope* r, int type, const void* x_dev, int
                                                 " (want 0 = F32, 1 = F16, 30 = BF16)");
     if (n < 0 || n > (int64_t)INT32_MAX || n_heads < 1 || n_heads > 65535)
         return fail(UNILLM_ERR_INVALID_ARG, what + "need n in [0, 2^31) and n_heads in [1, 65535]");
-    const int64_t width = n_heads * r->head_dim, far = (int64_t)1 << 31;
+    const int64_t width = n_heads * r->head_dim, far = (int64_t)1 << 27;
     if (x_stride < width || out_stride < width || x_stride > far || out_stride > far)
-        return fail(UNILLM_ERR_INVALID_ARG, what + "row strides must be at least " + std::to_string(width));
+        return fail(UNILLM_ERR_INVALID_ARG, what + "row strides must be in [" + std::to_string(width) + ", 2^27]");
     if (n == 0) return UNILLM_OK;
     if (!x_dev || !out_dev || !positions_dev)
         return fail(UNILLM_ERR_INVALID_ARG, what + "x, out or positions is NULL");
@@ -1382,7 +1382,7 @@ int check_kv8_heads(const unillm_paged_kv8* c, int64_t n, int64_t n_heads, const
 
 // Rows of f32 that a call reads.
 int check_rows(const float* p, int64_t stride, int64_t width, const std::string& what, const char* name) {
-    if (stride < width || stride % 4 != 0 || stride > (int64_t)1 << 40)
+    if (stride < width || stride % 4 != 0 || stride > (int64_t)1 << 32)
         return fail(UNILLM_ERR_INVALID_ARG, what + ": row strides must be multiples of 4 floats, of at least " +
                                                 std::to_string(width) + " (" + name + ")");
     if (!p) return fail(UNILLM_ERR_INVALID_ARG, what + ": " + name + " is NULL");
@@ -1558,7 +1558,7 @@ int unillm_hip_paged_kv8_read(const unillm_paged_kv8* c, const unillm_page_table
         return fail(UNILLM_ERR_INVALID_ARG, what + ": need n_seqs in [0, 2^22] and n_rows in [0, 2^26]");
     const int64_t width = c->n_kv_heads * c->head_dim;
     const size_t size = (size_t)dense_elem_bytes(out_type);
-    if (out_stride < width || out_stride > (int64_t)1 << 40 || (size_t)out_stride * size % 16 != 0)
+    if (out_stride < width || out_stride > (int64_t)1 << 32 || (size_t)out_stride * size % 16 != 0)
         return fail(UNILLM_ERR_INVALID_ARG,
                     what + ": out_stride must be at least " + std::to_string(width) + ", a multiple of 16 bytes");
     if (n_seqs == 0 || n_rows == 0) return UNILLM_OK;

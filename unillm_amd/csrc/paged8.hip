@@ -75,6 +75,16 @@ __device__ __forceinline__ uint32_t again4(uint32_t w, float f) {
     return encode4<C>(v[0], v[1], v[2], v[3]);
 }
 
+// A load of what no one else reads: it takes no place in the caches.  (32 sequences of 8192 keys, 8 kv heads of
+// 128, pages of 32: 115 us a call, 139 with ordinary loads.  ONCE, below: whether V comes so.  A visit's 64 keys
+// are half a line of V where a page is 128 positions or more, and the next wave reads the other half: on three
+// sequences of 70001 to 100000 a call takes 117 us with ordinary loads of V there, 124 with these, 225 with
+// these and neighbouring visits in one wave.  As two kernels: a branch around the loads costs 5 %.)
+template <class V>
+__device__ __forceinline__ V once(const V* p) {
+    return __builtin_nontemporal_load(p);
+}
+
 // ---- rows into their blocks -------------------------------------------------------------------
 //
 // Rows of consecutive slots in one block of 16 are a run: a wave writes a run of one kv head's keys, or
@@ -155,7 +165,7 @@ __device__ __forceinline__ int2 octet_at(const PagedKv8& c, int u) {
     return make_int2(8 * u, 8 * u + 4);
 }
 __device__ __forceinline__ Octet octet(const float* x, int2 d) {
-    return Octet{*reinterpret_cast<const f32x4*>(x + d.x), *reinterpret_cast<const f32x4*>(x + d.y)};
+    return Octet{once(reinterpret_cast<const f32x4*>(x + d.x)), once(reinterpret_cast<const f32x4*>(x + d.y))};
 }
 // It rotated, in f64, to f32.
 __device__ __forceinline__ void rotate(const PagedKv8& c, Octet& o, int u, const double2* turn) {
@@ -274,7 +284,9 @@ __device__ __forceinline__ void write_values(const PagedKv8& c, const float* x, 
     for (int p = 0; p < kBlock; ++p) {
 #pragma unroll
         for (int j = 0; j < N; ++j) v[p].v[j] = 0.0f;
-        if (p >= off && p < off + n) v[p] = *reinterpret_cast<const Dims*>(x + (p - off) * stride + N * lane);
+        if (p >= off && p < off + n)
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[p].v[j] = once(x + (p - off) * stride + N * lane + j);
     }
 #pragma unroll
     for (int p = 0; p < kBlock; ++p)
@@ -512,16 +524,6 @@ struct Narrow8Lds {
     static constexpr int OBYTES = 4 * OT * 1024;
     static constexpr int BYTES = Q + (QBYTES > OBYTES ? QBYTES : OBYTES);
 };
-
-// A load of what no one else reads: it takes no place in the caches.  (32 sequences of 8192 keys, 8 kv heads of
-// 128, pages of 32: 115 us a call, 139 with ordinary loads.  ONCE, below: whether V comes so.  A visit's 64 keys
-// are half a line of V where a page is 128 positions or more, and the next wave reads the other half: on three
-// sequences of 70001 to 100000 a call takes 117 us with ordinary loads of V there, 124 with these, 225 with
-// these and neighbouring visits in one wave.  As two kernels: a branch around the loads costs 5 %.)
-template <class V>
-__device__ __forceinline__ V once(const V* p) {
-    return __builtin_nontemporal_load(p);
-}
 
 // 8 codes -> f16 or bf16, exactly
 template <class C>
