@@ -99,7 +99,7 @@ int unillm_hip_paged_kv8_append(unillm_paged_kv8* c, const unillm_page_table* t,
  * cache's values.  append 1: qkv_dev's rows are q, k, v, and k and v are appended first; append 0: they are q
  * alone (n_heads head_dim floats), and the rows' keys and values are there already.  f32's precision:
  * q is held to 22 bits, an element 2^-17 below its row's largest to fewer, 2^-39 of that one; weights are
- * held whole where an entry has up to 64 query rows a kv head.  A row of a longer entry may be off
+ * held whole where an entry has up to 64 query rows a kv head (hd 128: 96, hd 64: 144).  A row of a longer entry may be off
  * by 2^-16 of its largest sum of |weight x value| besides, 2^-27 a key where it sees more than 2048, if keys
  * of almost no value in their blocks take almost all of its weight.
  */

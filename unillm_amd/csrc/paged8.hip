@@ -26,8 +26,11 @@ namespace unillm {
 namespace {
 
 constexpr int kBlock = 16;  // positions to an exponent
-// Most query rows of an entry (a kv head) for narrow tiles.
-constexpr int kNarrowRows8 = 64;
+// Most query rows of an entry (a kv head) for narrow tiles.  (8 entries on 4000 keys, pages of 32, int8, us a call:
+// hd 64, 8 kv heads, of 112 rows narrow 56, wide 64, of 160 rows 64 and 64; hd 128, 8 kv heads, of 80 rows 74 and
+// 85, of 112 rows 90 and 86; hd 256, 4 kv heads, of 64 rows 67 and 84, of 80 rows 122 and 85.  e4m3 the
+// same to 10 %.)
+__host__ __device__ constexpr int narrow_rows(int64_t D) { return D == 64 ? 144 : D == 128 ? 96 : 64; }
 struct Int8 {
     static constexpr float top = 127.0f, room = 127.0f / 128.0f;  // top = room 2^bits
     static constexpr int bits = 7;
@@ -448,8 +451,8 @@ __global__ __launch_bounds__(256, D == 256 ? 3 : 4) void kv8_prepare_kernel(Page
     }
     if (bx < 0) {
         if (blockIdx.x == 0 && tid == 0) *a.redo_count = 0;
-        if (blockIdx.x == 0) return plan<64, kNarrowRows8>(t, a, kNarrow, reinterpret_cast<int*>(lds));
-        return plan<D == 256 ? 32 : 64, kNarrowRows8>(t, a, kWide, reinterpret_cast<int*>(lds));
+        if (blockIdx.x == 0) return plan<64, narrow_rows(D)>(t, a, kNarrow, reinterpret_cast<int*>(lds));
+        return plan<D == 256 ? 32 : 64, narrow_rows(D)>(t, a, kWide, reinterpret_cast<int*>(lds));
     }
     const int total = t.counts[kPagesTokens];
     if (row0 >= total) return;
@@ -1628,12 +1631,12 @@ Layout layout(const PagedKv8& c, const unillm_page_table& t, int64_t n, int64_t 
         return here;
     };
     for (int k = 0; k < 2; ++k) {
-        // tiles: an entry's last may be ragged (a wide entry has more than kNarrowRows8 rows).  A
+        // tiles: an entry's last may be ragged (a wide entry has more than narrow_rows).  A
         // tile of nv visits makes at most nv / C + 1 pieces, and the nv / C add up to target /
         // KVH; more than one piece, at most 2 nv / C.
-        const int64_t entries = std::min<int64_t>(k == kNarrow ? n : n * G / (kNarrowRows8 + 1), t.st.max_seqs);
+        const int64_t entries = std::min<int64_t>(k == kNarrow ? n : n * G / (narrow_rows(D) + 1), t.st.max_seqs);
         const int64_t tiles = n * G / tile_rows(k, D) + entries;
-        const bool some = k == kNarrow || n * G > kNarrowRows8;
+        const bool some = k == kNarrow || n * G > narrow_rows(D);
         l.items[k] = some ? tiles + target_pieces(k) / KVH + 1 : 0;
         l.rows[k] = some ? 2 * (int64_t)target_pieces(k) * std::min<int64_t>(tile_rows(k, D), n * G) : 0;
         l.head_at[k] = take(2 * sizeof(int));
