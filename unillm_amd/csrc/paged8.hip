@@ -1204,6 +1204,7 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                     const bool all = ju + 31 <= wmin &&
                                      (a.window == 0 || ju > wmax - a.window || ju + 32 <= a.sinks);
                     if (!all) {
+                        asm volatile("");  // (a branch: without it every visit forms its masks)
                         const int at = ppos - ju - 8 * hf, far = a.window > 0 ? at - a.window : INT_MIN;
                         const int sk0 = a.sinks - ju - 8 * hf;
 #pragma unroll
@@ -1232,6 +1233,10 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                     const float f = ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
                     const float fo = __builtin_amdgcn_ldexpf(f, rise - up);
                     l *= f;
+                    // (held in accumulation registers: without this every visit copies all of them out, in case)
+                    if constexpr (D == 256)
+#pragma unroll
+                        for (int i = 0; i < OT; ++i) asm volatile("" : "+a"(o[i]));
 #pragma unroll
                     for (int i = 0; i < OT; ++i) o[i] *= fo;
                     ref = to;
