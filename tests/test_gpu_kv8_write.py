@@ -242,6 +242,32 @@ def test_read_back(kind, dtype, heads, hd, page):
             assert torch.equal(got[at:at + n].cpu(), want)
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("heads,hd,n", [(1, 64, 20011), (2, 128, 9001), (4, 64, 8200)])
+def test_read_of_many_rows(kind, heads, hd, n):
+    """Workgroups of 16, 32 and 64 rows; some rows are not their sequence's."""
+    table = PageTable(3, 2000, 2000, 16, 20600)
+    cache = PagedKvCache8(heads, hd, 2000, 16, KINDS[kind])
+    table.extend(ints([1, 0]), ints([n - 37, 500]))
+    kv = torch.randn(n - 37 + 500, 2 * heads * hd, device="cuda")
+    cache.append(table, kv)
+    k, v = cache.read(table, ints([1, 2, 0, 1]), ints([3, 0, 490, 0]), ints([0, n - 40, n - 30, n - 17, n]), n,
+                      dtype=torch.bfloat16)
+    with pytest.raises(HipError, match="does not hold"):
+        table.check()
+    whole_k, whole_v = cache.read(table, ints([0, 1]), ints([0, 0]), ints([0, 500, 500 + n - 37]), 500 + n - 37)
+    table.check()
+    for got, whole, x in ((k, whole_k, kv[:, :heads * hd]), (v, whole_v, kv[:, heads * hd:])):
+        assert torch.equal(got[:n - 40], whole[503:].bfloat16())
+        assert torch.isnan(got[n - 40:n - 30]).all() and torch.isnan(got[n - 20:n - 17]).all()
+        assert torch.equal(got[n - 30:n - 20], whole[490:500].bfloat16())
+        assert torch.equal(got[n - 17:], whole[500:517].bfloat16())
+        # (and the values are those that were written, to half a step: 1/127 of a block's largest at most, or 2^-4 of itself)
+        y, x = whole[500:].flatten(1), x[:n - 37]
+        top = x.abs().max()
+        assert ((y - x).abs() <= (top / 127 if kind == "int8" else x.abs() * 2.0 ** -4 + top * 2.0 ** -16)).all()
+
+
 def test_read_outside_a_sequence():
     run = Run("int8", 2, 64, 16)
     steps(run, 8, [([0, 1], [20, 3])])

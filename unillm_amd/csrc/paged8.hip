@@ -1478,13 +1478,13 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(PagedKv8 c, PageTable t,
 }
 
 // ---- values read back -------------------------------------------------------------------------
-constexpr int kReadRows = 16;  // rows of a workgroup
+constexpr int kReadRows = 64;  // rows of a workgroup, at most
 struct Read {
     const int *ids, *starts, *cu;
     int B, n;
     void *k, *v;
     int64_t stride;
-    int heads;  // of a workgroup
+    int rows, heads;  // of a workgroup
 };
 
 template <class O>
@@ -1497,12 +1497,11 @@ template <class C, class O, int D>
 __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, Read a) {
     constexpr int kHold = 1024;  // entries that are held, and searched, in LDS
     __shared__ Runs<kReadRows> runs;
-    __shared__ uint64_t bad_rows;
+    __shared__ uint64_t bad_rows[2];  // by row from row0 - 1 on
     __shared__ int cu[kHold], ids[kHold], starts[kHold];
     const int tid = threadIdx.x, lane = tid & 63;
     const int KVH = (int)c.n_kv_heads, groups = (KVH + a.heads - 1) / a.heads;
-    constexpr int NR = kReadRows;
-    const int bx = by_xcd(blockIdx.x, gridDim.x), row0 = bx / groups * NR, g0 = bx % groups * a.heads;
+    const int NR = a.rows, bx = by_xcd(blockIdx.x, gridDim.x), row0 = bx / groups * NR, g0 = bx % groups * a.heads;
     const int heads = min(a.heads, KVH - g0), end = min(a.n, a.cu[a.B]);
     const bool in_lds = a.B <= kHold;
     if (in_lds)
@@ -1532,19 +1531,19 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, 
             }
         }
     }
-    if (tid < 64) {
-        const uint64_t b = __ballot(bad) >> 1;  // (bit i: row row0 + i)
-        if (tid == 0) {
-            bad_rows = b & ((1ull << NR) - 1);
-            if (bad_rows != 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadRead);
+    if (tid < 128) {
+        const uint64_t b = __ballot(bad);
+        if ((tid & 63) == 0) {
+            bad_rows[tid >> 6] = b;
+            if (b != 0) atomicCAS(&t.counts[kPagesError], 0, (int)kPagesBadRead);
         }
     }
     find_runs(runs, slot, NR);
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     O* const outs[2] = {static_cast<O*>(a.k), static_cast<O*>(a.v)};
-    if (bad_rows != 0)
+    if ((bad_rows[0] | bad_rows[1]) != 0)
         for (int r = wv; r < NR; r += 4)
-            if (bad_rows >> r & 1)
+            if (bad_rows[(r + 1) / 64] >> (r + 1) % 64 & 1)
                 for (int w = 0; w < 2; ++w)
                     if (outs[w])
                         for (int d = lane; d < heads * D; d += 64)
@@ -1781,8 +1780,12 @@ size_t kv8_workspace_bytes(const PagedKv8& c, const unillm_page_table& t, int64_
 hipError_t launch_kv8_read(const PagedKv8& c, const unillm_page_table& t, const int* ids,
                            const int* starts, const int* cu, int64_t n_seqs, int64_t n, int type,
                            void* k_out, void* v_out, int64_t ostride, hipStream_t s) {
-    const int64_t blocks = (n + kReadRows - 1) / kReadRows;
-    Read a{ids, starts, cu, (int)n_seqs, (int)n, k_out, v_out, ostride, heads_each(blocks, c.n_kv_heads)};
+    // (a workgroup's tasks are its runs times its heads: of few heads it takes more rows, where they are many.
+    // 171000 rows of 2 heads of 256: 16 a workgroup 174 us, so 108)
+    int rows = kBlock;
+    while (rows < kReadRows && rows * c.n_kv_heads < 8 * kBlock && n >= (int64_t)4096 * rows / kBlock) rows *= 2;
+    const int64_t blocks = (n + rows - 1) / rows;
+    Read a{ids, starts, cu, (int)n_seqs, (int)n, k_out, v_out, ostride, rows, heads_each(blocks, c.n_kv_heads)};
     const unsigned grid = (unsigned)((blocks * ((c.n_kv_heads + a.heads - 1) / a.heads) + 7) / 8 * 8);
     return by_pool(c, [&](auto code, auto dim) {
         using C = decltype(code);
