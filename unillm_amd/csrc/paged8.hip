@@ -10,8 +10,9 @@
 // Attention is that of paged.hip (its plan, pieces and merge are shared, paged.hpp):
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = e^(q k_j / sqrt(hd) - max).
 // A code is exact in f16 and in bf16.  q k: codes in f16 against two f16 parts of q (22 bits), the block's
-// power of two multiplied onto the scores; w v: codes in bf16 against three bf16 parts of the weight
-// times its block's power of two, all 24 bits of it and of any size.
+// power of two multiplied onto the scores.  w v: the weight times its block's power of two, in narrow tiles in
+// three bf16 parts against codes in bf16, all 24 bits of it and of any size; in wide tiles, which the
+// matrix cores bound, in two f16 parts against codes in f16.
 #include <hip/hip_runtime.h>
 
 #include <limits.h>
@@ -92,6 +93,9 @@ __device__ __forceinline__ V once(const V* p) {
 //
 // Rows of consecutive slots in one block of 16 are a run: a wave writes a run of one kv head's keys, or
 // values, whole, so no two waves meet in a block, and an exponent's byte is its own.
+// Bound by HBM where rows are many: 4000 rows of 32 kv heads of 128, e4m3, 164 MB in 51 us, 3.2 TB/s (a copy 5.4:
+// V goes out in 16-byte pieces of its lines); by the latency of dependent loads where they are few: 96 rows of 8
+// heads 6 us.
 constexpr int kWriteRows = 16;  // rows of a workgroup whose runs it takes, at most
 
 template <int ROWS>
@@ -516,6 +520,9 @@ __global__ __launch_bounds__(256, D == 256 ? 3 : 4) void kv8_prepare_kernel(Page
 //     row l % 16, the scores of the 16 keys of block l / 16 of the visit, and one exponent is all of theirs.  Its
 //     16 bytes are dimensions 64 b + 16 (l / 16) .. of the key, 8 to each of two products;
 //   O^T += V^T . P^T: its 16 bytes are those 16 keys' values of dimension l % 16 of each 16.
+// Bound by HBM: 80 sequences of up to 9000, 8 kv heads of 128, pages of 32, e4m3, 441 MB in 84 us, 5.2 TB/s (a copy
+// 5.4); widening int8 codes takes 540 vector instructions a visit beside 80 MFMAs, e4m3 320, and 32 sequences
+// of 8192 take either at the same rate; for short sequences by latency (one of 1500 keys: 8 us).
 template <int D>
 struct Narrow8Lds {
     static constexpr int NB = D / 32, OT = D / 16;
@@ -884,6 +891,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
 // the row's largest weight times power of two so far, as 2^11: parts down to 2^-24 reach 2^-35 of it.  (A
 // whole power of two apart from the weights' own reference, so that sums and weights are scaled alike, to the
 // bit.)  What that may lose is looked at in the end.
+// Bound by the matrix cores at hd 128 (3001 tokens behind 8000, 32 heads on 8, int8: 950 us, 980 TFLOP/s of
+// products, where a large library product reaches 1152), by the vector units at hd 64 (700), and at hd 256 by
+// having one wave a SIMD, whose products nothing overlaps (780).
 constexpr int kWideShift = 11;
 constexpr float kWideSlack = 4.0f;
 // What a row may lose by the weights' parts, of its largest sum: 2^-16 over up to 2048 keys, 2^-27 a key over
@@ -1492,7 +1502,9 @@ struct alignas(16) Eight {  // (four, of f32)
     O v[16 / sizeof(O)];
 };
 
-// The mirror of the writes: runs of rows in one block, a wave a run of one kv head's keys or values.
+// The mirror of the writes: runs of rows in one block, a wave a run of one kv head's keys and values.
+// Bound by HBM: 90000 rows of 8 heads of 128, to f16, 553 MB, pages of 16 in 92 us (6.0 TB/s), of 128 in 133 (a line
+// of V is eight runs', which several workgroups fetch).
 template <class C, class O, int D>
 __global__ __launch_bounds__(256) void kv8_read_kernel(PagedKv8 c, PageTable t, Read a) {
     constexpr int kHold = 1024;  // entries that are held, and searched, in LDS

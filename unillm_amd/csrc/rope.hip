@@ -57,7 +57,8 @@ struct RopeCall {
 // A workgroup takes `rows` rows: a thread has a unit of a head, V elements (half-split: and their partners),
 // of every so many of their heads, four at a time, the first four requested before the rows' cosines and
 // sines are formed (in LDS).
-// Bound by HBM where rows are many, by latency for few.
+// Bound by HBM where rows are many (20001 rows of 32 heads of 128 in f32, 655 MB in 125 us: 5.2 TB/s, a copy's
+// rate), by latency for few (one row 3.3 us, 777 rows in f16 5.4).
 template <class T, int V, int W, bool HALF>
 __global__ __launch_bounds__(256) void rope_kernel(RopeCall a, int rows) {
     using S = Some<T, V, W>;
