@@ -419,6 +419,12 @@ def test_refusals():
                    dict(rope=Rope(64, rotary_dim=20)), dict(k=torch.zeros(4, 2, 16, 64, device="cuda", dtype=torch.int8))):
         with pytest.raises(RuntimeError):
             PagedKvCache8(**{**dict(n_kv_heads=2, head_dim=64, n_pages=4, page_size=16), **change})
+    closed = Rope(64)
+    closed.close()
+    with pytest.raises(RuntimeError, match="closed"):
+        PagedKvCache8(2, 64, 4, 16, rope=closed)
+    with pytest.raises(RuntimeError, match="NULL"):
+        closed.apply(torch.zeros(1, 1, 64, device="cuda"), ints([0]))
     mem = [torch.zeros(4, 2, 16, 64, device="cuda", dtype=torch.int8), torch.zeros(4, 2, 1, device="cuda", dtype=torch.uint8)]
     with pytest.raises(RuntimeError, match="share memory"):
         PagedKvCache8(2, 64, 4, 16, k=mem[0], v=mem[0].view(4, 2, 64, 16), k_exp=mem[1], v_exp=mem[1].clone())

@@ -33,6 +33,8 @@ class PagedKvCache8:
         self._h = None
         if dtype not in _KV8_TYPES:
             raise RuntimeError(f"PagedKvCache8: dtype {dtype} (want int8 or float8_e4m3fn)")
+        if rope is not None and rope._h is None:
+            raise RuntimeError("PagedKvCache8: the rope is closed")
         parts = [k, v, k_exp, v_exp]
         if any((p is None) != (k is None) for p in parts):
             raise RuntimeError("PagedKvCache8: give all of k, v, k_exp and v_exp, or none")
