@@ -51,6 +51,20 @@ def test_shapes_and_types(dtype, interleaved, n, heads, hd, rot):
     check(out, x, pos.tolist(), frequencies(rot), interleaved)
 
 
+@pytest.mark.parametrize("dtype", list(EPS))
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("n,heads,hd,rot", [(1, 1, 3, 2), (5, 3, 5, 4), (40, 2, 511, 2), (9, 7, 65, 64)])
+def test_heads_of_odd_sizes(dtype, interleaved, n, heads, hd, rot):
+    torch.manual_seed(hd)
+    x = torch.randn(n, heads, hd, device="cuda").to(dtype)
+    pos = torch.randint(0, 1 << 20, (n,), device="cuda", dtype=torch.int32)
+    rope = Rope(hd, rotary_dim=rot, interleaved=interleaved)
+    hold = torch.full((n, heads * hd + 3), 7.0, device="cuda", dtype=dtype)
+    check(rope.apply(x, pos, out=hold[:, 1:-2].unflatten(1, (heads, hd))), x, pos.tolist(), frequencies(rot), interleaved)
+    assert (hold[:, [0, -2, -1]] == 7).all()
+    assert torch.equal(rope.apply(x, pos, out=x), hold[:, 1:-2].unflatten(1, (heads, hd)))
+
+
 @pytest.mark.parametrize("scaling", list(SCALED))
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_scalings(scaling, interleaved):

@@ -63,13 +63,14 @@ template <class T, int V, int W, bool HALF>
 __global__ __launch_bounds__(256) void rope_kernel(RopeCall a, int rows) {
     using S = Some<T, V, W>;
     constexpr int B = 4, P = HALF ? V : V / 2;  // items at a time, pairs of a unit
+    constexpr bool kOdd = W < V;                // a head may end inside its last unit
     // [rows][rot / 2], pair p at p % P rot / 2 P + p / P: what lanes read together lies together
     extern __shared__ double2 turn[];
     const int tid = threadIdx.x, pairs = a.rot / 2, sets = pairs / P;
     const int64_t row0 = (int64_t)blockIdx.x * rows;
     const int n = (int)min((int64_t)rows, a.n - row0);
     // units of a head: those that turn first, then those that are copied
-    const int turning = (HALF ? pairs : a.rot) / V, units = turning + (a.copy ? (a.hd - a.rot) / V : 0);
+    const int turning = (HALF ? pairs : a.rot) / V, units = turning + (a.copy ? (a.hd - a.rot + (kOdd ? V - 1 : 0)) / V : 0);
     const int across = min(units, 256), side = tid / across, sides = 256 / across;
     const int dr = sides / a.heads, dh = sides % a.heads;
     int u = side < sides ? tid % across : units;
@@ -94,7 +95,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeCall a, int rows) {
             hh[i] = h;
             if (u < units && r < n) {
                 const T* x = static_cast<const T*>(a.x) + (row0 + r) * a.xstride + h * a.hd + d;
-                lo[i] = *reinterpret_cast<const S*>(x);
+                if (kOdd && d + V > a.hd) lo[i].v[0] = x[0];
+                else lo[i] = *reinterpret_cast<const S*>(x);
                 if (HALF && u < turning) hi[i] = *reinterpret_cast<const S*>(x + pairs);
             }
             next();
@@ -133,7 +135,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeCall a, int rows) {
                         lo[i].v[2 * e + 1] = rope_narrow<T>(p * z[e * sets].y + q * z[e * sets].x);
                     }
                 }
-                *reinterpret_cast<S*>(out) = lo[i];
+                if (kOdd && d + V > a.hd) out[0] = lo[i].v[0];
+                else *reinterpret_cast<S*>(out) = lo[i];
             }
     }
 }
