@@ -45,8 +45,9 @@ typedef struct unillm_paged_kv8 unillm_paged_kv8;
 /* Rotary positions of heads of head_dim (2 .. 512) elements, of which the first rotary_dim (even, 2 ..
  * head_dim) turn.  theta > 1 (finite).  factor >= 1 where a scaling takes it; low, high and original
  * (> 0) where LLAMA3 or YARN do; what a scaling does not take is not looked at.  freq_factors:
- * rotary_dim / 2 positive host values (a GGUF file's rope_freqs), or NULL: 1.  magnitude: of the
- * turned pairs, finite; 0: the scaling's own (YARN 0.1 ln factor + 1, else 1). */
+ * rotary_dim / 2 positive host values (a GGUF file's rope_freqs) that leave no frequency past 2^20,
+ * or NULL: 1.  magnitude: of the turned pairs, finite; 0: the scaling's own (YARN 0.1 ln factor + 1,
+ * else 1). */
 int unillm_hip_rope_create(int64_t head_dim, int64_t rotary_dim, int layout, double theta, int scaling,
                            double factor, double low, double high, int64_t original,
                            const double* freq_factors, double magnitude, unillm_rope** out);

@@ -79,6 +79,14 @@ def test_rope_shapes_are_checked_on_the_host(lib, change):
     assert lib.unillm_hip_rope_create(*{**ROPE, **change}.values(), None) == BAD
 
 
+@pytest.mark.parametrize("factor", [1e-7, 1e-310])
+def test_frequencies_past_2_to_the_20_are_refused(lib, factor):
+    out = ctypes.c_void_p(5)
+    factors = (ctypes.c_double * 32)(*[factor] + [1.0] * 31)
+    assert lib.unillm_hip_rope_create(*{**ROPE, "factors": factors}.values(), ctypes.byref(out)) == BAD
+    assert out.value is None and "frequency" in _capi.last_error()
+
+
 @pytest.mark.parametrize("change", [
     dict(kv_type=0), dict(kv_type=3), dict(kv_type=24), dict(heads=0), dict(heads=65536), dict(hd=96), dict(hd=0),
     dict(hd=512), dict(n_pages=0), dict(n_pages=1 << 28), dict(page=24), dict(page=8), dict(heads=40000, hd=256, page=256),

@@ -1267,7 +1267,6 @@ int unillm_hip_rope_create(int64_t head_dim, int64_t rotary_dim, int layout, dou
     for (int i = 0; freq_factors && i < pairs; ++i)
         if (!(freq_factors[i] > 0.0) || !isfinite(freq_factors[i]))
             return fail(UNILLM_ERR_INVALID_ARG, what + "freq_factors must be positive and finite");
-    if (int rc = ensure_init()) return rc;
     const double R = (double)rotary_dim, context = (double)original;
     double first = 0.0, last = 0.0;  // YARN's ramp, by the pair's number
     if (scaling == UNILLM_ROPE_SCALE_YARN) {
@@ -1287,10 +1286,13 @@ int unillm_hip_rope_create(int64_t head_dim, int64_t rotary_dim, int layout, dou
         if (scaling == UNILLM_ROPE_SCALE_YARN) r = 1.0 - (i - first) / std::max(last - first, 0.001);
         r = std::min(std::max(r, 0.0), 1.0);
         if (scaling != UNILLM_ROPE_SCALE_NONE) f *= r + (1.0 - r) / factor;
+        if (!(f <= 0x1p20))  // (one position's angle is held to 2^-52 of itself)
+            return fail(UNILLM_ERR_INVALID_ARG, what + "a frequency past 2^20 (its freq_factor is too small)");
         turns[i] = f / M_PI;
         turns[pairs + 2 * i] = cos(f);
         turns[pairs + 2 * i + 1] = sin(f);
     }
+    if (int rc = ensure_init()) return rc;
     unillm_rope* h = new (std::nothrow) unillm_rope{};
     if (!h) return fail(UNILLM_ERR_OUT_OF_MEMORY, "host allocation failed");
     *h = {g_device, layout, head_dim, rotary_dim, magnitude, nullptr};

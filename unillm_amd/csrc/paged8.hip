@@ -93,7 +93,7 @@ __device__ __forceinline__ V once(const V* p) {
 //
 // Rows of consecutive slots in one block of 16 are a run: a wave writes a run of one kv head's keys, or
 // values, whole, so no two waves meet in a block, and an exponent's byte is its own.
-// Bound by HBM where rows are many: 4000 rows of 32 kv heads of 128, e4m3, 164 MB in 51 us, 3.2 TB/s (a copy 5.4:
+// Bound by HBM where rows are many: 4000 rows of 32 kv heads of 128, e4m3, 164 MB in 48 us, 3.4 TB/s (a copy 5.4:
 // V goes out in 16-byte pieces of its lines); by the latency of dependent loads where they are few: 96 rows of 8
 // heads 6 us.
 constexpr int kWriteRows = 16;  // rows of a workgroup whose runs it takes, at most
