@@ -372,6 +372,27 @@ def test_serving_run_eager_captured_and_on_streams():
     assert torch.equal(aside, layers[0].attention(table, torch.ones(6, H * hd, device="cuda"), H))
 
 
+@pytest.mark.parametrize("kind,KVH,hd", [("int8", 8, 256), ("e4m3", 16, 128), ("int8", 32, 64)])
+def test_pages_past_4_gib_of_a_pool(kind, KVH, hd):
+    """The same rows on pages from 8200 on (512 KiB each, 4.3 GB before them) and on the first ones: the same bits."""
+    page, H, got = 256, 2 * KVH, []
+    for before in (8200, 0):
+        table = PageTable(3, 8200, before + 12, page, 1 << 22)
+        cache = PagedKvCache8(KVH, hd, before + 12, page, KINDS[kind], Rope(hd))
+        if before:
+            table.extend(ints([2]), ints([before * page]))
+        gen = torch.Generator(device="cuda").manual_seed(hd)
+        outs = [step(table, cache, gen, H, entries, True)[1]
+                for entries in ([(0, 700), (1, 40)], [(0, 1), (1, 300)], [(1, 1), (0, 20)], [(0, 1), (1, 1)])]
+        held = [p for p in table.block_table[:2].flatten().tolist() if p >= 0]
+        assert len(held) >= 5 and min(held) >= before
+        outs += cache.read(table, ints([0, 1]), ints([3, 0]), ints([0, 700, 1000]), 1000)
+        table.check()
+        got.append(outs)
+        del table, cache
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_capture_without_a_workspace_is_refused():
     table, cache, gen = make("int8", 1, 64, 16, [20])
     table.extend(ints([0]), ints([1]))
