@@ -48,8 +48,11 @@ __device__ __forceinline__ int least_exponent(float top) {
     const int e = __builtin_amdgcn_frexp_expf(top) - C::bits + (__builtin_amdgcn_frexp_mantf(top) > C::room ? 1 : 0);
     return max(1, e + 127);
 }
-// 2^(b - 127), of b in [1, 254] (0 and 255, which no block is given, as those)
-__device__ __forceinline__ float power(int b) { return __uint_as_float((uint32_t)min(max(b, 1), 254) << 23); }
+// A byte of the pool as the exponent it counts as (0 and 255, which no block is given, as 1 and 254).
+__device__ __forceinline__ int counted(int b) { return min(max(b, 1), 254); }
+// 2^(b - 127), and 2^(127 - b) of a counted b (of 254 a denormal, by which products are as exact)
+__device__ __forceinline__ float power(int b) { return __uint_as_float((uint32_t)counted(b) << 23); }
+__device__ __forceinline__ float inverse(int b) { return __uint_as_float(b < 254 ? (uint32_t)(254 - b) << 23 : 1u << 22); }
 
 // Four values, in steps, as codes: to nearest even, infinities to the largest code, NaN to 0.
 template <class C>
@@ -224,7 +227,7 @@ __device__ __forceinline__ void write_keys(const PagedKv8& c, const float* x, in
     const int64_t head = (int64_t)(sl >> c.page_shift) * c.n_kv_heads + g;
     uint8_t* dst = c.k + ((head << c.page_shift) + in_page) * D;
     uint8_t* exps = c.k_exp + ((head << c.page_shift >> 4) + in_page / kBlock);
-    const int had = off > 0 ? min((int)*exps, 254) : 0;
+    const int had = off > 0 ? counted(*exps) : 0;
     const int2 d = octet_at(c, u);
     Octet v[N];
     float top = 0.0f;
@@ -248,7 +251,7 @@ __device__ __forceinline__ void write_keys(const PagedKv8& c, const float* x, in
     }
     const int b = max(least_exponent<C>(wave_max(top)), had);
     if (lane == 0) *exps = (uint8_t)b;
-    const float inv = power(254 - b);
+    const float inv = inverse(b);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int r = i * RP + sub;
@@ -278,7 +281,7 @@ __device__ __forceinline__ void write_values(const PagedKv8& c, const float* x, 
     const int64_t head = (int64_t)(sl >> c.page_shift) * c.n_kv_heads + g;
     uint8_t* dst = c.v + ((head * D + N * lane) << c.page_shift) + in_page / kBlock * kBlock;
     uint8_t* exps = c.v_exp + ((head << c.page_shift >> 4) + in_page / kBlock);
-    const int had = off > 0 ? min((int)*exps, 254) : 0;
+    const int had = off > 0 ? counted(*exps) : 0;
     u32x4 old[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -301,7 +304,7 @@ __device__ __forceinline__ void write_values(const PagedKv8& c, const float* x, 
         for (int j = 0; j < N; ++j) top = fmaxf(top, magnitude(v[p].v[j], odd));
     const int b = max(least_exponent<C>(wave_max(top)), had);
     if (lane == 0) *exps = (uint8_t)b;
-    const float inv = power(254 - b), f = power(127 + had - b);
+    const float inv = inverse(b), f = power(127 + had - b);
     const bool anew = off > 0 && b > had;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -338,7 +341,7 @@ __device__ __forceinline__ void write_one_keys(const PagedKv8& c, const float* k
     uint8_t* exps = c.k_exp + ((head << c.page_shift >> 4) + in_page / kBlock);
     const int2 d = octet_at(c, u);
     Octet v = octet(kv + row * stride + (int64_t)g * D, d);
-    const int had = off > 0 ? min((int)*exps, 254) : 0;
+    const int had = off > 0 ? counted(*exps) : 0;
     rotate(c, v, u, turn + row * (c.rotary_dim / 2));
     asm volatile("" : "+v"(v.lo), "+v"(v.hi));  // (rows of f32 first)
     float top = 0.0f;
@@ -352,7 +355,7 @@ __device__ __forceinline__ void write_one_keys(const PagedKv8& c, const float* k
     const int b = max(least_exponent<C>(top), had);
     if (!live) return;
     if (u == 0) *exps = (uint8_t)b;
-    const float inv = power(254 - b);
+    const float inv = inverse(b);
     const f32x4 lo = v.lo * inv, hi = v.hi * inv;
     *reinterpret_cast<uint32_t*>(dst + d.x) = encode4<C>(lo[0], lo[1], lo[2], lo[3]);
     *reinterpret_cast<uint32_t*>(dst + d.y) = encode4<C>(hi[0], hi[1], hi[2], hi[3]);
@@ -390,11 +393,11 @@ __device__ __forceinline__ void write_one_values(const PagedKv8& c, const float*
         float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < N; ++j) top = fmaxf(top, magnitude(v[i].v[j], odd));
-        const int was = off > 0 ? min(had[i], 254) : 0;
+        const int was = off > 0 ? counted(had[i]) : 0;
         const int b = max(least_exponent<C>(wave_max(top)), was);
         if (lane == 0) c.v_exp[(head[i] << c.page_shift >> 4) + in_page / kBlock] = (uint8_t)b;
         uint8_t* dst = c.v + ((head[i] * D + N * lane) << c.page_shift) + in_page - off;
-        const float inv = power(254 - b);
+        const float inv = inverse(b);
         if (off > 0 && b > was) {  // (the codes before it, in the row's first words)
             const float f = power(127 + was - b);
             for (int j = 0; j < N; ++j)
@@ -1051,7 +1054,7 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                 *reinterpret_cast<u32x4*>(buf + L::K + at) = codes_f16<C>(sk[i][0], sk[i][1]);
                 if (lane == 0) {
                     steps[m % 4 * 4 + kgroup(i)] = power(ke[i]);
-                    vexps[m % 4 * 4 + kgroup(i)] = min(max(ve[i], 1), 254) - 127;
+                    vexps[m % 4 * 4 + kgroup(i)] = counted(ve[i]) - 127;
                 }
             }
             const int left = len - kstored;  // keys of V's visit and on
