@@ -602,6 +602,11 @@ __device__ __forceinline__ void parts_bf16(const f32x8& v, u32x4 (&p)[3]) {
 
 // How far above the reference a weight may come before the reference follows (log2).
 constexpr float kSlack = 8.0f;
+// Narrow tiles' weights times their blocks' powers of two, and the sums of both, are held 2^kLift times as large, so
+// that weights of small values keep their bits: with the least step, 2^-126, down to a weight of 2^-16 all of
+// them.  (Of values past 2^80 or so the products are infinite: their rows are done again.)
+constexpr int kLift = 32;
+__device__ __forceinline__ float lifted(int b) { return __uint_as_float((uint32_t)min(max(b, 1) + kLift, 255) << 23); }
 
 template <class C, int D, bool ONCE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(PagedKv8 c, PageTable t, Call a) {
@@ -783,7 +788,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
                     ref = up;
                 }
                 const float from = ref == -INFINITY ? 0.0f : ref;  // (all weights are 0 then)
-                const float step = power(ve);
+                const float step = lifted(ve);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     s[r] = __builtin_amdgcn_exp2f(s[r] - from);
@@ -822,6 +827,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
         // the four waves' sums: scaled to one reference, added through LDS
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
+        l *= (float)(1ull << kLift);  // (as the sums of values)
         if (bad) flags[0] = 1;
         __syncthreads();  // (q's parts are read)
         if (lane < 16) {
