@@ -56,3 +56,18 @@ def test_a_power_of_two_of_the_values(kind, hd, n, gap):
 @pytest.mark.parametrize("power", [-115, -100, 100, 115])
 def test_values_near_the_ends(kind, hd, n, power, gap):
     close(*(lambda out, want: (out, *want))(*attended(kind, hd, n, power, gap)))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("gap", [11.0, 13.0])
+@pytest.mark.parametrize("power", [-100, -105])
+def test_rows_of_small_values_are_done_again_as_others(kind, hd, gap, power):
+    """A chunk's rows beside a sink (wide tiles): those that are done again in f32 at the one size are at the other, by
+    the same steps.  What comes below f32's normal numbers, at most each of the 900 products and sums, is off by 2^-150,
+    2^-140 in all; a quotient's last bit may turn besides."""
+    out, _ = attended(kind, hd, 200, 0, gap)
+    got, want = attended(kind, hd, 200, power, gap)
+    close(got, *want)
+    off = (torch.ldexp(got.double(), torch.tensor(-power, device="cuda")) - out).abs()
+    assert (off <= 2.0 ** (-140 - power) + 2.0 ** -23 * out.abs()).all(), float((off / out.abs().amax()).max())

@@ -1332,13 +1332,13 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
         float chk = l * 0.0f, most = 0.0f;
         // Weights in two parts are off by up to 2^-25, and a row's sums by that times the item's keys and the
         // largest code: a row whose largest sum may have lost too much is done again (but where all values are
-        // 0, or next to it: their blocks' exponents are the least).
+        // 0, or next to it, below 2^-112: their blocks' exponents are the least, and rise is -126 or little more).
 #pragma unroll
         for (int i = 0; i < OT; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(o[i][e]));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
-        if (l > 0.0f && rise > -100 &&
+        if (l > 0.0f && rise > -120 &&
             most * kWideLoss < C::top * ((float)min(it.nv * U, kWideLossKeys) * 0x1p-25f)) chk = 1.0f;
         // the sums against the weights' reference
 #pragma unroll
