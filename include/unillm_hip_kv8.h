@@ -85,8 +85,10 @@ int unillm_hip_paged_kv8_buffers(const unillm_paged_kv8* c, void** k, void** v, 
  * block that gets new positions: its exponent becomes the least, at least -126, with which the new
  * values' largest magnitude is at most 127 (e4m3: 448) steps, and no less than it was if the
  * block holds positions before them; if it grows, their codes are rounded anew, each growth
- * doubling the step at least, so that a code is never off by more than one step.  New values
- * are rounded to nearest even.  What a block holds past the step's last position stays.  What is
+ * doubling the step at least.  New values are rounded to nearest even.  So of a block whose step is s an
+ * int8 value is off by at most s / 2, and by less than s where the block grew after it was written; an
+ * e4m3 one by at most 2^-4 of itself or 2^-10 s, whichever is more, and where the block grew by 2^-4 of
+ * itself and less than 2^-9 s.  What a block holds past the step's last position stays.  What is
  * not finite is held as the largest code (an infinity) or as 0 (NaN), counts for no exponent, and is
  * reported by unillm_hip_page_table_check.  Exponents do not shrink when positions are taken back
  * (truncate) and written again within a block.  If the table has no plan, or one of more than n_tokens

@@ -2,10 +2,11 @@
 //
 // A pool's codes are int8 or e4m3, and 16 positions of a kv head share a power of two, so a code c of a
 // block with byte b stands for c 2^(b - 127).  Powers of two: a block's exponent grows as further
-// positions come, and its codes are rounded anew then.  Each growth at least doubles the step, so the
-// roundings add up to less than one step however often it happens (with the tightest step, growing
-// by little each time, to several), and rounding to half the step or rounding a code to twice
-// the step is exact arithmetic: the same bits on every machine.
+// positions come, and its codes are rounded anew then.  Each growth at least doubles the step s, so an int8
+// code's roundings add up to less than s however often it happens, s / 2 (1 + 1/2 + ..) (with the tightest step,
+// growing by little each time, to several).  e4m3 codes have 4 significant bits, which a growth keeps until a code is
+// below 2^-6: 2^-4 of the value, and less than 2^-9 s.  Values times a power of two, and codes rounded from them, are
+// exact arithmetic: the same bits on every machine.
 //
 // Attention is that of paged.hip (its plan, pieces and merge are shared, paged.hpp):
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = e^(q k_j / sqrt(hd) - max).
