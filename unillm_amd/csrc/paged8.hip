@@ -1284,9 +1284,9 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
             }
             if (!kStoreEarly) store(n + 1 + grp);
             __syncthreads();  // the vector phase ends
-            // (where the matrix phase is the longer one, its wave goes first on the SIMD: three chunks
-            // among 24 sequences, bf16, 169 us against 175; at hd 64, f16, 233 against 224)
-            if (!kStoreEarly) __builtin_amdgcn_s_setprio(1);
+            // (the matrix phase's wave goes first on the SIMD: 3001 tokens behind 8000, int8, at hd 128 981 us, 1004 without;
+            // at hd 64 631 and 673.  At hd 256 there is one wave: 438 without, 445 so.)
+            if (GR == 2) __builtin_amdgcn_s_setprio(1);
             {
                 // o += p v of visit n.  Step i: dimensions 32 (i % OT) .., keys of MFMA i / OT
                 const uint8_t* buf = lds + (n + 1) % GR * L::PAIR;
@@ -1311,12 +1311,12 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
                 }
             }
             if (n + 1 == it.nv) {
-                __builtin_amdgcn_s_setprio(0);
+                if (GR == 2) __builtin_amdgcn_s_setprio(0);
                 break;
             }
             if (kStoreEarly) store(n + 2);
             scores(n + 1);
-            if (!kStoreEarly) __builtin_amdgcn_s_setprio(0);
+            if (GR == 2) __builtin_amdgcn_s_setprio(0);
             __syncthreads();  // the matrix phase ends
         }
         if (GR == 2) {  // (both groups pass 2 nv + 2 barriers from the first pair on)
