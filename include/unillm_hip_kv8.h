@@ -104,8 +104,10 @@ int unillm_hip_paged_kv8_append(unillm_paged_kv8* c, const unillm_page_table* t,
  * q is held to 22 bits, an element 2^-17 below its row's largest to fewer, 2^-39 of that one; weights are
  * held whole where an entry has up to 64 query rows a kv head (hd 128: 96, hd 64: 144).  A row of a longer entry may be off
  * by 2^-16 of its largest sum of |weight x value| besides, 2^-27 a key where it sees more than 2048, if keys
- * of almost no value in their blocks take almost all of its weight.
- */
+ * of almost no value in their blocks take almost all of its weight.  Rows of a longer entry that would be off by
+ * more are done again, by a wave each that reads all its keys: behind an attention sink of no value, where the
+ * other keys' weighted values come to less than 1/512 of the largest code at the sink's weight, a chunk takes tens of
+ * times as long. */
 int unillm_hip_paged_kv8_attention(unillm_paged_kv8* c, const unillm_page_table* t,
                                    const float* qkv_dev, int64_t qkv_stride, int64_t n_tokens,
                                    int64_t n_heads, int append, int64_t window, int64_t sinks,

@@ -83,11 +83,14 @@ __device__ __forceinline__ uint32_t again4(uint32_t w, float f) {
     return encode4<C>(v[0], v[1], v[2], v[3]);
 }
 
-// A load of what no one else reads: it takes no place in the caches.  (32 sequences of 8192 keys, 8 kv heads of
+// A load of what is read once: it takes no place in the caches.  (32 sequences of 8192 keys, 8 kv heads of
 // 128, pages of 32: 115 us a call, 139 with ordinary loads.  ONCE, below: whether V comes so.  A visit's 64 keys
 // are half a line of V where a page is 128 positions or more, and the next wave reads the other half: on three
 // sequences of 70001 to 100000 a call takes 117 us with ordinary loads of V there, 124 with these, 225 with
-// these and neighbouring visits in one wave.  As two kernels: a branch around the loads costs 5 %.)
+// these and neighbouring visits in one wave.  As two kernels: a branch around the loads costs 5 %.  The keys of an entry of
+// more than one narrow tile are read again by the tiles' other items, and there these loads cost time: 80 sequences
+// of up to 8750 keys, 32 heads on 8 of 128, e4m3, pages of 32, us a call with these and with ordinary loads: 16 rows
+// an entry and kv head 87 and 91, 32 rows 142 and 120, 64 rows 248 and 195.)
 template <class V>
 __device__ __forceinline__ V once(const V* p) {
     return __builtin_nontemporal_load(p);
@@ -422,7 +425,7 @@ __device__ __forceinline__ int by_xcd(int i, int n) { return i % 8 * (n / 8) + i
 // rows and q_heads heads each (rotated, times log2 e / sqrt(hd), f32, into q_out); the rest write the runs
 // that begin in `rows` rows, of `heads` kv heads. An append does only the last of these: its kernel is
 // compiled without the others (PLAN false: 400 B of LDS instead of 9 KB, and 4000 rotated rows of 32 heads of
-// 128 in 47.2 us instead of 49.4).
+// 128, e4m3, in 48.2 us instead of 49.5).
 struct Prepare {
     const float *q, *kv;
     int64_t stride;  // of both
@@ -905,7 +908,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_narrow_kernel(Paged
 // whole power of two apart from the weights' own reference, so that sums and weights are scaled alike, to the
 // bit.)  What that may lose is looked at in the end.
 // Bound by the matrix cores at hd 128 (3001 tokens behind 8000, 32 heads on 8, int8: 950 us, 980 TFLOP/s of
-// products, where a large library product reaches 1152), by the vector units at hd 64 (700), and at hd 256 by
+// products, where a large library product reaches 1152), by the vector units at hd 64 (750 over a call), and at hd 256 by
 // having one wave a SIMD, whose products nothing overlaps (780).
 constexpr int kWideShift = 11;
 constexpr float kWideSlack = 4.0f;
@@ -948,8 +951,9 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
     constexpr int VGROUPS = U / 16;
     // A buffer's pair m - 2 was last read in the second group's matrix phase m - 2, so either group may
     // store its share of pair m in the two phases after: its matrix phase m - 1, or the vector
-    // phase m - 1 (m - 2 in the second group).  The stores go with the shorter phase (f16: at hd 128
-    // a matrix phase takes 3000 cycles, the weights 1470; at hd 64 1350 and 1600).
+    // phase m - 1 (m - 2 in the second group).  The stores go with the shorter phase, at hd 128 the vector
+    // one, at hd 64 the matrix one (3001 tokens behind 8000, int8, 32 heads, us a call: hd 128 on 8 kv heads 976, 1331 the
+    // other way; hd 64 on 4 625, 719).
     constexpr bool kStoreEarly = GR == 2 && D == 64;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int* flags = reinterpret_cast<int*>(lds + L::STAT);  // [0] a bad page
@@ -1087,9 +1091,9 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
         __syncthreads();  // (the item before is done with the LDS)
         if (tid == 0) flags[0] = 0;
         float inv = 1.0f;
-        // The wave's rows of q and of their rotations come whole rows at a time and through its own
-        // part of the LDS: a lane's operand is 32 bytes of a row, and loaded so every request would
-        // touch 32 lines (22000 cycles an item at hd 128 before, of 115000).
+        // The wave's rows of q come whole rows at a time and through its own part of the LDS: a lane's operand
+        // is 32 bytes of a row, and loaded so every request would touch 32 lines (3001 tokens behind 8000, hd 128,
+        // int8: 981 us, 1031 so; without the 8000 227 and 231).
         {
             // (opaque lane numbers here and at the end: no address of these is kept through the visits)
             int el = lane;
@@ -1398,7 +1402,9 @@ __global__ __launch_bounds__((256 * Wide8Lds<D>::GR), (D == 256 ? 1 : 2)) void k
 }
 
 // One row and head by a wave, in plain f32: for rows whose products of parts came out non-finite (an
-// infinite query, or scores past f32's range).  qf: LDS [D], the query; sc: LDS [64].  Lane el gets
+// infinite query, or scores past f32's range), and those of wide tiles that lost too much: an attention sink of
+// value 0 may list every row of its head, and each reads all its keys for itself (2000 tokens behind 2000, 32 heads
+// on 8 of 128, int8, a sink of 10 nats in each head: 13.7 ms, 0.28 without).  qf: LDS [D], the query; sc: LDS [64].  Lane el gets
 // dimensions el + 64 i of out.
 template <class C, int D>
 __device__ void attend_row(const PagedKv8& c, const Call& a, const int* pages, int row, int h, int p,
