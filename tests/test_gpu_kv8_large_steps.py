@@ -40,3 +40,14 @@ def test_more_than_256_wide_tiles(kind):
     entries = [(i * 7 % 260, 5) for i in range(260)]
     q, out = step(table, cache, gen, 13, entries, True)
     close(out, *expect(cache, table, q, 13, entries, frequencies(256)))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("hd,G", [(64, 145), (64, 300), (128, 97), (256, 130)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (33, 5)])
+def test_many_heads_on_one(kind, hd, G, window, sinks):
+    """Single tokens of so many heads on one kv head that they are wide tiles' rows, beside a few of several tokens."""
+    table, cache, gen = make(kind, 1, hd, 32, [300, 1, 40], rope=Rope(hd, rotary_dim=hd // 2))
+    entries = [(1, 1), (0, 2), (2, 1)]
+    q, out = step(table, cache, gen, G, entries, True, window=window, sinks=sinks)
+    close(out, *expect(cache, table, q, G, entries, frequencies(hd // 2), window=window, sinks=sinks))
